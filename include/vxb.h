@@ -228,6 +228,31 @@ int vxb_kv_free_seq(vxb_kv *kv, int64_t seq_id);
  * once in kv_stats), a partly filled last block is copied; appends to either
  * sequence never touch a shared block. Synchronous on `stream`. */
 int vxb_kv_fork(vxb_kv *kv, int64_t src_seq, int64_t dst_seq, int64_t n_tokens, void *stream);
+/* append_kv for ragged chunks: h_n_tokens[i] (>= 0) consecutive tokens of
+ * sequence h_seq_ids[i] (no sequence twice), their rows packed one sequence
+ * after another: d_k / d_v bf16 [sum of h_n_tokens, num_kv_heads, head_dim],
+ * 16-byte aligned. Blocks come from the free stack sequence by sequence; the
+ * kernel builds each token's slot, the block-table entries and the lengths
+ * from the chunk lengths (no copy from host memory). All or nothing: on
+ * VXB_ENOBLOCKS no sequence has changed. */
+int vxb_kv_append_chunks(vxb_kv *kv, int layer, int n, const int64_t *h_seq_ids, const int32_t *h_n_tokens,
+                         const uint16_t *d_k, const uint16_t *d_v, void *stream);
+/* Takes appended tokens back (rejected drafts): afterwards every layer of
+ * sequence h_seq_ids[i] (no sequence twice) holds at most h_lens[i] tokens;
+ * layers that hold fewer, and sequences the cache does not know, stay as they
+ * are. Emptied blocks return to the free stack, the last one first. Where the
+ * cut falls inside a block that a forked sequence shares, the kept rows move
+ * to a block of the sequence's own (VXB_ENOBLOCKS, nothing changed, if there
+ * is none). Ordered on `stream`, does not synchronise. */
+int vxb_kv_truncate(vxb_kv *kv, int n, const int64_t *h_seq_ids, const int64_t *h_lens, void *stream);
+/* The cache's own device memory, for kernels and copies of the caller's (any
+ * output may be NULL): keys and values [max_blocks, num_kv_heads, block_size,
+ * head_dim] (bf16 or int8), int8 scales f32 [max_blocks, num_kv_heads,
+ * block_size] (NULL for bf16), block tables int32 [num_layers, max_seqs,
+ * max_blocks_per_seq] and lengths int32 [num_layers, max_seqs]. Sequences
+ * take slots 0, 1, ... of the last two as they first appear. */
+int vxb_kv_pages(const vxb_kv *kv, void **d_k, void **d_v, float **d_k_scale, float **d_v_scale, int32_t **d_tables,
+                 int32_t **d_lens);
 /* kv_cache_stats (src/kv_cache.rs:220-230): out6 = {used_blocks, free_blocks,
  * block_size, num_seqs (tables), device bytes in use, distinct sequences}. */
 int vxb_kv_stats(const vxb_kv *kv, int64_t *out6);
@@ -247,6 +272,24 @@ int vxb_kv_gather(vxb_kv *kv, int layer, int64_t seq_id, float *d_k_out, float *
 int vxb_decode_attention(vxb_kv *kv, int layer, int n, const int64_t *h_seq_ids, const uint16_t *d_q,
                          int num_q_heads, float softmax_scale, uint16_t *d_out, float *d_lse,
                          void *stream);
+
+/* Attention of chunks of new tokens over the cache: the h_n_queries[i] rows of
+ * sequence h_seq_ids[i] (rows packed one sequence after another, bf16
+ * [sum of h_n_queries, Hq, D]) are its last h_n_queries[i] cached tokens, and
+ * with len cached tokens row r attends to the keys j <= len - h_n_queries[i] +
+ * r (causal != 0) or to all len (causal == 0). out as q, lse (optional) f32
+ * [rows, Hq], natural log. A row that sees no key (an empty or unknown
+ * sequence, more queries than tokens) gives zeros and lse -inf; what the cache
+ * holds behind a sequence's last token is never used. Query head j reads kv
+ * head j / (Hq / Hkv), Hq / Hkv <= 128. Tensors are 16-byte aligned.
+ * d_ws: ws_bytes of device scratch (16-byte aligned), at least what
+ * vxb_chunk_attention_ws gives for this cache and head count, not shared with
+ * a call that may run at the same time. The lengths are those at the call:
+ * a captured call replays with them. Allocates nothing. */
+int vxb_chunk_attention_ws(const vxb_kv *kv, int num_q_heads, size_t *ws_bytes);
+int vxb_chunk_attention(vxb_kv *kv, int layer, int n, const int64_t *h_seq_ids, const int32_t *h_n_queries,
+                        const uint16_t *d_q, int num_q_heads, float softmax_scale, int causal, uint16_t *d_out,
+                        float *d_lse, void *d_ws, size_t ws_bytes, void *stream);
 
 /* ------------------------------------------------------------------------ */
 /* K2: prefill GEMM. Replaces weight_only_matmul (src/quantize.rs:845-852)  */
@@ -323,6 +366,33 @@ int vxb_add(vxb_ctx *ctx, const float *d_a, const float *d_b, size_t n, float *d
  * reference (ties included). vocab <= 131072. Synchronous on `stream`. */
 int vxb_sample_top_p(vxb_ctx *ctx, const float *d_logits, int rows, int vocab, double temperature, double top_p,
                      const int64_t *h_seeds, int32_t *d_out, void *stream);
+
+/* Probabilities of f32 logits [rows, vocab] (contiguous): d_probs f32 [rows,
+ * vocab] = exp((x - max) / t) / sum, with t = d_temperature[row] (f32 [rows])
+ * or, when d_temperature is NULL, `temperature` (finite). A temperature that
+ * is not at least 0.01 is greedy, as in the generate loop (argmax below it): 1
+ * at the first maximum, 0 elsewhere. -inf logits get 0; a row of -inf alone
+ * gives zeros. A NaN logit makes its row NaN (greedy: it is passed over). d_probs may be d_logits. Allocates nothing. */
+int vxb_token_probs(vxb_ctx *ctx, const float *d_logits, int rows, int vocab, const float *d_temperature,
+                    double temperature, float *d_probs, void *stream);
+
+/* Verification of drafted tokens (speculative sampling). Request i has
+ * h_n_drafts[i] (>= 0) drafts, packed one request after another: d_drafts and
+ * d_u_accept [sum of h_n_drafts], d_draft_probs f32 [sum of h_n_drafts, vocab]
+ * (the distributions q they were drawn from; NULL: q is 1 at the draft), and
+ * d_target_probs f32 [sum of h_n_drafts + n, vocab]: the target's p for each
+ * draft and for the token behind the last one. Drafts are accepted in order
+ * while u_accept * q(draft) < p(draft); a draft outside 0..vocab-1 is not.
+ * Then one token is drawn: from max(p - q, 0) of the first refused draft's row,
+ * or from p of the last row when all are accepted, as the first index whose
+ * cumulative sum exceeds d_u_sample[i] (f32 [n], in [0, 1)) times the row's
+ * sum. Products, differences and sums are f64. A row of max(p - q, 0) without
+ * mass draws from p; a p without mass gives token 0; NaN counts as 0.
+ * d_tokens int32 [sum of h_n_drafts + n] gets each request's accepted drafts,
+ * the drawn token, then -1; d_n_accepted int32 [n]. Allocates nothing. */
+int vxb_verify_drafts(vxb_ctx *ctx, int n, const int32_t *h_n_drafts, int vocab, const int32_t *d_drafts,
+                      const float *d_target_probs, const float *d_draft_probs, const float *d_u_accept,
+                      const float *d_u_sample, int32_t *d_tokens, int32_t *d_n_accepted, void *stream);
 
 /* ContinuousBatcher (src/kv_cache.rs:117-154) and the batcher_* builtins
  * (188-290): max_batch_size slots; add takes the lowest free slot and the

@@ -83,11 +83,16 @@ SIGNATURES = {
     "vxb_kv_append_seq": (_I, [_P, _I, _I64, _I, _P, _P, _P]),
     "vxb_kv_free_seq": (_I, [_P, _I64]),
     "vxb_kv_fork": (_I, [_P, _I64, _I64, _I64, _P]),
+    "vxb_kv_append_chunks": (_I, [_P, _I, _I, _P, _P, _P, _P, _P]),
+    "vxb_kv_truncate": (_I, [_P, _I, _P, _P, _P]),
+    "vxb_kv_pages": (_I, [_P, _P, _P, _P, _P, _P, _P]),
     "vxb_kv_stats": (_I, [_P, _P]),
     "vxb_kv_seq_len": (_I, [_P, _I, _I64, _P]),
     "vxb_kv_block_table": (_I, [_P, _I, _I64, _P, _I, _P]),
     "vxb_kv_gather": (_I, [_P, _I, _I64, _P, _P, _P]),
     "vxb_decode_attention": (_I, [_P, _I, _I, _P, _P, _I, ctypes.c_float, _P, _P, _P]),
+    "vxb_chunk_attention_ws": (_I, [_P, _I, ctypes.POINTER(_SZ)]),
+    "vxb_chunk_attention": (_I, [_P, _I, _I, _P, _P, _P, _I, ctypes.c_float, _I, _P, _P, _P, _SZ, _P]),
     "vxb_gemm_q": (_I, [_P, _I, _P, _I, _I, _P, _I, _I, _P, _P]),
     "vxb_flash_fwd": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, ctypes.c_float, _I, _P, _P, _P]),
     "vxb_flash_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, ctypes.c_float, _I, _P, _P, _P, _P]),
@@ -98,6 +103,8 @@ SIGNATURES = {
     "vxb_rope_angles": (_I, [_P, _P, _I, _I, _P, _I, _P, _P]),
     "vxb_add": (_I, [_P, _P, _P, _SZ, _P, _P]),
     "vxb_sample_top_p": (_I, [_P, _P, _I, _I, ctypes.c_double, ctypes.c_double, _P, _P, _P]),
+    "vxb_token_probs": (_I, [_P, _P, _I, _I, _P, ctypes.c_double, _P, _P]),
+    "vxb_verify_drafts": (_I, [_P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _P]),
     "vxb_batcher_create": (_I, [_I, ctypes.POINTER(_P)]),
     "vxb_batcher_destroy": (_I, [_P]),
     "vxb_batcher_add": (_I, [_P, _P, _SZ, ctypes.POINTER(_I)]),

@@ -11,6 +11,7 @@
 // (src/quantize.rs:585-591: absmax/127, all-zero -> 1.0) and codes
 // round-half-away(v/scale) clamped to [-128, 127] (src/quantize.rs:105-108).
 #include <algorithm>
+#include <climits>
 #include <cmath>
 
 #include "kv_cache.h"
@@ -70,6 +71,142 @@ __global__ void kv_append_kernel(const KVPlace *__restrict__ places, int layer, 
   const KVPlace p = places[i];
   append_token(p, i, layer, H, D, bs, max_seqs, mbps, is_int8, k, v, pool_k, pool_v, scale_k, scale_v, tables, lens);
 }
+
+// ---- ragged chunks (vxb_kv_append_chunks)
+//
+// A launch covers consecutive packed rows of the call: `n` pieces, piece i the
+// rows [row0_i, row0_{i+1}) that become tokens pos0_i, pos0_i + 1, ... of one
+// sequence; ids lists the pool blocks of its positions from block pos0_i /
+// block_size on, starting at ids[blk0_i]. The record travels by value (within
+// the 4 KB of kernel parameters that every launch carries), so an append needs
+// no host-to-device copy and no staging buffer that a later call could
+// overwrite.
+constexpr int kPieces = 64, kPieceIds = 640;
+struct ChunkPiece {
+  int32_t slot, pos0, row0, blk0;
+};
+struct ChunkArgs {
+  const uint16_t *k, *v;
+  void *pool_k, *pool_v;
+  float *scale_k, *scale_v;
+  int32_t *tables, *lens;  // of the layer
+  int H, bs, mbps, n, row_end, tokens;
+  ChunkPiece piece[kPieces];
+  int32_t ids[kPieceIds];
+};
+static_assert(sizeof(ChunkArgs) <= 4096, "kernel parameters");
+
+constexpr int kChunkThreads = 256;
+constexpr int kChunkTokens = 64;  // most tokens of a CTA
+
+// One (token, K or V, head) row of D values per D / 8 lanes, 16 bytes a lane;
+// every thread loads four pieces before it stores them. Memory-bound: the
+// rows are read once and written once (bf16), and the destination of a row is
+// 2 D contiguous bytes. A CTA takes `tokens` tokens, enough for two rounds of
+// loads at few heads.
+template <int D, bool INT8>
+__global__ void __launch_bounds__(kChunkThreads) kv_append_chunks_kernel(const __grid_constant__ ChunkArgs a) {
+  __shared__ int32_t s_block[kChunkTokens], s_off[kChunkTokens];
+  const int first = a.piece[0].row0 + (int)blockIdx.x * a.tokens;
+  const int count = min(a.tokens, a.row_end - first);
+  for (int t = threadIdx.x; t < count; t += kChunkThreads) {
+    const int row = first + t;
+    int lo = 0, hi = a.n - 1;  // the last piece whose row0 <= row
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (a.piece[mid].row0 <= row) lo = mid;
+      else hi = mid - 1;
+    }
+    const ChunkPiece p = a.piece[lo];
+    const int pos = p.pos0 + (row - p.row0);
+    const int index = pos / a.bs;
+    const int block = a.ids[p.blk0 + index - p.pos0 / a.bs];
+    s_block[t] = block;
+    s_off[t] = pos - index * a.bs;
+    if (s_off[t] == 0) a.tables[(size_t)p.slot * a.mbps + index] = block;
+    const int end = lo + 1 < a.n ? a.piece[lo + 1].row0 : a.row_end;
+    if (row + 1 == end) a.lens[p.slot] = pos + 1;
+  }
+  __syncthreads();
+  constexpr int LANES = D / 8, ROWS = kChunkThreads / LANES, UNROLL = 4;
+  const int lane = threadIdx.x % LANES, r0 = threadIdx.x / LANES;
+  const int rows = count * 2 * a.H;  // (token, K | V, head)
+  for (int first_row = 0; first_row < rows; first_row += ROWS * UNROLL) {  // the same rounds for every thread: warps shuffle below
+    const int base = first_row + r0;
+    uint4 val[UNROLL];
+    size_t dst[UNROLL];
+    bool isv[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; u++) {
+      const int r = base + u * ROWS;
+      if (r >= rows) break;
+      const int t = r / (2 * a.H), h2 = r - t * 2 * a.H;
+      isv[u] = h2 >= a.H;
+      const int h = isv[u] ? h2 - a.H : h2;
+      val[u] = __ldcs(reinterpret_cast<const uint4 *>((isv[u] ? a.v : a.k) + (((size_t)(first + t) * a.H + h) * D + lane * 8)));
+      dst[u] = ((size_t)s_block[t] * a.H + h) * a.bs + s_off[t];  // token row of the pool
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; u++) {
+      const bool live = base + u * ROWS < rows;
+      if constexpr (!INT8) {
+        if (live) *reinterpret_cast<uint4 *>((uint16_t *)(isv[u] ? a.pool_v : a.pool_k) + dst[u] * D + lane * 8) = val[u];
+      } else {
+        // calibrate_minmax: scale = absmax / 127 in f64 (1 for a row of
+        // zeros), code = v / scale rounded half away from zero. The f32
+        // quotient is within 1e-4 of the f64 one (|code| <= 127, two
+        // roundings and the reciprocal's), so only quotients within 1e-3 of
+        // a half need the f64 division.
+        const uint32_t w[4] = {live ? val[u].x : 0u, live ? val[u].y : 0u, live ? val[u].z : 0u, live ? val[u].w : 0u};
+        float x[8], m = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          x[2 * e] = __uint_as_float(w[e] << 16);
+          x[2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u);
+          m = fmaxf(m, fmaxf(fabsf(x[2 * e]), fabsf(x[2 * e + 1])));
+        }
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const double scale = m == 0.f ? 1.0 : (double)m / 127.0;
+        const float inv = m == 0.f ? 1.f : 127.f / m;
+        // a tiny or non-finite maximum leaves the f32 quotient's error bound
+        const bool plain = m == 0.f || (m > 1e-30f && m < 1e30f);
+        uint32_t out[2] = {0u, 0u};
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const float q = x[e] * inv, aq = fabsf(q);
+          const float n = floorf(aq + 0.5f);
+          int code;
+          if (plain && fabsf(aq - floorf(aq) - 0.5f) > 1e-3f) {
+            code = (int)copysignf(n, q);
+          } else {
+            const double e64 = round((double)x[e] / scale);
+            code = isnan(e64) ? 0 : (int)fmin(fmax(e64, -128.0), 127.0);
+          }
+          out[e >> 2] |= ((uint32_t)code & 0xFFu) << (8 * (e & 3));
+        }
+        if (live) {
+          *reinterpret_cast<uint2 *>((int8_t *)(isv[u] ? a.pool_v : a.pool_k) + dst[u] * D + lane * 8) = make_uint2(out[0], out[1]);
+          if (lane == 0) (isv[u] ? a.scale_v : a.scale_k)[dst[u]] = (float)scale;
+        }
+      }
+    }
+  }
+}
+
+// lens[layer][slot] = min(lens[layer][slot], len) for every layer
+constexpr int kCutSeqs = 256;
+struct CutArgs {
+  int32_t *lens;
+  int n, max_seqs;
+  int32_t slot[kCutSeqs], len[kCutSeqs];
+};
+__global__ void kv_cut_lens_kernel(const __grid_constant__ CutArgs a) {
+  int32_t *row = a.lens + (size_t)blockIdx.x * a.max_seqs;
+  for (int i = threadIdx.x; i < a.n; i += blockDim.x) row[a.slot[i]] = min(row[a.slot[i]], a.len[i]);
+}
+
+__global__ void kv_set_entry_kernel(int32_t *entry, int32_t block) { *entry = block; }
 
 // get_kv (src/kv_cache.rs:69-80) for tests: dequantized f32 [len, H, D].
 __global__ void kv_gather_kernel(const int32_t *__restrict__ table, int len, int H, int D, int bs, int is_int8,
@@ -199,6 +336,7 @@ VXB_API int vxb_kv_create(vxb_ctx *ctx, int num_layers, int num_kv_heads, int he
   if (kv_dtype != VXB_BF16 && kv_dtype != VXB_I8)
     return set_error(ctx, VXB_EINVAL, "vxb_kv_create: kv_dtype must be VXB_BF16 or VXB_I8");
   if (int rc = use_device(ctx)) return rc;
+  if (int rc = ws_reserve(ctx, 0, 0)) return rc;  // device error word: later calls allocate nothing
   vxb_kv *kv = new vxb_kv();
   kv->ctx = ctx;
   kv->num_layers = num_layers;
@@ -296,6 +434,243 @@ VXB_API int vxb_kv_append_seq(vxb_kv *kv, int layer, int64_t seq_id, int n_token
   cudaStream_t st = (cudaStream_t)stream;
   if (int rc = upload_places(kv, pl, st, &d_pl)) return rc;
   return kv_append_launch(kv, layer, n_tokens, d_pl, d_k, d_v, st);
+}
+
+namespace {
+
+// A sequence listed twice in one call (the calls below change each sequence once)
+bool listed_twice(std::vector<int64_t> ids) {
+  std::sort(ids.begin(), ids.end());
+  return std::adjacent_find(ids.begin(), ids.end()) != ids.end();
+}
+
+// Drop the tokens of one table behind `len` (host side): emptied blocks go
+// back to the free stack, the last one first, so that the same appends get the
+// same blocks again.
+void cut_table(vxb_kv *kv, vxb_kv::Table &t, int64_t len) {
+  const int64_t keep = (len + kv->block_size - 1) / kv->block_size;
+  while ((int64_t)t.blocks.size() > keep) {
+    kv_release_block(kv, t.blocks.back());
+    t.blocks.pop_back();
+  }
+  t.len = len;
+}
+
+int append_chunks(vxb_kv *kv, int layer, int n, const int64_t *ids, const int32_t *counts, const uint16_t *d_k,
+                  const uint16_t *d_v, cudaStream_t st) {
+  vxb_ctx *ctx = kv->ctx;
+  const int bs = kv->block_size;
+  int64_t total = 0, need = 0;
+  size_t new_slots = 0;
+  for (int i = 0; i < n; i++) {
+    if (counts[i] < 0) return set_error(ctx, VXB_EINVAL, "vxb_kv_append_chunks: sequence %lld has %d tokens", (long long)ids[i], counts[i]);
+    total += counts[i];
+  }
+  if (total > INT_MAX) return set_error(ctx, VXB_EINVAL, "vxb_kv_append_chunks: %lld rows", (long long)total);
+  if (total == 0) return VXB_OK;
+  if (!d_k || !d_v || ((uintptr_t)d_k | (uintptr_t)d_v) % 16)
+    return set_error(ctx, VXB_EINVAL, "vxb_kv_append_chunks: d_k and d_v must be 16-byte aligned device pointers");
+  if (listed_twice(std::vector<int64_t>(ids, ids + n)))
+    return set_error(ctx, VXB_EINVAL, "vxb_kv_append_chunks: a sequence is listed twice");
+  // everything is checked before anything is taken
+  for (int i = 0; i < n; i++) {
+    if (counts[i] == 0) continue;
+    auto it = kv->tables.find(std::make_pair(layer, ids[i]));
+    const int64_t len = it == kv->tables.end() ? 0 : it->second.len;
+    const int64_t have = (len + bs - 1) / bs, want = (len + counts[i] + bs - 1) / bs;
+    if (want > kv->max_blocks_per_seq || len + counts[i] > INT_MAX)
+      return set_error(ctx, VXB_ENOBLOCKS, "sequence %lld exceeds max_blocks_per_seq=%d", (long long)ids[i], kv->max_blocks_per_seq);
+    need += want - have;
+    if (!kv->slot_of.count(ids[i])) new_slots++;
+  }
+  if (need > (int64_t)kv->free_blocks.size()) return set_error(ctx, VXB_ENOBLOCKS, "KV cache out of blocks");
+  if (new_slots > kv->free_slots.size())
+    return set_error(ctx, VXB_ENOBLOCKS, "KV cache has no free sequence slot (max_seqs=%d)", kv->max_seqs);
+
+  // host tables: blocks and lengths, remembered for the launches
+  struct Seq {
+    vxb_kv::Table *table;
+    int64_t len;
+    int slot;
+  };
+  std::vector<Seq> seqs(n, Seq{nullptr, 0, 0});
+  for (int i = 0; i < n; i++) {
+    if (counts[i] == 0) continue;
+    vxb_kv::Table &t = kv->tables[std::make_pair(layer, ids[i])];
+    const int64_t want = (t.len + counts[i] + bs - 1) / bs;
+    t.blocks.reserve((size_t)want);
+    if (!kv->slot_of.count(ids[i])) {
+      kv->slot_of[ids[i]] = kv->free_slots.back();
+      kv->free_slots.pop_back();
+    }
+    seqs[i] = {&t, t.len, kv->slot_of.at(ids[i])};
+    while ((int64_t)t.blocks.size() < want) {
+      t.blocks.push_back(kv->free_blocks.back());
+      kv->refs[kv->free_blocks.back()] = 1;
+      kv->free_blocks.pop_back();
+    }
+    t.len += counts[i];
+  }
+
+  ChunkArgs a;
+  a.k = d_k;
+  a.v = d_v;
+  a.pool_k = kv->pool_k;
+  a.pool_v = kv->pool_v;
+  a.scale_k = kv->scale_k;
+  a.scale_v = kv->scale_v;
+  a.tables = kv->d_tables + (size_t)layer * kv->max_seqs * kv->max_blocks_per_seq;
+  a.lens = kv->d_lens + (size_t)layer * kv->max_seqs;
+  a.H = kv->num_kv_heads;
+  a.bs = bs;
+  a.mbps = kv->max_blocks_per_seq;
+  a.n = 0;
+  int used = 0, row = 0, rc = VXB_OK;
+  auto flush = [&]() {
+    if (a.n == 0 || rc) return;
+    a.row_end = row;
+    const int rows = row - a.piece[0].row0;
+    // two rounds of 4 x 16 bytes per thread at least, but CTAs for every SM first
+    const int per_token = 2 * a.H * (kv->head_dim / 8);
+    int tokens = (2 * 4 * kChunkThreads + per_token - 1) / per_token;
+    const int sms = kv->ctx->num_sms > 0 ? kv->ctx->num_sms : 148;
+    while (tokens > 1 && (rows + tokens - 1) / tokens < 2 * sms) tokens = (tokens + 1) / 2;
+    a.tokens = std::min(tokens, kChunkTokens);
+    const unsigned grid = (unsigned)((rows + a.tokens - 1) / a.tokens);
+    const bool i8 = kv->dtype == VXB_I8;
+    if (kv->head_dim == 128) {
+      if (i8) kv_append_chunks_kernel<128, true><<<grid, kChunkThreads, 0, st>>>(a);
+      else kv_append_chunks_kernel<128, false><<<grid, kChunkThreads, 0, st>>>(a);
+    } else {
+      if (i8) kv_append_chunks_kernel<64, true><<<grid, kChunkThreads, 0, st>>>(a);
+      else kv_append_chunks_kernel<64, false><<<grid, kChunkThreads, 0, st>>>(a);
+    }
+    rc = launch_check(ctx, "kv_append_chunks_kernel");
+    a.n = 0;
+    used = 0;
+  };
+  for (int i = 0; i < n && !rc; i++) {
+    int64_t pos = seqs[i].len;
+    int left = counts[i];
+    while (left > 0 && !rc) {
+      if (a.n == kPieces || used == kPieceIds) flush();
+      // as many of the chunk's tokens as the remaining ids reach
+      const int64_t b0 = pos / bs;
+      const int64_t room = (int64_t)(kPieceIds - used) * bs - pos % bs;
+      const int take = (int)std::min<int64_t>(left, room);
+      const int64_t b1 = (pos + take + bs - 1) / bs;
+      a.piece[a.n++] = {seqs[i].slot, (int32_t)pos, row, used};
+      for (int64_t b = b0; b < b1; b++) a.ids[used++] = seqs[i].table->blocks[(size_t)b];
+      pos += take;
+      row += take;
+      left -= take;
+    }
+  }
+  flush();
+  if (rc)  // nothing was launched behind the failed launch: the tokens are taken back
+    for (int i = n - 1; i >= 0; i--)
+      if (seqs[i].table) cut_table(kv, *seqs[i].table, seqs[i].len);
+  return rc;
+}
+
+int truncate(vxb_kv *kv, int n, const int64_t *ids, const int64_t *lens, cudaStream_t st) {
+  vxb_ctx *ctx = kv->ctx;
+  const int bs = kv->block_size;
+  for (int i = 0; i < n; i++)
+    if (lens[i] < 0) return set_error(ctx, VXB_EINVAL, "vxb_kv_truncate: sequence %lld to %lld tokens", (long long)ids[i], (long long)lens[i]);
+  if (listed_twice(std::vector<int64_t>(ids, ids + n))) return set_error(ctx, VXB_EINVAL, "vxb_kv_truncate: a sequence is listed twice");
+  struct Cut {
+    vxb_kv::Table *table;
+    int64_t len;
+    int layer, slot;
+  };
+  std::vector<Cut> cuts, moves;  // moves: cuts inside a shared block
+  int64_t freed = 0;
+  for (int layer = kv->num_layers - 1; layer >= 0; layer--)
+    for (int i = n - 1; i >= 0; i--) {
+      auto it = kv->tables.find(std::make_pair(layer, ids[i]));
+      if (it == kv->tables.end() || it->second.len <= lens[i]) continue;
+      vxb_kv::Table &t = it->second;
+      cuts.push_back({&t, lens[i], layer, kv->slot_of.at(ids[i])});
+      for (size_t b = (size_t)((lens[i] + bs - 1) / bs); b < t.blocks.size(); b++) freed += kv->refs[t.blocks[b]] == 1;
+      if (lens[i] % bs && kv->refs[t.blocks[(size_t)(lens[i] / bs)]] > 1) moves.push_back(cuts.back());
+    }
+  if (cuts.empty()) return VXB_OK;
+  if ((int64_t)moves.size() > (int64_t)kv->free_blocks.size() + freed) return set_error(ctx, VXB_ENOBLOCKS, "KV cache out of blocks");
+  CutArgs a;
+  a.lens = kv->d_lens;
+  a.max_seqs = kv->max_seqs;
+  for (const Cut &c : cuts) cut_table(kv, *c.table, c.len);
+  for (const Cut &c : moves) {
+    const size_t index = (size_t)(c.len / bs);
+    const int32_t from = c.table->blocks[index];
+    if (kv->refs[from] <= 1) continue;  // the other holders were cut in this call
+    const int32_t to = kv->free_blocks.back();
+    kv->free_blocks.pop_back();
+    kv->refs[to] = 1;
+    kv->refs[from]--;
+    c.table->blocks[index] = to;
+    kv_copy_rows_kernel<<<kv->num_kv_heads, 256, 0, st>>>((uint8_t *)kv->pool_k, (uint8_t *)kv->pool_v, kv->scale_k, kv->scale_v, from, to,
+                                                          kv->num_kv_heads, bs, kv->head_dim, (int)kv->elem_bytes, (int)(c.len % bs));
+    if (int rc = launch_check(ctx, "kv_copy_rows_kernel")) return rc;
+    kv_set_entry_kernel<<<1, 1, 0, st>>>(kv->d_tables + ((size_t)c.layer * kv->max_seqs + c.slot) * kv->max_blocks_per_seq + index, to);
+    if (int rc = launch_check(ctx, "kv_set_entry_kernel")) return rc;
+  }
+  for (int i0 = 0; i0 < n;) {
+    a.n = 0;
+    for (; i0 < n && a.n < kCutSeqs; i0++) {
+      auto si = kv->slot_of.find(ids[i0]);
+      if (si == kv->slot_of.end() || lens[i0] > INT_MAX) continue;
+      a.slot[a.n] = si->second;
+      a.len[a.n++] = (int32_t)lens[i0];
+    }
+    if (a.n == 0) continue;
+    kv_cut_lens_kernel<<<kv->num_layers, std::min(128, (a.n + 31) / 32 * 32), 0, st>>>(a);
+    if (int rc = launch_check(ctx, "kv_cut_lens_kernel")) return rc;
+  }
+  return VXB_OK;
+}
+
+}  // namespace
+
+VXB_API int vxb_kv_append_chunks(vxb_kv *kv, int layer, int n, const int64_t *h_seq_ids, const int32_t *h_n_tokens,
+                                 const uint16_t *d_k, const uint16_t *d_v, void *stream) {
+  if (int rc = kv_check(kv, "vxb_kv_append_chunks")) return rc;
+  if (layer < 0 || layer >= kv->num_layers) return set_error(kv->ctx, VXB_EINVAL, "vxb_kv_append_chunks: layer %d out of range", layer);
+  if (n < 0 || (n > 0 && (!h_seq_ids || !h_n_tokens))) return set_error(kv->ctx, VXB_EINVAL, "vxb_kv_append_chunks: bad arguments");
+  if (n == 0) return VXB_OK;
+  DeviceScope dev(kv->ctx);
+  if (dev.rc) return dev.rc;
+  try {
+    return append_chunks(kv, layer, n, h_seq_ids, h_n_tokens, d_k, d_v, (cudaStream_t)stream);
+  } catch (...) {
+    return set_error(kv->ctx, VXB_ENOMEM, "vxb_kv_append_chunks: out of host memory");
+  }
+}
+
+VXB_API int vxb_kv_truncate(vxb_kv *kv, int n, const int64_t *h_seq_ids, const int64_t *h_lens, void *stream) {
+  if (int rc = kv_check(kv, "vxb_kv_truncate")) return rc;
+  if (n < 0 || (n > 0 && (!h_seq_ids || !h_lens))) return set_error(kv->ctx, VXB_EINVAL, "vxb_kv_truncate: bad arguments");
+  if (n == 0) return VXB_OK;
+  DeviceScope dev(kv->ctx);
+  if (dev.rc) return dev.rc;
+  try {
+    return truncate(kv, n, h_seq_ids, h_lens, (cudaStream_t)stream);
+  } catch (...) {
+    return set_error(kv->ctx, VXB_ENOMEM, "vxb_kv_truncate: out of host memory");
+  }
+}
+
+VXB_API int vxb_kv_pages(const vxb_kv *kv, void **d_k, void **d_v, float **d_k_scale, float **d_v_scale,
+                         int32_t **d_tables, int32_t **d_lens) {
+  if (!kv) return set_error(nullptr, VXB_EINVAL, "vxb_kv_pages: null cache");
+  if (d_k) *d_k = kv->pool_k;
+  if (d_v) *d_v = kv->pool_v;
+  if (d_k_scale) *d_k_scale = kv->scale_k;
+  if (d_v_scale) *d_v_scale = kv->scale_v;
+  if (d_tables) *d_tables = kv->d_tables;
+  if (d_lens) *d_lens = kv->d_lens;
+  return VXB_OK;
 }
 
 VXB_API int vxb_kv_free_seq(vxb_kv *kv, int64_t seq_id) {

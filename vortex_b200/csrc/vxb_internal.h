@@ -47,6 +47,22 @@ int cuda_fail(vxb_ctx *ctx, cudaError_t e, const char *what);
 // Make the context's device current for this host thread.
 int use_device(vxb_ctx *ctx);
 
+// Makes the context's device current for the scope of an entry point and the
+// caller's device current again behind it.
+struct DeviceScope {
+  int prev = -1, rc = VXB_OK;
+  explicit DeviceScope(vxb_ctx *ctx) {
+    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+    rc = use_device(ctx);
+    if (prev == ctx->device) prev = -1;
+  }
+  ~DeviceScope() {
+    if (prev >= 0) cudaSetDevice(prev);
+  }
+  DeviceScope(const DeviceScope &) = delete;
+  DeviceScope &operator=(const DeviceScope &) = delete;
+};
+
 // Ensure the workspace holds `bytes` and `counters` reduction counters.
 // Allocation happens only when growing, so calls that fit the current size
 // (for example inside CUDA graph capture) allocate nothing.

@@ -16,6 +16,44 @@ BF16 = N.BF16
 I8 = N.I8
 
 
+def _ids_counts(who: str, seq_ids, counts, dtype=np.int32):
+    """Host arrays of one sequence id and one count (or length) each."""
+    ids = np.ascontiguousarray(np.atleast_1d(seq_ids), dtype=np.int64)
+    c = np.atleast_1d(np.asarray(counts))
+    if c.size and not np.issubdtype(c.dtype, np.integer):
+        raise N.VxbError(N.VXB_EINVAL, f"{who}: the counts must be whole numbers")
+    if ids.ndim != 1 or c.ndim != 1 or ids.size != c.size:
+        raise N.VxbError(N.VXB_EINVAL, f"{who}: {ids.size} sequences and {c.size} counts")
+    if c.size and (int(c.min()) < 0 or int(c.max()) > np.iinfo(dtype).max):
+        raise N.VxbError(N.VXB_EINVAL, f"{who}: a count is negative or too large")
+    return ids, np.ascontiguousarray(c, dtype=dtype)
+
+
+def _device_rows(who: str, name: str, t, shape, device: int):
+    """t as a contiguous bf16 tensor of this shape on the cache's device."""
+    import torch
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or not t.is_cuda or t.device.index != device:
+        raise N.VxbError(N.VXB_EINVAL, f"{who}: {name} must be a bf16 tensor on cuda:{device}")
+    if tuple(t.shape) != tuple(shape):
+        raise N.VxbError(N.VXB_EINVAL, f"{who}: {name} must be {tuple(shape)}, got {tuple(t.shape)}")
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _stream_on(device: int) -> int:
+    """The current stream of the cache's device (which need not be the current device)."""
+    import torch
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+class _DeviceArray:
+    """Device memory of a cache for torch.as_tensor; the tensor keeps the cache alive."""
+
+    def __init__(self, owner, ptr: int, shape, typestr: str):
+        self.owner = owner
+        self.__cuda_array_interface__ = {"data": (ptr, False), "shape": tuple(shape), "typestr": typestr, "version": 3}
+
+
 class PagedKVCache:
     """PagedKVCache::new(num_layers, num_heads, head_dim, block_size, max_blocks)
     (src/kv_cache.rs:41-45); num_heads are the KV heads of a token."""
@@ -28,6 +66,8 @@ class PagedKVCache:
         self.block_size, self.max_blocks = block_size, max_blocks
         self.kv_dtype = kv_dtype
         mbps = max_blocks_per_seq or max_blocks
+        self.max_seqs, self.max_blocks_per_seq = max_seqs, mbps
+        self._chunk_ws = {}  # num_q_heads -> scratch bytes of chunk_attention
         p = ctypes.c_void_p()
         N.check(N.lib().vxb_kv_create(self.ctx.ptr, num_layers, num_heads, head_dim, block_size, max_blocks,
                                       max_seqs, mbps, kv_dtype, ctypes.byref(p)), self.ctx.ptr)
@@ -59,6 +99,48 @@ class PagedKVCache:
         v = v.contiguous()
         T = k.shape[0]
         self._check(N.lib().vxb_kv_append_seq(self.ptr, layer, int(seq_id), T, _dptr(k), _dptr(v), _stream_ptr()))
+
+    def append_chunks(self, layer: int, seq_ids, n_tokens, k, v):
+        """Ragged chunks: n_tokens[i] consecutive tokens of each listed
+        sequence, their rows packed one sequence after another: k, v bf16
+        [sum(n_tokens), H, D]."""
+        ids, counts = _ids_counts("append_chunks", seq_ids, n_tokens)
+        want = (int(counts.sum()), self.num_heads, self.head_dim)
+        k = _device_rows("append_chunks", "k", k, want, self.ctx.device)
+        v = _device_rows("append_chunks", "v", v, want, self.ctx.device)
+        self._check(N.lib().vxb_kv_append_chunks(self.ptr, layer, ids.size, ids.ctypes.data, counts.ctypes.data,
+                                                 k.data_ptr(), v.data_ptr(), _stream_on(self.ctx.device)))
+
+    def truncate(self, seq_ids, lengths):
+        """Takes appended tokens back: every layer of seq_ids[i] holds at most
+        lengths[i] tokens afterwards."""
+        ids, lens = _ids_counts("truncate", seq_ids, lengths, np.int64)
+        self._check(N.lib().vxb_kv_truncate(self.ptr, ids.size, ids.ctypes.data, lens.ctypes.data,
+                                            _stream_on(self.ctx.device)))
+
+    def pages(self) -> dict:
+        """The cache's device memory as tensors that share it: k, v
+        [max_blocks, H, block_size, D], tables [layers, max_seqs,
+        max_blocks_per_seq] and lens [layers, max_seqs] (int32); int8 caches
+        also k_scale, v_scale [max_blocks, H, block_size]."""
+        import torch
+        p = [ctypes.c_void_p() for _ in range(6)]
+        self._check(N.lib().vxb_kv_pages(self.ptr, *(ctypes.addressof(x) for x in p)))
+        page = (self.max_blocks, self.num_heads, self.block_size, self.head_dim)
+        seqs = (self.num_layers, self.max_seqs, self.max_blocks_per_seq)
+
+        def view(ptr, shape, typestr):
+            return torch.as_tensor(_DeviceArray(self, ptr.value, shape, typestr), device=f"cuda:{self.ctx.device}")
+
+        int8 = self.kv_dtype == I8
+        out = {}
+        for name, ptr in (("k", p[0]), ("v", p[1])):
+            t = view(ptr, page, "|i1" if int8 else "<i2")
+            out[name] = t if int8 else t.view(torch.bfloat16)
+        if int8:
+            out["k_scale"], out["v_scale"] = view(p[2], page[:3], "<f4"), view(p[3], page[:3], "<f4")
+        out["tables"], out["lens"] = view(p[4], seqs, "<i4"), view(p[5], seqs[:2], "<i4")
+        return out
 
     def get_kv(self, layer: int, seq_id: int):
         """PagedKVCache::get_kv: (keys, values) as f32 [len, H, D] tensors."""
@@ -115,4 +197,39 @@ class PagedKVCache:
         self._check(N.lib().vxb_decode_attention(self.ptr, layer, ids.size, ids.ctypes.data_as(ctypes.c_void_p),
                                                  _dptr(q), Hq, ctypes.c_float(scale), _dptr(out),
                                                  _dptr(lse) if lse is not None else None, _stream_ptr()))
+        return out
+
+    def chunk_attention(self, layer: int, seq_ids, n_queries, q, softmax_scale: float | None = None,
+                        causal: bool = True, out=None, lse=None):
+        """Attention of several queries per sequence: the n_queries[i] rows of
+        seq_ids[i] (packed, q bf16 [sum(n_queries), Hq, D]) are its last
+        n_queries[i] cached tokens; each sees the tokens up to its own (all of
+        them with causal=False). Returns bf16 like q (and fills lse f32 [rows,
+        Hq] if given). Rows that see nothing are zeros with lse -inf."""
+        import torch
+        ids, counts = _ids_counts("chunk_attention", seq_ids, n_queries)
+        rows, dev = int(counts.sum()), self.ctx.device
+        if q.dim() != 3:
+            raise N.VxbError(N.VXB_EINVAL, "chunk_attention: q must be [rows, Hq, D]")
+        Hq = q.shape[1]
+        shape = (rows, Hq, self.head_dim)
+        q = _device_rows("chunk_attention", "q", q, shape, dev)
+        if out is None:
+            out = torch.empty_like(q)
+        elif out is not _device_rows("chunk_attention", "out", out, shape, dev):
+            raise N.VxbError(N.VXB_EINVAL, "chunk_attention: out must be contiguous and 16-byte aligned")
+        if lse is not None and (lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous()
+                                or tuple(lse.shape) != shape[:2]):
+            raise N.VxbError(N.VXB_EINVAL, f"chunk_attention: lse must be contiguous f32 {shape[:2]} on cuda:{dev}")
+        need = self._chunk_ws.get(Hq)
+        if need is None:
+            n = ctypes.c_size_t()
+            self._check(N.lib().vxb_chunk_attention_ws(self.ptr, Hq, ctypes.byref(n)))
+            need = self._chunk_ws[Hq] = n.value
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(self.head_dim)
+        self._check(N.lib().vxb_chunk_attention(self.ptr, layer, ids.size, ids.ctypes.data, counts.ctypes.data,
+                                                q.data_ptr(), Hq, scale, int(causal), out.data_ptr(),
+                                                lse.data_ptr() if lse is not None else None, ws.data_ptr(), need,
+                                                _stream_on(dev)))
         return out

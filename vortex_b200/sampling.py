@@ -36,6 +36,80 @@ def sample_top_p(logits, temperature: float, top_p: float, seeds):
     return out
 
 
+def _f32_rows(who: str, name: str, t, shape=None, device=None):
+    """t as a contiguous f32 CUDA tensor (of this shape, on this device)."""
+    import torch
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.float32:
+        raise N.VxbError(N.VXB_EINVAL, f"{who}: {name} must be an f32 tensor on the GPU")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise N.VxbError(N.VXB_EINVAL, f"{who}: {name} must be {tuple(shape)}, got {tuple(t.shape)}")
+    if device is not None and t.device != device:
+        raise N.VxbError(N.VXB_EINVAL, f"{who}: {name} is on {t.device}, not on {device}")
+    return t.contiguous()
+
+
+def token_probs(logits, temperature=1.0, out=None):
+    """Probabilities of f32 logits [..., vocab] at a temperature (one number,
+    or an f32 tensor with one per row on the logits' device): exp((x - max) /
+    t) / sum; below 0.01 1 at the first maximum. -inf logits (banned tokens)
+    get 0, a row of nothing else zeros. out may be logits."""
+    import torch
+    lg = _f32_rows("token_probs", "logits", logits)
+    if lg.dim() == 0 or lg.shape[-1] == 0:
+        raise N.VxbError(N.VXB_EINVAL, "token_probs: logits must be [..., vocab]")
+    vocab = lg.shape[-1]
+    rows = lg.numel() // vocab
+    if out is None:
+        out = torch.empty_like(lg)
+    elif _f32_rows("token_probs", "out", out, lg.shape, lg.device) is not out:
+        raise N.VxbError(N.VXB_EINVAL, "token_probs: out must be contiguous")
+    per_row = None
+    if isinstance(temperature, torch.Tensor):
+        per_row = _f32_rows("token_probs", "temperature", temperature.reshape(-1), (rows,), lg.device)
+    dev = lg.device.index
+    context(dev).call("vxb_token_probs", lg.data_ptr(), rows, vocab, per_row.data_ptr() if per_row is not None else None,
+                      1.0 if per_row is not None else float(temperature), out.data_ptr(),
+                      torch.cuda.current_stream(dev).cuda_stream)
+    return out
+
+
+def verify_drafts(drafts, n_drafts, target_probs, draft_probs, u_accept, u_sample):
+    """Speculative sampling: accepts each request's drafts in order while
+    u_accept * q(draft) < p(draft), then draws one token, from max(p - q, 0) of
+    the first refused draft's row or from p of the row behind the last draft.
+
+    drafts int32 [D] with n_drafts[i] (host counts) for request i, packed;
+    target_probs f32 [D + n, vocab] (one row more per request than drafts);
+    draft_probs f32 [D, vocab], or None where the drafts were not drawn (q is 1
+    at the draft); u_accept f32 [D] and u_sample f32 [n] uniform in [0, 1).
+    Returns (tokens int32 [D + n]: accepted drafts, the drawn token, then -1,
+    per request; accepted int32 [n])."""
+    import torch
+    counts = np.atleast_1d(np.asarray(n_drafts))
+    if counts.ndim != 1 or (counts.size and (not np.issubdtype(counts.dtype, np.integer) or int(counts.min()) < 0
+                                             or int(counts.max()) > np.iinfo(np.int32).max)):
+        raise N.VxbError(N.VXB_EINVAL, "verify_drafts: n_drafts must be whole numbers, none negative")
+    counts = np.ascontiguousarray(counts, dtype=np.int32)
+    n, total = counts.size, int(counts.sum())
+    if not isinstance(target_probs, torch.Tensor) or target_probs.dim() != 2 or target_probs.shape[1] == 0:
+        raise N.VxbError(N.VXB_EINVAL, "verify_drafts: target_probs must be [rows, vocab]")
+    vocab = target_probs.shape[1]
+    p = _f32_rows("verify_drafts", "target_probs", target_probs, (total + n, vocab))
+    q = None if draft_probs is None else _f32_rows("verify_drafts", "draft_probs", draft_probs, (total, vocab), p.device)
+    ua = _f32_rows("verify_drafts", "u_accept", u_accept, (total,), p.device)
+    us = _f32_rows("verify_drafts", "u_sample", u_sample, (n,), p.device)
+    if not isinstance(drafts, torch.Tensor) or drafts.dtype != torch.int32 or drafts.device != p.device or tuple(drafts.shape) != (total,):
+        raise N.VxbError(N.VXB_EINVAL, f"verify_drafts: drafts must be int32 ({total},) on {p.device}")
+    drafts = drafts.contiguous()
+    tokens = torch.empty(total + n, dtype=torch.int32, device=p.device)
+    accepted = torch.empty(n, dtype=torch.int32, device=p.device)
+    dev = p.device.index
+    context(dev).call("vxb_verify_drafts", n, counts.ctypes.data, vocab, drafts.data_ptr(), p.data_ptr(),
+                      q.data_ptr() if q is not None else None, ua.data_ptr(), us.data_ptr(), tokens.data_ptr(),
+                      accepted.data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
+    return tokens, accepted
+
+
 class ContinuousBatcher:
     """ContinuousBatcher::new(max_batch_size) (src/kv_cache.rs:128-154)."""
 
