@@ -1,143 +1,975 @@
-// Attention of chunks of new tokens over the paged KV cache: several queries
-// of a sequence at once, each seeing the cached tokens up to its own.
+// Attention of chunks of new tokens over the paged KV cache, on the
+// 5th-generation tensor cores.
 //
 //   O[r, h]   = sum_j exp(scale q_r . k_j - lse[r, h]) v_j,   j <= last(r)
 //   lse[r, h] = log sum_j exp(scale q_r . k_j)
 //
-// with last(r) = len - n_queries + r (causal) or len - 1. One warp per (row,
-// query head): the lanes share the head dimension, one pass over the visible
-// keys with the running maximum and sum of the softmax in f32.
+// with last(r) = len - n_queries + r (causal) or len - 1. Between one query
+// per sequence (drafted tokens: the cache is read once, HBM-bound) and
+// thousands (chunks of prompts: tensor- and exponential-bound).
+//
+// Rows. The G query heads of a kv head share its keys, so row t * G + g of a
+// tile is head g of the chunk's token t: a tile of 128 rows holds 128 / G
+// tokens, one TMA box of [tokens][G][64] per 64 columns. An item is (sequence,
+// kv head, 256 rows); a key tile is 128 tokens, K and V of one kv head.
+//
+// Two streams. A CTA runs two softmax warpgroups, each with its own S and O in
+// tensor memory. An item of more than 128 rows gives each stream half of the
+// rows and both the same key tiles; a smaller item gives both the same rows
+// and every other key tile, and the streams are joined at the end. Either way
+// the tensor core works on one stream while the other takes exponentials. P
+// (bf16) overwrites its own S: S, S, O, O fill the 512 columns at D = 128.
+//
+// Work split. The key tiles of all items in a row are cut into equal runs, one
+// per SM (the host gives each CTA its first item and tile), so ragged batches,
+// long caches with few rows and causal triangles balance alike. A run that
+// ends inside an item leaves its unnormalised sums in the caller's scratch and
+// a second kernel joins an item's parts.
+//
+// Warps: 0-3 and 4-7 softmax (thread = row = TMEM lane), 8 issues the MMAs, 9
+// the TMA copies; int8 caches add 12-15, which turn int8 pages into bf16
+// tiles (codes are exact in bf16; the K scale multiplies the scores and the V
+// scale the softmax weights, both per key). Pages come through one ring of
+// tiles in the order K, V, K, V, ...; a page box is up to 128 tokens of one
+// block, of which only those that hold tokens are copied.
+//
+// Keys behind the last token never count: S is masked by selection, the
+// MMA stops at the last 16 keys with a token and the rest of those 16 V rows
+// is zeroed. A key that only some rows of a tile see may hold inf or NaN: such
+// elements of V are taken out of the tile before the product and added to the
+// rows that see them (0 * inf would reach the others).
+//
+// P is rounded to bf16 once (2^-8 of a weight; the output's own rounding is as
+// large); the sums l are of the f32 weights. Every wait is bounded.
+#include <atomic>
 #include <climits>
 #include <cmath>
-
+#include <cuda.h>
 #include <cuda_bf16.h>
 
+#include <mutex>
+
 #include "kv_cache.h"
+#include "tc_common.h"
 
 using namespace vxb;
+using namespace vxb::tc;
 
 namespace {
 
-constexpr int kSeqs = 128;  // sequences of one launch (their record is a kernel parameter)
+constexpr int BM = 128, BN = 128;
+constexpr int kSeqs = 128;    // sequences of one launch (their record is a kernel parameter)
+constexpr int kMaxCtas = 160;
+constexpr int kRowsItem = 2 * BM;
+constexpr float RESCALE_THRESHOLD = 8.f;  // O is rescaled when a row's maximum grows by more (log2)
+
 struct ChunkSeq {
   int32_t slot, row0, rows, len;
 };
+struct Start {  // a CTA's first item and the first of its key tiles
+  int32_t seq, head, pair, tile;
+};
+struct Shape {
+  int tpt;  // tokens of a 128-row tile
+  int causal;
+};
 struct ChunkArgs {
-  const uint16_t *q;
   uint16_t *out;
   float *lse;
-  const void *pool_k, *pool_v;
+  float *ws;
+  int *err;
   const float *sk, *sv;
   const int32_t *tables;  // of the layer
-  int n, rows, Hq, Hkv, G, bs, mbps, causal;
+  int n, Hq, Hkv, G, bs, mbps, box, n_ctas;
+  Shape sh;
   float scale_log2;
+  long long units;
   ChunkSeq seq[kSeqs];
+  Start start[kMaxCtas + 1];
 };
-static_assert(sizeof(ChunkArgs) <= 4096, "kernel parameters");
+static_assert(sizeof(ChunkArgs) <= 8192, "kernel parameters");
+
+// Key tiles that the tokens before tok_end of a chunk see
+__host__ __device__ inline int tiles_of(const ChunkSeq &s, const Shape &sh, int tok_end) {
+  const int seen = sh.causal ? s.len - s.rows + tok_end : s.len;
+  return seen > 0 ? (seen + BN - 1) / BN : 0;
+}
+// Units of an item: its key tiles, one at least
+__host__ __device__ inline int units_of(const ChunkSeq &s, const Shape &sh, int pair) {
+  const int end = (pair + 1) * 2 * sh.tpt;
+  const int t = tiles_of(s, sh, end < s.rows ? end : s.rows);
+  return t > 0 ? t : 1;
+}
+
+// The run of a CTA as pieces: consecutive key tiles of one item.
+struct Piece {
+  ChunkSeq s;
+  int head, tok0, ntok, tb, te, units, te_u;
+  bool both;   // two tiles of rows, the same keys; else one tile, every other key tile
+  int n0, n1;  // steps of the streams
+  __device__ __forceinline__ int tile(int stream, int i) const { return both ? tb + i : tb + 2 * i + stream; }
+  __device__ __forceinline__ int steps(int stream) const { return stream ? n1 : n0; }
+  __device__ __forceinline__ bool whole() const { return tb == 0 && te_u == units; }
+};
+struct Run {
+  Start at;
+  int left;
+  __device__ Run(const ChunkArgs &a) {
+    at = a.start[blockIdx.x];
+    const long long u0 = a.units * blockIdx.x / a.n_ctas, u1 = a.units * (blockIdx.x + 1) / a.n_ctas;
+    left = (int)(u1 - u0);
+  }
+  __device__ __forceinline__ bool next(const ChunkArgs &a, Piece &p) {
+    if (left <= 0) return false;
+    p.s = a.seq[at.seq];
+    p.head = at.head;
+    p.tok0 = at.pair * 2 * a.sh.tpt;
+    p.ntok = min(2 * a.sh.tpt, p.s.rows - p.tok0);
+    p.both = p.ntok > a.sh.tpt;
+    const int n = tiles_of(p.s, a.sh, p.tok0 + p.ntok);
+    p.units = max(1, n);
+    p.tb = at.tile;
+    p.te_u = min(p.units, p.tb + left);
+    p.te = min(p.te_u, n);
+    const int count = max(0, p.te - p.tb);
+    if (p.both) {
+      p.n0 = max(0, min(p.te, tiles_of(p.s, a.sh, p.tok0 + a.sh.tpt)) - p.tb);
+      p.n1 = count;
+    } else {
+      p.n0 = (count + 1) / 2;
+      p.n1 = count / 2;
+    }
+    left -= p.te_u - p.tb;
+    at.tile = 0;
+    at.pair++;
+    if (at.pair * 2 * a.sh.tpt >= p.s.rows) {
+      at.pair = 0;
+      if (++at.head == a.Hkv) {
+        at.head = 0;
+        at.seq++;
+      }
+    }
+    return true;
+  }
+};
 
 template <int D, bool INT8>
-__global__ void __launch_bounds__(128) chunk_attn_kernel(const __grid_constant__ ChunkArgs a) {
-  constexpr int PER = D / 32;
-  const int lane = threadIdx.x & 31;
-  const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (item >= (long long)a.rows * a.Hq) return;
-  const int row = a.seq[0].row0 + (int)(item / a.Hq), head = (int)(item % a.Hq), hk = head / a.G;
-  int lo = 0, hi = a.n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.seq[mid].row0 <= row) lo = mid;
-    else hi = mid - 1;
-  }
-  const ChunkSeq s = a.seq[lo];
-  const int keys = a.causal ? s.len - s.rows + (row - s.row0) + 1 : s.len;
-  const int32_t *table = a.tables + (size_t)s.slot * a.mbps;
-  const size_t at = ((size_t)row * a.Hq + head) * D + lane * PER;
-  float q[PER], o[PER];
-#pragma unroll
-  for (int e = 0; e < PER; e++) {
-    q[e] = bf16_bits_to_f32(a.q[at + e]);
-    o[e] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  for (int j = 0; j < keys; j++) {
-    const size_t token = ((size_t)table[j / a.bs] * a.Hkv + hk) * a.bs + j % a.bs;
-    float k[PER], v[PER], dot = 0.f;
-#pragma unroll
-    for (int e = 0; e < PER; e++) {
-      if (INT8) {
-        k[e] = (float)((const int8_t *)a.pool_k)[token * D + lane * PER + e] * a.sk[token];
-        v[e] = (float)((const int8_t *)a.pool_v)[token * D + lane * PER + e] * a.sv[token];
-      } else {
-        k[e] = bf16_bits_to_f32(((const uint16_t *)a.pool_k)[token * D + lane * PER + e]);
-        v[e] = bf16_bits_to_f32(((const uint16_t *)a.pool_v)[token * D + lane * PER + e]);
-      }
-      dot = fmaf(q[e], k[e], dot);
+struct Cfg {
+  static constexpr int SLAB = BN * 128;             // 64 bf16 columns of 128 rows
+  static constexpr int TILE = SLAB * (D / 64);      // one bf16 tile
+  static constexpr int RAW = INT8 ? BN * D : 0;     // one int8 tile
+  static constexpr int SLOTS = INT8 ? (D == 128 ? 3 : 6) : (D == 128 ? 5 : 10);
+  static constexpr int RAWS = INT8 ? (D == 128 ? 3 : 6) : 0;
+  static constexpr int OFF_KV = 2 * TILE;
+  static constexpr int OFF_RAW = OFF_KV + SLOTS * TILE;
+  static constexpr int OFF_SCALE = OFF_RAW + RAWS * RAW;  // f32 per key: K and V scales of the last SLOTS tiles
+  static constexpr int OFF_ML = OFF_SCALE + (INT8 ? SLOTS * 2 * BN * 4 : 0);
+  static constexpr int OFF_BARS = OFF_ML + 2 * BM * 8;
+  static constexpr int SMEM = OFF_BARS + 512;
+  static constexpr int THREADS = INT8 ? 512 : 384;
+  // registers per thread: softmax, producer and converter warpgroups; their
+  // sum is what the block is launched with (128 x 512 resp. 168 x 384)
+  static constexpr int REG_SOFT = INT8 ? 192 : 208, REG_PROD = INT8 ? 56 : 88, REG_CONV = 72;
+  static_assert(INT8 ? 2 * REG_SOFT + REG_PROD + REG_CONV <= 512 : 2 * REG_SOFT + REG_PROD <= 504, "registers");
+  static_assert(SMEM <= 232448, "shared memory");
+};
+
+template <int SLOTS, int RAWS>
+struct Bars {
+  uint64_t q_full, q_empty, o_free, s_full[2], p_full[2], o_full[2], full[SLOTS], empty[SLOTS], raw_full[RAWS + 1],
+      raw_empty[RAWS + 1];
+  uint32_t tmem;
+  int acc[2];  // the stream's O already holds values that its first product adds to
+};
+
+// Bounded wait; once one has run out, the following ones of this thread do not
+// wait again, and the kernel ends.
+template <bool WARP>  // every lane of a warp waits, and they go on together
+struct Waiter {
+  int *err;
+  bool dead = false;
+  __device__ __forceinline__ void operator()(uint64_t *bar, uint32_t parity) {
+    if (!mbar_wait(bar, parity, dead ? 0 : kWaitBudget)) {
+      dead = true;
+      atomicExch(err, 1);
     }
-    const float x = warp_sum(dot) * a.scale_log2;
-    const float top = fmaxf(m, x);
-    const float f = top == -INFINITY ? 1.f : exp2f(m - top), p = top == -INFINITY ? 0.f : exp2f(x - top);
-    m = top;
-    l = l * f + p;
-#pragma unroll
-    for (int e = 0; e < PER; e++) o[e] = o[e] * f + p * v[e];
+    if (WARP) __syncwarp();
   }
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+};
+
+__device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ bool bar_or(int id, int threads, bool p) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, %2, %3, p;\n selp.u32 %0, 1, 0, q;\n}"
+      : "=r"(r)
+      : "r"((uint32_t)p), "r"(id), "r"(threads)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ float tmem_ld1(uint32_t taddr) {
+  uint32_t r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
+  tmem_wait_ld();
+  return __uint_as_float(r);
+}
+__device__ __forceinline__ void tmem_st1(uint32_t taddr, float v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(__float_as_uint(v)) : "memory");
+}
+
+// 16-byte chunk c (8 columns) of row r of a bf16 tile in shared memory
+__device__ __forceinline__ uint32_t chunk_off(int r, int c) {
+  return (uint32_t)((c >> 3) * (BN * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
+__device__ __forceinline__ uint32_t odd_bf16(uint32_t w) {  // a non-finite element in a pair
+  return (uint32_t)((w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u);
+}
+
+// ------------------------------------------------------------------ softmax warpgroup of stream ST
+template <int D, bool INT8, class B>
+__device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B &bars, const int st) {
+  using C = Cfg<D, INT8>;
+  const int warp4 = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31, r = warp4 * 32 + lane;
+  const uint32_t lane_off = (uint32_t)(warp4 * 32) << 16;
+  const uint32_t tS = bars.tmem + st * 128 + lane_off, tO = bars.tmem + 256 + st * 128 + lane_off;
+  const uint32_t tO_other = bars.tmem + 256 + (st ^ 1) * 128 + lane_off;
+  float2 *ml = reinterpret_cast<float2 *>(sm + C::OFF_ML);  // [2][BM]
+  Waiter<true> wait{a.err};
+  Run run(a);
+  Piece p;
+  uint32_t step = 0, pieces = 0, ring = 0;  // this stream's steps; pieces; first ring index of the piece
+  while (run.next(a, p)) {
+    const int base = p.s.len - p.s.rows;
+    const int tile_tok = p.tok0 + (p.both ? st * a.sh.tpt : 0);          // first token of this stream's rows
+    const int toks = min(a.sh.tpt, p.tok0 + p.ntok - tile_tok);
+    const int live = toks * a.G;
+    const int tok = tile_tok + r / a.G;
+    // last visible key; rows that do not exist are never masked (nor read)
+    const int lim = r < live ? (a.sh.causal ? base + tok : p.s.len - 1) : INT_MAX;
+    const int lim_first = a.sh.causal ? base + tile_tok : p.s.len - 1;
+    const bool warp_live = warp4 * 32 < live;
+    float m = -INFINITY, l = 0.f;
+    const int steps = p.steps(st);
+    for (int i = 0; i < steps; i++, step++) {
+      const int t = p.tile(st, i), k0 = t * BN;
+      const uint32_t kv = ring + 2 * (uint32_t)(t - p.tb);  // ring index of K; V is the next
+      wait(&bars.s_full[st], step & 1);
+      tc_fence_after();
+      // V elements that only some rows may see, and rows behind the last token
+      const int valid = min(BN, p.s.len - k0);
+      bool odd = false;
+      const bool both_here = p.both && i < p.n0;  // the other stream works on the same tile
+      // a tile that hides keys from some row of either stream that uses it
+      const int lim_item = a.sh.causal ? base + p.tok0 : p.s.len - 1;
+      const bool diagonal = (both_here ? lim_item : lim_first) < min(k0 + BN, p.s.len) - 1;
+      uint8_t *sv_tile = sm + C::OFF_KV + ((kv + 1) % C::SLOTS) * C::TILE;
+      if constexpr (!INT8) {
+        if (diagonal || valid < BN) {
+          wait(&bars.full[(kv + 1) % C::SLOTS], ((kv + 1) / C::SLOTS) & 1);
+          if (valid < BN && !(both_here && st == 1)) {
+            const int rows = (valid + 15) / 16 * 16 - valid;
+            for (int c = r; c < rows * (D / 8); c += 128)
+              *reinterpret_cast<uint4 *>(sv_tile + chunk_off(valid + c / (D / 8), c % (D / 8))) = make_uint4(0u, 0u, 0u, 0u);
+            fence_async_smem();
+          }
+          if (diagonal) {
+            uint32_t found = 0;
+            for (int c = r; c < valid * (D / 8); c += 128) {
+              const uint4 w = *reinterpret_cast<const uint4 *>(sv_tile + chunk_off(c / (D / 8), c % (D / 8)));
+              found |= odd_bf16(w.x) | odd_bf16(w.y) | odd_bf16(w.z) | odd_bf16(w.w);
+            }
+            __syncwarp();
+            odd = bar_or(2 + st, 128, found != 0);
+          }
+        }
+      }
+      if (warp_live) {
+        float s[BN];
 #pragma unroll
-  for (int e = 0; e < PER; e++) a.out[at + e] = __bfloat16_as_ushort(__float2bfloat16_rn(o[e] * inv));
-  if (a.lse && lane == 0) a.lse[(size_t)row * a.Hq + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+        for (int c = 0; c < BN / 32; c++) tmem_ld32(tS + c * 32, *reinterpret_cast<float(*)[32]>(s + c * 32));
+        tmem_wait_ld();
+        // K and V scales of this tile: there until its V is released, after P
+        const float *key_scale = reinterpret_cast<const float *>(sm + C::OFF_SCALE) + (kv / 2 % C::SLOTS) * 2 * BN;
+        if constexpr (INT8) {
+#pragma unroll
+          for (int c = 0; c < BN; c += 4) {
+            const float4 f = *reinterpret_cast<const float4 *>(key_scale + c);
+            s[c] *= f.x;
+            s[c + 1] *= f.y;
+            s[c + 2] *= f.z;
+            s[c + 3] *= f.w;
+          }
+        }
+        const bool masked = !__all_sync(0xffffffffu, k0 + BN - 1 <= lim);
+        if (masked) {
+#pragma unroll
+          for (int c = 0; c < BN; c++) s[c] = k0 + c <= lim ? s[c] : -INFINITY;
+        }
+        float mx4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int c = 4; c < BN; c++) mx4[c & 3] = fmaxf(mx4[c & 3], s[c]);
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale_log2;
+        const bool grow = mx > m + RESCALE_THRESHOLD;
+        const float m_new = grow ? mx : m;
+        const float mb = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = grow ? ex2(m - mb) : 1.f;
+        m = m_new;
+        if (i > 0 && __any_sync(0xffffffffu, grow)) {
+          // s_full of this step came behind the products of the last: O is whole
+#pragma unroll
+          for (int c = 0; c < D / 32; c++) {
+            float o[32];
+            tmem_ld32(tO + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; e++) o[e] *= alpha;
+            tmem_st32(tO + c * 32, o);
+          }
+        }
+        float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < BN; c++) {
+          s[c] = ex2(fmaf(s[c], a.scale_log2, -mb));
+          sum4[c & 3] += s[c];
+        }
+        l = l * alpha + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
+        if constexpr (INT8) {
+          // ready: the K tile's full came before S; V's scales come with V
+          wait(&bars.full[(kv + 1) % C::SLOTS], ((kv + 1) / C::SLOTS) & 1);
+          const float *val_scale = key_scale + BN;
+#pragma unroll
+          for (int c = 0; c < BN; c += 4) {
+            const float4 f = *reinterpret_cast<const float4 *>(val_scale + c);
+            s[c] *= f.x;
+            s[c + 1] *= f.y;
+            s[c + 2] *= f.z;
+            s[c + 3] *= f.w;
+          }
+          if (masked) {  // 0 * a scale that is not finite
+#pragma unroll
+            for (int c = 0; c < BN; c++) s[c] = k0 + c <= lim ? s[c] : 0.f;
+          }
+        }
+        if constexpr (!INT8) {
+          if (odd) {
+            // rare: every non-finite V element, added to the rows that see its key
+#pragma unroll
+            for (int c = 0; c < BN / 32; c++) tmem_st32(tS + c * 32, *reinterpret_cast<float(*)[32]>(s + c * 32));
+            if (i == 0) {
+              float z[32];
+#pragma unroll
+              for (int e = 0; e < 32; e++) z[e] = 0.f;
+#pragma unroll
+              for (int c = 0; c < D / 32; c++) tmem_st32(tO + c * 32, z);
+            }
+            tmem_wait_st();
+            for (int k = 0; k < valid; k++)
+              for (int c = 0; c < D / 8; c++) {
+                const uint4 w = *reinterpret_cast<const uint4 *>(sv_tile + chunk_off(k, c));
+                if (!(odd_bf16(w.x) | odd_bf16(w.y) | odd_bf16(w.z) | odd_bf16(w.w))) continue;
+                const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll 1
+                for (int e = 0; e < 8; e++) {
+                  const uint32_t bits = (ww[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
+                  if ((bits & 0x7F80u) != 0x7F80u) continue;
+                  const float pk = tmem_ld1(tS + k), o = tmem_ld1(tO + c * 8 + e);
+                  tmem_st1(tO + c * 8 + e, k0 + k <= lim ? fmaf(pk, __uint_as_float(bits << 16), o) : o);
+                  tmem_wait_st();
+                }
+              }
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < BN / 64; c++) {
+          uint32_t h[32];
+#pragma unroll
+          for (int e = 0; e < 32; e++) h[e] = pack_bf16(s[c * 64 + 2 * e], s[c * 64 + 2 * e + 1]);
+          tmem_st32u(tS + c * 32, h);
+        }
+        tmem_wait_st();
+      }
+      if constexpr (!INT8) {
+        if (odd) {
+          if (i == 0 && r == 0) bars.acc[st] = 1;
+          // every row has taken the odd elements: out of the tile with them
+          __syncwarp();
+          if (both_here) bar_sync(1, 256);
+          else bar_sync(2 + st, 128);
+          if (!(both_here && st == 1)) {
+            for (int c = r; c < valid * (D / 8); c += 128) {
+              uint4 *at = reinterpret_cast<uint4 *>(sv_tile + chunk_off(c / (D / 8), c % (D / 8)));
+              uint32_t w[4] = {at->x, at->y, at->z, at->w};
+#pragma unroll
+              for (int e = 0; e < 4; e++) {
+                if ((w[e] & 0x7F80u) == 0x7F80u) w[e] &= 0xFFFF0000u;
+                if ((w[e] & 0x7F800000u) == 0x7F800000u) w[e] &= 0xFFFFu;
+              }
+              *at = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            fence_async_smem();
+          }
+          __syncwarp();
+          if (both_here) bar_sync(1, 256);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.p_full[st]);
+    }
+    // ---------------- end of the piece
+    wait(&bars.o_full[st], pieces & 1);
+    if (!p.both) {
+      ml[st * BM + r] = make_float2(m, l);
+      wait(&bars.o_full[st ^ 1], pieces & 1);
+      bar_sync(1, 256);
+    }
+    tc_fence_after();
+    const bool mine = r < live;
+    const size_t row = (size_t)(p.s.row0 + tok) * a.Hq + (size_t)p.head * a.G + r % a.G;
+    const bool whole = p.whole();
+    // scratch of an unfinished item: the CTA's first or last part
+    float *part = a.ws + (size_t)(blockIdx.x * 2 + (p.tb > 0 ? 0 : 1)) * (kRowsItem * (D + 2));
+    const int prow = p.both ? st * BM + r : r;
+    float f0 = 1.f, f1 = 0.f;  // factors of this stream's and the other's O
+    if (!p.both) {
+      const float2 o = ml[(st ^ 1) * BM + r];
+      const float top = fmaxf(m, o.x);
+      f0 = m == -INFINITY ? 0.f : ex2(m - top);
+      f1 = o.x == -INFINITY ? 0.f : ex2(o.x - top);
+      // NaN sums stay: a stream with steps whose maximum is -inf has l = 0 or NaN
+      l = (m == -INFINITY ? l : l * f0) + (o.x == -INFINITY ? o.y : o.y * f1);
+      m = top;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (warp_live) {
+      // one tile of rows: the streams write half of the columns each
+      const int c0 = p.both ? 0 : st * (D / 2), c1 = p.both ? D : c0 + D / 2;
+      const bool has0 = steps > 0, has1 = !p.both && p.steps(st ^ 1) > 0;
+#pragma unroll 1
+      for (int c = c0; c < c1; c += 32) {
+        float o[32];
+#pragma unroll
+        for (int e = 0; e < 32; e++) o[e] = 0.f;
+        if (has0) {
+          tmem_ld32(tO + c, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; e++) o[e] *= f0;
+        }
+        if (has1) {
+          float x[32];
+          tmem_ld32(tO_other + c, x);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; e++) o[e] = fmaf(x[e], f1, o[e]);
+        }
+        if (mine && whole) {
+          uint4 *dst = reinterpret_cast<uint4 *>(a.out + row * D + c);
+#pragma unroll
+          for (int q = 0; q < 4; q++)
+            dst[q] = make_uint4(pack_bf16(o[q * 8] * inv, o[q * 8 + 1] * inv), pack_bf16(o[q * 8 + 2] * inv, o[q * 8 + 3] * inv),
+                                pack_bf16(o[q * 8 + 4] * inv, o[q * 8 + 5] * inv), pack_bf16(o[q * 8 + 6] * inv, o[q * 8 + 7] * inv));
+        } else if (mine) {
+          float4 *dst = reinterpret_cast<float4 *>(part + (size_t)prow * D + c);
+#pragma unroll
+          for (int q = 0; q < 8; q++) __stcg(dst + q, make_float4(o[q * 4], o[q * 4 + 1], o[q * 4 + 2], o[q * 4 + 3]));
+        }
+      }
+      if (mine && (p.both || st == 0)) {
+        if (whole) {
+          if (a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+        } else {
+          __stcg(reinterpret_cast<float2 *>(part + (size_t)kRowsItem * D) + prow, make_float2(m, l));
+        }
+      }
+    }
+    tc_fence_before();
+    if (!p.both) bar_sync(1, 256);  // ml has been read
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars.o_free);
+    pieces++;
+    ring += 2 * (uint32_t)max(0, p.te - p.tb);
+  }
+}
+
+// ------------------------------------------------------------------ MMA thread
+template <int D, bool INT8, class B>
+__device__ __forceinline__ void mma_role(const ChunkArgs &a, uint8_t *sm, B &bars) {
+  using C = Cfg<D, INT8>;
+  constexpr uint32_t ID_QK = idesc_bf16(BM, BN, false), ID_PV = idesc_bf16(BM, D, true);
+  const uint32_t s_q = smem_u32(sm), s_kv = smem_u32(sm + C::OFF_KV), tmem = bars.tmem;
+  Waiter<false> wait{a.err};
+  Run run(a);
+  Piece p;
+  uint32_t ring = 0, pieces = 0, psteps[2] = {0, 0};
+  while (run.next(a, p)) {
+    const int tiles = max(0, p.te - p.tb);
+    bool o_mine = pieces == 0;  // the softmax warps have read the last piece's O
+    auto own_o = [&]() {
+      if (!o_mine) wait(&bars.o_free, (pieces - 1) & 1);
+      o_mine = true;
+    };
+    wait(&bars.q_full, pieces & 1);
+    auto issue_s = [&](int st, int i) {
+      const uint32_t kv = ring + 2 * (uint32_t)(p.tile(st, i) - p.tb), slot = kv % C::SLOTS;
+      wait(&bars.full[slot], (kv / C::SLOTS) & 1);
+      tc_fence_after();
+      const uint32_t q = s_q + (p.both ? st : 0) * C::TILE, k = s_kv + slot * C::TILE;
+#pragma unroll
+      for (int x = 0; x < D / 16; x++) {
+        const uint32_t off = (x >> 2) * C::SLAB + (x & 3) * 32;
+        umma_bf16(tmem + st * 128, sw128_desc(q + off, 16, 1024), sw128_desc(k + off, 16, 1024), ID_QK, x > 0 ? 1u : 0u);
+      }
+      umma_commit(&bars.s_full[st]);
+      if (!p.both || st == 1) umma_commit(&bars.empty[slot]);  // stream 1 is the last to use a shared tile
+    };
+    auto issue_pv = [&](int st, int i) {
+      const int t = p.tile(st, i);
+      const uint32_t kv = ring + 2 * (uint32_t)(t - p.tb) + 1, slot = kv % C::SLOTS;
+      own_o();
+      wait(&bars.p_full[st], psteps[st]++ & 1);
+      wait(&bars.full[slot], (kv / C::SLOTS) & 1);
+      tc_fence_after();
+      const uint32_t v = s_kv + slot * C::TILE;
+      uint32_t acc = i > 0 ? 1u : 0u;
+      if (!INT8 && i == 0 && *(volatile int *)&bars.acc[st]) {
+        acc = 1u;
+        *(volatile int *)&bars.acc[st] = 0;
+      }
+      const int k16 = (min(BN, p.s.len - t * BN) + 15) / 16;
+      for (int x = 0; x < k16; x++)
+        umma_bf16_ts(tmem + 256 + st * 128, tmem + st * 128 + x * 8, sw128_desc(v + x * 2048, C::SLAB, 1024), ID_PV, x > 0 ? 1u : acc);
+      if (!p.both || st == 1) umma_commit(&bars.empty[slot]);
+    };
+    if (p.n0 > 0) issue_s(0, 0);
+    if (p.n1 > 0) issue_s(1, 0);
+    const int steps = max(p.n0, p.n1);
+    for (int i = 0; i < steps; i++)
+#pragma unroll
+      for (int st = 0; st < 2; st++) {
+        const int n = p.steps(st);
+        if (i < n) {
+          issue_pv(st, i);
+          if (i + 1 < n) issue_s(st, i + 1);
+          else umma_commit(&bars.o_full[st]);
+        }
+      }
+    umma_commit(&bars.q_empty);
+    own_o();
+    if (p.n0 == 0) umma_commit(&bars.o_full[0]);
+    if (p.n1 == 0) umma_commit(&bars.o_full[1]);
+    ring += 2 * (uint32_t)tiles;
+    pieces++;
+  }
+}
+
+// ------------------------------------------------------------------ TMA warp
+template <int D, bool INT8, class B>
+__device__ __forceinline__ void tma_role(const CUtensorMap *tq, const CUtensorMap *tk, const CUtensorMap *tv, const ChunkArgs &a,
+                                         uint8_t *sm, B &bars) {
+  using C = Cfg<D, INT8>;
+  constexpr int SLABS = INT8 ? 1 : D / 64;
+  constexpr int RING = INT8 ? C::RAWS : C::SLOTS;
+  constexpr int ROW = INT8 ? D : 128;  // bytes of a box row
+  const int lane = threadIdx.x & 31;
+  const int per_tile = BN / a.box;  // boxes of a tile and slab
+  uint8_t *tiles = sm + (INT8 ? C::OFF_RAW : C::OFF_KV);
+  Waiter<true> wait{a.err};
+  Run run(a);
+  Piece p;
+  uint32_t idx = 0, pieces = 0;
+  while (run.next(a, p)) {
+    const int32_t *table = a.tables + (size_t)p.s.slot * a.mbps;
+    // pool rows of this lane's box in the tiles t .. t + 32 / per_tile - 1
+    const int group = 32 / per_tile;
+    int rows = 0;
+    auto look_up = [&](int t) {
+      const int tok = (t + lane / per_tile) * BN + lane % per_tile * a.box;
+      if (tok < p.s.len && t + lane / per_tile < p.te) {
+        const int b = tok / a.bs;
+        rows = (int)(((long long)__ldg(table + b) * a.Hkv + p.head) * a.bs + (tok - b * a.bs));
+      }
+    };
+    auto load = [&](const CUtensorMap *map, int t) {
+      const uint32_t slot = idx % RING;
+      uint64_t *full = INT8 ? &bars.raw_full[slot] : &bars.full[slot], *empty = INT8 ? &bars.raw_empty[slot] : &bars.empty[slot];
+      if (idx >= RING) wait(empty, (idx / RING - 1) & 1);
+      const int boxes = (min(BN, p.s.len - t * BN) + a.box - 1) / a.box;
+      if (lane == 0) mbar_expect_tx(full, (uint32_t)(boxes * SLABS * a.box * ROW));
+      __syncwarp();
+      const int row = __shfl_sync(0xffffffffu, rows, (t - p.tb) % group * per_tile + lane / SLABS % per_tile);
+      if (lane < boxes * SLABS) {
+        const int b = lane / SLABS, sl = lane % SLABS;
+        tma_load_2d(tiles + slot * (INT8 ? C::RAW : C::TILE) + sl * C::SLAB + b * a.box * ROW, map, sl * 64, row, full);
+      }
+      __syncwarp();
+      idx++;
+    };
+    auto load_q = [&]() {
+      if (pieces > 0) wait(&bars.q_empty, (pieces - 1) & 1);
+      if (lane == 0) {
+        const int halves = p.both ? 2 : 1;
+        mbar_expect_tx(&bars.q_full, (uint32_t)(halves * (D / 64) * a.sh.tpt * a.G * 128));
+        for (int h = 0; h < halves; h++)
+          for (int sl = 0; sl < D / 64; sl++)
+            tma_load_3d(sm + h * C::TILE + sl * C::SLAB, tq, sl * 64, p.head * a.G, p.s.row0 + p.tok0 + h * a.sh.tpt, &bars.q_full);
+      }
+      __syncwarp();
+    };
+    if (p.te <= p.tb) load_q();
+    for (int t = p.tb; t < p.te; t++) {
+      if ((t - p.tb) % group == 0) look_up(t);
+      load(tk, t);
+      if (t == p.tb) load_q();  // behind the first keys: the last piece may still use Q
+      load(tv, t);
+    }
+    pieces++;
+  }
+}
+
+// ------------------------------------------------------------------ converter warpgroup (int8)
+template <int D, class B>
+__device__ __forceinline__ void convert_role(const ChunkArgs &a, uint8_t *sm, B &bars) {
+  using C = Cfg<D, true>;
+  const int r = threadIdx.x & 127, lane = threadIdx.x & 31;
+  Waiter<true> wait{a.err};
+  Run run(a);
+  Piece p;
+  uint32_t idx = 0;
+  while (run.next(a, p)) {
+    const int32_t *table = a.tables + (size_t)p.s.slot * a.mbps;
+    for (int t = p.tb; t < p.te; t++) {
+      const int tok = t * BN + r, valid = min(BN, p.s.len - t * BN);
+      size_t row = 0;
+      if (r < valid) row = ((size_t)__ldg(table + tok / a.bs) * a.Hkv + p.head) * a.bs + tok % a.bs;
+      const float scale[2] = {r < valid ? __ldcg(a.sk + row) : 0.f, r < valid ? __ldcg(a.sv + row) : 0.f};
+#pragma unroll
+      for (int v = 0; v < 2; v++, idx++) {
+        const uint32_t raw = idx % C::RAWS, slot = idx % C::SLOTS;
+        wait(&bars.raw_full[raw], (idx / C::RAWS) & 1);
+        if (idx >= C::SLOTS) wait(&bars.empty[slot], (idx / C::SLOTS - 1) & 1);
+        const uint8_t *src = sm + C::OFF_RAW + raw * C::RAW;
+        uint8_t *dst = sm + C::OFF_KV + slot * C::TILE;
+        // V of tile t holds its slot until the softmax has used both of the
+        // tile's scales, so this warpgroup is less than SLOTS tiles ahead
+        reinterpret_cast<float *>(sm + C::OFF_SCALE)[(idx / 2 % C::SLOTS * 2 + v) * BN + r] = scale[v];
+        // 16 codes at a time; rows behind the last token become zeros
+#pragma unroll 4
+        for (int c = r; c < BN * D / 16; c += 128) {
+          const int row_t = c / (D / 16), ch = c % (D / 16);
+          const uint4 w = row_t < valid ? *reinterpret_cast<const uint4 *>(src + c * 16) : make_uint4(0u, 0u, 0u, 0u);
+          const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+          uint32_t o[8];
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+              // bytes (b0, b1) -> bf16 pair of the codes: low 7 bits on the magic
+              // 0x43 give 128 + low7, the sign bit on it 128 or 256; their
+              // difference is the code, exactly
+              const uint32_t x = __byte_perm(in[e], 0x43434343u, half ? 0x4342u | 0x0000u : 0x4140u);
+              uint32_t d;
+              asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(x & 0xFF7FFF7Fu), "r"(x & 0xFF80FF80u));
+              o[e * 2 + half] = d;
+            }
+          *reinterpret_cast<uint4 *>(dst + chunk_off(row_t, 2 * ch)) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4 *>(dst + chunk_off(row_t, 2 * ch + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&bars.raw_empty[raw]);
+          mbar_arrive(&bars.full[slot]);
+        }
+      }
+    }
+  }
+}
+
+template <int N>
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+
+template <int D, bool INT8>
+__global__ void __launch_bounds__(Cfg<D, INT8>::THREADS, 1)
+    chunk_attn_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                      const __grid_constant__ CUtensorMap tv, const __grid_constant__ ChunkArgs a) {
+  using C = Cfg<D, INT8>;
+  using B = Bars<C::SLOTS, C::RAWS>;
+  static_assert(sizeof(B) <= 512, "barriers");
+  extern __shared__ __align__(1024) uint8_t sm[];
+  B &bars = *reinterpret_cast<B *>(sm + C::OFF_BARS);
+  const int warp = threadIdx.x >> 5;
+  // the kernel that joins the parts may launch; it waits for this grid's end
+  asm volatile("griddepcontrol.launch_dependents;");
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem)), "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  if (threadIdx.x == 32) {
+    mbar_init(&bars.q_full, 1);
+    mbar_init(&bars.q_empty, 1);
+    mbar_init(&bars.o_free, 8);
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&bars.s_full[i], 1);
+      mbar_init(&bars.p_full[i], 4);
+      mbar_init(&bars.o_full[i], 1);
+      bars.acc[i] = 0;
+    }
+    for (int i = 0; i < C::SLOTS; i++) {
+      mbar_init(&bars.full[i], INT8 ? 4 : 1);
+      mbar_init(&bars.empty[i], 1);
+    }
+    for (int i = 0; i < C::RAWS; i++) {
+      mbar_init(&bars.raw_full[i], 1);
+      mbar_init(&bars.raw_empty[i], 4);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars.tmem;
+  if (warp < 8) {
+    regs_inc<C::REG_SOFT>();
+    softmax_role<D, INT8>(a, sm, bars, warp >> 2);
+  } else if (warp < 12) {
+    regs_dec<C::REG_PROD>();
+    if (warp == 8) {
+      if ((threadIdx.x & 31) == 0) mma_role<D, INT8>(a, sm, bars);
+      __syncwarp();
+    } else if (warp == 9) {
+      tma_role<D, INT8>(&tq, &tk, &tv, a, sm, bars);
+    }
+  } else {
+    if constexpr (INT8) {
+      regs_dec<C::REG_CONV>();
+      convert_role<D>(a, sm, bars);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+}
+
+// Joins the parts of the items that CTA boundaries cut: block x belongs to the
+// boundary before CTA x + 1 and takes the item if that boundary is its first.
+constexpr int kJoinThreads = 128;
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) chunk_join_kernel(const __grid_constant__ ChunkArgs a) {
+  constexpr int ROWS = kJoinThreads / (D / 4);
+  const int c = (int)blockIdx.x + 1;
+  const Start it = a.start[c], before = a.start[c - 1];
+  auto same = [&](const Start &x) { return x.seq == it.seq && x.head == it.head && x.pair == it.pair && x.tile > 0; };
+  if (it.tile == 0 || same(before)) return;
+  const ChunkSeq s = a.seq[it.seq];
+  const int tok0 = it.pair * 2 * a.sh.tpt, ntok = min(2 * a.sh.tpt, s.rows - tok0);
+  const bool both = ntok > a.sh.tpt;
+  const int rows = ntok * a.G;
+  int last = c;  // CTAs c - 1 .. last hold parts
+  while (last + 1 < a.n_ctas && same(a.start[last + 1])) last++;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int col = threadIdx.x % (D / 4);
+  for (int r = (int)blockIdx.y * ROWS + threadIdx.x / (D / 4); r < rows; r += gridDim.y * ROWS) {
+    // row r of the item in the scratch: the second tile starts at 128
+    const int tile_rows = a.sh.tpt * a.G, prow = both && r >= tile_rows ? BM + r - tile_rows : r;
+    auto part = [&](int x) { return a.ws + (size_t)(x * 2 + (x == c - 1 ? 1 : 0)) * (kRowsItem * (D + 2)); };
+    float m = -INFINITY;
+    for (int x = c - 1; x <= last; x++) m = fmaxf(m, __ldcg(reinterpret_cast<const float2 *>(part(x) + (size_t)kRowsItem * D) + prow).x);
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int x = c - 1; x <= last; x++) {
+      const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part(x) + (size_t)kRowsItem * D) + prow);
+      const float f = ml.x == -INFINITY ? 1.f : ex2(ml.x - m);  // without a maximum l and O are 0, or NaN
+      const float4 y = __ldcg(reinterpret_cast<const float4 *>(part(x) + (size_t)prow * D) + col);
+      l = fmaf(ml.y, f, l);
+      o.x = fmaf(y.x, f, o.x);
+      o.y = fmaf(y.y, f, o.y);
+      o.z = fmaf(y.z, f, o.z);
+      o.w = fmaf(y.w, f, o.w);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int tok = tok0 + r / a.G;
+    const size_t row = (size_t)(s.row0 + tok) * a.Hq + (size_t)it.head * a.G + r % a.G;
+    *reinterpret_cast<uint2 *>(a.out + row * D + col * 4) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+    if (col == 0 && a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+  }
+}
+
+// ------------------------------------------------------------------ host
+using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                   const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn(vxb_ctx *ctx) {
+  static std::mutex mu;
+  static EncodeTiledFn fn = nullptr;
+  std::lock_guard<std::mutex> lk(mu);
+  if (!fn) {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess || !p) {
+      cudaGetLastError();
+      set_error(ctx, VXB_ECUDA, "vxb_chunk_attention: cuTensorMapEncodeTiled is not available from the driver");
+      return nullptr;
+    }
+    fn = reinterpret_cast<EncodeTiledFn>(p);
+  }
+  return fn;
+}
+
+int encode(vxb_ctx *ctx, EncodeTiledFn fn, CUtensorMap *map, CUtensorMapDataType type, int rank, const void *base,
+           const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box, CUtensorMapSwizzle swizzle) {
+  const cuuint32_t one[3] = {1, 1, 1};
+  const CUresult r = fn(map, type, (cuuint32_t)rank, const_cast<void *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(ctx, VXB_EINVAL, "vxb_chunk_attention: cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return VXB_OK;
+}
+
+size_t part_floats(int D) { return (size_t)kRowsItem * (D + 2); }
+int ctas_of(const vxb_ctx *ctx) {
+  const int sms = ctx->num_sms > 0 ? ctx->num_sms : 148;
+  return sms < kMaxCtas ? sms : kMaxCtas;
+}
+
+template <int D, bool INT8>
+int launch(vxb_ctx *ctx, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, const ChunkArgs &a, bool cut, int max_rows,
+           cudaStream_t st) {
+  using C = Cfg<D, INT8>;
+  static std::atomic<bool> configured[64];  // kernel attributes set on this device (zero-initialized)
+  if (!configured[ctx->device & 63]) {
+    VXB_CUDA_TRY(ctx, cudaFuncSetAttribute(chunk_attn_kernel<D, INT8>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    configured[ctx->device & 63] = true;
+  }
+  chunk_attn_kernel<D, INT8><<<a.n_ctas, C::THREADS, C::SMEM, st>>>(q, k, v, a);
+  if (int rc = launch_check(ctx, "chunk_attn_kernel")) return rc;
+  if (!cut) return VXB_OK;
+  cudaLaunchConfig_t cfg = {};
+  constexpr int ROWS = kJoinThreads / (D / 4);
+  cfg.gridDim = dim3((unsigned)(a.n_ctas - 1), (unsigned)((max_rows + ROWS - 1) / ROWS));
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  VXB_CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, chunk_join_kernel<D>, a));
+  return launch_check(ctx, "chunk_join_kernel");
 }
 
 int chunk_attention(vxb_kv *kv, int layer, int n, const int64_t *ids, const int32_t *counts, const uint16_t *d_q, int Hq,
-                    float scale, int causal, uint16_t *d_out, float *d_lse, cudaStream_t st) {
+                    float scale, int causal, uint16_t *d_out, float *d_lse, float *ws, cudaStream_t st) {
   vxb_ctx *ctx = kv->ctx;
+  const int D = kv->head_dim, Hkv = kv->num_kv_heads, bs = kv->block_size;
   int64_t total = 0;
   for (int i = 0; i < n; i++) {
     if (counts[i] < 0) return set_error(ctx, VXB_EINVAL, "vxb_chunk_attention: sequence %lld has %d queries", (long long)ids[i], counts[i]);
     total += counts[i];
   }
-  if (total > INT_MAX) return set_error(ctx, VXB_EINVAL, "vxb_chunk_attention: %lld rows", (long long)total);
+  if (total > INT_MAX - kRowsItem) return set_error(ctx, VXB_EINVAL, "vxb_chunk_attention: %lld rows", (long long)total);
   if (total == 0) return VXB_OK;
   if (!d_q || !d_out || ((uintptr_t)d_q | (uintptr_t)d_out) % 16)
     return set_error(ctx, VXB_EINVAL, "vxb_chunk_attention: d_q and d_out must be 16-byte aligned device pointers");
+  if ((int64_t)kv->max_blocks * Hkv * bs > INT_MAX)  // TMA coordinates
+    return set_error(ctx, VXB_EUNSUPPORTED, "vxb_chunk_attention: a pool of more than 2^31 token rows");
+  EncodeTiledFn fn = encode_fn(ctx);
+  if (!fn) return VXB_ECUDA;
+  const bool i8 = kv->dtype == VXB_I8;
   ChunkArgs a;
-  a.q = d_q;
   a.out = d_out;
   a.lse = d_lse;
-  a.pool_k = kv->pool_k;
-  a.pool_v = kv->pool_v;
+  a.ws = ws;
+  a.err = ctx->d_err;
   a.sk = kv->scale_k;
   a.sv = kv->scale_v;
   a.tables = kv->d_tables + (size_t)layer * kv->max_seqs * kv->max_blocks_per_seq;
   a.Hq = Hq;
-  a.Hkv = kv->num_kv_heads;
-  a.G = Hq / kv->num_kv_heads;
-  a.bs = kv->block_size;
+  a.Hkv = Hkv;
+  a.G = Hq / Hkv;
+  a.bs = bs;
   a.mbps = kv->max_blocks_per_seq;
-  a.causal = causal;
+  a.sh = {BM / a.G, causal != 0};
   a.scale_log2 = scale * 1.44269504088896340736f;
-  const bool i8 = kv->dtype == VXB_I8;
+  a.box = bs % 128 == 0 ? 128 : bs % 64 == 0 ? 64 : bs % 32 == 0 ? 32 : 16;  // tokens of a page copy: within a block
+  CUtensorMap mq, mk, mv;
+  {
+    const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)Hq, (cuuint64_t)total};
+    const cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)Hq * D * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)a.G, (cuuint32_t)a.sh.tpt};
+    if (int rc = encode(ctx, fn, &mq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, d_q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  }
+  for (int v = 0; v < 2; v++) {
+    const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)kv->max_blocks * Hkv * bs};
+    const cuuint64_t strides[1] = {(cuuint64_t)D * kv->elem_bytes};
+    const cuuint32_t box[2] = {i8 ? (cuuint32_t)D : 64u, (cuuint32_t)a.box};
+    if (int rc = encode(ctx, fn, v ? &mv : &mk, i8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                        v ? kv->pool_v : kv->pool_k, dims, strides, box, i8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B))
+      return rc;
+  }
   int row = 0;
   for (int i = 0; i < n;) {
     a.n = 0;
-    a.rows = -row;
+    a.units = 0;
+    long long per_head[kSeqs];
+    int max_rows = 0;
     for (; i < n && a.n < kSeqs; i++) {
       if (counts[i] == 0) continue;
       auto it = kv->tables.find(std::make_pair(layer, ids[i]));
       const int len = it == kv->tables.end() ? 0 : (int)it->second.len;
-      a.seq[a.n++] = {len > 0 ? kv->slot_of.at(ids[i]) : 0, row, counts[i], len};
+      ChunkSeq &s = a.seq[a.n];
+      s = {len > 0 ? kv->slot_of.at(ids[i]) : 0, row, counts[i], len};
+      per_head[a.n] = 0;
+      const int pairs = (counts[i] + 2 * a.sh.tpt - 1) / (2 * a.sh.tpt);
+      for (int p = 0; p < pairs; p++) per_head[a.n] += units_of(s, a.sh, p);
+      a.units += per_head[a.n] * Hkv;
+      max_rows = max_rows > counts[i] ? max_rows : counts[i];
       row += counts[i];
+      a.n++;
     }
-    a.rows += row;
     if (a.n == 0) continue;
-    const unsigned grid = (unsigned)(((long long)a.rows * Hq + 3) / 4);
-    if (kv->head_dim == 128) {
-      if (i8) chunk_attn_kernel<128, true><<<grid, 128, 0, st>>>(a);
-      else chunk_attn_kernel<128, false><<<grid, 128, 0, st>>>(a);
-    } else {
-      if (i8) chunk_attn_kernel<64, true><<<grid, 128, 0, st>>>(a);
-      else chunk_attn_kernel<64, false><<<grid, 128, 0, st>>>(a);
+    a.n_ctas = (int)(a.units < ctas_of(ctx) ? a.units : ctas_of(ctx));
+    if (a.units / a.n_ctas >= INT_MAX / 4) return set_error(ctx, VXB_EINVAL, "vxb_chunk_attention: too much work for one call");
+    // the item and key tile where each CTA's run starts
+    int sq = 0, hd = 0, pr = 0;
+    long long at = 0;  // first unit of (sq, hd, pr)
+    bool cut = false;
+    for (int c = 0; c < a.n_ctas; c++) {
+      const long long u = a.units * c / a.n_ctas;
+      while (true) {
+        if (pr == 0 && u - at >= per_head[sq]) {  // whole heads at a time
+          const long long skip = (u - at) / per_head[sq] < Hkv - hd ? (u - at) / per_head[sq] : Hkv - hd;
+          at += skip * per_head[sq];
+          hd += (int)skip;
+        } else {
+          const int w = units_of(a.seq[sq], a.sh, pr);
+          if (u - at < w) break;
+          at += w;
+          pr++;
+          if (pr * 2 * a.sh.tpt >= a.seq[sq].rows) {
+            pr = 0;
+            hd++;
+          }
+        }
+        if (hd == Hkv) {
+          hd = 0;
+          sq++;
+        }
+      }
+      a.start[c] = {sq, hd, pr, (int32_t)(u - at)};
+      cut |= u > at;
     }
-    if (int rc = launch_check(ctx, "chunk_attn_kernel")) return rc;
+    max_rows = max_rows < 2 * a.sh.tpt ? max_rows * a.G : 2 * a.sh.tpt * a.G;
+    int rc;
+    if (D == 128) rc = i8 ? launch<128, true>(ctx, mq, mk, mv, a, cut, max_rows, st) : launch<128, false>(ctx, mq, mk, mv, a, cut, max_rows, st);
+    else rc = i8 ? launch<64, true>(ctx, mq, mk, mv, a, cut, max_rows, st) : launch<64, false>(ctx, mq, mk, mv, a, cut, max_rows, st);
+    if (rc) return rc;
   }
   return VXB_OK;
 }
@@ -155,7 +987,7 @@ VXB_API int vxb_chunk_attention_ws(const vxb_kv *kv, int num_q_heads, size_t *ws
   if (!kv || !kv->ctx) return set_error(nullptr, VXB_EINVAL, "vxb_chunk_attention_ws: null cache");
   if (!ws_bytes) return set_error(kv->ctx, VXB_EINVAL, "vxb_chunk_attention_ws: null output");
   if (int rc = check_heads(kv, num_q_heads)) return rc;
-  *ws_bytes = 256;
+  *ws_bytes = (size_t)2 * ctas_of(kv->ctx) * part_floats(kv->head_dim) * sizeof(float);
   return VXB_OK;
 }
 
@@ -175,7 +1007,8 @@ VXB_API int vxb_chunk_attention(vxb_kv *kv, int layer, int n, const int64_t *h_s
   DeviceScope dev(ctx);
   if (dev.rc) return dev.rc;
   try {
-    return chunk_attention(kv, layer, n, h_seq_ids, h_n_queries, d_q, num_q_heads, softmax_scale, causal, d_out, d_lse, (cudaStream_t)stream);
+    return chunk_attention(kv, layer, n, h_seq_ids, h_n_queries, d_q, num_q_heads, softmax_scale, causal, d_out, d_lse, (float *)d_ws,
+                           (cudaStream_t)stream);
   } catch (...) {
     return set_error(ctx, VXB_ENOMEM, "vxb_chunk_attention: out of host memory");
   }
