@@ -281,6 +281,36 @@ def test_chunk_attention_vs_f64(KV, H, G, D, bs, lens, counts, int8, causal):
     assert torch.equal(out, c.chunk_attention(1, ids, counts, q, causal=causal)), "not deterministic"
 
 
+FEW = [
+    # H kv, G, block, lens, counts: up to 64 rows a head, short and long, many and few sequences
+    (1, 1, 16, [128 * i + 1 for i in range(20)], [1 + i % 16 for i in range(20)]),
+    (4, 4, 16, [3000, 127, 128, 129, 5000], [4, 8, 16, 1, 5]),
+    (2, 8, 32, [40, 9000], [8, 8]),
+    (1, 64, 16, [700, 31], [1, 1]),
+    (1, 24, 128, [2000, 2, 640], [2, 2, 1]),
+    (3, 7, 16, [255, 1, 400, 256, 17, 1030], [9, 1, 2, 0, 4, 3]),
+    (8, 1, 64, [600] * 40, [64, 1, 3, 33] * 10),
+]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("H,G,bs,lens,counts", FEW)
+def test_chunk_attention_few_rows(KV, H, G, bs, lens, counts, D, int8, causal):
+    n = len(lens)
+    c = make(KV, 1, H, D, bs, sum(-(-x // bs) for x in lens), n, int8)
+    v = rnd((sum(lens), H, D), 2)
+    v[::5] *= 100.0  # scales of an int8 cache that differ from key to key
+    v[1::7] *= 0.001
+    c.append_chunks(0, range(n), lens, rnd((sum(lens), H, D), 1), v)
+    q = rnd((sum(counts), H * G, D), 3, 2.0)
+    lse = torch.full((sum(counts), H * G), 7.0, device="cuda")
+    out = c.chunk_attention(0, range(n), counts, q, causal=causal, lse=lse)
+    check_rows(out, lse, q, c, 0, range(n), counts, causal, 1 / math.sqrt(D))
+    assert torch.equal(out, c.chunk_attention(0, range(n), counts, q, causal=causal)), "not deterministic"
+
+
 @pytest.mark.parametrize("int8", [False, True])
 def test_chunk_attention_rows_that_see_nothing(KV, int8):
     # empty and unknown sequences, more queries than tokens, sequences without queries
@@ -303,10 +333,11 @@ def test_chunk_attention_rows_that_see_nothing(KV, int8):
 
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 @pytest.mark.parametrize("D", [64, 128])
-def test_chunk_attention_masked_tokens_do_not_matter(KV, D, bad):
+@pytest.mark.parametrize("m", [200, 64])
+def test_chunk_attention_masked_tokens_do_not_matter(KV, D, m, bad):
     # a later token of the same chunk with a non-finite key or value changes
     # no earlier row; a finite softmax sees only visible tokens
-    H, n, m = 2, 300, 200
+    H, n = 2, 300
     k, v = rnd((n, H, D), 1), rnd((n, H, D), 2)
     q = rnd((m, H, D), 3)
     outs = []
@@ -318,11 +349,12 @@ def test_chunk_attention_masked_tokens_do_not_matter(KV, D, bad):
         c.append_chunks(0, [0], [n], kk, vv)
         outs.append(c.chunk_attention(0, [0], [m], q))
     clean, dirty = outs
-    assert torch.equal(clean[:150], dirty[:150])            # rows up to token 249
-    assert torch.equal(clean[:151, 0], dirty[:151, 0])
-    assert torch.equal(clean[151:, 0, 6:], dirty[151:, 0, 6:])  # one dimension of one value row
-    assert not bool(torch.isfinite(dirty[151:, 0, 5]).any())
-    assert not bool(torch.isfinite(dirty[160:, 1]).any())
+    at = n - m                                              # the first row's token
+    assert torch.equal(clean[:250 - at], dirty[:250 - at])
+    assert torch.equal(clean[:251 - at, 0], dirty[:251 - at, 0])
+    assert torch.equal(clean[251 - at:, 0, 6:], dirty[251 - at:, 0, 6:])  # one dimension of one value row
+    assert not bool(torch.isfinite(dirty[251 - at:, 0, 5]).any())
+    assert not bool(torch.isfinite(dirty[260 - at:, 1]).any())
 
 
 def test_chunk_attention_many_sequences_streams_and_graphs(KV):

@@ -49,109 +49,13 @@
 
 #include <mutex>
 
-#include "kv_cache.h"
-#include "tc_common.h"
+#include "chunk_attn.h"
 
 using namespace vxb;
 using namespace vxb::tc;
+using namespace vxb::chunk;
 
 namespace {
-
-constexpr int BM = 128, BN = 128;
-constexpr int kSeqs = 128;    // sequences of one launch (their record is a kernel parameter)
-constexpr int kMaxCtas = 160;
-constexpr int kRowsItem = 2 * BM;
-constexpr float RESCALE_THRESHOLD = 8.f;  // O is rescaled when a row's maximum grows by more (log2)
-
-struct ChunkSeq {
-  int32_t slot, row0, rows, len;
-};
-struct Start {  // a CTA's first item and the first of its key tiles
-  int32_t seq, head, pair, tile;
-};
-struct Shape {
-  int tpt;  // tokens of a 128-row tile
-  int causal;
-};
-struct ChunkArgs {
-  uint16_t *out;
-  float *lse;
-  float *ws;
-  int *err;
-  const float *sk, *sv;
-  const int32_t *tables;  // of the layer
-  int n, Hq, Hkv, G, bs, mbps, box, n_ctas;
-  Shape sh;
-  float scale_log2;
-  long long units;
-  ChunkSeq seq[kSeqs];
-  Start start[kMaxCtas + 1];
-};
-static_assert(sizeof(ChunkArgs) <= 8192, "kernel parameters");
-
-// Key tiles that the tokens before tok_end of a chunk see
-__host__ __device__ inline int tiles_of(const ChunkSeq &s, const Shape &sh, int tok_end) {
-  const int seen = sh.causal ? s.len - s.rows + tok_end : s.len;
-  return seen > 0 ? (seen + BN - 1) / BN : 0;
-}
-// Units of an item: its key tiles, one at least
-__host__ __device__ inline int units_of(const ChunkSeq &s, const Shape &sh, int pair) {
-  const int end = (pair + 1) * 2 * sh.tpt;
-  const int t = tiles_of(s, sh, end < s.rows ? end : s.rows);
-  return t > 0 ? t : 1;
-}
-
-// The run of a CTA as pieces: consecutive key tiles of one item.
-struct Piece {
-  ChunkSeq s;
-  int head, tok0, ntok, tb, te, units, te_u;
-  bool both;   // two tiles of rows, the same keys; else one tile, every other key tile
-  int n0, n1;  // steps of the streams
-  __device__ __forceinline__ int tile(int stream, int i) const { return both ? tb + i : tb + 2 * i + stream; }
-  __device__ __forceinline__ int steps(int stream) const { return stream ? n1 : n0; }
-  __device__ __forceinline__ bool whole() const { return tb == 0 && te_u == units; }
-};
-struct Run {
-  Start at;
-  int left;
-  __device__ Run(const ChunkArgs &a) {
-    at = a.start[blockIdx.x];
-    const long long u0 = a.units * blockIdx.x / a.n_ctas, u1 = a.units * (blockIdx.x + 1) / a.n_ctas;
-    left = (int)(u1 - u0);
-  }
-  __device__ __forceinline__ bool next(const ChunkArgs &a, Piece &p) {
-    if (left <= 0) return false;
-    p.s = a.seq[at.seq];
-    p.head = at.head;
-    p.tok0 = at.pair * 2 * a.sh.tpt;
-    p.ntok = min(2 * a.sh.tpt, p.s.rows - p.tok0);
-    p.both = p.ntok > a.sh.tpt;
-    const int n = tiles_of(p.s, a.sh, p.tok0 + p.ntok);
-    p.units = max(1, n);
-    p.tb = at.tile;
-    p.te_u = min(p.units, p.tb + left);
-    p.te = min(p.te_u, n);
-    const int count = max(0, p.te - p.tb);
-    if (p.both) {
-      p.n0 = max(0, min(p.te, tiles_of(p.s, a.sh, p.tok0 + a.sh.tpt)) - p.tb);
-      p.n1 = count;
-    } else {
-      p.n0 = (count + 1) / 2;
-      p.n1 = count / 2;
-    }
-    left -= p.te_u - p.tb;
-    at.tile = 0;
-    at.pair++;
-    if (at.pair * 2 * a.sh.tpt >= p.s.rows) {
-      at.pair = 0;
-      if (++at.head == a.Hkv) {
-        at.head = 0;
-        at.seq++;
-      }
-    }
-    return true;
-  }
-};
 
 template <int D, bool INT8>
 struct Cfg {
@@ -182,49 +86,9 @@ struct Bars {
   int acc[2];  // the stream's O already holds values that its first product adds to
 };
 
-// Bounded wait; once one has run out, the following ones of this thread do not
-// wait again, and the kernel ends.
-template <bool WARP>  // every lane of a warp waits, and they go on together
-struct Waiter {
-  int *err;
-  bool dead = false;
-  __device__ __forceinline__ void operator()(uint64_t *bar, uint32_t parity) {
-    if (!mbar_wait(bar, parity, dead ? 0 : kWaitBudget)) {
-      dead = true;
-      atomicExch(err, 1);
-    }
-    if (WARP) __syncwarp();
-  }
-};
-
-__device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
-__device__ __forceinline__ bool bar_or(int id, int threads, bool p) {
-  uint32_t r;
-  asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, %2, %3, p;\n selp.u32 %0, 1, 0, q;\n}"
-      : "=r"(r)
-      : "r"((uint32_t)p), "r"(id), "r"(threads)
-      : "memory");
-  return r != 0;
-}
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ float tmem_ld1(uint32_t taddr) {
-  uint32_t r;
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
-  tmem_wait_ld();
-  return __uint_as_float(r);
-}
-__device__ __forceinline__ void tmem_st1(uint32_t taddr, float v) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(__float_as_uint(v)) : "memory");
-}
-
 // 16-byte chunk c (8 columns) of row r of a bf16 tile in shared memory
 __device__ __forceinline__ uint32_t chunk_off(int r, int c) {
   return (uint32_t)((c >> 3) * (BN * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-}
-
-__device__ __forceinline__ uint32_t odd_bf16(uint32_t w) {  // a non-finite element in a pair
-  return (uint32_t)((w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u);
 }
 
 // ------------------------------------------------------------------ softmax warpgroup of stream ST
@@ -238,7 +102,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
   float2 *ml = reinterpret_cast<float2 *>(sm + C::OFF_ML);  // [2][BM]
   Waiter<true> wait{a.err};
   Run run(a);
-  Piece p;
+  Piece p{};
   uint32_t step = 0, pieces = 0, ring = 0;  // this stream's steps; pieces; first ring index of the piece
   while (run.next(a, p)) {
     const int base = p.s.len - p.s.rows;
@@ -400,13 +264,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
           if (!(both_here && st == 1)) {
             for (int c = r; c < valid * (D / 8); c += 128) {
               uint4 *at = reinterpret_cast<uint4 *>(sv_tile + chunk_off(c / (D / 8), c % (D / 8)));
-              uint32_t w[4] = {at->x, at->y, at->z, at->w};
-#pragma unroll
-              for (int e = 0; e < 4; e++) {
-                if ((w[e] & 0x7F80u) == 0x7F80u) w[e] &= 0xFFFF0000u;
-                if ((w[e] & 0x7F800000u) == 0x7F800000u) w[e] &= 0xFFFFu;
-              }
-              *at = make_uint4(w[0], w[1], w[2], w[3]);
+              *at = make_uint4(even_bf16(at->x), even_bf16(at->y), even_bf16(at->z), even_bf16(at->w));
             }
             fence_async_smem();
           }
@@ -502,7 +360,7 @@ __device__ __forceinline__ void mma_role(const ChunkArgs &a, uint8_t *sm, B &bar
   const uint32_t s_q = smem_u32(sm), s_kv = smem_u32(sm + C::OFF_KV), tmem = bars.tmem;
   Waiter<false> wait{a.err};
   Run run(a);
-  Piece p;
+  Piece p{};
   uint32_t ring = 0, pieces = 0, psteps[2] = {0, 0};
   while (run.next(a, p)) {
     const int tiles = max(0, p.te - p.tb);
@@ -578,7 +436,7 @@ __device__ __forceinline__ void tma_role(const CUtensorMap *tq, const CUtensorMa
   uint8_t *tiles = sm + (INT8 ? C::OFF_RAW : C::OFF_KV);
   Waiter<true> wait{a.err};
   Run run(a);
-  Piece p;
+  Piece p{};
   uint32_t idx = 0, pieces = 0;
   while (run.next(a, p)) {
     const int32_t *table = a.tables + (size_t)p.s.slot * a.mbps;
@@ -636,7 +494,7 @@ __device__ __forceinline__ void convert_role(const ChunkArgs &a, uint8_t *sm, B 
   const int r = threadIdx.x & 127, lane = threadIdx.x & 31;
   Waiter<true> wait{a.err};
   Run run(a);
-  Piece p;
+  Piece p{};
   uint32_t idx = 0;
   while (run.next(a, p)) {
     const int32_t *table = a.tables + (size_t)p.s.slot * a.mbps;
@@ -832,27 +690,47 @@ int encode(vxb_ctx *ctx, EncodeTiledFn fn, CUtensorMap *map, CUtensorMapDataType
   return VXB_OK;
 }
 
-size_t part_floats(int D) { return (size_t)kRowsItem * (D + 2); }
-int ctas_of(const vxb_ctx *ctx) {
-  const int sms = ctx->num_sms > 0 ? ctx->num_sms : 148;
-  return sms < kMaxCtas ? sms : kMaxCtas;
-}
-
 template <int D, bool INT8>
-int launch(vxb_ctx *ctx, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, const ChunkArgs &a, bool cut, int max_rows,
-           cudaStream_t st) {
+int launch_many(vxb_kv *kv, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, const ChunkArgs &a, cudaStream_t st) {
   using C = Cfg<D, INT8>;
   static std::atomic<bool> configured[64];  // kernel attributes set on this device (zero-initialized)
-  if (!configured[ctx->device & 63]) {
-    VXB_CUDA_TRY(ctx, cudaFuncSetAttribute(chunk_attn_kernel<D, INT8>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-    configured[ctx->device & 63] = true;
+  if (!configured[kv->ctx->device & 63]) {
+    VXB_CUDA_TRY(kv->ctx, cudaFuncSetAttribute(chunk_attn_kernel<D, INT8>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    configured[kv->ctx->device & 63] = true;
   }
   chunk_attn_kernel<D, INT8><<<a.n_ctas, C::THREADS, C::SMEM, st>>>(q, k, v, a);
-  if (int rc = launch_check(ctx, "chunk_attn_kernel")) return rc;
-  if (!cut) return VXB_OK;
+  return launch_check(kv->ctx, "chunk_attn_kernel");
+}
+
+int launch_many(vxb_kv *kv, const ChunkArgs &a, int64_t rows, cudaStream_t st) {
+  vxb_ctx *ctx = kv->ctx;
+  const int D = kv->head_dim;
+  const bool i8 = kv->dtype == VXB_I8;
+  EncodeTiledFn fn = encode_fn(ctx);
+  if (!fn) return VXB_ECUDA;
+  CUtensorMap mq, mk, mv;
+  {
+    const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)a.Hq, (cuuint64_t)rows};
+    const cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)a.Hq * D * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)a.G, (cuuint32_t)a.sh.tpt};
+    if (int rc = encode(ctx, fn, &mq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, a.q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  }
+  for (int v = 0; v < 2; v++) {
+    const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)kv->max_blocks * a.Hkv * a.bs};
+    const cuuint64_t strides[1] = {(cuuint64_t)D * kv->elem_bytes};
+    const cuuint32_t box[2] = {i8 ? (cuuint32_t)D : 64u, (cuuint32_t)a.box};
+    if (int rc = encode(ctx, fn, v ? &mv : &mk, i8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                        v ? a.pool_v : a.pool_k, dims, strides, box, i8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B))
+      return rc;
+  }
+  if (D == 128) return i8 ? launch_many<128, true>(kv, mq, mk, mv, a, st) : launch_many<128, false>(kv, mq, mk, mv, a, st);
+  return i8 ? launch_many<64, true>(kv, mq, mk, mv, a, st) : launch_many<64, false>(kv, mq, mk, mv, a, st);
+}
+
+int launch_join(vxb_kv *kv, const ChunkArgs &a, int max_rows, cudaStream_t st) {
+  const int rows = kJoinThreads / (kv->head_dim / 4);
   cudaLaunchConfig_t cfg = {};
-  constexpr int ROWS = kJoinThreads / (D / 4);
-  cfg.gridDim = dim3((unsigned)(a.n_ctas - 1), (unsigned)((max_rows + ROWS - 1) / ROWS));
+  cfg.gridDim = dim3((unsigned)(a.n_ctas - 1), (unsigned)((max_rows + rows - 1) / rows));
   cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -860,14 +738,64 @@ int launch(vxb_ctx *ctx, const CUtensorMap &q, const CUtensorMap &k, const CUten
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  VXB_CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, chunk_join_kernel<D>, a));
-  return launch_check(ctx, "chunk_join_kernel");
+  if (kv->head_dim == 128) VXB_CUDA_TRY(kv->ctx, cudaLaunchKernelEx(&cfg, chunk_join_kernel<128>, a));
+  else VXB_CUDA_TRY(kv->ctx, cudaLaunchKernelEx(&cfg, chunk_join_kernel<64>, a));
+  return launch_check(kv->ctx, "chunk_join_kernel");
+}
+
+int ctas_of(const vxb_ctx *ctx) {
+  const int sms = ctx->num_sms > 0 ? ctx->num_sms : 148;
+  return sms < kMaxCtas ? sms : kMaxCtas;
+}
+
+// Cuts the key tiles of a.seq[0 .. a.n) into one run per CTA; whether a cut
+// falls inside an item.
+int cut_runs(const vxb_ctx *ctx, ChunkArgs &a, bool *cut) {
+  long long per_head[kSeqs];
+  a.units = 0;
+  for (int i = 0; i < a.n; i++) {
+    per_head[i] = 0;
+    const int pairs = (a.seq[i].rows + 2 * a.sh.tpt - 1) / (2 * a.sh.tpt);
+    for (int p = 0; p < pairs; p++) per_head[i] += units_of(a.seq[i], a.sh, p);
+    a.units += per_head[i] * a.Hkv;
+  }
+  a.n_ctas = (int)(a.units < ctas_of(ctx) ? a.units : ctas_of(ctx));
+  if (a.units / a.n_ctas >= INT_MAX / 4) return VXB_EINVAL;
+  int sq = 0, hd = 0, pr = 0;
+  long long at = 0;  // first unit of (sq, hd, pr)
+  *cut = false;
+  for (int c = 0; c < a.n_ctas; c++) {
+    const long long u = a.units * c / a.n_ctas;
+    while (true) {
+      if (pr == 0 && u - at >= per_head[sq]) {  // whole heads at a time
+        const long long fit = (u - at) / per_head[sq], skip = fit < a.Hkv - hd ? fit : a.Hkv - hd;
+        at += skip * per_head[sq];
+        hd += (int)skip;
+      } else {
+        const int w = units_of(a.seq[sq], a.sh, pr);
+        if (u - at < w) break;
+        at += w;
+        pr++;
+        if (pr * 2 * a.sh.tpt >= a.seq[sq].rows) {
+          pr = 0;
+          hd++;
+        }
+      }
+      if (hd == a.Hkv) {
+        hd = 0;
+        sq++;
+      }
+    }
+    a.start[c] = {sq, hd, pr, (int32_t)(u - at)};
+    *cut |= u > at;
+  }
+  return VXB_OK;
 }
 
 int chunk_attention(vxb_kv *kv, int layer, int n, const int64_t *ids, const int32_t *counts, const uint16_t *d_q, int Hq,
                     float scale, int causal, uint16_t *d_out, float *d_lse, float *ws, cudaStream_t st) {
   vxb_ctx *ctx = kv->ctx;
-  const int D = kv->head_dim, Hkv = kv->num_kv_heads, bs = kv->block_size;
+  const int Hkv = kv->num_kv_heads, bs = kv->block_size;
   int64_t total = 0;
   for (int i = 0; i < n; i++) {
     if (counts[i] < 0) return set_error(ctx, VXB_EINVAL, "vxb_chunk_attention: sequence %lld has %d queries", (long long)ids[i], counts[i]);
@@ -877,12 +805,12 @@ int chunk_attention(vxb_kv *kv, int layer, int n, const int64_t *ids, const int3
   if (total == 0) return VXB_OK;
   if (!d_q || !d_out || ((uintptr_t)d_q | (uintptr_t)d_out) % 16)
     return set_error(ctx, VXB_EINVAL, "vxb_chunk_attention: d_q and d_out must be 16-byte aligned device pointers");
-  if ((int64_t)kv->max_blocks * Hkv * bs > INT_MAX)  // TMA coordinates
+  if ((int64_t)kv->max_blocks * Hkv * bs > INT_MAX)  // token rows of the pool are counted in 32 bits
     return set_error(ctx, VXB_EUNSUPPORTED, "vxb_chunk_attention: a pool of more than 2^31 token rows");
-  EncodeTiledFn fn = encode_fn(ctx);
-  if (!fn) return VXB_ECUDA;
-  const bool i8 = kv->dtype == VXB_I8;
   ChunkArgs a;
+  a.q = d_q;
+  a.pool_k = kv->pool_k;
+  a.pool_v = kv->pool_v;
   a.out = d_out;
   a.lse = d_lse;
   a.ws = ws;
@@ -895,81 +823,32 @@ int chunk_attention(vxb_kv *kv, int layer, int n, const int64_t *ids, const int3
   a.G = Hq / Hkv;
   a.bs = bs;
   a.mbps = kv->max_blocks_per_seq;
-  a.sh = {BM / a.G, causal != 0};
   a.scale_log2 = scale * 1.44269504088896340736f;
   a.box = bs % 128 == 0 ? 128 : bs % 64 == 0 ? 64 : bs % 32 == 0 ? 32 : 16;  // tokens of a page copy: within a block
-  CUtensorMap mq, mk, mv;
-  {
-    const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)Hq, (cuuint64_t)total};
-    const cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)Hq * D * 2};
-    const cuuint32_t box[3] = {64, (cuuint32_t)a.G, (cuuint32_t)a.sh.tpt};
-    if (int rc = encode(ctx, fn, &mq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, d_q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
-  }
-  for (int v = 0; v < 2; v++) {
-    const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)kv->max_blocks * Hkv * bs};
-    const cuuint64_t strides[1] = {(cuuint64_t)D * kv->elem_bytes};
-    const cuuint32_t box[2] = {i8 ? (cuuint32_t)D : 64u, (cuuint32_t)a.box};
-    if (int rc = encode(ctx, fn, v ? &mv : &mk, i8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
-                        v ? kv->pool_v : kv->pool_k, dims, strides, box, i8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B))
-      return rc;
-  }
-  int row = 0;
-  for (int i = 0; i < n;) {
-    a.n = 0;
-    a.units = 0;
-    long long per_head[kSeqs];
-    int max_rows = 0;
-    for (; i < n && a.n < kSeqs; i++) {
-      if (counts[i] == 0) continue;
-      auto it = kv->tables.find(std::make_pair(layer, ids[i]));
-      const int len = it == kv->tables.end() ? 0 : (int)it->second.len;
-      ChunkSeq &s = a.seq[a.n];
-      s = {len > 0 ? kv->slot_of.at(ids[i]) : 0, row, counts[i], len};
-      per_head[a.n] = 0;
-      const int pairs = (counts[i] + 2 * a.sh.tpt - 1) / (2 * a.sh.tpt);
-      for (int p = 0; p < pairs; p++) per_head[a.n] += units_of(s, a.sh, p);
-      a.units += per_head[a.n] * Hkv;
-      max_rows = max_rows > counts[i] ? max_rows : counts[i];
-      row += counts[i];
-      a.n++;
-    }
-    if (a.n == 0) continue;
-    a.n_ctas = (int)(a.units < ctas_of(ctx) ? a.units : ctas_of(ctx));
-    if (a.units / a.n_ctas >= INT_MAX / 4) return set_error(ctx, VXB_EINVAL, "vxb_chunk_attention: too much work for one call");
-    // the item and key tile where each CTA's run starts
-    int sq = 0, hd = 0, pr = 0;
-    long long at = 0;  // first unit of (sq, hd, pr)
-    bool cut = false;
-    for (int c = 0; c < a.n_ctas; c++) {
-      const long long u = a.units * c / a.n_ctas;
-      while (true) {
-        if (pr == 0 && u - at >= per_head[sq]) {  // whole heads at a time
-          const long long skip = (u - at) / per_head[sq] < Hkv - hd ? (u - at) / per_head[sq] : Hkv - hd;
-          at += skip * per_head[sq];
-          hd += (int)skip;
-        } else {
-          const int w = units_of(a.seq[sq], a.sh, pr);
-          if (u - at < w) break;
-          at += w;
-          pr++;
-          if (pr * 2 * a.sh.tpt >= a.seq[sq].rows) {
-            pr = 0;
-            hd++;
-          }
-        }
-        if (hd == Hkv) {
-          hd = 0;
-          sq++;
-        }
+  // chunks of few rows and the others go to a kernel each
+  for (int few = 0; few < 2; few++) {
+    a.sh = {few ? kFewRows : BM / a.G, causal != 0};
+    int row = 0;
+    for (int i = 0; i < n;) {
+      a.n = 0;
+      int max_rows = 0;
+      for (; i < n && a.n < kSeqs; i++) {
+        const int at = row;
+        row += counts[i];
+        if (counts[i] == 0 || ((int64_t)counts[i] * a.G <= kFewRows) != (few == 1)) continue;
+        auto it = kv->tables.find(std::make_pair(layer, ids[i]));
+        const int len = it == kv->tables.end() ? 0 : (int)it->second.len;
+        a.seq[a.n++] = {len > 0 ? kv->slot_of.at(ids[i]) : 0, at, counts[i], len};
+        max_rows = max_rows > counts[i] ? max_rows : counts[i];
       }
-      a.start[c] = {sq, hd, pr, (int32_t)(u - at)};
-      cut |= u > at;
+      if (a.n == 0) continue;
+      bool cut = false;
+      if (cut_runs(ctx, a, &cut)) return set_error(ctx, VXB_EINVAL, "vxb_chunk_attention: too much work for one call");
+      max_rows = (max_rows < 2 * a.sh.tpt ? max_rows : 2 * a.sh.tpt) * a.G;
+      if (int rc = few ? launch_few(kv, a, max_rows, st) : launch_many(kv, a, total, st)) return rc;
+      if (cut)
+        if (int rc = launch_join(kv, a, max_rows, st)) return rc;
     }
-    max_rows = max_rows < 2 * a.sh.tpt ? max_rows * a.G : 2 * a.sh.tpt * a.G;
-    int rc;
-    if (D == 128) rc = i8 ? launch<128, true>(ctx, mq, mk, mv, a, cut, max_rows, st) : launch<128, false>(ctx, mq, mk, mv, a, cut, max_rows, st);
-    else rc = i8 ? launch<64, true>(ctx, mq, mk, mv, a, cut, max_rows, st) : launch<64, false>(ctx, mq, mk, mv, a, cut, max_rows, st);
-    if (rc) return rc;
   }
   return VXB_OK;
 }

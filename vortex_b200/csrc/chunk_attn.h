@@ -1,0 +1,168 @@
+// What the kernels of the chunk attention share: a launch's record, the cut of
+// its key tiles into one run per CTA, bounded waits.
+#pragma once
+
+#include "kv_cache.h"
+#include "tc_common.h"
+
+namespace vxb {
+namespace chunk {
+
+constexpr int BM = 128, BN = 128;
+constexpr int kSeqs = 128;    // sequences of one launch (their record is a kernel parameter)
+constexpr int kMaxCtas = 160;
+constexpr int kRowsItem = 2 * BM;
+constexpr float RESCALE_THRESHOLD = 8.f;  // O is rescaled when a row's maximum grows by more (log2)
+
+struct ChunkSeq {
+  int32_t slot, row0, rows, len;
+};
+struct Start {  // a CTA's first item and the first of its key tiles
+  int32_t seq, head, pair, tile;
+};
+struct Shape {
+  int tpt;  // tokens of a 128-row tile
+  int causal;
+};
+struct ChunkArgs {
+  const uint16_t *q;
+  const void *pool_k, *pool_v;
+  uint16_t *out;
+  float *lse;
+  float *ws;
+  int *err;
+  const float *sk, *sv;
+  const int32_t *tables;  // of the layer
+  int n, Hq, Hkv, G, bs, mbps, box, n_ctas;
+  Shape sh;
+  float scale_log2;
+  long long units;
+  ChunkSeq seq[kSeqs];
+  Start start[kMaxCtas + 1];
+};
+static_assert(sizeof(ChunkArgs) <= 8192, "kernel parameters");
+
+// Key tiles that the tokens before tok_end of a chunk see
+__host__ __device__ inline int tiles_of(const ChunkSeq &s, const Shape &sh, int tok_end) {
+  const int seen = sh.causal ? s.len - s.rows + tok_end : s.len;
+  return seen > 0 ? (seen + BN - 1) / BN : 0;
+}
+// Units of an item: its key tiles, one at least
+__host__ __device__ inline int units_of(const ChunkSeq &s, const Shape &sh, int pair) {
+  const int end = (pair + 1) * 2 * sh.tpt;
+  const int t = tiles_of(s, sh, end < s.rows ? end : s.rows);
+  return t > 0 ? t : 1;
+}
+
+#ifdef __CUDACC__
+// Bounded wait; once one has run out, the following ones of this thread do not
+// wait again, and the kernel ends.
+using namespace vxb::tc;
+
+template <bool WARP>  // every lane of a warp waits, and they go on together
+struct Waiter {
+  int *err;
+  bool dead = false;
+  __device__ __forceinline__ void operator()(uint64_t *bar, uint32_t parity) {
+    if (!mbar_wait(bar, parity, dead ? 0 : kWaitBudget)) {
+      dead = true;
+      atomicExch(err, 1);
+    }
+    if (WARP) __syncwarp();
+  }
+};
+
+// The run of a CTA as pieces: consecutive key tiles of one item.
+struct Piece {
+  ChunkSeq s;
+  int head, tok0, ntok, tb, te, units, te_u;
+  bool both;   // two tiles of rows, the same keys; else one tile, every other key tile
+  int n0, n1;  // steps of the streams
+  __device__ __forceinline__ int tile(int stream, int i) const { return both ? tb + i : tb + 2 * i + stream; }
+  __device__ __forceinline__ int steps(int stream) const { return stream ? n1 : n0; }
+  __device__ __forceinline__ bool whole() const { return tb == 0 && te_u == units; }
+};
+struct Run {
+  Start at;
+  int left;
+  __device__ Run(const ChunkArgs &a) {
+    at = a.start[blockIdx.x];
+    const long long u0 = a.units * blockIdx.x / a.n_ctas, u1 = a.units * (blockIdx.x + 1) / a.n_ctas;
+    left = (int)(u1 - u0);
+  }
+  __device__ __forceinline__ bool next(const ChunkArgs &a, Piece &p) {
+    if (left <= 0) return false;
+    p.s = a.seq[at.seq];
+    p.head = at.head;
+    p.tok0 = at.pair * 2 * a.sh.tpt;
+    p.ntok = min(2 * a.sh.tpt, p.s.rows - p.tok0);
+    p.both = p.ntok > a.sh.tpt;
+    const int n = tiles_of(p.s, a.sh, p.tok0 + p.ntok);
+    p.units = max(1, n);
+    p.tb = at.tile;
+    p.te_u = min(p.units, p.tb + left);
+    p.te = min(p.te_u, n);
+    const int count = max(0, p.te - p.tb);
+    if (p.both) {
+      p.n0 = max(0, min(p.te, tiles_of(p.s, a.sh, p.tok0 + a.sh.tpt)) - p.tb);
+      p.n1 = count;
+    } else {
+      p.n0 = (count + 1) / 2;
+      p.n1 = count / 2;
+    }
+    left -= p.te_u - p.tb;
+    at.tile = 0;
+    at.pair++;
+    if (at.pair * 2 * a.sh.tpt >= p.s.rows) {
+      at.pair = 0;
+      if (++at.head == a.Hkv) {
+        at.head = 0;
+        at.seq++;
+      }
+    }
+    return true;
+  }
+};
+
+__device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ bool bar_or(int id, int threads, bool p) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, %2, %3, p;\n selp.u32 %0, 1, 0, q;\n}"
+      : "=r"(r)
+      : "r"((uint32_t)p), "r"(id), "r"(threads)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ float tmem_ld1(uint32_t taddr) {
+  uint32_t r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
+  tmem_wait_ld();
+  return __uint_as_float(r);
+}
+__device__ __forceinline__ void tmem_st1(uint32_t taddr, float v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(__float_as_uint(v)) : "memory");
+}
+
+__device__ __forceinline__ uint32_t odd_bf16(uint32_t w) {  // a non-finite element in a pair
+  return (uint32_t)((w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u);
+}
+
+__device__ __forceinline__ uint32_t even_bf16(uint32_t w) {  // the pair with zeros for those
+  if ((w & 0x7F80u) == 0x7F80u) w &= 0xFFFF0000u;
+  if ((w & 0x7F800000u) == 0x7F800000u) w &= 0xFFFFu;
+  return w;
+}
+#endif
+
+// Scratch of an item's part: 256 rows of D sums, then (maximum, sum) pairs.
+inline size_t part_floats(int D) { return (size_t)kRowsItem * (D + 2); }
+
+// Chunks of up to kFewRows rows per kv head (few_rows.cu); everything else goes
+// to the kernel in chunk_attn.cu.
+constexpr int kFewRows = 64;
+int launch_few(vxb_kv *kv, const ChunkArgs &a, int max_rows, cudaStream_t st);
+
+}  // namespace chunk
+}  // namespace vxb
