@@ -546,11 +546,6 @@ __device__ __forceinline__ void convert_role(const ChunkArgs &a, uint8_t *sm, B 
   }
 }
 
-template <int N>
-__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-
 template <int D, bool INT8>
 __global__ void __launch_bounds__(Cfg<D, INT8>::THREADS, 1)
     chunk_attn_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,

@@ -145,6 +145,12 @@ __device__ __forceinline__ void tmem_st1(uint32_t taddr, float v) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(__float_as_uint(v)) : "memory");
 }
 
+// A warpgroup's share of the block's registers.
+template <int N>
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+
 __device__ __forceinline__ uint32_t odd_bf16(uint32_t w) {  // a non-finite element in a pair
   return (uint32_t)((w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u);
 }

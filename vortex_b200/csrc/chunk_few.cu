@@ -4,7 +4,7 @@
 // columns:
 //
 //   S^T = K Q^T         A = the K tile, B = the query rows
-//   P^T = 2^(S^T - m)   thread = key: N values each
+//   P^T = 2^(S^T - m)   thread = key and half of the rows
 //   O^T += V^T P^T      A = the V tile read MN-major, B = P from shared memory
 //
 // With the queries as rows (chunk_attn.cu) a tile costs 128 exponentials per
@@ -14,7 +14,8 @@
 // warpgroup and no reduction; l is summed per thread and reduced at the end.
 //
 // Loader warps bring tiles of 128 keys into a ring in the order they are used
-// (K0, K1, V0, K2, V1, ...): bf16 rows with cp.async (a 16-token page is only
+// (K of three tiles, then K of tile t + 3 before V of tile t, so that three S
+// can be on their way while a softmax runs): bf16 rows with cp.async (a 16-token page is only
 // 4 KB: as many TMA boxes reach 5.6 TB/s, 16-byte copies the memory rate),
 // int8 rows through registers, K to bf16 and V to f16 (codes are exact in
 // both). Rows behind the last token become zeros.
@@ -43,34 +44,46 @@ template <int D, bool INT8, int NR>
 struct Cfg {
   static constexpr int SLAB = BN * 128;         // 64 columns of 128 keys
   static constexpr int TILE = SLAB * (D / 64);
-  // fewer where Q, P and the scales of int8 leave less room (int8 loads run ahead in registers)
-  static constexpr int SLOTS = D == 128 ? (INT8 ? (NR == 64 ? 4 : NR == 32 ? 5 : 6) : NR == 64 ? 5 : 6) : 10;
-  static constexpr int LAG = D == 128 ? 3 : 6;  // slots whose copies are in flight before the oldest is waited for
+  static constexpr int AHEAD = 3;               // tiles whose S may be computed before the oldest one's P is there
+  // int8: slots of codes on their way, in shared memory of the thread that will
+  // convert them (two groups of threads, RAWS slots each)
+  static constexpr int RAWS = INT8 ? 2 : 0, RAW = BN * D + BN * 8;
+  static constexpr int SLOTS = !INT8 ? (D == 128 ? (NR == 64 ? 5 : 6) : 10) : D == 128 ? (NR == 64 ? 3 : 4) : 8;
+  static constexpr int QBUFS = INT8 && D == 128 && NR > 16 ? 1 : 2;
   static constexpr int Q = NR * D * 2, P = NR * BN * 2;
-  static constexpr int OFF_Q = SLOTS * TILE;    // two pieces
-  static constexpr int OFF_P = OFF_Q + 2 * Q;   // two tiles
-  static constexpr int OFF_SCALE = OFF_P + 2 * P;
-  static constexpr int SCALES = 8;              // tiles whose K and V scales are kept
-  static constexpr int OFF_RED = OFF_SCALE + (INT8 ? SCALES * 2 * BN * 4 : 0);  // [4][NR] per warp, m, reference, factor [NR]
+  static constexpr int OFF_Q = SLOTS * TILE;
+  static constexpr int OFF_P = OFF_Q + QBUFS * Q;  // two tiles
+  static constexpr int OFF_RAW = OFF_P + 2 * P;
+  static constexpr int OFF_SCALE = OFF_RAW + 2 * RAWS * RAW;
+  // Tiles whose K and V scales are kept. K of tile t takes slot 2 t - AHEAD of
+  // the order above once the slot SLOTS before it is used up: then S of tile
+  // t - SLOTS / 2 is done, for which the softmax of the tile AHEAD before it is.
+  static constexpr int SCALES = INT8 ? AHEAD + (SLOTS + 1) / 2 : 0;
+  static constexpr int OFF_RED = OFF_SCALE + SCALES * 2 * BN * 4;  // per-warp results and per-row values of the softmax
   static constexpr int OFF_BARS = OFF_RED + 7 * NR * 4;
-  static constexpr int SMEM = OFF_BARS + 512;
+  static constexpr int SMEM = OFF_BARS + 320;
   static constexpr int LOADERS = INT8 ? 8 : 4;  // warps
-  static constexpr int THREADS = 128 + LOADERS * 32 + 32;
-  static constexpr int COLS = 4 * NR;           // TMEM: S, S, O, O
+  // warps: softmax 0-7, loaders, MMA, Q. int8: five warpgroups at 96 registers
+  static constexpr int THREADS = INT8 ? 640 : 448;
+  static constexpr int REG_SOFT = NR == 64 ? 112 : 96, REG_LOAD = NR == 64 ? 96 : 112, REG_MMA = 56;
+  static_assert(2 * REG_SOFT + 2 * REG_LOAD + REG_MMA <= 5 * 96, "registers");
+  static constexpr int COLS = (AHEAD + 2) * NR <= 128 ? 128 : (AHEAD + 2) * NR <= 256 ? 256 : 512;  // TMEM: S x AHEAD, O, O
   static_assert(SMEM <= 232448, "shared memory");
-  static_assert(LAG < SLOTS && SCALES >= (SLOTS + 3 + 1) / 2, "ring");
 };
 
 template <int SLOTS>
 struct Bars {
-  uint64_t full[SLOTS], empty[SLOTS], q_empty[2], s_full[2], p_full[2], pv_done[2], o_full[2], o_free[2];
+  uint64_t full[SLOTS], empty[SLOTS], q_full[2], q_empty[2], s_full[3], p_full[2], pv_done[2], o_full[2], o_free[2];
   uint32_t tmem;
   int acc;  // O already holds values that the piece's first product adds to
 };
 
-// ring index, within a piece of T tiles, of K and V of tile t
-__device__ __forceinline__ uint32_t k_at(int t) { return t == 0 ? 0u : 2u * (uint32_t)t - 1u; }
-__device__ __forceinline__ uint32_t v_at(int t, int T) { return t < T - 1 ? 2u * (uint32_t)t + 2u : 2u * (uint32_t)T - 1u; }
+// The slots of a piece of T tiles, in the order they are used: K of the first
+// AHEAD tiles, then K of tile t + AHEAD before V of tile t.
+template <int AHEAD>
+__device__ __forceinline__ uint32_t k_at(int t) { return (uint32_t)(t < AHEAD ? t : 2 * t - AHEAD); }
+template <int AHEAD>
+__device__ __forceinline__ uint32_t v_at(int t, int T) { return (uint32_t)(t + AHEAD < T ? 2 * t + AHEAD + 1 : T + t); }
 
 // 16-byte chunk c of row r of a tile, 128-byte swizzle
 __device__ __forceinline__ uint32_t chunk_off(int r, int c) {
@@ -80,6 +93,10 @@ __device__ __forceinline__ uint32_t chunk_off(int r, int c) {
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void cp4(uint32_t dst, const void *src, bool live) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
@@ -97,8 +114,26 @@ __device__ __forceinline__ void tmem_ld<16>(uint32_t taddr, float (&v)[16]) {
 #pragma unroll
   for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
 }
+template <>
+__device__ __forceinline__ void tmem_ld<8>(uint32_t taddr, float (&v)[8]) {
+  uint32_t r[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+#pragma unroll
+  for (int i = 0; i < 8; i++) v[i] = __uint_as_float(r[i]);
+}
 template <int N>
 __device__ __forceinline__ void tmem_st(uint32_t taddr, const float (&v)[N]);
+template <>
+__device__ __forceinline__ void tmem_st<32>(uint32_t taddr, const float (&v)[32]) { tmem_st32(taddr, v); }
+template <>
+__device__ __forceinline__ void tmem_st<8>(uint32_t taddr, const float (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(__float_as_uint(v[0])),
+               "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])), "r"(__float_as_uint(v[4])),
+               "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7]))
+               : "memory");
+}
 template <>
 __device__ __forceinline__ void tmem_st<16>(uint32_t taddr, const float (&v)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
@@ -115,181 +150,181 @@ __host__ __device__ constexpr uint32_t idesc(int N, bool a_mn_major, bool f16) {
   return (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10)) | ((a_mn_major ? 1u : 0u) << 15) | ((uint32_t)(N >> 3) << 17) | (8u << 24);
 }
 
-// ------------------------------------------------------------------ softmax: thread = key
+// Column of a query row, or of V, that 16-byte chunk c of a tile's row holds.
+// int8 rows of 128: a lane converts 16 codes, and its two chunks go to the same
+// place of the two slabs (neighbouring chunks of one row would meet in the
+// same banks), so the head dimension is permuted alike in Q, K, V and O.
+template <int D, bool INT8>
+__device__ __forceinline__ int chunk_of(int c) {
+  return INT8 && D == 128 ? (c & 7) * 2 + (c >> 3) : c;
+}
+
+// ------------------------------------------------------------------ softmax: thread = (key, half of the rows)
 template <int D, bool INT8, int NR>
 __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Bars<Cfg<D, INT8, NR>::SLOTS> &bars) {
   using C = Cfg<D, INT8, NR>;
-  constexpr int CH = NR < 32 ? NR : 32;  // columns in registers at a time
+  constexpr int N = NR / 2;  // rows of this warpgroup
   constexpr float SHIFT = INT8 ? 6.f : 0.f;  // P (and l) hold 2^SHIFT times the weights
-  const int key = threadIdx.x, warp = key >> 5, lane = key & 31;
+  const int wg = threadIdx.x >> 7, key = threadIdx.x & 127, warp = key >> 5, lane = key & 31;
+  const int row_base = wg * N;
   const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
-  float *red = reinterpret_cast<float *>(sm + C::OFF_RED), *m_s = red + 4 * NR, *ref_s = m_s + NR, *f_s = ref_s + NR;
+  // this warpgroup's: per-warp results [4][N], maxima, negated references, factors [N]
+  float *red = reinterpret_cast<float *>(sm + C::OFF_RED) + wg * 7 * N, *m_s = red + 4 * N, *ref_s = m_s + N, *f_s = ref_s + N;
   const float *scales = reinterpret_cast<const float *>(sm + C::OFF_SCALE);
+  const int bar = 1 + wg;
   Waiter<true> wait{a.err};
   Run run(a);
   Piece p{};
   uint32_t g = 0, pieces = 0, ring = 0;  // tiles and pieces so far; first ring index of the piece
   while (run.next(a, p)) {
-    const int T = max(0, p.te - p.tb), live = p.ntok * a.G;
+    const int T = max(0, p.te - p.tb), live = p.ntok * a.G - row_base;  // of this warpgroup's rows
     const int base = p.s.len - p.s.rows + p.tok0;  // last key that the first token sees
-    const uint32_t tO = bars.tmem + lane_off + (2 + (pieces & 1)) * NR;
-    float l[NR];
+    const uint32_t tO = bars.tmem + lane_off + (C::AHEAD + (pieces & 1)) * NR + row_base;
+    float l[N];
 #pragma unroll
-    for (int n = 0; n < NR; n++) l[n] = 0.f;
+    for (int n = 0; n < N; n++) l[n] = 0.f;
     for (int t = 0; t < T; t++, g++) {
       const int k0 = (p.tb + t) * BN, k = k0 + key;
-      const uint32_t tS = bars.tmem + lane_off + (g & 1) * NR;
-      wait(&bars.s_full[g & 1], (g >> 1) & 1);
+      const uint32_t tS = bars.tmem + lane_off + (g % C::AHEAD) * NR + row_base;
+      wait(&bars.s_full[g % C::AHEAD], (g / C::AHEAD) & 1);
       tc_fence_after();
-      // the first row that sees this thread's key
-      const int n_min = k >= p.s.len ? INT_MAX : a.sh.causal && k > base ? (k - base) * a.G : 0;
+      // the first of these rows that sees this thread's key
+      const int n_min = k >= p.s.len ? INT_MAX : (a.sh.causal && k > base ? (k - base) * a.G : 0) - row_base;
       const bool masked = k0 + BN > p.s.len || (a.sh.causal && k0 + BN - 1 > base);
-      float sc = a.scale_log2, add = 0.f, isv = 1.f;
+      float sc = a.scale_log2, add = SHIFT, isv = 1.f;
       if constexpr (INT8) {
         const float *tile = scales + g % C::SCALES * 2 * BN;
         sc *= tile[key];
         const float sv = tile[BN + key];
-        add = log2f(sv);
+        add += log2f(sv);
         isv = 1.f / sv;
       }
-      float s[CH];
-      // log2 of the weight, without the reference
-      auto load = [&](int c0) {
-        tmem_ld<CH>(tS + c0, s);
+      float x[N];  // log2 of what goes into P
+      auto load = [&](bool with_ref) {
+        tmem_ld<N>(tS, x);
         tmem_wait_ld();
 #pragma unroll
-        for (int n = 0; n < CH; n++) {
-          s[n] = INT8 ? fmaf(s[n], sc, add) : s[n] * sc;
-          if (masked) s[n] = c0 + n >= n_min ? s[n] : -INFINITY;
+        for (int n = 0; n < N; n += 4) {
+          const float4 r4 = with_ref ? *reinterpret_cast<const float4 *>(ref_s + n) : make_float4(0.f, 0.f, 0.f, 0.f);
+          const float ref[4] = {r4.x, r4.y, r4.z, r4.w};
+#pragma unroll
+          for (int e = 0; e < 4; e++) x[n + e] = fmaf(x[n + e], sc, INT8 ? add + ref[e] : ref[e]);
+        }
+        if (masked) {
+#pragma unroll
+          for (int n = 0; n < N; n++) x[n] = n >= n_min ? x[n] : -INFINITY;
         }
       };
-      bool over = t == 0;
+      bool over = true;
+      if (t > 0) {
+        load(true);
+        float top = x[0];
 #pragma unroll
-      for (int c0 = 0; c0 < NR; c0 += CH) {
-        load(c0);
-        if (t > 0) {
-#pragma unroll
-          for (int n = 0; n < CH; n += 4) {
-            const float4 m = *reinterpret_cast<const float4 *>(ref_s + c0 + n);
-            over |= s[n] > m.x + RESCALE_THRESHOLD || s[n + 1] > m.y + RESCALE_THRESHOLD || s[n + 2] > m.z + RESCALE_THRESHOLD ||
-                    s[n + 3] > m.w + RESCALE_THRESHOLD;
-          }
-        }
+        for (int n = 1; n < N; n++) top = fmaxf(top, x[n]);
+        over = bar_or(bar, 128, top > RESCALE_THRESHOLD + SHIFT);
       }
-      over = t == 0 || bar_or(1, 128, over);
       if (over) {
         // new references: the rows' maxima over this tile and before
-#pragma unroll 1
-        for (int c0 = 0; c0 < NR; c0 += CH) {
-          if (NR > CH) load(c0);
-          float top = -INFINITY;
+        load(false);
+        float top = -INFINITY;
 #pragma unroll
-          for (int n = 0; n < CH; n++) {
-            const float x = warp_max(s[n]);
-            top = lane == n ? x : top;
-          }
-          if (lane < CH) red[warp * NR + c0 + lane] = top;
+        for (int n = 0; n < N; n++) {
+          float y;
+          asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x[n]));
+          top = lane == n ? y : top;
         }
-        bar_sync(1, 128);
-        if (key < NR) {
+        if (lane < N) red[warp * N + lane] = top;
+        bar_sync(bar, 128);
+        if (key < N) {
           const float old = t == 0 ? -INFINITY : m_s[key];
-          const float m = fmaxf(fmaxf(fmaxf(red[key], red[NR + key]), fmaxf(red[2 * NR + key], red[3 * NR + key])), old);
+          const float m = fmaxf(fmaxf(fmaxf(red[key], red[N + key]), fmaxf(red[2 * N + key], red[3 * N + key])) - SHIFT, old);
           m_s[key] = m;
-          ref_s[key] = m == -INFINITY ? -1e30f : m;  // no score yet: any one passes it
+          ref_s[key] = m == -INFINITY ? 1e30f : -m;  // no score yet: any one passes it
           f_s[key] = m == old ? 1.f : ex2(old - m);
         }
-        bar_sync(1, 128);
+        bar_sync(bar, 128);
         if (t > 0) {
           wait(&bars.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
           tc_fence_after();
+          float o[N];
+          tmem_ld<N>(tO, o);
+          tmem_wait_ld();
 #pragma unroll
-          for (int c0 = 0; c0 < NR; c0 += 16) {
-            float o[16];
-            tmem_ld<16>(tO + c0, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int n = 0; n < 16; n++) {
-              const float f = f_s[c0 + n];
-              o[n] *= f;
-              l[c0 + n] *= f;
-            }
-            tmem_st<16>(tO + c0, o);
+          for (int n = 0; n < N; n++) {
+            const float f = f_s[n];
+            o[n] *= f;
+            l[n] *= f;
           }
+          tmem_st<N>(tO, o);
           tmem_wait_st();
         }
+        load(true);
       }
       // P of two tiles ago has been used
       uint8_t *P = sm + C::OFF_P + (g & 1) * C::P;
       if (g >= 2) wait(&bars.pv_done[g & 1], ((g - 2) >> 1) & 1);
-      uint8_t *prow = P + (key >> 6) * (NR * 128) + (key & 7) * 2;
-      const uint32_t chunk = (uint32_t)(key & 63) >> 3 << 4;
+      uint8_t *prow = P + (key >> 6) * (NR * 128) + row_base * 128 + (key & 7) * 2;
+      const uint32_t chunk = (uint32_t)(key & 63) >> 3;
 #pragma unroll
-      for (int c0 = 0; c0 < NR; c0 += CH) {
-        if (NR > CH) load(c0);
-#pragma unroll
-        for (int n = 0; n < CH; n += 4) {
-          const float4 ref = *reinterpret_cast<const float4 *>(ref_s + c0 + n);
-          const float m4[4] = {ref.x, ref.y, ref.z, ref.w};
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const int r = c0 + n + e;
-            const float w = ex2(INT8 ? s[n + e] - (m4[e] - SHIFT) : s[n + e] - m4[e]);
-            uint16_t bits;
-            if constexpr (INT8) {
-              // a row without this key: no product with a scale that is not finite
-              l[r] = !masked || r >= n_min ? fmaf(w, isv, l[r]) : l[r];
-              bits = __half_as_ushort(__float2half_rn(w));
-            } else {
-              l[r] += w;
-              bits = (uint16_t)pack_bf16(w, 0.f);
-            }
-            *reinterpret_cast<uint16_t *>(prow + r * 128 + (chunk ^ ((uint32_t)(r & 7) << 4))) = bits;
-          }
+      for (int n = 0; n < N; n += 2) {
+        const float w0 = ex2(x[n]), w1 = ex2(x[n + 1]);
+        uint32_t pair;
+        if constexpr (INT8) {
+          // a row without this key: no product with a scale that is not finite
+          l[n] = !masked || n >= n_min ? fmaf(w0, isv, l[n]) : l[n];
+          l[n + 1] = !masked || n + 1 >= n_min ? fmaf(w1, isv, l[n + 1]) : l[n + 1];
+          asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(pair) : "f"(w1), "f"(w0));
+        } else {
+          l[n] += w0;
+          l[n + 1] += w1;
+          pair = pack_bf16(w0, w1);
         }
+        *reinterpret_cast<uint16_t *>(prow + n * 128 + ((chunk ^ (n & 7)) << 4)) = (uint16_t)pair;
+        *reinterpret_cast<uint16_t *>(prow + (n + 1) * 128 + ((chunk ^ ((n + 1) & 7)) << 4)) = (uint16_t)(pair >> 16);
       }
       if constexpr (!INT8) {
         if (a.sh.causal && min(k0 + BN, p.s.len) - 1 > base) {
           // some row does not see all of this tile's keys
           const int valid = min(BN, p.s.len - k0);
-          const uint32_t vi = ring + v_at(t, T);
+          const uint32_t vi = ring + v_at<C::AHEAD>(t, T);
           wait(&bars.full[vi % C::SLOTS], (vi / C::SLOTS) & 1);
           uint8_t *V = sm + (vi % C::SLOTS) * C::TILE;
           uint32_t found = 0;
-          for (int c = key; c < valid * (D / 8); c += 128) {
+          for (int c = threadIdx.x; c < valid * (D / 8); c += 256) {
             const uint4 w = *reinterpret_cast<const uint4 *>(V + chunk_off(c / (D / 8), c % (D / 8)));
             found |= odd_bf16(w.x) | odd_bf16(w.y) | odd_bf16(w.z) | odd_bf16(w.w);
           }
           __syncwarp();
-          if (bar_or(1, 128, found != 0)) {
+          if (bar_or(3, 256, found != 0)) {
             // rare: lane d of O^T takes every non-finite value of column d of V
             if (t > 0) {
               wait(&bars.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
               tc_fence_after();
             } else {
-              float z[16];
+              float z[N];
 #pragma unroll
-              for (int n = 0; n < 16; n++) z[n] = 0.f;
-#pragma unroll
-              for (int c0 = 0; c0 < NR; c0 += 16) tmem_st<16>(tO + c0, z);
+              for (int n = 0; n < N; n++) z[n] = 0.f;
+              tmem_st<N>(tO, z);
               tmem_wait_st();
-              if (key == 0) bars.acc = 1;
+              if (threadIdx.x == 0) bars.acc = 1;
             }
             const int d = key % D;
             for (int j = 0; j < valid; j++) {
               const uint32_t bits = *reinterpret_cast<const uint16_t *>(V + chunk_off(j, d >> 3) + (d & 7) * 2);
               const bool odd = (bits & 0x7F80u) == 0x7F80u;
               if (!__any_sync(0xffffffffu, odd)) continue;
-              const int first = a.sh.causal && k0 + j > base ? (k0 + j - base) * a.G : 0;
-              for (int n = first; n < NR; n++) {
-                const uint32_t off = (uint32_t)(j >> 6) * (NR * 128) + (uint32_t)n * 128 + ((((uint32_t)(j & 63) >> 3) ^ ((uint32_t)n & 7)) << 4) + (j & 7) * 2;
+              const int first = max(0, (k0 + j > base ? (k0 + j - base) * a.G : 0) - row_base);
+              for (int n = first; n < N; n++) {
+                const uint32_t off = (uint32_t)(j >> 6) * (NR * 128) + (uint32_t)(row_base + n) * 128 +
+                                     ((((uint32_t)(j & 63) >> 3) ^ ((uint32_t)n & 7)) << 4) + (j & 7) * 2;
                 const float w = __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t *>(P + off) << 16);
                 const float o = tmem_ld1(tO + n);
                 tmem_st1(tO + n, odd ? fmaf(w, __uint_as_float(bits << 16), o) : o);
                 tmem_wait_st();
               }
             }
-            bar_sync(1, 128);
-            for (int c = key; c < valid * (D / 8); c += 128) {
+            bar_sync(3, 256);
+            for (int c = threadIdx.x; c < valid * (D / 8); c += 256) {
               uint4 *at = reinterpret_cast<uint4 *>(V + chunk_off(c / (D / 8), c % (D / 8)));
               *at = make_uint4(even_bf16(at->x), even_bf16(at->y), even_bf16(at->z), even_bf16(at->w));
             }
@@ -303,56 +338,53 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
     }
     // ---------------- end of the piece
     // l of every row: over the lanes, then the warps
-    bar_sync(1, 128);  // red is free
+    bar_sync(bar, 128);  // red is free
 #pragma unroll
-    for (int n = 0; n < NR; n++) {
-      const float x = warp_sum(l[n]);
-      if (lane == (n & 31)) red[warp * NR + n] = x;
+    for (int n = 0; n < N; n++) {
+      const float y = warp_sum(l[n]);
+      if (lane == n) red[warp * N + n] = y;
     }
-    bar_sync(1, 128);
-    if (key < NR) f_s[key] = red[key] + red[NR + key] + red[2 * NR + key] + red[3 * NR + key];
-    bar_sync(1, 128);
+    bar_sync(bar, 128);
     const bool whole = p.whole();
     float *part = a.ws + (size_t)(blockIdx.x * 2 + (p.tb > 0 ? 0 : 1)) * (kRowsItem * (D + 2));
     const size_t row0 = (size_t)(p.s.row0 + p.tok0) * a.Hq + (size_t)p.head * a.G;
-    if (key < live) {
-      const float m = T > 0 ? m_s[key] : -INFINITY, L = f_s[key];
-      if (!whole) {
-        __stcg(reinterpret_cast<float2 *>(part + (size_t)kRowsItem * D) + key, make_float2(m - SHIFT, L));
-      } else if (a.lse) {
-        a.lse[row0 + (size_t)(key / a.G) * a.Hq + key % a.G] = L == 0.f ? -INFINITY : (m - SHIFT + log2f(L)) * 0.69314718055994531f;
+    if (key < N) {
+      const float L = red[key] + red[N + key] + red[2 * N + key] + red[3 * N + key];
+      const float m = T > 0 ? m_s[key] : -INFINITY;
+      f_s[key] = whole ? (L == 0.f ? 0.f : 1.f / L) : 1.f;
+      const int r = row_base + key;
+      if (key < live) {
+        if (!whole) __stcg(reinterpret_cast<float2 *>(part + (size_t)kRowsItem * D) + r, make_float2(m - SHIFT, L));
+        else if (a.lse) a.lse[row0 + (size_t)(r / a.G) * a.Hq + r % a.G] = L == 0.f ? -INFINITY : (m - SHIFT + log2f(L)) * 0.69314718055994531f;
       }
     }
+    bar_sync(bar, 128);
     wait(&bars.o_full[pieces & 1], (pieces >> 1) & 1);
     tc_fence_after();
-#pragma unroll 1
-    for (int c0 = 0; c0 < NR && c0 < live; c0 += 16) {
-      float o[16];
+    if (live > 0) {
+      float o[N];
 #pragma unroll
-      for (int n = 0; n < 16; n++) o[n] = 0.f;
+      for (int n = 0; n < N; n++) o[n] = 0.f;
       if (T > 0) {
-        tmem_ld<16>(tO + c0, o);
+        tmem_ld<N>(tO, o);
         tmem_wait_ld();
       }
-      int tok = c0 / a.G, h = c0 - tok * a.G;
       if (key < D) {
+        const int d = chunk_of<D, INT8>(key >> 3) * 8 + (key & 7);
+        int tok = row_base / a.G, h = row_base - tok * a.G;
 #pragma unroll
-        for (int n = 0; n < 16; n++) {
-          if (c0 + n < live) {
-            if (whole) {
-              const float L = f_s[c0 + n];
-              a.out[(row0 + (size_t)tok * a.Hq + h) * D + key] = (uint16_t)pack_bf16(L == 0.f ? 0.f : o[n] * (1.f / L), 0.f);
-            } else {
-              __stcg(part + (size_t)(c0 + n) * D + key, o[n]);
+        for (int n = 0; n < N; n++) {
+          if (n < live) {
+            const float y = o[n] * f_s[n];
+            if (whole) a.out[(row0 + (size_t)tok * a.Hq + h) * D + d] = (uint16_t)pack_bf16(y, 0.f);
+            else __stcg(part + (size_t)(row_base + n) * D + d, y);
+            if (++h == a.G) {
+              h = 0;
+              tok++;
             }
-          }
-          if (++h == a.G) {
-            h = 0;
-            tok++;
           }
         }
       }
-      __syncwarp();
     }
     tc_fence_before();
     __syncwarp();
@@ -374,12 +406,14 @@ __device__ __forceinline__ void mma_role(const ChunkArgs &a, uint8_t *sm, Bars<C
   uint32_t g = 0, pieces = 0, ring = 0;
   while (run.next(a, p)) {
     const int T = max(0, p.te - p.tb);
-    const uint32_t pb = pieces & 1;
+    const uint32_t pb = pieces & 1, qb = pieces % C::QBUFS;
+    wait(&bars.q_full[qb], (pieces / C::QBUFS) & 1);
     auto issue_s = [&](int t) {
-      const uint32_t i = ring + k_at(t), slot = i % C::SLOTS, buf = (g + t) & 1;
+      const uint32_t i = ring + k_at<C::AHEAD>(t), slot = i % C::SLOTS, buf = (g + t) % C::AHEAD;
       wait(&bars.full[slot], (i / C::SLOTS) & 1);
+      fence_async_smem();  // the loaders' cp.async (bf16) are announced without one
       tc_fence_after();
-      const uint32_t k = s_kv + slot * C::TILE, q = s_q + pb * C::Q;
+      const uint32_t k = s_kv + slot * C::TILE, q = s_q + qb * C::Q;
 #pragma unroll
       for (int x = 0; x < D / 16; x++)
         umma_bf16(tmem + buf * NR, sw128_desc(k + (x >> 2) * C::SLAB + (x & 3) * 32, 16, 1024),
@@ -387,13 +421,14 @@ __device__ __forceinline__ void mma_role(const ChunkArgs &a, uint8_t *sm, Bars<C
       umma_commit(&bars.s_full[buf]);
       umma_commit(&bars.empty[slot]);
     };
-    if (T > 0) issue_s(0);
-    if (T > 1) issue_s(1);
+    for (int t = 0; t < C::AHEAD && t < T; t++) issue_s(t);
     if (pieces >= 2) wait(&bars.o_free[pb], ((pieces >> 1) - 1) & 1);
     for (int t = 0; t < T; t++) {
-      const uint32_t i = ring + v_at(t, T), slot = i % C::SLOTS, buf = (g + t) & 1;
+      const uint32_t i = ring + v_at<C::AHEAD>(t, T), slot = i % C::SLOTS, buf = (g + t) & 1;
       wait(&bars.p_full[buf], ((g + t) >> 1) & 1);
+      if (t + C::AHEAD < T) issue_s(t + C::AHEAD);  // S of tile t has been read
       wait(&bars.full[slot], (i / C::SLOTS) & 1);
+      fence_async_smem();
       tc_fence_after();
       uint32_t acc = t > 0 ? 1u : 0u;
       if (!INT8 && t == 0 && *(volatile int *)&bars.acc) {
@@ -404,13 +439,12 @@ __device__ __forceinline__ void mma_role(const ChunkArgs &a, uint8_t *sm, Bars<C
       // heads of 64: the second 64 rows of A are the first again, and are not read back
 #pragma unroll
       for (int x = 0; x < BN / 16; x++)
-        umma_bf16(tmem + (2 + pb) * NR, sw128_desc(v + x * 2048, D == 128 ? C::SLAB : 0, 1024),
+        umma_bf16(tmem + (C::AHEAD + pb) * NR, sw128_desc(v + x * 2048, D == 128 ? C::SLAB : 0, 1024),
                   sw128_desc(pp + (x >> 2) * (NR * 128) + (x & 3) * 32, 16, 1024), ID_O, x > 0 ? 1u : acc);
       umma_commit(&bars.empty[slot]);
       umma_commit(&bars.pv_done[buf]);
-      if (t + 2 < T) issue_s(t + 2);
     }
-    umma_commit(&bars.q_empty[pb]);
+    umma_commit(&bars.q_empty[qb]);
     umma_commit(&bars.o_full[pb]);
     g += (uint32_t)T;
     ring += 2 * (uint32_t)T;
@@ -428,45 +462,48 @@ __device__ __forceinline__ int group_row(const ChunkArgs &a, const Piece &p, con
   return (__ldg(table + b) * a.Hkv + p.head) * a.bs + (tok - b * a.bs);
 }
 
-// Query rows of the piece into its buffer (zeros behind the last), by `threads` threads
-template <int D, int NR>
-__device__ __forceinline__ void load_q(const ChunkArgs &a, const Piece &p, uint32_t dst, int tid, int threads) {
-  const int live = p.ntok * a.G;
-  for (int c = tid; c < NR * (D / 8); c += threads) {
-    const int n = c / (D / 8), ch = c % (D / 8), tok = n / a.G;
-    const uint16_t *src = a.q + ((size_t)(p.s.row0 + p.tok0 + (n < live ? tok : 0)) * a.Hq + (size_t)p.head * a.G + (n < live ? n - tok * a.G : 0)) * D + ch * 8;
-    cp16(dst + (ch >> 3) * (NR * 128) + n * 128 + (((ch & 7) ^ (n & 7)) << 4), src, n < live);
+// Q warp: the query rows of each piece (zeros behind the last)
+template <int D, bool INT8, int NR>
+__device__ __forceinline__ void q_role(const ChunkArgs &a, uint8_t *sm, Bars<Cfg<D, INT8, NR>::SLOTS> &bars) {
+  using C = Cfg<D, INT8, NR>;
+  const int lane = threadIdx.x & 31;
+  Waiter<true> wait{a.err};
+  Run run(a);
+  Piece p{};
+  uint32_t pieces = 0;
+  while (run.next(a, p)) {
+    const uint32_t qb = pieces % C::QBUFS;
+    if (pieces >= C::QBUFS) wait(&bars.q_empty[qb], (pieces / C::QBUFS - 1) & 1);
+    const uint32_t dst = smem_u32(sm + C::OFF_Q) + qb * C::Q;
+    const int live = p.ntok * a.G;
+#pragma unroll 4
+    for (int c = lane; c < NR * (D / 8); c += 32) {
+      const int n = c / (D / 8), ch = c % (D / 8), tok = n < live ? n / a.G : 0, h = n < live ? n - tok * a.G : 0;  // ch: chunk of the tile's row
+      const uint16_t *src = a.q + ((size_t)(p.s.row0 + p.tok0 + tok) * a.Hq + (size_t)p.head * a.G + h) * D + chunk_of<D, INT8>(ch) * 8;
+      cp16(dst + (ch >> 3) * (NR * 128) + n * 128 + (((ch & 7) ^ (n & 7)) << 4), src, n < live);
+    }
+    cp_wait_all();
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars.q_full[qb]);
+    pieces++;
   }
 }
 
 template <int D, int NR>
 __device__ __forceinline__ void load_role(const ChunkArgs &a, uint8_t *sm, Bars<Cfg<D, false, NR>::SLOTS> &bars) {
   using C = Cfg<D, false, NR>;
-  const int tid = threadIdx.x - 128, lane = threadIdx.x & 31;
-  const uint32_t s_kv = smem_u32(sm), s_q = smem_u32(sm + C::OFF_Q);
+  const int tid = threadIdx.x - 256;
+  const uint32_t s_kv = smem_u32(sm);
   constexpr int CHUNKS = D / 8, STEP = 128 / CHUNKS;  // rows per round of the 128 threads
   const int ch = tid % CHUNKS, r0 = tid / CHUNKS;
   Waiter<true> wait{a.err};
   Run run(a);
   Piece p{};
-  uint32_t idx = 0, told = 0, pieces = 0;  // copied and announced slots
-  auto tell = [&](uint32_t upto) {  // their copies have landed
-    fence_async_smem();
-    __syncwarp();
-    if (lane == 0)
-      for (uint32_t i = told; i < upto; i++) mbar_arrive(&bars.full[i % C::SLOTS]);
-    told = upto;
-  };
-  // waiting for the MMA side: the tiles that it may need first are announced first
-  auto wait_told = [&](uint64_t *bar, uint32_t ph) {
-    if (__all_sync(0xffffffffu, mbar_try(smem_u32(bar), ph))) return;
-    cp_wait<0>();
-    tell(idx);
-    wait(bar, ph);
-  };
+  uint32_t idx = 0;
   auto copy = [&](const void *pool, int rows, int tile) {
     const uint32_t slot = idx % C::SLOTS;
-    if (idx >= C::SLOTS) wait_told(&bars.empty[slot], (idx / C::SLOTS - 1) & 1);
+    if (idx >= C::SLOTS) wait(&bars.empty[slot], (idx / C::SLOTS - 1) & 1);
     const uint32_t dst = s_kv + slot * C::TILE;
     const int valid = p.s.len - tile * BN;
     const uint16_t *src = reinterpret_cast<const uint16_t *>(pool) + ch * 8;
@@ -476,116 +513,127 @@ __device__ __forceinline__ void load_role(const ChunkArgs &a, uint8_t *sm, Bars<
       const int row = __shfl_sync(0xffffffffu, rows, r >> 4) + (r & 15);
       cp16(dst + chunk_off(r, ch), src + (size_t)row * D, r < valid);
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    // arrives when this thread's copies have landed; the MMA thread, behind all
+    // of them, orders them before its reads (fence.proxy.async)
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&bars.full[slot])) : "memory");
     idx++;
-    if (idx - told > C::LAG) {
-      cp_wait<C::LAG>();
-      tell(idx - C::LAG);
-    }
   };
   while (run.next(a, p)) {
     const int32_t *table = a.tables + (size_t)p.s.slot * a.mbps;
     const int T = max(0, p.te - p.tb);
-    if (pieces >= 2) wait_told(&bars.q_empty[pieces & 1], ((pieces >> 1) - 1) & 1);
-    if (T > 0) {
-      load_q<D, NR>(a, p, s_q + (pieces & 1) * C::Q, tid, 128);  // lands with the first K
-      int next = group_row(a, p, table, p.tb);
-      copy(a.pool_k, next, p.tb);
-      for (int t = 0; t < T; t++) {
-        const int now = next;
-        if (t + 1 < T) {
-          next = group_row(a, p, table, p.tb + t + 1);
-          copy(a.pool_k, next, p.tb + t + 1);
-        }
-        copy(a.pool_v, now, p.tb + t);
+    // the pool rows of the last AHEAD tiles' K, for their V
+    int rows[C::AHEAD];
+#pragma unroll
+    for (int t = 0; t < C::AHEAD; t++)
+      if (t < T) {
+        rows[t] = group_row(a, p, table, p.tb + t);
+        copy(a.pool_k, rows[t], p.tb + t);
       }
+    for (int t = 0; t < T; t++) {
+      const int now = rows[0];
+#pragma unroll
+      for (int i = 0; i + 1 < C::AHEAD; i++) rows[i] = rows[i + 1];
+      if (t + C::AHEAD < T) {
+        rows[C::AHEAD - 1] = group_row(a, p, table, p.tb + t + C::AHEAD);
+        copy(a.pool_k, rows[C::AHEAD - 1], p.tb + t + C::AHEAD);
+      }
+      copy(a.pool_v, now, p.tb + t);
     }
-    pieces++;
   }
-  cp_wait<0>();
-  tell(idx);
+  cp_wait_all();
 }
 
-// int8: two groups of four warps take the slots in turn; the codes of a group's
-// next slot are on their way in registers while it converts this one's.
+// int8: two groups of four warps take the slots in turn. A thread copies the
+// codes that it will convert RAWS slots ahead into its own part of shared
+// memory (loads into registers would not survive the fences between them).
 template <int D, int NR>
 __device__ __forceinline__ void load_role_i8(const ChunkArgs &a, uint8_t *sm, Bars<Cfg<D, true, NR>::SLOTS> &bars) {
   using C = Cfg<D, true, NR>;
-  const int tid = (threadIdx.x - 128) & 127, lane = threadIdx.x & 31;
-  const uint32_t half = (threadIdx.x - 128) >> 7;
+  const int tid = threadIdx.x & 127, lane = threadIdx.x & 31;
+  const uint32_t half = (threadIdx.x - 256) >> 7;
   constexpr int CHUNKS = D / 16, STEP = 128 / CHUNKS, N = BN / STEP;
   const int ch = tid % CHUNKS, r0 = tid / CHUNKS;
   Waiter<true> wait{a.err};
-  // this group's next slot: j (of parity `half`) of the 2 T slots of piece p
-  Run run(a);
-  Piece p{};
-  uint32_t ring = 0, tiles = 0, pieces = 0, q_seen = 0;  // ring and tiles: before p; pieces: with p
-  int T = 0, j = 0;
-  auto next_piece = [&]() {
-    do {
-      ring += 2 * (uint32_t)T;
-      tiles += (uint32_t)T;
-      if (!run.next(a, p)) return false;
-      pieces++;
-      T = max(0, p.te - p.tb);
-    } while (T == 0);
-    j = (int)half;
-    return true;
+  // a slot of the group: slot j (of parity `half`) of the 2 T slots of piece p
+  struct Cursor {
+    Run run;
+    Piece p;
+    uint32_t ring, tiles;  // before p
+    int T, j;
+    bool more;
   };
-  uint4 w[N];
-  float scale_k = 1.f, scale_v = 1.f;
-  // slot j: K of tile 0, then K of the next tile and V in turn, V of the last at the end
-  auto tile_of = [&]() { return j == 0 ? 0 : j == 2 * T - 1 ? T - 1 : j & 1 ? (j + 1) / 2 : j / 2 - 1; };
-  auto is_v = [&]() { return j == 2 * T - 1 || (j > 0 && !(j & 1)); };
-  auto fetch = [&]() {
-    const bool v = is_v();
-    const int tile = p.tb + tile_of(), valid = p.s.len - tile * BN;
-    const int rows = group_row(a, p, a.tables + (size_t)p.s.slot * a.mbps, tile);
+  auto next_piece = [&](Cursor &c) {
+    do {
+      c.ring += 2 * (uint32_t)c.T;
+      c.tiles += (uint32_t)c.T;
+      if (!c.run.next(a, c.p)) {
+        c.more = false;
+        return;
+      }
+      c.T = max(0, c.p.te - c.p.tb);
+    } while (c.T == 0);
+    c.j = (int)half;
+  };
+  auto advance = [&](Cursor &c) {
+    c.j += 2;
+    if (c.j >= 2 * c.T) next_piece(c);
+  };
+  // the tile of slot j, and whether it is V (inverse of k_at and v_at)
+  auto what = [&](const Cursor &c, bool &v) {
+    const int first = min(C::AHEAD, c.T), pairs = 2 * (c.T - first), m = c.j - first;
+    v = m >= 0 && (m >= pairs || (m & 1));
+    return m < 0 ? c.j : m >= pairs ? m - pairs + (c.T - first) : (m & 1) ? m >> 1 : first + (m >> 1);
+  };
+  uint8_t *raw = sm + C::OFF_RAW + half * C::RAWS * C::RAW;
+  auto fetch = [&](const Cursor &c, uint32_t stage) {
+    bool v;
+    const int tile = c.p.tb + what(c, v), valid = c.p.s.len - tile * BN;
+    const int rows = group_row(a, c.p, a.tables + (size_t)c.p.s.slot * a.mbps, tile);
     const uint8_t *src = reinterpret_cast<const uint8_t *>(v ? a.pool_v : a.pool_k) + ch * 16;
+    const uint32_t dst = smem_u32(raw + stage * C::RAW) + tid * 16;
 #pragma unroll
     for (int i = 0; i < N; i++) {
       const int r = r0 + i * STEP;
       const int row = __shfl_sync(0xffffffffu, rows, r >> 4) + (r & 15);
-      w[i] = r < valid ? __ldcg(reinterpret_cast<const uint4 *>(src + (size_t)row * D)) : make_uint4(0u, 0u, 0u, 0u);
+      cp16(dst + i * 2048, src + (size_t)row * D, r < valid);
     }
     const int row = __shfl_sync(0xffffffffu, rows, tid >> 4) + (tid & 15);
-    if (!v) {  // both scales come with K; a key that does not exist has scale 1
-      scale_k = tid < valid ? __ldcg(a.sk + row) : 1.f;
-      scale_v = tid < valid ? __ldcg(a.sv + row) : 1.f;
+    if (!v) {  // both scales come with K
+      const uint32_t at = smem_u32(raw + stage * C::RAW + BN * D) + tid * 8;
+      cp4(at, a.sk + row, tid < valid);
+      cp4(at + 4, a.sv + row, tid < valid);
     }
   };
-  bool more = next_piece();
-  if (more) fetch();
-  while (more) {
-    const bool v = is_v(), first = j == 0;
-    const uint32_t idx = ring + (uint32_t)j, slot = idx % C::SLOTS, tile = tiles + (uint32_t)tile_of();
-    const float sk = scale_k, sv = scale_v;
-    if (first) {
-      // Q lands with the first K. Every piece's buffer is waited for in turn,
-      // also of pieces without tiles: a phase must not be missed.
-      for (; q_seen < pieces; q_seen++)
-        if (q_seen >= 2) wait(&bars.q_empty[q_seen & 1], ((q_seen >> 1) - 1) & 1);
-      load_q<D, NR>(a, p, smem_u32(sm + C::OFF_Q) + ((pieces - 1) & 1) * C::Q, tid, 128);
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    }
-    uint4 x[N];
+  Cursor f{Run(a), Piece{}, 0, 0, 0, 0, true}, c = f;
+  next_piece(f);
+  next_piece(c);
 #pragma unroll
-    for (int i = 0; i < N; i++) x[i] = w[i];
-    j += 2;
-    more = j < 2 * T || next_piece();
-    if (more) fetch();
+  for (int i = 0; i < C::RAWS; i++) {
+    if (f.more) {
+      fetch(f, i);
+      advance(f);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  for (uint32_t n = 0; c.more; n++) {
+    bool v;
+    const int tile = what(c, v), valid = c.p.s.len - (c.p.tb + tile) * BN;
+    const uint32_t idx = c.ring + (uint32_t)c.j, slot = idx % C::SLOTS, stage = n % C::RAWS;
+    cp_wait<C::RAWS - 1>();
     if (idx >= C::SLOTS) wait(&bars.empty[slot], (idx / C::SLOTS - 1) & 1);
+    const uint8_t *src = raw + stage * C::RAW;
     if (!v) {
-      // read before tile + 2's K is used up, and this K is at most SLOTS behind
-      float *at = reinterpret_cast<float *>(sm + C::OFF_SCALE) + tile % C::SCALES * 2 * BN + tid;
-      at[0] = sk;
-      at[BN] = sv;
+      float *at = reinterpret_cast<float *>(sm + C::OFF_SCALE) + (c.tiles + tile) % C::SCALES * 2 * BN + tid;
+      const float2 f2 = *reinterpret_cast<const float2 *>(src + BN * D + tid * 8);
+      at[0] = tid < valid ? f2.x : 1.f;
+      at[BN] = tid < valid ? f2.y : 1.f;
     }
     uint8_t *dst = sm + slot * C::TILE;
 #pragma unroll
     for (int i = 0; i < N; i++) {
       const int r = r0 + i * STEP;
-      const uint32_t in[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+      const uint4 x = *reinterpret_cast<const uint4 *>(src + i * 2048 + tid * 16);
+      const uint32_t in[4] = {x.x, x.y, x.z, x.w};
       uint32_t o[8];
 #pragma unroll
       for (int e = 0; e < 8; e++) {
@@ -601,21 +649,29 @@ __device__ __forceinline__ void load_role_i8(const ChunkArgs &a, uint8_t *sm, Ba
           asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(o[e]) : "r"(h & 0xFF7FFF7Fu), "r"(h & 0xFF80FF80u));
         }
       }
-      *reinterpret_cast<uint4 *>(dst + chunk_off(r, 2 * ch)) = make_uint4(o[0], o[1], o[2], o[3]);
-      *reinterpret_cast<uint4 *>(dst + chunk_off(r, 2 * ch + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
+      // columns 16 ch .. + 7 and .. + 15 (chunk_of)
+      *reinterpret_cast<uint4 *>(dst + chunk_off(r, D == 128 ? ch : 2 * ch)) = make_uint4(o[0], o[1], o[2], o[3]);
+      *reinterpret_cast<uint4 *>(dst + chunk_off(r, D == 128 ? ch + 8 : 2 * ch + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
     }
-    if (first) cp_wait<0>();
+    // the stage's codes are in registers, or used: the next may come
+    if (f.more) {
+      fetch(f, stage);
+      advance(f);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
     fence_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(&bars.full[slot]);
+    advance(c);
   }
+  cp_wait_all();
 }
 
 template <int D, bool INT8, int NR>
 __global__ void __launch_bounds__(Cfg<D, INT8, NR>::THREADS, 1) chunk_few_kernel(const __grid_constant__ ChunkArgs a) {
   using C = Cfg<D, INT8, NR>;
   using B = Bars<C::SLOTS>;
-  static_assert(sizeof(B) <= 512, "barriers");
+  static_assert(sizeof(B) <= 320, "barriers");
   extern __shared__ __align__(1024) uint8_t sm[];
   B &bars = *reinterpret_cast<B *>(sm + C::OFF_BARS);
   const int warp = threadIdx.x >> 5;
@@ -626,17 +682,18 @@ __global__ void __launch_bounds__(Cfg<D, INT8, NR>::THREADS, 1) chunk_few_kernel
   }
   if (threadIdx.x == 32) {
     for (int i = 0; i < C::SLOTS; i++) {
-      mbar_init(&bars.full[i], 4);
+      mbar_init(&bars.full[i], INT8 ? 4 : 128);
       mbar_init(&bars.empty[i], 1);
     }
     for (int i = 0; i < 2; i++) {
+      mbar_init(&bars.q_full[i], 1);
       mbar_init(&bars.q_empty[i], 1);
-      mbar_init(&bars.s_full[i], 1);
-      mbar_init(&bars.p_full[i], 4);
+      mbar_init(&bars.p_full[i], 8);
       mbar_init(&bars.pv_done[i], 1);
       mbar_init(&bars.o_full[i], 1);
-      mbar_init(&bars.o_free[i], 4);
+      mbar_init(&bars.o_free[i], 8);
     }
+    for (int i = 0; i < C::AHEAD; i++) mbar_init(&bars.s_full[i], 1);
     bars.acc = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -644,14 +701,24 @@ __global__ void __launch_bounds__(Cfg<D, INT8, NR>::THREADS, 1) chunk_few_kernel
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars.tmem;
-  if (warp < 4) {
+  if (warp < 8) {
+    if constexpr (INT8 && C::REG_SOFT > 96) regs_inc<C::REG_SOFT>();
     softmax_role<D, INT8, NR>(a, sm, bars);
-  } else if (warp < 4 + C::LOADERS) {
-    if constexpr (INT8) load_role_i8<D, NR>(a, sm, bars);
-    else load_role<D, NR>(a, sm, bars);
+  } else if (warp < 8 + C::LOADERS) {
+    if constexpr (INT8) {
+      if constexpr (C::REG_LOAD > 96) regs_inc<C::REG_LOAD>();
+      load_role_i8<D, NR>(a, sm, bars);
+    } else {
+      load_role<D, NR>(a, sm, bars);
+    }
   } else {
-    if ((threadIdx.x & 31) == 0) mma_role<D, INT8, NR>(a, sm, bars);
-    __syncwarp();
+    if constexpr (INT8) regs_dec<C::REG_MMA>();
+    if (warp == 8 + C::LOADERS) {
+      if ((threadIdx.x & 31) == 0) mma_role<D, INT8, NR>(a, sm, bars);
+      __syncwarp();
+    } else if (warp == 9 + C::LOADERS) {
+      q_role<D, INT8, NR>(a, sm, bars);
+    }
   }
   tc_fence_before();
   __syncthreads();
