@@ -62,10 +62,10 @@ struct Cfg {
   static constexpr int OFF_RED = OFF_SCALE + SCALES * 2 * BN * 4;  // per-warp results and per-row values of the softmax
   static constexpr int OFF_BARS = OFF_RED + 7 * NR * 4;
   static constexpr int SMEM = OFF_BARS + 320;
-  static constexpr int LOADERS = INT8 ? 8 : 4;  // warps
-  // warps: softmax 0-7, loaders, MMA, Q. int8: five warpgroups at 96 registers
-  static constexpr int THREADS = INT8 ? 640 : 448;
-  static constexpr int REG_SOFT = NR == 64 ? 112 : 96, REG_LOAD = NR == 64 ? 96 : 112, REG_MMA = 56;
+  static constexpr int LOADERS = 8;  // warps
+  // warps: softmax 0-7, loaders, MMA, Q: five warpgroups at 96 registers
+  static constexpr int THREADS = 640;
+  static constexpr int REG_SOFT = NR == 64 ? (INT8 ? 112 : 128) : 96, REG_LOAD = INT8 ? (NR == 64 ? 96 : 112) : (NR == 64 ? 80 : 96), REG_MMA = 56;
   static_assert(2 * REG_SOFT + 2 * REG_LOAD + REG_MMA <= 5 * 96, "registers");
   static constexpr int COLS = (AHEAD + 2) * NR <= 128 ? 128 : (AHEAD + 2) * NR <= 256 ? 256 : 512;  // TMEM: S x AHEAD, O, O
   static_assert(SMEM <= 232448, "shared memory");
@@ -490,23 +490,65 @@ __device__ __forceinline__ void q_role(const ChunkArgs &a, uint8_t *sm, Bars<Cfg
   }
 }
 
+// The slots of one of the two loader groups (four warps each, which take the
+// ring's slots in turn): slot j, of the group's parity, of the 2 T slots of a
+// piece.
+template <int AHEAD>
+struct Cursor {
+  Run run;
+  Piece p;
+  uint32_t ring, tiles, half;  // slots and tiles before p; the group
+  int T, j;
+  bool more;
+  __device__ __forceinline__ Cursor(const ChunkArgs &a, uint32_t group)
+      : run(a), p{}, ring(0), tiles(0), half(group), T(0), j(0), more(true) { piece(a); }
+  __device__ __forceinline__ void piece(const ChunkArgs &a) {
+    do {
+      ring += 2 * (uint32_t)T;
+      tiles += (uint32_t)T;
+      if (!run.next(a, p)) {
+        more = false;
+        return;
+      }
+      T = max(0, p.te - p.tb);
+    } while (T == 0);
+    j = (int)half;
+  }
+  __device__ __forceinline__ void advance(const ChunkArgs &a) {
+    j += 2;
+    if (j >= 2 * T) piece(a);
+  }
+  // the tile of slot j, and whether it is V (inverse of k_at and v_at)
+  __device__ __forceinline__ int tile(bool &v) const {
+    const int first = min(AHEAD, T), pairs = 2 * (T - first), m = j - first;
+    v = m >= 0 && (m >= pairs || (m & 1));
+    return m < 0 ? j : m >= pairs ? m - pairs + (T - first) : (m & 1) ? m >> 1 : first + (m >> 1);
+  }
+  __device__ __forceinline__ int rows(const ChunkArgs &a) const {
+    bool v;
+    return more ? group_row(a, p, a.tables + (size_t)p.s.slot * a.mbps, p.tb + tile(v)) : 0;
+  }
+};
+
 template <int D, int NR>
 __device__ __forceinline__ void load_role(const ChunkArgs &a, uint8_t *sm, Bars<Cfg<D, false, NR>::SLOTS> &bars) {
   using C = Cfg<D, false, NR>;
-  const int tid = threadIdx.x - 256;
+  const int tid = threadIdx.x & 127;
   const uint32_t s_kv = smem_u32(sm);
   constexpr int CHUNKS = D / 8, STEP = 128 / CHUNKS;  // rows per round of the 128 threads
   const int ch = tid % CHUNKS, r0 = tid / CHUNKS;
   Waiter<true> wait{a.err};
-  Run run(a);
-  Piece p{};
-  uint32_t idx = 0;
-  auto copy = [&](const void *pool, int rows, int tile) {
-    const uint32_t slot = idx % C::SLOTS;
+  Cursor<C::AHEAD> c(a, (threadIdx.x - 256) >> 7);
+  int next = c.rows(a);
+  while (c.more) {
+    bool v;
+    const int tile = c.p.tb + c.tile(v), valid = c.p.s.len - tile * BN, rows = next;
+    const uint32_t idx = c.ring + (uint32_t)c.j, slot = idx % C::SLOTS;
+    c.advance(a);
+    next = c.rows(a);  // the table's answer comes while this slot is copied
     if (idx >= C::SLOTS) wait(&bars.empty[slot], (idx / C::SLOTS - 1) & 1);
     const uint32_t dst = s_kv + slot * C::TILE;
-    const int valid = p.s.len - tile * BN;
-    const uint16_t *src = reinterpret_cast<const uint16_t *>(pool) + ch * 8;
+    const uint16_t *src = reinterpret_cast<const uint16_t *>(v ? a.pool_v : a.pool_k) + ch * 8;
 #pragma unroll
     for (int i = 0; i < BN / STEP; i++) {
       const int r = r0 + i * STEP;
@@ -516,36 +558,13 @@ __device__ __forceinline__ void load_role(const ChunkArgs &a, uint8_t *sm, Bars<
     // arrives when this thread's copies have landed; the MMA thread, behind all
     // of them, orders them before its reads (fence.proxy.async)
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&bars.full[slot])) : "memory");
-    idx++;
-  };
-  while (run.next(a, p)) {
-    const int32_t *table = a.tables + (size_t)p.s.slot * a.mbps;
-    const int T = max(0, p.te - p.tb);
-    // the pool rows of the last AHEAD tiles' K, for their V
-    int rows[C::AHEAD];
-#pragma unroll
-    for (int t = 0; t < C::AHEAD; t++)
-      if (t < T) {
-        rows[t] = group_row(a, p, table, p.tb + t);
-        copy(a.pool_k, rows[t], p.tb + t);
-      }
-    for (int t = 0; t < T; t++) {
-      const int now = rows[0];
-#pragma unroll
-      for (int i = 0; i + 1 < C::AHEAD; i++) rows[i] = rows[i + 1];
-      if (t + C::AHEAD < T) {
-        rows[C::AHEAD - 1] = group_row(a, p, table, p.tb + t + C::AHEAD);
-        copy(a.pool_k, rows[C::AHEAD - 1], p.tb + t + C::AHEAD);
-      }
-      copy(a.pool_v, now, p.tb + t);
-    }
   }
   cp_wait_all();
 }
 
-// int8: two groups of four warps take the slots in turn. A thread copies the
-// codes that it will convert RAWS slots ahead into its own part of shared
-// memory (loads into registers would not survive the fences between them).
+// int8: a thread copies the codes that it will convert RAWS slots ahead into
+// its own part of shared memory (loads into registers would not survive the
+// fences between them).
 template <int D, int NR>
 __device__ __forceinline__ void load_role_i8(const ChunkArgs &a, uint8_t *sm, Bars<Cfg<D, true, NR>::SLOTS> &bars) {
   using C = Cfg<D, true, NR>;
@@ -554,77 +573,47 @@ __device__ __forceinline__ void load_role_i8(const ChunkArgs &a, uint8_t *sm, Ba
   constexpr int CHUNKS = D / 16, STEP = 128 / CHUNKS, N = BN / STEP;
   const int ch = tid % CHUNKS, r0 = tid / CHUNKS;
   Waiter<true> wait{a.err};
-  // a slot of the group: slot j (of parity `half`) of the 2 T slots of piece p
-  struct Cursor {
-    Run run;
-    Piece p;
-    uint32_t ring, tiles;  // before p
-    int T, j;
-    bool more;
-  };
-  auto next_piece = [&](Cursor &c) {
-    do {
-      c.ring += 2 * (uint32_t)c.T;
-      c.tiles += (uint32_t)c.T;
-      if (!c.run.next(a, c.p)) {
-        c.more = false;
-        return;
-      }
-      c.T = max(0, c.p.te - c.p.tb);
-    } while (c.T == 0);
-    c.j = (int)half;
-  };
-  auto advance = [&](Cursor &c) {
-    c.j += 2;
-    if (c.j >= 2 * c.T) next_piece(c);
-  };
-  // the tile of slot j, and whether it is V (inverse of k_at and v_at)
-  auto what = [&](const Cursor &c, bool &v) {
-    const int first = min(C::AHEAD, c.T), pairs = 2 * (c.T - first), m = c.j - first;
-    v = m >= 0 && (m >= pairs || (m & 1));
-    return m < 0 ? c.j : m >= pairs ? m - pairs + (c.T - first) : (m & 1) ? m >> 1 : first + (m >> 1);
-  };
   uint8_t *raw = sm + C::OFF_RAW + half * C::RAWS * C::RAW;
-  auto fetch = [&](const Cursor &c, uint32_t stage) {
-    bool v;
-    const int tile = c.p.tb + what(c, v), valid = c.p.s.len - tile * BN;
-    const int rows = group_row(a, c.p, a.tables + (size_t)c.p.s.slot * a.mbps, tile);
-    const uint8_t *src = reinterpret_cast<const uint8_t *>(v ? a.pool_v : a.pool_k) + ch * 16;
-    const uint32_t dst = smem_u32(raw + stage * C::RAW) + tid * 16;
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-      const int r = r0 + i * STEP;
-      const int row = __shfl_sync(0xffffffffu, rows, r >> 4) + (r & 15);
-      cp16(dst + i * 2048, src + (size_t)row * D, r < valid);
-    }
-    const int row = __shfl_sync(0xffffffffu, rows, tid >> 4) + (tid & 15);
-    if (!v) {  // both scales come with K
-      const uint32_t at = smem_u32(raw + stage * C::RAW + BN * D) + tid * 8;
-      cp4(at, a.sk + row, tid < valid);
-      cp4(at + 4, a.sv + row, tid < valid);
-    }
-  };
-  Cursor f{Run(a), Piece{}, 0, 0, 0, 0, true}, c = f;
-  next_piece(f);
-  next_piece(c);
-#pragma unroll
-  for (int i = 0; i < C::RAWS; i++) {
+  Cursor<C::AHEAD> f(a, half), c(a, half);  // what is fetched, what is converted
+  int next = f.rows(a);
+  auto fetch = [&](uint32_t stage) {
     if (f.more) {
-      fetch(f, i);
-      advance(f);
+      bool v;
+      const int tile = f.p.tb + f.tile(v), valid = f.p.s.len - tile * BN, rows = next;
+      f.advance(a);
+      next = f.rows(a);
+      const uint8_t *src = reinterpret_cast<const uint8_t *>(v ? a.pool_v : a.pool_k) + ch * 16;
+      const uint32_t dst = smem_u32(raw + stage * C::RAW) + tid * 16;
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        const int r = r0 + i * STEP;
+        const int row = __shfl_sync(0xffffffffu, rows, r >> 4) + (r & 15);
+        cp16(dst + i * 2048, src + (size_t)row * D, r < valid);
+      }
+      const int row = __shfl_sync(0xffffffffu, rows, tid >> 4) + (tid & 15);
+      if (!v) {  // both scales come with K
+        const uint32_t at = smem_u32(raw + stage * C::RAW + BN * D) + tid * 8;
+        cp4(at, a.sk + row, tid < valid);
+        cp4(at + 4, a.sv + row, tid < valid);
+      }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
-  }
+  };
+#pragma unroll
+  for (int i = 0; i < C::RAWS; i++) fetch(i);
   for (uint32_t n = 0; c.more; n++) {
     bool v;
-    const int tile = what(c, v), valid = c.p.s.len - (c.p.tb + tile) * BN;
+    const int tile = c.tile(v), valid = c.p.s.len - (c.p.tb + tile) * BN;
     const uint32_t idx = c.ring + (uint32_t)c.j, slot = idx % C::SLOTS, stage = n % C::RAWS;
     cp_wait<C::RAWS - 1>();
-    if (idx >= C::SLOTS) wait(&bars.empty[slot], (idx / C::SLOTS - 1) & 1);
     const uint8_t *src = raw + stage * C::RAW;
+    uint4 x[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] = *reinterpret_cast<const uint4 *>(src + i * 2048 + tid * 16);
+    const float2 f2 = *reinterpret_cast<const float2 *>(src + BN * D + tid * 8);
+    if (idx >= C::SLOTS) wait(&bars.empty[slot], (idx / C::SLOTS - 1) & 1);
     if (!v) {
       float *at = reinterpret_cast<float *>(sm + C::OFF_SCALE) + (c.tiles + tile) % C::SCALES * 2 * BN + tid;
-      const float2 f2 = *reinterpret_cast<const float2 *>(src + BN * D + tid * 8);
       at[0] = tid < valid ? f2.x : 1.f;
       at[BN] = tid < valid ? f2.y : 1.f;
     }
@@ -632,8 +621,7 @@ __device__ __forceinline__ void load_role_i8(const ChunkArgs &a, uint8_t *sm, Ba
 #pragma unroll
     for (int i = 0; i < N; i++) {
       const int r = r0 + i * STEP;
-      const uint4 x = *reinterpret_cast<const uint4 *>(src + i * 2048 + tid * 16);
-      const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+      const uint32_t in[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
       uint32_t o[8];
 #pragma unroll
       for (int e = 0; e < 8; e++) {
@@ -653,16 +641,11 @@ __device__ __forceinline__ void load_role_i8(const ChunkArgs &a, uint8_t *sm, Ba
       *reinterpret_cast<uint4 *>(dst + chunk_off(r, D == 128 ? ch : 2 * ch)) = make_uint4(o[0], o[1], o[2], o[3]);
       *reinterpret_cast<uint4 *>(dst + chunk_off(r, D == 128 ? ch + 8 : 2 * ch + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
     }
-    // the stage's codes are in registers, or used: the next may come
-    if (f.more) {
-      fetch(f, stage);
-      advance(f);
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
     fence_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(&bars.full[slot]);
-    advance(c);
+    fetch(stage);  // its codes have been used
+    c.advance(a);
   }
   cp_wait_all();
 }
@@ -702,17 +685,15 @@ __global__ void __launch_bounds__(Cfg<D, INT8, NR>::THREADS, 1) chunk_few_kernel
   tc_fence_after();
   const uint32_t tmem = bars.tmem;
   if (warp < 8) {
-    if constexpr (INT8 && C::REG_SOFT > 96) regs_inc<C::REG_SOFT>();
+    if constexpr (C::REG_SOFT > 96) regs_inc<C::REG_SOFT>();
     softmax_role<D, INT8, NR>(a, sm, bars);
   } else if (warp < 8 + C::LOADERS) {
-    if constexpr (INT8) {
-      if constexpr (C::REG_LOAD > 96) regs_inc<C::REG_LOAD>();
-      load_role_i8<D, NR>(a, sm, bars);
-    } else {
-      load_role<D, NR>(a, sm, bars);
-    }
+    if constexpr (C::REG_LOAD > 96) regs_inc<C::REG_LOAD>();
+    if constexpr (C::REG_LOAD < 96) regs_dec<C::REG_LOAD>();
+    if constexpr (INT8) load_role_i8<D, NR>(a, sm, bars);
+    else load_role<D, NR>(a, sm, bars);
   } else {
-    if constexpr (INT8) regs_dec<C::REG_MMA>();
+    regs_dec<C::REG_MMA>();
     if (warp == 8 + C::LOADERS) {
       if ((threadIdx.x & 31) == 0) mma_role<D, INT8, NR>(a, sm, bars);
       __syncwarp();
