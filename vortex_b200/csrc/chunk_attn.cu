@@ -352,13 +352,16 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
   }
 }
 
-// ------------------------------------------------------------------ MMA thread
+// ------------------------------------------------------------------ MMA warp
 template <int D, bool INT8, class B>
 __device__ __forceinline__ void mma_role(const ChunkArgs &a, uint8_t *sm, B &bars) {
   using C = Cfg<D, INT8>;
   constexpr uint32_t ID_QK = idesc_bf16(BM, BN, false), ID_PV = idesc_bf16(BM, D, true);
-  const uint32_t s_q = smem_u32(sm), s_kv = smem_u32(sm + C::OFF_KV), tmem = bars.tmem;
-  Waiter<false> wait{a.err};
+  constexpr uint64_t KMAJOR = desc_base(16, 1024), VMAJOR = desc_base(C::SLAB, 1024);
+  const uint32_t s_q = smem_u32(sm) >> 4, s_kv = smem_u32(sm + C::OFF_KV) >> 4;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, bars.tmem, 0);
+  const uint32_t one = elect_one();
+  Waiter<true> wait{a.err};
   Run run(a);
   Piece p{};
   uint32_t ring = 0, pieces = 0, psteps[2] = {0, 0};
@@ -374,14 +377,14 @@ __device__ __forceinline__ void mma_role(const ChunkArgs &a, uint8_t *sm, B &bar
       const uint32_t kv = ring + 2 * (uint32_t)(p.tile(st, i) - p.tb), slot = kv % C::SLOTS;
       wait(&bars.full[slot], (kv / C::SLOTS) & 1);
       tc_fence_after();
-      const uint32_t q = s_q + (p.both ? st : 0) * C::TILE, k = s_kv + slot * C::TILE;
+      const uint64_t q = KMAJOR + (s_q + (p.both ? st : 0) * (C::TILE >> 4)), k = KMAJOR + (s_kv + slot * (C::TILE >> 4));
 #pragma unroll
       for (int x = 0; x < D / 16; x++) {
-        const uint32_t off = (x >> 2) * C::SLAB + (x & 3) * 32;
-        umma_bf16(tmem + st * 128, sw128_desc(q + off, 16, 1024), sw128_desc(k + off, 16, 1024), ID_QK, x > 0 ? 1u : 0u);
+        const uint32_t off = ((x >> 2) * C::SLAB + (x & 3) * 32) >> 4;
+        mma_ss(one, tmem + st * 128, q + off, k + off, ID_QK, x > 0 ? 1u : 0u);
       }
-      umma_commit(&bars.s_full[st]);
-      if (!p.both || st == 1) umma_commit(&bars.empty[slot]);  // stream 1 is the last to use a shared tile
+      mma_commit(one, &bars.s_full[st]);
+      if (!p.both || st == 1) mma_commit(one, &bars.empty[slot]);  // stream 1 is the last to use a shared tile
     };
     auto issue_pv = [&](int st, int i) {
       const int t = p.tile(st, i);
@@ -390,16 +393,23 @@ __device__ __forceinline__ void mma_role(const ChunkArgs &a, uint8_t *sm, B &bar
       wait(&bars.p_full[st], psteps[st]++ & 1);
       wait(&bars.full[slot], (kv / C::SLOTS) & 1);
       tc_fence_after();
-      const uint32_t v = s_kv + slot * C::TILE;
+      const uint64_t v = VMAJOR + (s_kv + slot * (C::TILE >> 4));
       uint32_t acc = i > 0 ? 1u : 0u;
-      if (!INT8 && i == 0 && *(volatile int *)&bars.acc[st]) {
+      if (!INT8 && i == 0 && __shfl_sync(0xffffffffu, *(volatile int *)&bars.acc[st], 0)) {
         acc = 1u;
+        __syncwarp();
         *(volatile int *)&bars.acc[st] = 0;
       }
       const int k16 = (min(BN, p.s.len - t * BN) + 15) / 16;
-      for (int x = 0; x < k16; x++)
-        umma_bf16_ts(tmem + 256 + st * 128, tmem + st * 128 + x * 8, sw128_desc(v + x * 2048, C::SLAB, 1024), ID_PV, x > 0 ? 1u : acc);
-      if (!p.both || st == 1) umma_commit(&bars.empty[slot]);
+      if (k16 == BN / 16) {
+#pragma unroll
+        for (int x = 0; x < BN / 16; x++)
+          mma_ts(one, tmem + 256 + st * 128, tmem + st * 128 + x * 8, v + (x * 2048 >> 4), ID_PV, x > 0 ? 1u : acc);
+      } else {
+        for (int x = 0; x < k16; x++)
+          mma_ts(one, tmem + 256 + st * 128, tmem + st * 128 + x * 8, v + (x * 2048 >> 4), ID_PV, x > 0 ? 1u : acc);
+      }
+      if (!p.both || st == 1) mma_commit(one, &bars.empty[slot]);
     };
     if (p.n0 > 0) issue_s(0, 0);
     if (p.n1 > 0) issue_s(1, 0);
@@ -411,13 +421,13 @@ __device__ __forceinline__ void mma_role(const ChunkArgs &a, uint8_t *sm, B &bar
         if (i < n) {
           issue_pv(st, i);
           if (i + 1 < n) issue_s(st, i + 1);
-          else umma_commit(&bars.o_full[st]);
+          else mma_commit(one, &bars.o_full[st]);
         }
       }
-    umma_commit(&bars.q_empty);
+    mma_commit(one, &bars.q_empty);
     own_o();
-    if (p.n0 == 0) umma_commit(&bars.o_full[0]);
-    if (p.n1 == 0) umma_commit(&bars.o_full[1]);
+    if (p.n0 == 0) mma_commit(one, &bars.o_full[0]);
+    if (p.n1 == 0) mma_commit(one, &bars.o_full[1]);
     ring += 2 * (uint32_t)tiles;
     pieces++;
   }
@@ -592,8 +602,7 @@ __global__ void __launch_bounds__(Cfg<D, INT8>::THREADS, 1)
   } else if (warp < 12) {
     regs_dec<C::REG_PROD>();
     if (warp == 8) {
-      if ((threadIdx.x & 31) == 0) mma_role<D, INT8>(a, sm, bars);
-      __syncwarp();
+      mma_role<D, INT8>(a, sm, bars);
     } else if (warp == 9) {
       tma_role<D, INT8>(&tq, &tk, &tv, a, sm, bars);
     }

@@ -145,6 +145,41 @@ __device__ __forceinline__ void tmem_st1(uint32_t taddr, float v) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(__float_as_uint(v)) : "memory");
 }
 
+// MMA issue. A whole warp runs the issuing loop and one elected lane's
+// instructions take effect: the operands are then uniform over the warp and
+// stay in uniform registers. (One lane alone in the loop took 80 cycles per
+// instruction to move them there.)
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(r));
+  return r;
+}
+// 128-byte-swizzled matrix descriptor without its address; adding (address >> 4) gives the whole
+__device__ __forceinline__ constexpr uint64_t desc_base(uint32_t lbo, uint32_t sbo) {
+  return ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void mma_ss(uint32_t one, uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(adesc), "l"(bdesc), "r"(id), "r"(acc), "r"(one)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t one, uint32_t d, uint32_t a, uint64_t bdesc, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(bdesc), "r"(id), "r"(acc), "r"(one)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t one, uint64_t *bar) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(smem_u32(bar)),
+      "r"(one)
+      : "memory");
+}
+
 // A warpgroup's share of the block's registers.
 template <int N>
 __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }

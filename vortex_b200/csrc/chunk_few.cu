@@ -394,13 +394,18 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
   }
 }
 
-// ------------------------------------------------------------------ MMA thread
+// ------------------------------------------------------------------ MMA warp
 template <int D, bool INT8, int NR>
 __device__ __forceinline__ void mma_role(const ChunkArgs &a, uint8_t *sm, Bars<Cfg<D, INT8, NR>::SLOTS> &bars) {
   using C = Cfg<D, INT8, NR>;
   constexpr uint32_t ID_S = idesc(NR, false, false), ID_O = idesc(NR, true, INT8);
-  const uint32_t s_kv = smem_u32(sm), s_q = smem_u32(sm + C::OFF_Q), s_p = smem_u32(sm + C::OFF_P), tmem = bars.tmem;
-  Waiter<false> wait{a.err};
+  constexpr uint64_t KMAJOR = desc_base(16, 1024);
+  // heads of 64: the second 64 rows of A are the first again, and are not read back
+  constexpr uint64_t VMAJOR = desc_base(D == 128 ? C::SLAB : 0, 1024);
+  const uint32_t s_kv = smem_u32(sm) >> 4, s_q = smem_u32(sm + C::OFF_Q) >> 4, s_p = smem_u32(sm + C::OFF_P) >> 4;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, bars.tmem, 0);
+  const uint32_t one = elect_one();
+  Waiter<true> wait{a.err};
   Run run(a);
   Piece p{};
   uint32_t g = 0, pieces = 0, ring = 0;
@@ -413,13 +418,13 @@ __device__ __forceinline__ void mma_role(const ChunkArgs &a, uint8_t *sm, Bars<C
       wait(&bars.full[slot], (i / C::SLOTS) & 1);
       fence_async_smem();  // the loaders' cp.async (bf16) are announced without one
       tc_fence_after();
-      const uint32_t k = s_kv + slot * C::TILE, q = s_q + qb * C::Q;
+      const uint64_t k = KMAJOR + (s_kv + slot * (C::TILE >> 4)), q = KMAJOR + (s_q + qb * (C::Q >> 4));
 #pragma unroll
       for (int x = 0; x < D / 16; x++)
-        umma_bf16(tmem + buf * NR, sw128_desc(k + (x >> 2) * C::SLAB + (x & 3) * 32, 16, 1024),
-                  sw128_desc(q + (x >> 2) * (NR * 128) + (x & 3) * 32, 16, 1024), ID_S, x > 0 ? 1u : 0u);
-      umma_commit(&bars.s_full[buf]);
-      umma_commit(&bars.empty[slot]);
+        mma_ss(one, tmem + buf * NR, k + (((x >> 2) * C::SLAB + (x & 3) * 32) >> 4), q + (((x >> 2) * (NR * 128) + (x & 3) * 32) >> 4), ID_S,
+               x > 0 ? 1u : 0u);
+      mma_commit(one, &bars.s_full[buf]);
+      mma_commit(one, &bars.empty[slot]);
     };
     for (int t = 0; t < C::AHEAD && t < T; t++) issue_s(t);
     if (pieces >= 2) wait(&bars.o_free[pb], ((pieces >> 1) - 1) & 1);
@@ -431,21 +436,21 @@ __device__ __forceinline__ void mma_role(const ChunkArgs &a, uint8_t *sm, Bars<C
       fence_async_smem();
       tc_fence_after();
       uint32_t acc = t > 0 ? 1u : 0u;
-      if (!INT8 && t == 0 && *(volatile int *)&bars.acc) {
+      if (!INT8 && t == 0 && __shfl_sync(0xffffffffu, *(volatile int *)&bars.acc, 0)) {
         acc = 1u;
+        __syncwarp();
         *(volatile int *)&bars.acc = 0;
       }
-      const uint32_t v = s_kv + slot * C::TILE, pp = s_p + buf * C::P;
-      // heads of 64: the second 64 rows of A are the first again, and are not read back
+      const uint64_t v = VMAJOR + (s_kv + slot * (C::TILE >> 4)), pp = KMAJOR + (s_p + buf * (C::P >> 4));
 #pragma unroll
       for (int x = 0; x < BN / 16; x++)
-        umma_bf16(tmem + (C::AHEAD + pb) * NR, sw128_desc(v + x * 2048, D == 128 ? C::SLAB : 0, 1024),
-                  sw128_desc(pp + (x >> 2) * (NR * 128) + (x & 3) * 32, 16, 1024), ID_O, x > 0 ? 1u : acc);
-      umma_commit(&bars.empty[slot]);
-      umma_commit(&bars.pv_done[buf]);
+        mma_ss(one, tmem + (C::AHEAD + pb) * NR, v + (x * 2048 >> 4), pp + (((x >> 2) * (NR * 128) + (x & 3) * 32) >> 4), ID_O,
+               x > 0 ? 1u : acc);
+      mma_commit(one, &bars.empty[slot]);
+      mma_commit(one, &bars.pv_done[buf]);
     }
-    umma_commit(&bars.q_empty[qb]);
-    umma_commit(&bars.o_full[pb]);
+    mma_commit(one, &bars.q_empty[qb]);
+    mma_commit(one, &bars.o_full[pb]);
     g += (uint32_t)T;
     ring += 2 * (uint32_t)T;
     pieces++;
@@ -555,7 +560,7 @@ __device__ __forceinline__ void load_role(const ChunkArgs &a, uint8_t *sm, Bars<
       const int row = __shfl_sync(0xffffffffu, rows, r >> 4) + (r & 15);
       cp16(dst + chunk_off(r, ch), src + (size_t)row * D, r < valid);
     }
-    // arrives when this thread's copies have landed; the MMA thread, behind all
+    // arrives when this thread's copies have landed; the MMA warp, behind all
     // of them, orders them before its reads (fence.proxy.async)
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&bars.full[slot])) : "memory");
   }
@@ -695,8 +700,7 @@ __global__ void __launch_bounds__(Cfg<D, INT8, NR>::THREADS, 1) chunk_few_kernel
   } else {
     regs_dec<C::REG_MMA>();
     if (warp == 8 + C::LOADERS) {
-      if ((threadIdx.x & 31) == 0) mma_role<D, INT8, NR>(a, sm, bars);
-      __syncwarp();
+      mma_role<D, INT8, NR>(a, sm, bars);
     } else if (warp == 9 + C::LOADERS) {
       q_role<D, INT8, NR>(a, sm, bars);
     }
