@@ -13,9 +13,8 @@
 // only when a score passes it by 2^8, so a tile needs one vote of the
 // warpgroup and no reduction; l is summed per thread and reduced at the end.
 //
-// Loader warps bring tiles of 128 keys into a ring in the order they are used
-// (K of three tiles, then K of tile t + 3 before V of tile t, so that three S
-// can be on their way while a softmax runs): bf16 rows with cp.async (a 16-token page is only
+// Loader warps bring tiles of 128 keys into two rings, one of K and one of V
+// (K is used up as soon as its S is done, three tiles ahead of V): bf16 rows with cp.async (a 16-token page is only
 // 4 KB: as many TMA boxes reach 5.6 TB/s, 16-byte copies the memory rate),
 // int8 rows through registers, K to bf16 and V to f16 (codes are exact in
 // both). Rows behind the last token become zeros.
@@ -31,6 +30,7 @@
 #include <climits>
 #include <cmath>
 #include <cuda_fp16.h>
+#include <type_traits>
 
 #include "chunk_attn.h"
 
@@ -45,45 +45,55 @@ struct Cfg {
   static constexpr int SLAB = BN * 128;         // 64 columns of 128 keys
   static constexpr int TILE = SLAB * (D / 64);
   static constexpr int AHEAD = 3;               // tiles whose S may be computed before the oldest one's P is there
-  // int8: slots of codes on their way, in shared memory of the thread that will
-  // convert them (two groups of threads, RAWS slots each)
+  // int8: tiles of codes on their way, in shared memory of the thread that will
+  // convert them (RAWS each of K and V)
   static constexpr int RAWS = INT8 ? 2 : 0, RAW = BN * D + BN * 8;
-  static constexpr int SLOTS = !INT8 ? (D == 128 ? (NR == 64 ? 5 : 6) : 10) : D == 128 ? (NR == 64 ? 3 : 4) : 8;
+  // ring slots of K and of V
+  static constexpr int KS = D == 64 ? (INT8 ? 4 : 5) : INT8 ? (NR == 64 ? 1 : 2) : NR == 64 ? 2 : 3;
+  static constexpr int VS = D == 64 ? (INT8 ? 4 : 5) : INT8 ? 2 : 3;
   static constexpr int QBUFS = INT8 && D == 128 && NR > 16 ? 1 : 2;
   static constexpr int Q = NR * D * 2, P = NR * BN * 2;
-  static constexpr int OFF_Q = SLOTS * TILE;
+  static constexpr int OFF_V = KS * TILE, OFF_Q = OFF_V + VS * TILE;
   static constexpr int OFF_P = OFF_Q + QBUFS * Q;  // two tiles
   static constexpr int OFF_RAW = OFF_P + 2 * P;
   static constexpr int OFF_SCALE = OFF_RAW + 2 * RAWS * RAW;
-  // Tiles whose K and V scales are kept. K of tile t takes slot 2 t - AHEAD of
-  // the order above once the slot SLOTS before it is used up: then S of tile
-  // t - SLOTS / 2 is done, for which the softmax of the tile AHEAD before it is.
-  static constexpr int SCALES = INT8 ? AHEAD + (SLOTS + 1) / 2 : 0;
+  // Tiles whose K and V scales are kept: K of tile t is written when S of tile
+  // t - KS is done, for which the softmax of the tile AHEAD before it is.
+  static constexpr int SCALES = INT8 ? AHEAD + KS : 0;
   static constexpr int OFF_RED = OFF_SCALE + SCALES * 2 * BN * 4;  // per-warp results and per-row values of the softmax
   static constexpr int OFF_BARS = OFF_RED + 7 * NR * 4;
   static constexpr int SMEM = OFF_BARS + 320;
-  static constexpr int LOADERS = 8;  // warps
-  // warps: softmax 0-7, loaders, MMA, Q: five warpgroups at 96 registers
-  static constexpr int THREADS = 640;
-  static constexpr int REG_SOFT = NR == 64 ? (INT8 ? 112 : 128) : 96, REG_LOAD = INT8 ? (NR == 64 ? 96 : 112) : (NR == 64 ? 80 : 96), REG_MMA = 56;
-  static_assert(2 * REG_SOFT + 2 * REG_LOAD + REG_MMA <= 5 * 96, "registers");
+  // Warpgroups: two of softmax, PER_SLOT each that load K and V (int8 converts
+  // as it loads), one with the MMA and Q warps.
+  static constexpr int PER_SLOT = INT8 ? 2 : 1, LOADERS = 8 * PER_SLOT;  // warpgroups of a group; warps in all
+  static constexpr int THREADS = 256 + LOADERS * 32 + 128;
+  static constexpr int REGS = INT8 ? 72 : 96;  // at launch
+  static constexpr int REG_SOFT = NR < 64 ? 96 : INT8 ? 112 : 128, REG_LOAD = INT8 ? (NR < 64 ? 64 : 56) : NR < 64 ? 96 : 80, REG_MMA = 56;
+  static_assert(2 * REG_SOFT + 2 * PER_SLOT * REG_LOAD + REG_MMA <= THREADS / 128 * REGS, "registers");
   static constexpr int COLS = (AHEAD + 2) * NR <= 128 ? 128 : (AHEAD + 2) * NR <= 256 ? 256 : 512;  // TMEM: S x AHEAD, O, O
   static_assert(SMEM <= 232448, "shared memory");
 };
 
-template <int SLOTS>
+template <int KS, int VS>
 struct Bars {
-  uint64_t full[SLOTS], empty[SLOTS], q_full[2], q_empty[2], s_full[3], p_full[2], pv_done[2], o_full[2], o_free[2];
+  uint64_t k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], q_full[2], q_empty[2], s_full[3], p_full[2], pv_done[2], o_full[2], o_free[2];
   uint32_t tmem;
   int acc;  // O already holds values that the piece's first product adds to
 };
+template <int D, bool INT8, int NR>
+using BarsOf = Bars<Cfg<D, INT8, NR>::KS, Cfg<D, INT8, NR>::VS>;
 
-// The slots of a piece of T tiles, in the order they are used: K of the first
-// AHEAD tiles, then K of tile t + AHEAD before V of tile t.
-template <int AHEAD>
-__device__ __forceinline__ uint32_t k_at(int t) { return (uint32_t)(t < AHEAD ? t : 2 * t - AHEAD); }
-template <int AHEAD>
-__device__ __forceinline__ uint32_t v_at(int t, int T) { return (uint32_t)(t + AHEAD < T ? 2 * t + AHEAD + 1 : T + t); }
+// A ring's next slot, and how often it has gone around.
+template <int SLOTS>
+struct Ring {
+  uint32_t slot = 0, phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == SLOTS) {
+      slot = 0;
+      phase ^= 1;
+    }
+  }
+};
 
 // 16-byte chunk c of row r of a tile, 128-byte swizzle
 __device__ __forceinline__ uint32_t chunk_off(int r, int c) {
@@ -100,22 +110,7 @@ __device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-template <int N>
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[N]);
-template <>
-__device__ __forceinline__ void tmem_ld<32>(uint32_t taddr, float (&v)[32]) { tmem_ld32(taddr, v); }
-template <>
-__device__ __forceinline__ void tmem_ld<16>(uint32_t taddr, float (&v)[16]) {
-  uint32_t r[16];
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-                 "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-               : "r"(taddr));
-#pragma unroll
-  for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
-}
-template <>
-__device__ __forceinline__ void tmem_ld<8>(uint32_t taddr, float (&v)[8]) {
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&v)[8]) {
   uint32_t r[8];
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
@@ -123,24 +118,10 @@ __device__ __forceinline__ void tmem_ld<8>(uint32_t taddr, float (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; i++) v[i] = __uint_as_float(r[i]);
 }
-template <int N>
-__device__ __forceinline__ void tmem_st(uint32_t taddr, const float (&v)[N]);
-template <>
-__device__ __forceinline__ void tmem_st<32>(uint32_t taddr, const float (&v)[32]) { tmem_st32(taddr, v); }
-template <>
-__device__ __forceinline__ void tmem_st<8>(uint32_t taddr, const float (&v)[8]) {
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const float (&v)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(__float_as_uint(v[0])),
                "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])), "r"(__float_as_uint(v[4])),
                "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7]))
-               : "memory");
-}
-template <>
-__device__ __forceinline__ void tmem_st<16>(uint32_t taddr, const float (&v)[16]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-               "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])),
-               "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7])),
-               "r"(__float_as_uint(v[8])), "r"(__float_as_uint(v[9])), "r"(__float_as_uint(v[10])), "r"(__float_as_uint(v[11])),
-               "r"(__float_as_uint(v[12])), "r"(__float_as_uint(v[13])), "r"(__float_as_uint(v[14])), "r"(__float_as_uint(v[15]))
                : "memory");
 }
 
@@ -159,37 +140,62 @@ __device__ __forceinline__ int chunk_of(int c) {
   return INT8 && D == 128 ? (c & 7) * 2 + (c >> 3) : c;
 }
 
+// Sums of each of N values over the lanes: lane i gets that of value i / (32 / N) in v[0].
+template <int N, int OFF>
+__device__ __forceinline__ void halve(float *v, int lane) {
+  if constexpr (OFF > 0) {
+    if constexpr (N > 1) {
+      const bool up = (lane & OFF) != 0;
+#pragma unroll
+      for (int n = 0; n < N / 2; n++) {
+        const float send = up ? v[n] : v[n + N / 2];
+        v[n] = (up ? v[n + N / 2] : v[n]) + __shfl_xor_sync(0xffffffffu, send, OFF);
+      }
+      halve<N / 2, OFF / 2>(v, lane);
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], OFF);
+      halve<1, OFF / 2>(v, lane);
+    }
+  }
+}
+
 // ------------------------------------------------------------------ softmax: thread = (key, half of the rows)
+// Rows go to the two warpgroups in groups of eight in turn; groups without a
+// live row are passed over.
 template <int D, bool INT8, int NR>
-__device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Bars<Cfg<D, INT8, NR>::SLOTS> &bars) {
+__device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, BarsOf<D, INT8, NR> &bars) {
   using C = Cfg<D, INT8, NR>;
-  constexpr int N = NR / 2;  // rows of this warpgroup
+  constexpr int N = NR / 2, GROUPS = N / 8;  // rows of this warpgroup
   constexpr float SHIFT = INT8 ? 6.f : 0.f;  // P (and l) hold 2^SHIFT times the weights
   const int wg = threadIdx.x >> 7, key = threadIdx.x & 127, warp = key >> 5, lane = key & 31;
-  const int row_base = wg * N;
   const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
-  // this warpgroup's: per-warp results [4][N], maxima, negated references, factors [N]
-  float *red = reinterpret_cast<float *>(sm + C::OFF_RED) + wg * 7 * N, *m_s = red + 4 * N, *ref_s = m_s + N, *f_s = ref_s + N;
+  // row n of the warpgroup's N is row row_of(n) of the item
+  auto row_of = [&](int n) { return (n >> 3) * 16 + wg * 8 + (n & 7); };
+  // this warpgroup's: per-warp results [4][N]; per row the negated reference, a factor, a change of the reference
+  float *red = reinterpret_cast<float *>(sm + C::OFF_RED) + wg * 7 * N, *ref_s = red + 4 * N, *f_s = ref_s + N, *d_s = f_s + N;
   const float *scales = reinterpret_cast<const float *>(sm + C::OFF_SCALE);
   const int bar = 1 + wg;
   Waiter<true> wait{a.err};
   Run run(a);
   Piece p{};
-  uint32_t g = 0, pieces = 0, ring = 0;  // tiles and pieces so far; first ring index of the piece
+  uint32_t g = 0, pieces = 0;  // tiles and pieces so far
+  if (key < N) ref_s[key] = 0.f;
+  bar_sync(bar, 128);
   while (run.next(a, p)) {
-    const int T = max(0, p.te - p.tb), live = p.ntok * a.G - row_base;  // of this warpgroup's rows
+    const int T = max(0, p.te - p.tb), live = p.ntok * a.G;
+    const int groups = live > wg * 8 ? (live - wg * 8 + 15) / 16 : 0;  // of this warpgroup's, with a live row
     const int base = p.s.len - p.s.rows + p.tok0;  // last key that the first token sees
-    const uint32_t tO = bars.tmem + lane_off + (C::AHEAD + (pieces & 1)) * NR + row_base;
+    const uint32_t tO = bars.tmem + lane_off + (C::AHEAD + (pieces & 1)) * NR + wg * 8;
     float l[N];
 #pragma unroll
     for (int n = 0; n < N; n++) l[n] = 0.f;
     for (int t = 0; t < T; t++, g++) {
       const int k0 = (p.tb + t) * BN, k = k0 + key;
-      const uint32_t tS = bars.tmem + lane_off + (g % C::AHEAD) * NR + row_base;
+      const uint32_t tS = bars.tmem + lane_off + (g % C::AHEAD) * NR + wg * 8;
       wait(&bars.s_full[g % C::AHEAD], (g / C::AHEAD) & 1);
       tc_fence_after();
-      // the first of these rows that sees this thread's key
-      const int n_min = k >= p.s.len ? INT_MAX : (a.sh.causal && k > base ? (k - base) * a.G : 0) - row_base;
+      // the first row that sees this thread's key
+      const int n_min = k >= p.s.len ? INT_MAX : a.sh.causal && k > base ? (k - base) * a.G : 0;
       const bool masked = k0 + BN > p.s.len || (a.sh.causal && k0 + BN - 1 > base);
       float sc = a.scale_log2, add = SHIFT, isv = 1.f;
       if constexpr (INT8) {
@@ -200,95 +206,118 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
         isv = 1.f / sv;
       }
       float x[N];  // log2 of what goes into P
-      auto load = [&](bool with_ref) {
-        tmem_ld<N>(tS, x);
+      // (the usual case of only live groups has code without their branches,
+      // which keep the rows' chains apart)
+      float top = -INFINITY;
+      auto load = [&](auto all) {
+#pragma unroll
+        for (int j = 0; j < GROUPS; j++)
+          if (decltype(all)::value || j < groups) tmem_ld8(tS + j * 16, *reinterpret_cast<float(*)[8]>(x + j * 8));
         tmem_wait_ld();
 #pragma unroll
-        for (int n = 0; n < N; n += 4) {
-          const float4 r4 = with_ref ? *reinterpret_cast<const float4 *>(ref_s + n) : make_float4(0.f, 0.f, 0.f, 0.f);
-          const float ref[4] = {r4.x, r4.y, r4.z, r4.w};
+        for (int j = 0; j < GROUPS; j++)
+          if (decltype(all)::value || j < groups) {
 #pragma unroll
-          for (int e = 0; e < 4; e++) x[n + e] = fmaf(x[n + e], sc, INT8 ? add + ref[e] : ref[e]);
-        }
-        if (masked) {
+            for (int n = j * 8; n < j * 8 + 8; n += 4) {
+              const float4 r4 = *reinterpret_cast<const float4 *>(ref_s + n);
+              const float ref[4] = {r4.x, r4.y, r4.z, r4.w};
 #pragma unroll
-          for (int n = 0; n < N; n++) x[n] = n >= n_min ? x[n] : -INFINITY;
-        }
+              for (int e = 0; e < 4; e++) x[n + e] = fmaf(x[n + e], sc, INT8 ? add + ref[e] : ref[e]);
+            }
+            if (masked) {
+#pragma unroll
+              for (int n = j * 8; n < j * 8 + 8; n++) x[n] = row_of(n) >= n_min ? x[n] : -INFINITY;
+            }
+#pragma unroll
+            for (int n = j * 8; n < j * 8 + 8; n++) top = fmaxf(top, x[n]);
+          }
       };
-      bool over = true;
-      if (t > 0) {
-        load(true);
-        float top = x[0];
+      if (groups == GROUPS) load(std::true_type{});
+      else load(std::false_type{});
+      if (t == 0 || bar_or(bar, 128, top > RESCALE_THRESHOLD + SHIFT)) {
+        // New references: a first tile's maximum, later the maximum of the rows
+        // that passed it, becomes 2^SHIFT. (A row without a visible key in its
+        // first tile has none in the others.)
+        float most = -INFINITY;
 #pragma unroll
-        for (int n = 1; n < N; n++) top = fmaxf(top, x[n]);
-        over = bar_or(bar, 128, top > RESCALE_THRESHOLD + SHIFT);
-      }
-      if (over) {
-        // new references: the rows' maxima over this tile and before
-        load(false);
-        float top = -INFINITY;
+        for (int j = 0; j < GROUPS; j++)
+          if (j < groups) {
 #pragma unroll
-        for (int n = 0; n < N; n++) {
-          float y;
-          asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x[n]));
-          top = lane == n ? y : top;
-        }
-        if (lane < N) red[warp * N + lane] = top;
+            for (int n = j * 8; n < j * 8 + 8; n++) {
+              float y;
+              asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x[n]));
+              most = lane == n ? y : most;
+            }
+          }
+        if (lane < N) red[warp * N + lane] = most;
         bar_sync(bar, 128);
         if (key < N) {
-          const float old = t == 0 ? -INFINITY : m_s[key];
-          const float m = fmaxf(fmaxf(fmaxf(red[key], red[N + key]), fmaxf(red[2 * N + key], red[3 * N + key])) - SHIFT, old);
-          m_s[key] = m;
-          ref_s[key] = m == -INFINITY ? 1e30f : -m;  // no score yet: any one passes it
-          f_s[key] = m == old ? 1.f : ex2(old - m);
+          const float m = fmaxf(fmaxf(red[key], red[N + key]), fmaxf(red[2 * N + key], red[3 * N + key]));
+          const float d = t == 0 ? (m > -INFINITY ? SHIFT - m : 0.f) : fminf(SHIFT - m, 0.f);
+          ref_s[key] += d;
+          d_s[key] = d;
+          f_s[key] = ex2(d);
         }
         bar_sync(bar, 128);
+#pragma unroll
+        for (int n = 0; n < N; n++) x[n] += d_s[n];
         if (t > 0) {
           wait(&bars.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
           tc_fence_after();
-          float o[N];
-          tmem_ld<N>(tO, o);
-          tmem_wait_ld();
 #pragma unroll
-          for (int n = 0; n < N; n++) {
-            const float f = f_s[n];
-            o[n] *= f;
-            l[n] *= f;
-          }
-          tmem_st<N>(tO, o);
+          for (int j = 0; j < GROUPS; j++)
+            if (j < groups) {
+              float o[8];
+              tmem_ld8(tO + j * 16, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int n = 0; n < 8; n++) {
+                const float f = f_s[j * 8 + n];
+                o[n] *= f;
+                l[j * 8 + n] *= f;
+              }
+              tmem_st8(tO + j * 16, o);
+            }
           tmem_wait_st();
         }
-        load(true);
       }
       // P of two tiles ago has been used
       uint8_t *P = sm + C::OFF_P + (g & 1) * C::P;
       if (g >= 2) wait(&bars.pv_done[g & 1], ((g - 2) >> 1) & 1);
-      uint8_t *prow = P + (key >> 6) * (NR * 128) + row_base * 128 + (key & 7) * 2;
+      uint8_t *prow = P + (key >> 6) * (NR * 128) + wg * 8 * 128 + (key & 7) * 2;
       const uint32_t chunk = (uint32_t)(key & 63) >> 3;
+      auto weights = [&](auto all) {
 #pragma unroll
-      for (int n = 0; n < N; n += 2) {
-        const float w0 = ex2(x[n]), w1 = ex2(x[n + 1]);
-        uint32_t pair;
-        if constexpr (INT8) {
-          // a row without this key: no product with a scale that is not finite
-          l[n] = !masked || n >= n_min ? fmaf(w0, isv, l[n]) : l[n];
-          l[n + 1] = !masked || n + 1 >= n_min ? fmaf(w1, isv, l[n + 1]) : l[n + 1];
-          asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(pair) : "f"(w1), "f"(w0));
-        } else {
-          l[n] += w0;
-          l[n + 1] += w1;
-          pair = pack_bf16(w0, w1);
-        }
-        *reinterpret_cast<uint16_t *>(prow + n * 128 + ((chunk ^ (n & 7)) << 4)) = (uint16_t)pair;
-        *reinterpret_cast<uint16_t *>(prow + (n + 1) * 128 + ((chunk ^ ((n + 1) & 7)) << 4)) = (uint16_t)(pair >> 16);
-      }
+        for (int j = 0; j < GROUPS; j++)
+          if (decltype(all)::value || j < groups) {
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+              const int n = j * 8 + e;
+              const float w0 = ex2(x[n]), w1 = ex2(x[n + 1]);
+              uint32_t pair;
+              if constexpr (INT8) {
+                // a row without this key: no product with a scale that is not finite
+                l[n] = !masked || row_of(n) >= n_min ? fmaf(w0, isv, l[n]) : l[n];
+                l[n + 1] = !masked || row_of(n + 1) >= n_min ? fmaf(w1, isv, l[n + 1]) : l[n + 1];
+                asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(pair) : "f"(w1), "f"(w0));
+              } else {
+                l[n] += w0;
+                l[n + 1] += w1;
+                pair = pack_bf16(w0, w1);
+              }
+              *reinterpret_cast<uint16_t *>(prow + j * 2048 + e * 128 + ((chunk ^ e) << 4)) = (uint16_t)pair;
+              *reinterpret_cast<uint16_t *>(prow + j * 2048 + (e + 1) * 128 + ((chunk ^ (e + 1)) << 4)) = (uint16_t)(pair >> 16);
+            }
+          }
+      };
+      if (groups == GROUPS) weights(std::true_type{});
+      else weights(std::false_type{});
       if constexpr (!INT8) {
         if (a.sh.causal && min(k0 + BN, p.s.len) - 1 > base) {
           // some row does not see all of this tile's keys
           const int valid = min(BN, p.s.len - k0);
-          const uint32_t vi = ring + v_at<C::AHEAD>(t, T);
-          wait(&bars.full[vi % C::SLOTS], (vi / C::SLOTS) & 1);
-          uint8_t *V = sm + (vi % C::SLOTS) * C::TILE;
+          wait(&bars.v_full[g % C::VS], (g / C::VS) & 1);
+          uint8_t *V = sm + C::OFF_V + (g % C::VS) * C::TILE;
           uint32_t found = 0;
           for (int c = threadIdx.x; c < valid * (D / 8); c += 256) {
             const uint4 w = *reinterpret_cast<const uint4 *>(V + chunk_off(c / (D / 8), c % (D / 8)));
@@ -301,25 +330,25 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
               wait(&bars.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
               tc_fence_after();
             } else {
-              float z[N];
-#pragma unroll
-              for (int n = 0; n < N; n++) z[n] = 0.f;
-              tmem_st<N>(tO, z);
+              const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+              for (int j = 0; j < GROUPS; j++) tmem_st8(tO + j * 16, z);
               tmem_wait_st();
               if (threadIdx.x == 0) bars.acc = 1;
             }
             const int d = key % D;
-            for (int j = 0; j < valid; j++) {
-              const uint32_t bits = *reinterpret_cast<const uint16_t *>(V + chunk_off(j, d >> 3) + (d & 7) * 2);
+            for (int i = 0; i < valid; i++) {
+              const uint32_t bits = *reinterpret_cast<const uint16_t *>(V + chunk_off(i, d >> 3) + (d & 7) * 2);
               const bool odd = (bits & 0x7F80u) == 0x7F80u;
               if (!__any_sync(0xffffffffu, odd)) continue;
-              const int first = max(0, (k0 + j > base ? (k0 + j - base) * a.G : 0) - row_base);
-              for (int n = first; n < N; n++) {
-                const uint32_t off = (uint32_t)(j >> 6) * (NR * 128) + (uint32_t)(row_base + n) * 128 +
-                                     ((((uint32_t)(j & 63) >> 3) ^ ((uint32_t)n & 7)) << 4) + (j & 7) * 2;
+              const int first = k0 + i > base ? (k0 + i - base) * a.G : 0;
+              for (int n = 0; n < groups * 8; n++) {
+                const int r = row_of(n);
+                if (r < first) continue;
+                const uint32_t off = (uint32_t)(i >> 6) * (NR * 128) + (uint32_t)r * 128 + ((((uint32_t)(i & 63) >> 3) ^ ((uint32_t)n & 7)) << 4) + (i & 7) * 2;
                 const float w = __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t *>(P + off) << 16);
-                const float o = tmem_ld1(tO + n);
-                tmem_st1(tO + n, odd ? fmaf(w, __uint_as_float(bits << 16), o) : o);
+                const uint32_t at = tO + (n >> 3) * 16 + (n & 7);
+                const float o = tmem_ld1(at);
+                tmem_st1(at, odd ? fmaf(w, __uint_as_float(bits << 16), o) : o);
                 tmem_wait_st();
               }
             }
@@ -336,13 +365,13 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.p_full[g & 1]);
     }
-    // ---------------- end of the piece
-    // l of every row: over the lanes, then the warps
+    // ---------------- end of the piece (its code runs once a piece: kept short,
+    // since it comes from beyond the instruction cache)
     bar_sync(bar, 128);  // red is free
-#pragma unroll
-    for (int n = 0; n < N; n++) {
-      const float y = warp_sum(l[n]);
-      if (lane == n) red[warp * N + n] = y;
+    {
+      // l of every row over the lanes: halves are exchanged until a lane has one row
+      halve<N, 16>(l, lane);
+      if (lane % (32 / N) == 0) red[warp * N + lane / (32 / N)] = l[0];
     }
     bar_sync(bar, 128);
     const bool whole = p.whole();
@@ -350,109 +379,121 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
     const size_t row0 = (size_t)(p.s.row0 + p.tok0) * a.Hq + (size_t)p.head * a.G;
     if (key < N) {
       const float L = red[key] + red[N + key] + red[2 * N + key] + red[3 * N + key];
-      const float m = T > 0 ? m_s[key] : -INFINITY;
+      const float m = L == 0.f ? -INFINITY : -ref_s[key] - SHIFT;
       f_s[key] = whole ? (L == 0.f ? 0.f : 1.f / L) : 1.f;
-      const int r = row_base + key;
-      if (key < live) {
-        if (!whole) __stcg(reinterpret_cast<float2 *>(part + (size_t)kRowsItem * D) + r, make_float2(m - SHIFT, L));
-        else if (a.lse) a.lse[row0 + (size_t)(r / a.G) * a.Hq + r % a.G] = L == 0.f ? -INFINITY : (m - SHIFT + log2f(L)) * 0.69314718055994531f;
+      ref_s[key] = 0.f;
+      const int r = row_of(key);
+      if (r < live) {
+        if (!whole) __stcg(reinterpret_cast<float2 *>(part + (size_t)kRowsItem * D) + r, make_float2(m, L));
+        else if (a.lse) a.lse[row0 + (size_t)(r / a.G) * a.Hq + r % a.G] = (m + log2f(L)) * 0.69314718055994531f;
       }
     }
     bar_sync(bar, 128);
     wait(&bars.o_full[pieces & 1], (pieces >> 1) & 1);
     tc_fence_after();
-    if (live > 0) {
-      float o[N];
-#pragma unroll
-      for (int n = 0; n < N; n++) o[n] = 0.f;
+    const int d = key < D ? chunk_of<D, INT8>(key >> 3) * 8 + (key & 7) : 0;
+#pragma unroll 1
+    for (int j = 0; j < groups; j++) {
+      float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       if (T > 0) {
-        tmem_ld<N>(tO, o);
+        tmem_ld8(tO + j * 16, o);
         tmem_wait_ld();
       }
-      if (key < D) {
-        const int d = chunk_of<D, INT8>(key >> 3) * 8 + (key & 7);
-        int tok = row_base / a.G, h = row_base - tok * a.G;
+      const int r0 = j * 16 + wg * 8, count = key < D ? live - r0 : 0;
+      const float *f8 = f_s + j * 8;
+      if (whole) {
+        int h = r0 % a.G;
+        uint16_t *to = a.out + (row0 + (size_t)(r0 / a.G) * a.Hq + h) * D + d;
+        const size_t over = (size_t)(a.Hq - a.G) * D;  // from a token's last head of the group to the next token's first
 #pragma unroll
-        for (int n = 0; n < N; n++) {
-          if (n < live) {
-            const float y = o[n] * f_s[n];
-            if (whole) a.out[(row0 + (size_t)tok * a.Hq + h) * D + d] = (uint16_t)pack_bf16(y, 0.f);
-            else __stcg(part + (size_t)(row_base + n) * D + d, y);
-            if (++h == a.G) {
-              h = 0;
-              tok++;
-            }
+        for (int e = 0; e < 8; e++) {
+          if (e < count) *to = (uint16_t)pack_bf16(o[e] * f8[e], 0.f);
+          to += D;
+          if (++h == a.G) {
+            h = 0;
+            to += over;
           }
         }
+      } else {
+        float *to = part + (size_t)r0 * D + d;
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          if (e < count) __stcg(to + e * D, o[e]);
       }
+      __syncwarp();
     }
     tc_fence_before();
     __syncwarp();
     if (lane == 0) mbar_arrive(&bars.o_free[pieces & 1]);
     pieces++;
-    ring += 2 * (uint32_t)T;
   }
 }
 
 // ------------------------------------------------------------------ MMA warp
 template <int D, bool INT8, int NR>
-__device__ __forceinline__ void mma_role(const ChunkArgs &a, uint8_t *sm, Bars<Cfg<D, INT8, NR>::SLOTS> &bars) {
+__device__ __forceinline__ void mma_role(const ChunkArgs &a, uint8_t *sm, BarsOf<D, INT8, NR> &bars) {
   using C = Cfg<D, INT8, NR>;
-  constexpr uint32_t ID_S = idesc(NR, false, false), ID_O = idesc(NR, true, INT8);
   constexpr uint64_t KMAJOR = desc_base(16, 1024);
   // heads of 64: the second 64 rows of A are the first again, and are not read back
   constexpr uint64_t VMAJOR = desc_base(D == 128 ? C::SLAB : 0, 1024);
-  const uint32_t s_kv = smem_u32(sm) >> 4, s_q = smem_u32(sm + C::OFF_Q) >> 4, s_p = smem_u32(sm + C::OFF_P) >> 4;
+  const uint32_t s_k = smem_u32(sm) >> 4, s_v = smem_u32(sm + C::OFF_V) >> 4, s_q = smem_u32(sm + C::OFF_Q) >> 4, s_p = smem_u32(sm + C::OFF_P) >> 4;
   const uint32_t tmem = __shfl_sync(0xffffffffu, bars.tmem, 0);
   const uint32_t one = elect_one();
   Waiter<true> wait{a.err};
   Run run(a);
   Piece p{};
-  uint32_t g = 0, pieces = 0, ring = 0;
+  uint32_t g = 0, pieces = 0;
+  Ring<C::KS> kr;
+  Ring<C::VS> vr;
+  uint32_t s_buf = 0;  // S of the next tile
+  auto filled = [&](uint64_t *full, uint32_t phase) {
+    wait(full, phase);
+    fence_async_smem();  // the loaders' cp.async (bf16) are announced without one
+    tc_fence_after();
+  };
   while (run.next(a, p)) {
     const int T = max(0, p.te - p.tb);
     const uint32_t pb = pieces & 1, qb = pieces % C::QBUFS;
+    const int cols = (p.ntok * a.G + 15) / 16 * 16;  // of the NR, those with live rows
+    const uint32_t id_s = idesc(cols, false, false), id_o = idesc(cols, true, INT8);
+    const uint64_t q = KMAJOR + (s_q + qb * (C::Q >> 4));
+    const uint32_t t_o = tmem + (C::AHEAD + pb) * NR;
     wait(&bars.q_full[qb], (pieces / C::QBUFS) & 1);
-    auto issue_s = [&](int t) {
-      const uint32_t i = ring + k_at<C::AHEAD>(t), slot = i % C::SLOTS, buf = (g + t) % C::AHEAD;
-      wait(&bars.full[slot], (i / C::SLOTS) & 1);
-      fence_async_smem();  // the loaders' cp.async (bf16) are announced without one
-      tc_fence_after();
-      const uint64_t k = KMAJOR + (s_kv + slot * (C::TILE >> 4)), q = KMAJOR + (s_q + qb * (C::Q >> 4));
+    auto issue_s = [&]() {
+      filled(&bars.k_full[kr.slot], kr.phase);
+      const uint64_t k = KMAJOR + (s_k + kr.slot * (C::TILE >> 4));
 #pragma unroll
       for (int x = 0; x < D / 16; x++)
-        mma_ss(one, tmem + buf * NR, k + (((x >> 2) * C::SLAB + (x & 3) * 32) >> 4), q + (((x >> 2) * (NR * 128) + (x & 3) * 32) >> 4), ID_S,
+        mma_ss(one, tmem + s_buf * NR, k + (((x >> 2) * C::SLAB + (x & 3) * 32) >> 4), q + (((x >> 2) * (NR * 128) + (x & 3) * 32) >> 4), id_s,
                x > 0 ? 1u : 0u);
-      mma_commit(one, &bars.s_full[buf]);
-      mma_commit(one, &bars.empty[slot]);
+      mma_commit(one, &bars.s_full[s_buf]);
+      mma_commit(one, &bars.k_empty[kr.slot]);
+      kr.next();
+      s_buf = s_buf + 1 == C::AHEAD ? 0 : s_buf + 1;
     };
-    for (int t = 0; t < C::AHEAD && t < T; t++) issue_s(t);
+    for (int t = 0; t < C::AHEAD && t < T; t++) issue_s();
     if (pieces >= 2) wait(&bars.o_free[pb], ((pieces >> 1) - 1) & 1);
-    for (int t = 0; t < T; t++) {
-      const uint32_t i = ring + v_at<C::AHEAD>(t, T), slot = i % C::SLOTS, buf = (g + t) & 1;
-      wait(&bars.p_full[buf], ((g + t) >> 1) & 1);
-      if (t + C::AHEAD < T) issue_s(t + C::AHEAD);  // S of tile t has been read
-      wait(&bars.full[slot], (i / C::SLOTS) & 1);
-      fence_async_smem();
-      tc_fence_after();
+    for (int t = 0; t < T; t++, g++) {
+      const uint32_t buf = g & 1;
+      wait(&bars.p_full[buf], (g >> 1) & 1);
+      if (t + C::AHEAD < T) issue_s();  // S of tile t has been read
+      filled(&bars.v_full[vr.slot], vr.phase);
+      const uint64_t v = VMAJOR + (s_v + vr.slot * (C::TILE >> 4)), pp = KMAJOR + (s_p + buf * (C::P >> 4));
       uint32_t acc = t > 0 ? 1u : 0u;
       if (!INT8 && t == 0 && __shfl_sync(0xffffffffu, *(volatile int *)&bars.acc, 0)) {
         acc = 1u;
         __syncwarp();
         *(volatile int *)&bars.acc = 0;
       }
-      const uint64_t v = VMAJOR + (s_kv + slot * (C::TILE >> 4)), pp = KMAJOR + (s_p + buf * (C::P >> 4));
 #pragma unroll
       for (int x = 0; x < BN / 16; x++)
-        mma_ss(one, tmem + (C::AHEAD + pb) * NR, v + (x * 2048 >> 4), pp + (((x >> 2) * (NR * 128) + (x & 3) * 32) >> 4), ID_O,
-               x > 0 ? 1u : acc);
-      mma_commit(one, &bars.empty[slot]);
+        mma_ss(one, t_o, v + (x * 2048 >> 4), pp + (((x >> 2) * (NR * 128) + (x & 3) * 32) >> 4), id_o, x > 0 ? 1u : acc);
+      mma_commit(one, &bars.v_empty[vr.slot]);
       mma_commit(one, &bars.pv_done[buf]);
+      vr.next();
     }
     mma_commit(one, &bars.q_empty[qb]);
     mma_commit(one, &bars.o_full[pb]);
-    g += (uint32_t)T;
-    ring += 2 * (uint32_t)T;
     pieces++;
   }
 }
@@ -469,7 +510,7 @@ __device__ __forceinline__ int group_row(const ChunkArgs &a, const Piece &p, con
 
 // Q warp: the query rows of each piece (zeros behind the last)
 template <int D, bool INT8, int NR>
-__device__ __forceinline__ void q_role(const ChunkArgs &a, uint8_t *sm, Bars<Cfg<D, INT8, NR>::SLOTS> &bars) {
+__device__ __forceinline__ void q_role(const ChunkArgs &a, uint8_t *sm, BarsOf<D, INT8, NR> &bars) {
   using C = Cfg<D, INT8, NR>;
   const int lane = threadIdx.x & 31;
   Waiter<true> wait{a.err};
@@ -495,108 +536,91 @@ __device__ __forceinline__ void q_role(const ChunkArgs &a, uint8_t *sm, Bars<Cfg
   }
 }
 
-// The slots of one of the two loader groups (four warps each, which take the
-// ring's slots in turn): slot j, of the group's parity, of the 2 T slots of a
-// piece.
-template <int AHEAD>
-struct Cursor {
+// A loader group's tiles, one after another over the pieces of the run.
+struct Tiles {
   Run run;
   Piece p;
-  uint32_t ring, tiles, half;  // slots and tiles before p; the group
-  int T, j;
+  int t, T;
   bool more;
-  __device__ __forceinline__ Cursor(const ChunkArgs &a, uint32_t group)
-      : run(a), p{}, ring(0), tiles(0), half(group), T(0), j(0), more(true) { piece(a); }
-  __device__ __forceinline__ void piece(const ChunkArgs &a) {
+  __device__ __forceinline__ Tiles(const ChunkArgs &a) : run(a), p{}, t(0), T(0), more(true) { next(a); }
+  __device__ __forceinline__ void next(const ChunkArgs &a) {
+    if (++t < T) return;
+    t = 0;
     do {
-      ring += 2 * (uint32_t)T;
-      tiles += (uint32_t)T;
-      if (!run.next(a, p)) {
-        more = false;
-        return;
-      }
+      more = run.next(a, p);
       T = max(0, p.te - p.tb);
-    } while (T == 0);
-    j = (int)half;
+    } while (more && T == 0);
   }
-  __device__ __forceinline__ void advance(const ChunkArgs &a) {
-    j += 2;
-    if (j >= 2 * T) piece(a);
-  }
-  // the tile of slot j, and whether it is V (inverse of k_at and v_at)
-  __device__ __forceinline__ int tile(bool &v) const {
-    const int first = min(AHEAD, T), pairs = 2 * (T - first), m = j - first;
-    v = m >= 0 && (m >= pairs || (m & 1));
-    return m < 0 ? j : m >= pairs ? m - pairs + (T - first) : (m & 1) ? m >> 1 : first + (m >> 1);
-  }
+  __device__ __forceinline__ int tile() const { return p.tb + t; }
   __device__ __forceinline__ int rows(const ChunkArgs &a) const {
-    bool v;
-    return more ? group_row(a, p, a.tables + (size_t)p.s.slot * a.mbps, p.tb + tile(v)) : 0;
+    return more ? group_row(a, p, a.tables + (size_t)p.s.slot * a.mbps, tile()) : 0;
   }
 };
 
-template <int D, int NR>
-__device__ __forceinline__ void load_role(const ChunkArgs &a, uint8_t *sm, Bars<Cfg<D, false, NR>::SLOTS> &bars) {
+// One group of four warps loads K, the other V.
+template <int D, int NR, bool V>
+__device__ __forceinline__ void load_role(const ChunkArgs &a, uint8_t *sm, BarsOf<D, false, NR> &bars) {
   using C = Cfg<D, false, NR>;
   const int tid = threadIdx.x & 127;
-  const uint32_t s_kv = smem_u32(sm);
   constexpr int CHUNKS = D / 8, STEP = 128 / CHUNKS;  // rows per round of the 128 threads
   const int ch = tid % CHUNKS, r0 = tid / CHUNKS;
+  uint64_t *full = V ? bars.v_full : bars.k_full, *empty = V ? bars.v_empty : bars.k_empty;
+  const uint32_t ring = smem_u32(sm + (V ? C::OFF_V : 0));
+  const uint16_t *pool = reinterpret_cast<const uint16_t *>(V ? a.pool_v : a.pool_k) + ch * 8;
   Waiter<true> wait{a.err};
-  Cursor<C::AHEAD> c(a, (threadIdx.x - 256) >> 7);
+  Tiles c(a);
+  Ring<V ? C::VS : C::KS> at;
   int next = c.rows(a);
-  while (c.more) {
-    bool v;
-    const int tile = c.p.tb + c.tile(v), valid = c.p.s.len - tile * BN, rows = next;
-    const uint32_t idx = c.ring + (uint32_t)c.j, slot = idx % C::SLOTS;
-    c.advance(a);
-    next = c.rows(a);  // the table's answer comes while this slot is copied
-    if (idx >= C::SLOTS) wait(&bars.empty[slot], (idx / C::SLOTS - 1) & 1);
-    const uint32_t dst = s_kv + slot * C::TILE;
-    const uint16_t *src = reinterpret_cast<const uint16_t *>(v ? a.pool_v : a.pool_k) + ch * 8;
+  for (bool first = true; c.more; at.next()) {
+    const int valid = c.p.s.len - c.tile() * BN, rows = next;
+    c.next(a);
+    next = c.rows(a);  // the table's answer comes while this tile is copied
+    if (!first) wait(&empty[at.slot], at.phase ^ 1);
+    if (at.slot + 1 == (V ? C::VS : C::KS)) first = false;
+    const uint32_t dst = ring + at.slot * C::TILE;
 #pragma unroll
     for (int i = 0; i < BN / STEP; i++) {
       const int r = r0 + i * STEP;
       const int row = __shfl_sync(0xffffffffu, rows, r >> 4) + (r & 15);
-      cp16(dst + chunk_off(r, ch), src + (size_t)row * D, r < valid);
+      cp16(dst + chunk_off(r, ch), pool + (size_t)row * D, r < valid);
     }
     // arrives when this thread's copies have landed; the MMA warp, behind all
     // of them, orders them before its reads (fence.proxy.async)
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&bars.full[slot])) : "memory");
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[at.slot])) : "memory");
   }
   cp_wait_all();
 }
 
-// int8: a thread copies the codes that it will convert RAWS slots ahead into
+// int8: a thread copies the codes that it will convert RAWS tiles ahead into
 // its own part of shared memory (loads into registers would not survive the
 // fences between them).
-template <int D, int NR>
-__device__ __forceinline__ void load_role_i8(const ChunkArgs &a, uint8_t *sm, Bars<Cfg<D, true, NR>::SLOTS> &bars) {
+template <int D, int NR, bool V>
+__device__ __forceinline__ void load_role_i8(const ChunkArgs &a, uint8_t *sm, BarsOf<D, true, NR> &bars) {
   using C = Cfg<D, true, NR>;
-  const int tid = threadIdx.x & 127, lane = threadIdx.x & 31;
-  const uint32_t half = (threadIdx.x - 256) >> 7;
-  constexpr int CHUNKS = D / 16, STEP = 128 / CHUNKS, N = BN / STEP;
+  constexpr int THREADS = 128 * C::PER_SLOT;
+  const int tid = threadIdx.x % THREADS, lane = threadIdx.x & 31;
+  constexpr int CHUNKS = D / 16, STEP = THREADS / CHUNKS, N = BN / STEP;
   const int ch = tid % CHUNKS, r0 = tid / CHUNKS;
+  uint64_t *full = V ? bars.v_full : bars.k_full, *empty = V ? bars.v_empty : bars.k_empty;
+  uint8_t *ring = sm + (V ? C::OFF_V : 0), *raw = sm + C::OFF_RAW + (V ? C::RAWS * C::RAW : 0);
+  const uint8_t *pool = reinterpret_cast<const uint8_t *>(V ? a.pool_v : a.pool_k) + ch * 16;
   Waiter<true> wait{a.err};
-  uint8_t *raw = sm + C::OFF_RAW + half * C::RAWS * C::RAW;
-  Cursor<C::AHEAD> f(a, half), c(a, half);  // what is fetched, what is converted
+  Tiles f(a), c(a);  // what is fetched, what is converted
   int next = f.rows(a);
   auto fetch = [&](uint32_t stage) {
     if (f.more) {
-      bool v;
-      const int tile = f.p.tb + f.tile(v), valid = f.p.s.len - tile * BN, rows = next;
-      f.advance(a);
+      const int valid = f.p.s.len - f.tile() * BN, rows = next;
+      f.next(a);
       next = f.rows(a);
-      const uint8_t *src = reinterpret_cast<const uint8_t *>(v ? a.pool_v : a.pool_k) + ch * 16;
       const uint32_t dst = smem_u32(raw + stage * C::RAW) + tid * 16;
 #pragma unroll
       for (int i = 0; i < N; i++) {
         const int r = r0 + i * STEP;
         const int row = __shfl_sync(0xffffffffu, rows, r >> 4) + (r & 15);
-        cp16(dst + i * 2048, src + (size_t)row * D, r < valid);
+        cp16(dst + i * (THREADS * 16), pool + (size_t)row * D, r < valid);
       }
-      const int row = __shfl_sync(0xffffffffu, rows, tid >> 4) + (tid & 15);
-      if (!v) {  // both scales come with K
+      if (!V && tid < BN) {  // both scales come with K
+        const int row = __shfl_sync(0xffffffffu, rows, tid >> 4) + (tid & 15);
         const uint32_t at = smem_u32(raw + stage * C::RAW + BN * D) + tid * 8;
         cp4(at, a.sk + row, tid < valid);
         cp4(at + 4, a.sv + row, tid < valid);
@@ -606,23 +630,25 @@ __device__ __forceinline__ void load_role_i8(const ChunkArgs &a, uint8_t *sm, Ba
   };
 #pragma unroll
   for (int i = 0; i < C::RAWS; i++) fetch(i);
-  for (uint32_t n = 0; c.more; n++) {
-    bool v;
-    const int tile = c.tile(v), valid = c.p.s.len - (c.p.tb + tile) * BN;
-    const uint32_t idx = c.ring + (uint32_t)c.j, slot = idx % C::SLOTS, stage = n % C::RAWS;
+  Ring<V ? C::VS : C::KS> at;
+  Ring<C::RAWS> stage;
+  Ring<V ? 1 : C::SCALES> scales;
+  for (bool first = true; c.more; at.next(), stage.next(), scales.next(), c.next(a)) {
     cp_wait<C::RAWS - 1>();
-    const uint8_t *src = raw + stage * C::RAW;
+    const uint8_t *src = raw + stage.slot * C::RAW;
     uint4 x[N];
 #pragma unroll
-    for (int i = 0; i < N; i++) x[i] = *reinterpret_cast<const uint4 *>(src + i * 2048 + tid * 16);
-    const float2 f2 = *reinterpret_cast<const float2 *>(src + BN * D + tid * 8);
-    if (idx >= C::SLOTS) wait(&bars.empty[slot], (idx / C::SLOTS - 1) & 1);
-    if (!v) {
-      float *at = reinterpret_cast<float *>(sm + C::OFF_SCALE) + (c.tiles + tile) % C::SCALES * 2 * BN + tid;
-      at[0] = tid < valid ? f2.x : 1.f;
-      at[BN] = tid < valid ? f2.y : 1.f;
+    for (int i = 0; i < N; i++) x[i] = *reinterpret_cast<const uint4 *>(src + i * (THREADS * 16) + tid * 16);
+    if (!first) wait(&empty[at.slot], at.phase ^ 1);
+    if (at.slot + 1 == (V ? C::VS : C::KS)) first = false;
+    if (!V && tid < BN) {
+      const bool live = tid < c.p.s.len - c.tile() * BN;  // a key that does not exist has scale 1
+      const float2 f2 = *reinterpret_cast<const float2 *>(src + BN * D + tid * 8);
+      float *to = reinterpret_cast<float *>(sm + C::OFF_SCALE) + scales.slot * 2 * BN + tid;
+      to[0] = live ? f2.x : 1.f;
+      to[BN] = live ? f2.y : 1.f;
     }
-    uint8_t *dst = sm + slot * C::TILE;
+    uint8_t *dst = ring + at.slot * C::TILE;
 #pragma unroll
     for (int i = 0; i < N; i++) {
       const int r = r0 + i * STEP;
@@ -631,7 +657,7 @@ __device__ __forceinline__ void load_role_i8(const ChunkArgs &a, uint8_t *sm, Ba
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         const uint32_t word = in[e >> 1], sel = e & 1 ? 0x4342u : 0x4140u;
-        if (v) {
+        if constexpr (V) {
           // f16: (code ^ 0x80) under the magic 0x64 is 1024 + 128 + code
           const uint32_t h = __byte_perm(word ^ 0x80808080u, 0x64646464u, sel);
           asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(o[e]) : "r"(h), "r"(0x64806480u));
@@ -648,9 +674,8 @@ __device__ __forceinline__ void load_role_i8(const ChunkArgs &a, uint8_t *sm, Ba
     }
     fence_async_smem();
     __syncwarp();
-    if (lane == 0) mbar_arrive(&bars.full[slot]);
-    fetch(stage);  // its codes have been used
-    c.advance(a);
+    if (lane == 0) mbar_arrive(&full[at.slot]);
+    fetch(stage.slot);  // its codes have been used
   }
   cp_wait_all();
 }
@@ -658,7 +683,7 @@ __device__ __forceinline__ void load_role_i8(const ChunkArgs &a, uint8_t *sm, Ba
 template <int D, bool INT8, int NR>
 __global__ void __launch_bounds__(Cfg<D, INT8, NR>::THREADS, 1) chunk_few_kernel(const __grid_constant__ ChunkArgs a) {
   using C = Cfg<D, INT8, NR>;
-  using B = Bars<C::SLOTS>;
+  using B = BarsOf<D, INT8, NR>;
   static_assert(sizeof(B) <= 320, "barriers");
   extern __shared__ __align__(1024) uint8_t sm[];
   B &bars = *reinterpret_cast<B *>(sm + C::OFF_BARS);
@@ -669,9 +694,14 @@ __global__ void __launch_bounds__(Cfg<D, INT8, NR>::THREADS, 1) chunk_few_kernel
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   if (threadIdx.x == 32) {
-    for (int i = 0; i < C::SLOTS; i++) {
-      mbar_init(&bars.full[i], INT8 ? 4 : 128);
-      mbar_init(&bars.empty[i], 1);
+    constexpr uint32_t LOADING = INT8 ? 4 * C::PER_SLOT : 128;
+    for (int i = 0; i < C::KS; i++) {
+      mbar_init(&bars.k_full[i], LOADING);
+      mbar_init(&bars.k_empty[i], 1);
+    }
+    for (int i = 0; i < C::VS; i++) {
+      mbar_init(&bars.v_full[i], LOADING);
+      mbar_init(&bars.v_empty[i], 1);
     }
     for (int i = 0; i < 2; i++) {
       mbar_init(&bars.q_full[i], 1);
@@ -690,13 +720,18 @@ __global__ void __launch_bounds__(Cfg<D, INT8, NR>::THREADS, 1) chunk_few_kernel
   tc_fence_after();
   const uint32_t tmem = bars.tmem;
   if (warp < 8) {
-    if constexpr (C::REG_SOFT > 96) regs_inc<C::REG_SOFT>();
+    if constexpr (C::REG_SOFT > C::REGS) regs_inc<C::REG_SOFT>();
     softmax_role<D, INT8, NR>(a, sm, bars);
   } else if (warp < 8 + C::LOADERS) {
-    if constexpr (C::REG_LOAD > 96) regs_inc<C::REG_LOAD>();
-    if constexpr (C::REG_LOAD < 96) regs_dec<C::REG_LOAD>();
-    if constexpr (INT8) load_role_i8<D, NR>(a, sm, bars);
-    else load_role<D, NR>(a, sm, bars);
+    if constexpr (C::REG_LOAD < C::REGS) regs_dec<C::REG_LOAD>();
+    const bool v = warp >= 8 + C::LOADERS / 2;
+    if constexpr (INT8) {
+      if (v) load_role_i8<D, NR, true>(a, sm, bars);
+      else load_role_i8<D, NR, false>(a, sm, bars);
+    } else {
+      if (v) load_role<D, NR, true>(a, sm, bars);
+      else load_role<D, NR, false>(a, sm, bars);
+    }
   } else {
     regs_dec<C::REG_MMA>();
     if (warp == 8 + C::LOADERS) {
