@@ -67,14 +67,14 @@ struct Cfg {
   static constexpr int OFF_KV = 2 * TILE;
   static constexpr int OFF_RAW = OFF_KV + SLOTS * TILE;
   static constexpr int OFF_SCALE = OFF_RAW + RAWS * RAW;  // f32 per key: K and V scales of the last SLOTS tiles
-  static constexpr int OFF_ML = OFF_SCALE + (INT8 ? SLOTS * 2 * BN * 4 : 0);
-  static constexpr int OFF_BARS = OFF_ML + 2 * BM * 8;
-  static constexpr int SMEM = OFF_BARS + 512;
-  static constexpr int THREADS = INT8 ? 512 : 384;
-  // registers per thread: softmax, producer and converter warpgroups; their
-  // sum is what the block is launched with (128 x 512 resp. 168 x 384)
-  static constexpr int REG_SOFT = INT8 ? 192 : 208, REG_PROD = INT8 ? 56 : 88, REG_CONV = 72;
-  static_assert(INT8 ? 2 * REG_SOFT + REG_PROD + REG_CONV <= 512 : 2 * REG_SOFT + REG_PROD <= 504, "registers");
+  static constexpr int OFF_X = OFF_SCALE + (INT8 ? SLOTS * 2 * BN * 4 : 0);  // what the two halves of a row tell each other
+  static constexpr int OFF_BARS = OFF_X + 4 * BM * 4;
+  static constexpr int SMEM = OFF_BARS + 768;
+  // warpgroups: two of softmax for each stream, one of the MMA and TMA warps,
+  // int8: two that convert; registers at launch and of each
+  static constexpr int THREADS = INT8 ? 896 : 640, REGS = INT8 ? 72 : 96;
+  static constexpr int REG_SOFT = INT8 ? 88 : 104, REG_PROD = INT8 ? 56 : 64, REG_CONV = 48;
+  static_assert(4 * REG_SOFT + REG_PROD + (INT8 ? 2 * REG_CONV : 0) <= THREADS / 128 * REGS, "registers");
   static_assert(SMEM <= 232448, "shared memory");
 };
 
@@ -84,6 +84,11 @@ struct Bars {
       raw_empty[RAWS + 1];
   uint32_t tmem;
   int acc[2];  // the stream's O already holds values that its first product adds to
+  // the softmax warps' run and its piece (of even and odd number): in shared
+  // memory, to leave their registers to the scores
+  Run run;
+  Piece piece[2];
+  int more[2];
 };
 
 // 16-byte chunk c (8 columns) of row r of a bf16 tile in shared memory
@@ -91,260 +96,325 @@ __device__ __forceinline__ uint32_t chunk_off(int r, int c) {
   return (uint32_t)((c >> 3) * (BN * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
-// ------------------------------------------------------------------ softmax warpgroup of stream ST
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t as_u64(float2 v) {
+  uint64_t u;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(u) : "f"(v.x), "f"(v.y));
+  return u;
+}
+__device__ __forceinline__ float2 as_f2(uint64_t u) {
+  float2 v;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(u));
+  return v;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(as_u64(a)), "l"(as_u64(b)), "l"(as_u64(c)));
+  return as_f2(d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(as_u64(a)), "l"(as_u64(b)));
+  return as_f2(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(as_u64(a)), "l"(as_u64(b)));
+  return as_f2(d);
+}
+__device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+               "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                 "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr));
+#pragma unroll
+  for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
+}
+
+// v[i] *= f[i], f in shared memory (the same for every lane)
+template <int N>
+__device__ __forceinline__ void scale_keys(float *v, const float *f) {
+#pragma unroll
+  for (int c = 0; c < N; c += 4) {
+    const float4 x = *reinterpret_cast<const float4 *>(f + c);
+    const float2 lo = mul2(make_float2(v[c], v[c + 1]), make_float2(x.x, x.y)), hi = mul2(make_float2(v[c + 2], v[c + 3]), make_float2(x.z, x.w));
+    v[c] = lo.x;
+    v[c + 1] = lo.y;
+    v[c + 2] = hi.x;
+    v[c + 3] = hi.y;
+  }
+}
+
+// ------------------------------------------------------------------ softmax: thread = (stream, row, half of a tile's keys)
 template <int D, bool INT8, class B>
-__device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B &bars, const int st) {
+__device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B &bars) {
   using C = Cfg<D, INT8>;
-  const int warp4 = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31, r = warp4 * 32 + lane;
+  constexpr int N = BN / 2;
+  const int st = threadIdx.x >> 8, half = (threadIdx.x >> 7) & 1, warp4 = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
+  const int r = warp4 * 32 + lane, tid = threadIdx.x & 255;  // row of the tile; thread of the stream
   const uint32_t lane_off = (uint32_t)(warp4 * 32) << 16;
-  const uint32_t tS = bars.tmem + st * 128 + lane_off, tO = bars.tmem + 256 + st * 128 + lane_off;
-  const uint32_t tO_other = bars.tmem + 256 + (st ^ 1) * 128 + lane_off;
-  float2 *ml = reinterpret_cast<float2 *>(sm + C::OFF_ML);  // [2][BM]
+  const uint32_t tS = bars.tmem + st * 128 + half * N + lane_off;  // this half's scores, then (bf16) its weights
+  const uint32_t tO = bars.tmem + 256 + st * 128 + lane_off, tO_other = bars.tmem + 256 + (st ^ 1) * 128 + lane_off;
+  float *x_row = reinterpret_cast<float *>(sm + C::OFF_X) + r;  // [stream][half][row]
+  float *x_mine = x_row + (st * 2 + half) * BM, *x_half = x_row + (st * 2 + (half ^ 1)) * BM;
+  const int pair = 4 + st * 4 + warp4;  // barrier of the two warps that share these rows
   Waiter<true> wait{a.err};
-  Run run(a);
-  Piece p{};
   uint32_t step = 0, pieces = 0, ring = 0;  // this stream's steps; pieces; first ring index of the piece
-  while (run.next(a, p)) {
-    const int base = p.s.len - p.s.rows;
-    const int tile_tok = p.tok0 + (p.both ? st * a.sh.tpt : 0);          // first token of this stream's rows
-    const int toks = min(a.sh.tpt, p.tok0 + p.ntok - tile_tok);
-    const int live = toks * a.G;
-    const int tok = tile_tok + r / a.G;
+  while (true) {
+    if (threadIdx.x == 0) {
+      Run run = bars.run;
+      Piece next;
+      bars.more[pieces & 1] = run.next(a, next);
+      bars.piece[pieces & 1] = next;
+      bars.run = run;
+    }
+    __syncwarp();
+    bar_sync(1, 512);
+    if (!bars.more[pieces & 1]) break;
+    const Piece &p = bars.piece[pieces & 1];
+    const int tile_tok = p.tok0 + (p.both ? st * a.sh.tpt : 0);  // first token of this stream's rows
+    const int live = min(a.sh.tpt, p.tok0 + p.ntok - tile_tok) * a.G;
     // last visible key; rows that do not exist are never masked (nor read)
-    const int lim = r < live ? (a.sh.causal ? base + tok : p.s.len - 1) : INT_MAX;
-    const int lim_first = a.sh.causal ? base + tile_tok : p.s.len - 1;
+    const int lim = r < live ? (a.sh.causal ? p.s.len - p.s.rows + tile_tok + r / a.G : p.s.len - 1) : INT_MAX;
+    // the same of the first row of this stream, and of both
+    const int lim_first = a.sh.causal ? p.s.len - p.s.rows + tile_tok : p.s.len - 1, lim_item = a.sh.causal ? p.s.len - p.s.rows + p.tok0 : p.s.len - 1;
     const bool warp_live = warp4 * 32 < live;
     float m = -INFINITY, l = 0.f;
     const int steps = p.steps(st);
     for (int i = 0; i < steps; i++, step++) {
-      const int t = p.tile(st, i), k0 = t * BN;
+      const int t = p.tile(st, i), k0 = t * BN, kh = k0 + half * N;
       const uint32_t kv = ring + 2 * (uint32_t)(t - p.tb);  // ring index of K; V is the next
       wait(&bars.s_full[st], step & 1);
       tc_fence_after();
       // V elements that only some rows may see, and rows behind the last token
-      const int valid = min(BN, p.s.len - k0);
       bool odd = false;
       const bool both_here = p.both && i < p.n0;  // the other stream works on the same tile
       // a tile that hides keys from some row of either stream that uses it
-      const int lim_item = a.sh.causal ? base + p.tok0 : p.s.len - 1;
       const bool diagonal = (both_here ? lim_item : lim_first) < min(k0 + BN, p.s.len) - 1;
-      uint8_t *sv_tile = sm + C::OFF_KV + ((kv + 1) % C::SLOTS) * C::TILE;
       if constexpr (!INT8) {
-        if (diagonal || valid < BN) {
+        if (diagonal || p.s.len - k0 < BN) {
+          const int valid = min(BN, p.s.len - k0);
+          uint8_t *sv_tile = sm + C::OFF_KV + ((kv + 1) % C::SLOTS) * C::TILE;
           wait(&bars.full[(kv + 1) % C::SLOTS], ((kv + 1) / C::SLOTS) & 1);
           if (valid < BN && !(both_here && st == 1)) {
             const int rows = (valid + 15) / 16 * 16 - valid;
-            for (int c = r; c < rows * (D / 8); c += 128)
+            for (int c = tid; c < rows * (D / 8); c += 256)
               *reinterpret_cast<uint4 *>(sv_tile + chunk_off(valid + c / (D / 8), c % (D / 8))) = make_uint4(0u, 0u, 0u, 0u);
             fence_async_smem();
           }
           if (diagonal) {
             uint32_t found = 0;
-            for (int c = r; c < valid * (D / 8); c += 128) {
+            for (int c = tid; c < valid * (D / 8); c += 256) {
               const uint4 w = *reinterpret_cast<const uint4 *>(sv_tile + chunk_off(c / (D / 8), c % (D / 8)));
               found |= odd_bf16(w.x) | odd_bf16(w.y) | odd_bf16(w.z) | odd_bf16(w.w);
             }
             __syncwarp();
-            odd = bar_or(2 + st, 128, found != 0);
+            odd = bar_or(2 + st, 256, found != 0);
           }
         }
       }
       if (warp_live) {
-        float s[BN];
+        float s[N];
 #pragma unroll
-        for (int c = 0; c < BN / 32; c++) tmem_ld32(tS + c * 32, *reinterpret_cast<float(*)[32]>(s + c * 32));
+        for (int c = 0; c < N / 32; c++) tmem_ld32(tS + c * 32, *reinterpret_cast<float(*)[32]>(s + c * 32));
         tmem_wait_ld();
         // K and V scales of this tile: there until its V is released, after P
-        const float *key_scale = reinterpret_cast<const float *>(sm + C::OFF_SCALE) + (kv / 2 % C::SLOTS) * 2 * BN;
-        if constexpr (INT8) {
-#pragma unroll
-          for (int c = 0; c < BN; c += 4) {
-            const float4 f = *reinterpret_cast<const float4 *>(key_scale + c);
-            s[c] *= f.x;
-            s[c + 1] *= f.y;
-            s[c + 2] *= f.z;
-            s[c + 3] *= f.w;
-          }
-        }
-        const bool masked = !__all_sync(0xffffffffu, k0 + BN - 1 <= lim);
+        const float *key_scale = reinterpret_cast<const float *>(sm + C::OFF_SCALE) + (kv / 2 % C::SLOTS) * 2 * BN + half * N;
+        if constexpr (INT8) scale_keys<N>(s, key_scale);
+        const bool masked = !__all_sync(0xffffffffu, kh + N - 1 <= lim);
         if (masked) {
 #pragma unroll
-          for (int c = 0; c < BN; c++) s[c] = k0 + c <= lim ? s[c] : -INFINITY;
+          for (int c = 0; c < N; c++) s[c] = kh + c <= lim ? s[c] : -INFINITY;
         }
         float mx4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int c = 4; c < BN; c++) mx4[c & 3] = fmaxf(mx4[c & 3], s[c]);
-        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale_log2;
+        for (int c = 4; c + 7 < N; c += 8) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) mx4[e] = max3(mx4[e], s[c + 2 * e], s[c + 2 * e + 1]);
+        }
+        float mx = max3(max3(mx4[0], mx4[1], mx4[2]), max3(mx4[3], s[N - 4], s[N - 3]), fmaxf(s[N - 2], s[N - 1]));
+        // the row's maximum over both halves (the next S, so the next write
+        // here, waits for both halves' P)
+        *x_mine = mx;
+        bar_sync(pair, 64);
+        mx = fmaxf(mx, *x_half) * a.scale_log2;
         const bool grow = mx > m + RESCALE_THRESHOLD;
         const float m_new = grow ? mx : m;
         const float mb = m_new == -INFINITY ? 0.f : m_new;
         const float alpha = grow ? ex2(m - mb) : 1.f;
         m = m_new;
         if (i > 0 && __any_sync(0xffffffffu, grow)) {
-          // s_full of this step came behind the products of the last: O is whole
-#pragma unroll
-          for (int c = 0; c < D / 32; c++) {
-            float o[32];
-            tmem_ld32(tO + c * 32, o);
+          // s_full of this step came behind the products of the last: O is whole.
+          // Each half takes half of its columns.
+#pragma unroll 1
+          for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 8) {
+            float o[8];
+            tmem_ld8(tO + c, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; e++) o[e] *= alpha;
-            tmem_st32(tO + c * 32, o);
+            for (int e = 0; e < 8; e++) o[e] *= alpha;
+            tmem_st8(tO + c, o);
           }
         }
-        float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (INT8) wait(&bars.full[(kv + 1) % C::SLOTS], ((kv + 1) / C::SLOTS) & 1);  // V's scales come with V
+        const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), ref2 = make_float2(-mb, -mb);
+        float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-        for (int c = 0; c < BN; c++) {
-          s[c] = ex2(fmaf(s[c], a.scale_log2, -mb));
-          sum4[c & 3] += s[c];
-        }
-        l = l * alpha + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
-        if constexpr (INT8) {
-          // ready: the K tile's full came before S; V's scales come with V
-          wait(&bars.full[(kv + 1) % C::SLOTS], ((kv + 1) / C::SLOTS) & 1);
-          const float *val_scale = key_scale + BN;
+        for (int c = 0; c < N / 32; c++) {
+          float *v = s + c * 32;
 #pragma unroll
-          for (int c = 0; c < BN; c += 4) {
-            const float4 f = *reinterpret_cast<const float4 *>(val_scale + c);
-            s[c] *= f.x;
-            s[c + 1] *= f.y;
-            s[c + 2] *= f.z;
-            s[c + 3] *= f.w;
+          for (int e = 0; e < 32; e += 2) {
+            const float2 x = fma2(make_float2(v[e], v[e + 1]), scale2, ref2);
+            v[e] = ex2(x.x);
+            v[e + 1] = ex2(x.y);
+            sum2[(e >> 1) & 1] = add2(sum2[(e >> 1) & 1], make_float2(v[e], v[e + 1]));
           }
-          if (masked) {  // 0 * a scale that is not finite
+          if constexpr (INT8) {
+            scale_keys<32>(v, key_scale + BN + c * 32);
+            if (masked) {  // 0 * a scale that is not finite
 #pragma unroll
-            for (int c = 0; c < BN; c++) s[c] = k0 + c <= lim ? s[c] : 0.f;
-          }
-        }
-        if constexpr (!INT8) {
-          if (odd) {
-            // rare: every non-finite V element, added to the rows that see its key
-#pragma unroll
-            for (int c = 0; c < BN / 32; c++) tmem_st32(tS + c * 32, *reinterpret_cast<float(*)[32]>(s + c * 32));
-            if (i == 0) {
-              float z[32];
-#pragma unroll
-              for (int e = 0; e < 32; e++) z[e] = 0.f;
-#pragma unroll
-              for (int c = 0; c < D / 32; c++) tmem_st32(tO + c * 32, z);
+              for (int e = 0; e < 32; e++) v[e] = kh + c * 32 + e <= lim ? v[e] : 0.f;
             }
-            tmem_wait_st();
-            for (int k = 0; k < valid; k++)
-              for (int c = 0; c < D / 8; c++) {
-                const uint4 w = *reinterpret_cast<const uint4 *>(sv_tile + chunk_off(k, c));
-                if (!(odd_bf16(w.x) | odd_bf16(w.y) | odd_bf16(w.z) | odd_bf16(w.w))) continue;
-                const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll 1
-                for (int e = 0; e < 8; e++) {
-                  const uint32_t bits = (ww[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
-                  if ((bits & 0x7F80u) != 0x7F80u) continue;
-                  const float pk = tmem_ld1(tS + k), o = tmem_ld1(tO + c * 8 + e);
-                  tmem_st1(tO + c * 8 + e, k0 + k <= lim ? fmaf(pk, __uint_as_float(bits << 16), o) : o);
-                  tmem_wait_st();
-                }
-              }
           }
-        }
+          uint32_t h[16];
 #pragma unroll
-        for (int c = 0; c < BN / 64; c++) {
-          uint32_t h[32];
-#pragma unroll
-          for (int e = 0; e < 32; e++) h[e] = pack_bf16(s[c * 64 + 2 * e], s[c * 64 + 2 * e + 1]);
-          tmem_st32u(tS + c * 32, h);
+          for (int e = 0; e < 16; e++) h[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
+          tmem_st16u(tS + c * 16, h);
         }
+        l = l * alpha + ((sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y));
         tmem_wait_st();
       }
       if constexpr (!INT8) {
         if (odd) {
-          if (i == 0 && r == 0) bars.acc[st] = 1;
+          // rare: every non-finite V element, added to the rows that see its
+          // key (each half: its keys), one half after the other
+          const int valid = min(BN, p.s.len - k0);
+          uint8_t *sv_tile = sm + C::OFF_KV + ((ring + 2 * (uint32_t)(t - p.tb) + 1) % C::SLOTS) * C::TILE;
+#pragma unroll 1
+          for (int turn = 0; turn < 2; turn++) {
+            if (warp_live && turn == half) {
+              if (i == 0 && half == 0) {
+                const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                for (int c = 0; c < D; c += 8) tmem_st8(tO + c, z);
+                tmem_wait_st();
+              }
+              for (int k = half * N; k < min(valid, (half + 1) * N); k++)
+                for (int c = 0; c < D / 8; c++) {
+                  const uint4 w = *reinterpret_cast<const uint4 *>(sv_tile + chunk_off(k, c));
+                  if (!(odd_bf16(w.x) | odd_bf16(w.y) | odd_bf16(w.z) | odd_bf16(w.w))) continue;
+                  const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll 1
+                  for (int e = 0; e < 8; e++) {
+                    const uint32_t bits = (ww[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
+                    if ((bits & 0x7F80u) != 0x7F80u) continue;
+                    const uint32_t two = __float_as_uint(tmem_ld1(tS + ((k - half * N) >> 1)));
+                    const float pk = __uint_as_float(k & 1 ? two & 0xFFFF0000u : two << 16), o = tmem_ld1(tO + c * 8 + e);
+                    tmem_st1(tO + c * 8 + e, k0 + k <= lim ? fmaf(pk, __uint_as_float(bits << 16), o) : o);
+                    tmem_wait_st();
+                  }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            bar_sync(2 + st, 256);
+            tc_fence_after();
+          }
+          if (i == 0 && tid == 0) bars.acc[st] = 1;
           // every row has taken the odd elements: out of the tile with them
-          __syncwarp();
-          if (both_here) bar_sync(1, 256);
-          else bar_sync(2 + st, 128);
+          if (both_here) bar_sync(1, 512);
           if (!(both_here && st == 1)) {
-            for (int c = r; c < valid * (D / 8); c += 128) {
+            for (int c = tid; c < valid * (D / 8); c += 256) {
               uint4 *at = reinterpret_cast<uint4 *>(sv_tile + chunk_off(c / (D / 8), c % (D / 8)));
               *at = make_uint4(even_bf16(at->x), even_bf16(at->y), even_bf16(at->z), even_bf16(at->w));
             }
             fence_async_smem();
           }
           __syncwarp();
-          if (both_here) bar_sync(1, 256);
+          if (both_here) bar_sync(1, 512);
         }
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.p_full[st]);
     }
-    // ---------------- end of the piece
-    wait(&bars.o_full[st], pieces & 1);
+    // ---------------- end of the piece: l of both halves, of a shared row of
+    // both streams, then O
+    bar_sync(pair, 64);  // the last step's maxima have been read
+    *x_mine = l;
+    bar_sync(pair, 64);
+    l += *x_half;
+    float f0 = 1.f, f1 = 0.f;  // factors of this stream's and the other's O
     if (!p.both) {
-      ml[st * BM + r] = make_float2(m, l);
+      bar_sync(1, 512);
+      *x_mine = half ? l : m;
+      bar_sync(1, 512);
+      const float om = x_row[(st ^ 1) * 2 * BM], ol = x_row[((st ^ 1) * 2 + 1) * BM];
+      const float top = fmaxf(m, om);
+      f0 = m == -INFINITY ? 0.f : ex2(m - top);
+      f1 = om == -INFINITY ? 0.f : ex2(om - top);
+      // NaN sums stay: a stream with steps whose maximum is -inf has l = 0 or NaN
+      l = (m == -INFINITY ? l : l * f0) + (om == -INFINITY ? ol : ol * f1);
+      m = top;
+      bar_sync(1, 512);  // read by all
       wait(&bars.o_full[st ^ 1], pieces & 1);
-      bar_sync(1, 256);
+    } else {
+      bar_sync(pair, 64);
     }
+    wait(&bars.o_full[st], pieces & 1);
     tc_fence_after();
-    const bool mine = r < live;
+    const bool mine = r < live, whole = p.whole();
+    const int tok = tile_tok + r / a.G;
     const size_t row = (size_t)(p.s.row0 + tok) * a.Hq + (size_t)p.head * a.G + r % a.G;
-    const bool whole = p.whole();
     // scratch of an unfinished item: the CTA's first or last part
     float *part = a.ws + (size_t)(blockIdx.x * 2 + (p.tb > 0 ? 0 : 1)) * (kRowsItem * (D + 2));
     const int prow = p.both ? st * BM + r : r;
-    float f0 = 1.f, f1 = 0.f;  // factors of this stream's and the other's O
-    if (!p.both) {
-      const float2 o = ml[(st ^ 1) * BM + r];
-      const float top = fmaxf(m, o.x);
-      f0 = m == -INFINITY ? 0.f : ex2(m - top);
-      f1 = o.x == -INFINITY ? 0.f : ex2(o.x - top);
-      // NaN sums stay: a stream with steps whose maximum is -inf has l = 0 or NaN
-      l = (m == -INFINITY ? l : l * f0) + (o.x == -INFINITY ? o.y : o.y * f1);
-      m = top;
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
     if (warp_live) {
-      // one tile of rows: the streams write half of the columns each
-      const int c0 = p.both ? 0 : st * (D / 2), c1 = p.both ? D : c0 + D / 2;
+      const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+      // the row's threads take D / 2 columns each, or D / 4
+      const int width = p.both ? D / 2 : D / 4, first = p.both ? half * width : (st * 2 + half) * width;
       const bool has0 = steps > 0, has1 = !p.both && p.steps(st ^ 1) > 0;
+      f0 *= inv;
+      f1 *= inv;
 #pragma unroll 1
-      for (int c = c0; c < c1; c += 32) {
-        float o[32];
+      for (int c = first; c < first + width; c += 16) {
+        float o[16], x[16];
 #pragma unroll
-        for (int e = 0; e < 32; e++) o[e] = 0.f;
-        if (has0) {
-          tmem_ld32(tO + c, o);
-          tmem_wait_ld();
+        for (int e = 0; e < 16; e++) o[e] = x[e] = 0.f;
+        if (has0) tmem_ld16(tO + c, o);
+        if (has1) tmem_ld16(tO_other + c, x);
+        tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; e++) o[e] *= f0;
-        }
-        if (has1) {
-          float x[32];
-          tmem_ld32(tO_other + c, x);
-          tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 32; e++) o[e] = fmaf(x[e], f1, o[e]);
-        }
+        for (int e = 0; e < 16; e++) o[e] = has1 ? fmaf(x[e], f1, o[e] * f0) : o[e] * f0;
         if (mine && whole) {
           uint4 *dst = reinterpret_cast<uint4 *>(a.out + row * D + c);
 #pragma unroll
-          for (int q = 0; q < 4; q++)
-            dst[q] = make_uint4(pack_bf16(o[q * 8] * inv, o[q * 8 + 1] * inv), pack_bf16(o[q * 8 + 2] * inv, o[q * 8 + 3] * inv),
-                                pack_bf16(o[q * 8 + 4] * inv, o[q * 8 + 5] * inv), pack_bf16(o[q * 8 + 6] * inv, o[q * 8 + 7] * inv));
+          for (int q = 0; q < 2; q++)
+            dst[q] = make_uint4(pack_bf16(o[q * 8], o[q * 8 + 1]), pack_bf16(o[q * 8 + 2], o[q * 8 + 3]), pack_bf16(o[q * 8 + 4], o[q * 8 + 5]),
+                                pack_bf16(o[q * 8 + 6], o[q * 8 + 7]));
         } else if (mine) {
           float4 *dst = reinterpret_cast<float4 *>(part + (size_t)prow * D + c);
 #pragma unroll
-          for (int q = 0; q < 8; q++) __stcg(dst + q, make_float4(o[q * 4], o[q * 4 + 1], o[q * 4 + 2], o[q * 4 + 3]));
+          for (int q = 0; q < 4; q++) __stcg(dst + q, make_float4(o[q * 4], o[q * 4 + 1], o[q * 4 + 2], o[q * 4 + 3]));
         }
       }
-      if (mine && (p.both || st == 0)) {
-        if (whole) {
-          if (a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
-        } else {
-          __stcg(reinterpret_cast<float2 *>(part + (size_t)kRowsItem * D) + prow, make_float2(m, l));
-        }
+      if (mine && half == 0 && (p.both || st == 0)) {
+        if (!whole) __stcg(reinterpret_cast<float2 *>(part + (size_t)kRowsItem * D) + prow, make_float2(m, l));
+        else if (a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
       }
     }
     tc_fence_before();
-    if (!p.both) bar_sync(1, 256);  // ml has been read
     __syncwarp();
     if (lane == 0) mbar_arrive(&bars.o_free);
     pieces++;
@@ -353,6 +423,19 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
 }
 
 // ------------------------------------------------------------------ MMA warp
+// A ring slot that walks on: K and V of a tile are neighbours, tiles two apart.
+template <int SLOTS>
+struct Slot {
+  uint32_t slot, phase;
+  __device__ __forceinline__ void skip(uint32_t n) {  // n <= SLOTS
+    slot += n;
+    if (slot >= SLOTS) {
+      slot -= SLOTS;
+      phase ^= 1;
+    }
+  }
+};
+
 template <int D, bool INT8, class B>
 __device__ __forceinline__ void mma_role(const ChunkArgs &a, uint8_t *sm, B &bars) {
   using C = Cfg<D, INT8>;
@@ -364,71 +447,92 @@ __device__ __forceinline__ void mma_role(const ChunkArgs &a, uint8_t *sm, B &bar
   Waiter<true> wait{a.err};
   Run run(a);
   Piece p{};
-  uint32_t ring = 0, pieces = 0, psteps[2] = {0, 0};
+  Slot<C::SLOTS> ring{0, 0};  // K of the piece's first tile
+  uint32_t pieces = 0, p_phase = 0;  // p_phase: bit of each stream
+  // S of a stream from the K tile in a slot
+  auto qk = [&](uint32_t st, const Slot<C::SLOTS> &k, bool fresh, bool release) {
+    if (fresh) wait(&bars.full[k.slot], k.phase);
+    tc_fence_after();
+    const uint64_t q = KMAJOR + (s_q + (p.both ? st : 0) * (C::TILE >> 4)), kd = KMAJOR + (s_kv + k.slot * (C::TILE >> 4));
+#pragma unroll
+    for (int x = 0; x < D / 16; x++) {
+      const uint32_t off = ((x >> 2) * C::SLAB + (x & 3) * 32) >> 4;
+      mma_ss(one, tmem + st * 128, q + off, kd + off, ID_QK, x > 0 ? 1u : 0u);
+    }
+    mma_commit(one, &bars.s_full[st]);
+    if (release) mma_commit(one, &bars.empty[k.slot]);
+  };
+  // O of a stream plus its P times the V tile in a slot (k16: its 16s of keys)
+  auto pv = [&](uint32_t st, const Slot<C::SLOTS> &v, bool first, int k16, bool fresh, bool release) {
+    if (fresh) wait(&bars.full[v.slot], v.phase);
+    wait(&bars.p_full[st], (p_phase >> st) & 1);
+    p_phase ^= 1u << st;
+    tc_fence_after();
+    uint32_t acc = first ? 0u : 1u;
+    if (!INT8 && first && __shfl_sync(0xffffffffu, *(volatile int *)&bars.acc[st], 0)) {
+      acc = 1u;
+      __syncwarp();
+      *(volatile int *)&bars.acc[st] = 0;
+    }
+    const uint64_t vd = VMAJOR + (s_kv + v.slot * (C::TILE >> 4));
+    const uint32_t t_o = tmem + 256 + st * 128, t_p = tmem + st * 128;
+    // P of 64 keys is in the first 32 columns of each half of S
+#pragma unroll
+    for (int x = 0; x < BN / 16; x++)
+      if (x < k16) mma_ts(one, t_o, t_p + (x >> 2) * 64 + (x & 3) * 8, vd + (x * 2048 >> 4), ID_PV, x > 0 ? 1u : acc);
+    if (release) mma_commit(one, &bars.empty[v.slot]);
+  };
   while (run.next(a, p)) {
     const int tiles = max(0, p.te - p.tb);
-    bool o_mine = pieces == 0;  // the softmax warps have read the last piece's O
-    auto own_o = [&]() {
-      if (!o_mine) wait(&bars.o_free, (pieces - 1) & 1);
-      o_mine = true;
-    };
+    // the last tile of the sequence holds fewer keys
+    const int last = (p.s.len - 1) / BN - p.tb, last16 = (p.s.len - (p.tb + last) * BN + 15) / 16;
+    Slot<C::SLOTS> k = ring, v = ring;
+    v.skip(1);
     wait(&bars.q_full, pieces & 1);
-    auto issue_s = [&](int st, int i) {
-      const uint32_t kv = ring + 2 * (uint32_t)(p.tile(st, i) - p.tb), slot = kv % C::SLOTS;
-      wait(&bars.full[slot], (kv / C::SLOTS) & 1);
-      tc_fence_after();
-      const uint64_t q = KMAJOR + (s_q + (p.both ? st : 0) * (C::TILE >> 4)), k = KMAJOR + (s_kv + slot * (C::TILE >> 4));
-#pragma unroll
-      for (int x = 0; x < D / 16; x++) {
-        const uint32_t off = ((x >> 2) * C::SLAB + (x & 3) * 32) >> 4;
-        mma_ss(one, tmem + st * 128, q + off, k + off, ID_QK, x > 0 ? 1u : 0u);
-      }
-      mma_commit(one, &bars.s_full[st]);
-      if (!p.both || st == 1) mma_commit(one, &bars.empty[slot]);  // stream 1 is the last to use a shared tile
-    };
-    auto issue_pv = [&](int st, int i) {
-      const int t = p.tile(st, i);
-      const uint32_t kv = ring + 2 * (uint32_t)(t - p.tb) + 1, slot = kv % C::SLOTS;
-      own_o();
-      wait(&bars.p_full[st], psteps[st]++ & 1);
-      wait(&bars.full[slot], (kv / C::SLOTS) & 1);
-      tc_fence_after();
-      const uint64_t v = VMAJOR + (s_kv + slot * (C::TILE >> 4));
-      uint32_t acc = i > 0 ? 1u : 0u;
-      if (!INT8 && i == 0 && __shfl_sync(0xffffffffu, *(volatile int *)&bars.acc[st], 0)) {
-        acc = 1u;
-        __syncwarp();
-        *(volatile int *)&bars.acc[st] = 0;
-      }
-      const int k16 = (min(BN, p.s.len - t * BN) + 15) / 16;
-      if (k16 == BN / 16) {
-#pragma unroll
-        for (int x = 0; x < BN / 16; x++)
-          mma_ts(one, tmem + 256 + st * 128, tmem + st * 128 + x * 8, v + (x * 2048 >> 4), ID_PV, x > 0 ? 1u : acc);
-      } else {
-        for (int x = 0; x < k16; x++)
-          mma_ts(one, tmem + 256 + st * 128, tmem + st * 128 + x * 8, v + (x * 2048 >> 4), ID_PV, x > 0 ? 1u : acc);
-      }
-      if (!p.both || st == 1) mma_commit(one, &bars.empty[slot]);
-    };
-    if (p.n0 > 0) issue_s(0, 0);
-    if (p.n1 > 0) issue_s(1, 0);
-    const int steps = max(p.n0, p.n1);
-    for (int i = 0; i < steps; i++)
-#pragma unroll
-      for (int st = 0; st < 2; st++) {
-        const int n = p.steps(st);
-        if (i < n) {
-          issue_pv(st, i);
-          if (i + 1 < n) issue_s(st, i + 1);
-          else mma_commit(one, &bars.o_full[st]);
+    // the softmax warps have read the last piece's O before the first product
+    if (tiles == 0 && pieces > 0) wait(&bars.o_free, (pieces - 1) & 1);
+    if (p.both) {
+      // both streams use a tile; stream 1 sees at least as many
+      if (p.n0 > 0) qk(0, k, true, false);
+      if (p.n1 > 0) qk(1, k, p.n0 == 0, true);
+      if (tiles > 0 && pieces > 0) wait(&bars.o_free, (pieces - 1) & 1);
+#pragma unroll 1
+      for (int i = 0; i < p.n1; i++) {
+        const int k16 = i == last ? last16 : BN / 16;
+        k.skip(2);
+        if (i < p.n0) {
+          pv(0, v, i == 0, k16, true, false);
+          if (i + 1 < p.n0) qk(0, k, true, false);
+          else mma_commit(one, &bars.o_full[0]);
         }
+        pv(1, v, i == 0, k16, i >= p.n0, true);
+        if (i + 1 < p.n1) qk(1, k, i + 1 >= p.n0, true);
+        else mma_commit(one, &bars.o_full[1]);
+        v.skip(2);
       }
+    } else {
+      // tile i belongs to stream i & 1; S runs two tiles ahead
+      for (int i = 0; i < 2 && i < tiles; i++) {
+        qk(i, k, true, true);
+        k.skip(2);
+      }
+      if (tiles > 0 && pieces > 0) wait(&bars.o_free, (pieces - 1) & 1);
+#pragma unroll 1
+      for (int i = 0; i < tiles; i++) {
+        const uint32_t st = i & 1;
+        pv(st, v, i < 2, i == last ? last16 : BN / 16, true, true);
+        if (i + 2 < tiles) qk(st, k, true, true);
+        else mma_commit(one, &bars.o_full[st]);
+        k.skip(2);
+        v.skip(2);
+      }
+    }
     mma_commit(one, &bars.q_empty);
-    own_o();
     if (p.n0 == 0) mma_commit(one, &bars.o_full[0]);
     if (p.n1 == 0) mma_commit(one, &bars.o_full[1]);
-    ring += 2 * (uint32_t)tiles;
+    ring = v;
+    ring.skip(C::SLOTS - 1);  // V of the tile behind the last, less one
+    ring.phase ^= 1;
     pieces++;
   }
 }
@@ -501,7 +605,9 @@ __device__ __forceinline__ void tma_role(const CUtensorMap *tq, const CUtensorMa
 template <int D, class B>
 __device__ __forceinline__ void convert_role(const ChunkArgs &a, uint8_t *sm, B &bars) {
   using C = Cfg<D, true>;
-  const int r = threadIdx.x & 127, lane = threadIdx.x & 31;
+  const int tid = threadIdx.x - 640, lane = threadIdx.x & 31;
+  const int r = tid & 127, v_scale = tid >> 7;  // thread of K scales, or of V scales
+  constexpr int N = BN * D / 16 / 256;
   Waiter<true> wait{a.err};
   Run run(a);
   Piece p{};
@@ -512,7 +618,7 @@ __device__ __forceinline__ void convert_role(const ChunkArgs &a, uint8_t *sm, B 
       const int tok = t * BN + r, valid = min(BN, p.s.len - t * BN);
       size_t row = 0;
       if (r < valid) row = ((size_t)__ldg(table + tok / a.bs) * a.Hkv + p.head) * a.bs + tok % a.bs;
-      const float scale[2] = {r < valid ? __ldcg(a.sk + row) : 0.f, r < valid ? __ldcg(a.sv + row) : 0.f};
+      const float scale = r < valid ? __ldcg((v_scale ? a.sv : a.sk) + row) : 0.f;
 #pragma unroll
       for (int v = 0; v < 2; v++, idx++) {
         const uint32_t raw = idx % C::RAWS, slot = idx % C::SLOTS;
@@ -522,13 +628,18 @@ __device__ __forceinline__ void convert_role(const ChunkArgs &a, uint8_t *sm, B 
         uint8_t *dst = sm + C::OFF_KV + slot * C::TILE;
         // V of tile t holds its slot until the softmax has used both of the
         // tile's scales, so this warpgroup is less than SLOTS tiles ahead
-        reinterpret_cast<float *>(sm + C::OFF_SCALE)[(idx / 2 % C::SLOTS * 2 + v) * BN + r] = scale[v];
+        if (v_scale == v) reinterpret_cast<float *>(sm + C::OFF_SCALE)[(idx / 2 % C::SLOTS * 2 + v) * BN + r] = scale;
         // 16 codes at a time; rows behind the last token become zeros
-#pragma unroll 4
-        for (int c = r; c < BN * D / 16; c += 128) {
-          const int row_t = c / (D / 16), ch = c % (D / 16);
-          const uint4 w = row_t < valid ? *reinterpret_cast<const uint4 *>(src + c * 16) : make_uint4(0u, 0u, 0u, 0u);
-          const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+        uint4 codes[N];
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+          const int c = tid + n * 256;
+          codes[n] = c / (D / 16) < valid ? *reinterpret_cast<const uint4 *>(src + c * 16) : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+          const int c = tid + n * 256, row_t = c / (D / 16), ch = c % (D / 16);
+          const uint32_t in[4] = {codes[n].x, codes[n].y, codes[n].z, codes[n].w};
           uint32_t o[8];
 #pragma unroll
           for (int e = 0; e < 4; e++)
@@ -537,7 +648,7 @@ __device__ __forceinline__ void convert_role(const ChunkArgs &a, uint8_t *sm, B 
               // bytes (b0, b1) -> bf16 pair of the codes: low 7 bits on the magic
               // 0x43 give 128 + low7, the sign bit on it 128 or 256; their
               // difference is the code, exactly
-              const uint32_t x = __byte_perm(in[e], 0x43434343u, half ? 0x4342u | 0x0000u : 0x4140u);
+              const uint32_t x = __byte_perm(in[e], 0x43434343u, half ? 0x4342u : 0x4140u);
               uint32_t d;
               asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(x & 0xFF7FFF7Fu), "r"(x & 0xFF80FF80u));
               o[e * 2 + half] = d;
@@ -562,7 +673,7 @@ __global__ void __launch_bounds__(Cfg<D, INT8>::THREADS, 1)
                       const __grid_constant__ CUtensorMap tv, const __grid_constant__ ChunkArgs a) {
   using C = Cfg<D, INT8>;
   using B = Bars<C::SLOTS, C::RAWS>;
-  static_assert(sizeof(B) <= 512, "barriers");
+  static_assert(sizeof(B) <= 768, "barriers");
   extern __shared__ __align__(1024) uint8_t sm[];
   B &bars = *reinterpret_cast<B *>(sm + C::OFF_BARS);
   const int warp = threadIdx.x >> 5;
@@ -573,22 +684,23 @@ __global__ void __launch_bounds__(Cfg<D, INT8>::THREADS, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   if (threadIdx.x == 32) {
+    bars.run = Run(a);
     mbar_init(&bars.q_full, 1);
     mbar_init(&bars.q_empty, 1);
-    mbar_init(&bars.o_free, 8);
+    mbar_init(&bars.o_free, 16);
     for (int i = 0; i < 2; i++) {
       mbar_init(&bars.s_full[i], 1);
-      mbar_init(&bars.p_full[i], 4);
+      mbar_init(&bars.p_full[i], 8);
       mbar_init(&bars.o_full[i], 1);
       bars.acc[i] = 0;
     }
     for (int i = 0; i < C::SLOTS; i++) {
-      mbar_init(&bars.full[i], INT8 ? 4 : 1);
+      mbar_init(&bars.full[i], INT8 ? 8 : 1);
       mbar_init(&bars.empty[i], 1);
     }
     for (int i = 0; i < C::RAWS; i++) {
       mbar_init(&bars.raw_full[i], 1);
-      mbar_init(&bars.raw_empty[i], 4);
+      mbar_init(&bars.raw_empty[i], 8);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -596,14 +708,14 @@ __global__ void __launch_bounds__(Cfg<D, INT8>::THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars.tmem;
-  if (warp < 8) {
+  if (warp < 16) {
     regs_inc<C::REG_SOFT>();
-    softmax_role<D, INT8>(a, sm, bars, warp >> 2);
-  } else if (warp < 12) {
+    softmax_role<D, INT8>(a, sm, bars);
+  } else if (warp < 20) {
     regs_dec<C::REG_PROD>();
-    if (warp == 8) {
+    if (warp == 16) {
       mma_role<D, INT8>(a, sm, bars);
-    } else if (warp == 9) {
+    } else if (warp == 17) {
       tma_role<D, INT8>(&tq, &tk, &tv, a, sm, bars);
     }
   } else {
