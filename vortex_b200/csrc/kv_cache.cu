@@ -439,9 +439,16 @@ VXB_API int vxb_kv_append_seq(vxb_kv *kv, int layer, int64_t seq_id, int n_token
 namespace {
 
 // A sequence listed twice in one call (the calls below change each sequence once)
-bool listed_twice(std::vector<int64_t> ids) {
-  std::sort(ids.begin(), ids.end());
-  return std::adjacent_find(ids.begin(), ids.end()) != ids.end();
+bool listed_twice(const int64_t *ids, int n) {
+  if (n <= 48) {
+    for (int i = 1; i < n; i++)
+      for (int j = 0; j < i; j++)
+        if (ids[i] == ids[j]) return true;
+    return false;
+  }
+  std::vector<int64_t> sorted(ids, ids + n);
+  std::sort(sorted.begin(), sorted.end());
+  return std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end();
 }
 
 // Drop the tokens of one table behind `len` (host side): emptied blocks go
@@ -470,40 +477,52 @@ int append_chunks(vxb_kv *kv, int layer, int n, const int64_t *ids, const int32_
   if (total == 0) return VXB_OK;
   if (!d_k || !d_v || ((uintptr_t)d_k | (uintptr_t)d_v) % 16)
     return set_error(ctx, VXB_EINVAL, "vxb_kv_append_chunks: d_k and d_v must be 16-byte aligned device pointers");
-  if (listed_twice(std::vector<int64_t>(ids, ids + n)))
+  if (listed_twice(ids, n))
     return set_error(ctx, VXB_EINVAL, "vxb_kv_append_chunks: a sequence is listed twice");
   // everything is checked before anything is taken
+  struct Seq {
+    vxb_kv::Table *table;  // null: not there yet, or no tokens
+    int64_t len;
+    int slot;  // -1: none yet
+  };
+  std::vector<Seq> seqs(n, Seq{nullptr, 0, -1});
   for (int i = 0; i < n; i++) {
     if (counts[i] == 0) continue;
     auto it = kv->tables.find(std::make_pair(layer, ids[i]));
-    const int64_t len = it == kv->tables.end() ? 0 : it->second.len;
-    const int64_t have = (len + bs - 1) / bs, want = (len + counts[i] + bs - 1) / bs;
-    if (want > kv->max_blocks_per_seq || len + counts[i] > INT_MAX)
+    auto si = kv->slot_of.find(ids[i]);
+    Seq &q = seqs[i];
+    if (it != kv->tables.end()) {
+      q.table = &it->second;
+      q.len = it->second.len;
+    }
+    if (si == kv->slot_of.end()) new_slots++;
+    else q.slot = si->second;
+    const int64_t have = (q.len + bs - 1) / bs, want = (q.len + counts[i] + bs - 1) / bs;
+    if (want > kv->max_blocks_per_seq || q.len + counts[i] > INT_MAX)
       return set_error(ctx, VXB_ENOBLOCKS, "sequence %lld exceeds max_blocks_per_seq=%d", (long long)ids[i], kv->max_blocks_per_seq);
     need += want - have;
-    if (!kv->slot_of.count(ids[i])) new_slots++;
   }
   if (need > (int64_t)kv->free_blocks.size()) return set_error(ctx, VXB_ENOBLOCKS, "KV cache out of blocks");
   if (new_slots > kv->free_slots.size())
     return set_error(ctx, VXB_ENOBLOCKS, "KV cache has no free sequence slot (max_seqs=%d)", kv->max_seqs);
 
-  // host tables: blocks and lengths, remembered for the launches
-  struct Seq {
-    vxb_kv::Table *table;
-    int64_t len;
-    int slot;
-  };
-  std::vector<Seq> seqs(n, Seq{nullptr, 0, 0});
+  // host tables: blocks and lengths, remembered for the launches. What may
+  // throw comes before what takes blocks.
   for (int i = 0; i < n; i++) {
     if (counts[i] == 0) continue;
-    vxb_kv::Table &t = kv->tables[std::make_pair(layer, ids[i])];
-    const int64_t want = (t.len + counts[i] + bs - 1) / bs;
-    t.blocks.reserve((size_t)want);
-    if (!kv->slot_of.count(ids[i])) {
-      kv->slot_of[ids[i]] = kv->free_slots.back();
+    Seq &q = seqs[i];
+    if (!q.table) q.table = &kv->tables[std::make_pair(layer, ids[i])];
+    const int64_t want = (q.len + counts[i] + bs - 1) / bs;
+    if ((int64_t)q.table->blocks.capacity() < want) q.table->blocks.reserve((size_t)std::max<int64_t>(want, 2 * q.len / bs));
+    if (q.slot < 0) {
+      q.slot = kv->slot_of[ids[i]] = kv->free_slots.back();
       kv->free_slots.pop_back();
     }
-    seqs[i] = {&t, t.len, kv->slot_of.at(ids[i])};
+  }
+  for (int i = 0; i < n; i++) {
+    if (counts[i] == 0) continue;
+    vxb_kv::Table &t = *seqs[i].table;
+    const int64_t want = (t.len + counts[i] + bs - 1) / bs;
     while ((int64_t)t.blocks.size() < want) {
       t.blocks.push_back(kv->free_blocks.back());
       kv->refs[kv->free_blocks.back()] = 1;
@@ -578,20 +597,26 @@ int truncate(vxb_kv *kv, int n, const int64_t *ids, const int64_t *lens, cudaStr
   const int bs = kv->block_size;
   for (int i = 0; i < n; i++)
     if (lens[i] < 0) return set_error(ctx, VXB_EINVAL, "vxb_kv_truncate: sequence %lld to %lld tokens", (long long)ids[i], (long long)lens[i]);
-  if (listed_twice(std::vector<int64_t>(ids, ids + n))) return set_error(ctx, VXB_EINVAL, "vxb_kv_truncate: a sequence is listed twice");
+  if (listed_twice(ids, n)) return set_error(ctx, VXB_EINVAL, "vxb_kv_truncate: a sequence is listed twice");
   struct Cut {
     vxb_kv::Table *table;
     int64_t len;
     int layer, slot;
   };
   std::vector<Cut> cuts, moves;  // moves: cuts inside a shared block
+  std::vector<int> slots(n, -1);
+  for (int i = 0; i < n; i++) {
+    auto si = kv->slot_of.find(ids[i]);
+    if (si != kv->slot_of.end()) slots[i] = si->second;
+  }
   int64_t freed = 0;
   for (int layer = kv->num_layers - 1; layer >= 0; layer--)
     for (int i = n - 1; i >= 0; i--) {
+      if (slots[i] < 0) continue;
       auto it = kv->tables.find(std::make_pair(layer, ids[i]));
       if (it == kv->tables.end() || it->second.len <= lens[i]) continue;
       vxb_kv::Table &t = it->second;
-      cuts.push_back({&t, lens[i], layer, kv->slot_of.at(ids[i])});
+      cuts.push_back({&t, lens[i], layer, slots[i]});
       for (size_t b = (size_t)((lens[i] + bs - 1) / bs); b < t.blocks.size(); b++) freed += kv->refs[t.blocks[b]] == 1;
       if (lens[i] % bs && kv->refs[t.blocks[(size_t)(lens[i] / bs)]] > 1) moves.push_back(cuts.back());
     }
@@ -619,9 +644,8 @@ int truncate(vxb_kv *kv, int n, const int64_t *ids, const int64_t *lens, cudaStr
   for (int i0 = 0; i0 < n;) {
     a.n = 0;
     for (; i0 < n && a.n < kCutSeqs; i0++) {
-      auto si = kv->slot_of.find(ids[i0]);
-      if (si == kv->slot_of.end() || lens[i0] > INT_MAX) continue;
-      a.slot[a.n] = si->second;
+      if (slots[i0] < 0 || lens[i0] > INT_MAX) continue;
+      a.slot[a.n] = slots[i0];
       a.len[a.n++] = (int32_t)lens[i0];
     }
     if (a.n == 0) continue;

@@ -1,9 +1,12 @@
 // Token probabilities and verification of drafted tokens.
 //
-// vxb_token_probs: p = exp((x - max) / t) / sum per row of logits. Bound by
-// reading the row once and writing it once, so a row stays in registers
-// between the two: a cluster of up to 8 CTAs takes a row (32 values a thread
-// at most), its maximum and its sum go through distributed shared memory.
+// vxb_token_probs: p = exp((x - max) / t) / sum per row of logits: the row is
+// read once from HBM and written once. Few rows: a cluster of up to 8 CTAs
+// keeps its row in registers (latency: 4.7 us for 5 rows of 32,000). Many rows:
+// one pass for the running maximum and sum and a second over the row, which
+// the L2 still holds; no registers are tied up, so the SMs stay full of loads
+// (the register form reached 2.0 TB/s on 160 rows of 131,071). Maximum and sum
+// go through distributed shared memory.
 //
 // vxb_verify_drafts: the accept tests are a handful of gathers; the token that
 // is drawn needs one row of p (and q): a cluster per request sums its slices
@@ -23,7 +26,7 @@ namespace {
 constexpr int kMaxCluster = 8;
 
 // ------------------------------------------------------------------ probabilities
-constexpr int kProbThreads = 512;
+constexpr int kProbThreads = 512, kRowThreads = 256;  // of the two forms
 
 struct ProbArgs {
   const float *x, *temp;
@@ -33,50 +36,67 @@ struct ProbArgs {
 };
 
 // max over a CTA (every thread gets it); NaN passed over
+template <int THREADS>
 __device__ float block_max(float v, float *s) {
   v = warp_max(v);
   if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
   __syncthreads();
   float r = s[0];
-  for (int i = 1; i < kProbThreads / 32; i++) r = fmaxf(r, s[i]);
+  for (int i = 1; i < THREADS / 32; i++) r = fmaxf(r, s[i]);
   __syncthreads();
   return r;
 }
 
+template <int THREADS>
 __device__ float block_sum(float v, float *s) {
   v = warp_sum(v);
   if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
   __syncthreads();
   float r = 0.f;
-  for (int i = 0; i < kProbThreads / 32; i++) r += s[i];
+  for (int i = 0; i < THREADS / 32; i++) r += s[i];
   __syncthreads();
   return r;
 }
 
+template <int THREADS>
 __device__ int block_min(int v, int *s) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = min(v, __shfl_xor_sync(0xffffffffu, v, o));
   if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
   __syncthreads();
   int r = s[0];
-  for (int i = 1; i < kProbThreads / 32; i++) r = min(r, s[i]);
+  for (int i = 1; i < THREADS / 32; i++) r = min(r, s[i]);
   __syncthreads();
   return r;
 }
 
-// exp(d) with d = (x - max) / t <= 0. c + c_lo = log2(e) / t: the rounding of
-// d * c and the low part of c enter to first order, so the result keeps the
-// special-function unit's 2 ulp however far d is from 0.
-__device__ __forceinline__ float exp_scaled(float d, float c, float c_lo) {
-  const float y = d * c;
-  const float rest = fmaf(d, c_lo, fmaf(d, c, -y));
+// exp(d / t) with d = x - max <= 0 and c = log2(e) / t: the roundings of c and
+// of the product cost 1.5 * 2^-24 of |d| / t, the special-function unit 2 ulp.
+__device__ __forceinline__ float exp_scaled(float d, float c) {
   float e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(y));
-  return d == -INFINITY ? 0.f : fmaf(e, rest * 0.69314718055994531f, e);
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(d * c));
+  return e;
+}
+// (never 0: -inf, a banned token, stays -inf at any temperature)
+__device__ __forceinline__ float log2e_over(double t) { return fmaxf((float)(1.4426950408889634074 / t), 1e-37f); }
+
+// The cluster's maximum (NaN passed over), and its first index: 1 there, 0
+// elsewhere. Ranks take [begin, end) of the row; every thread's `m` is the
+// maximum of what it has seen.
+template <int THREADS>
+__device__ void one_hot(cg::cluster_group &cl, const float *x, float *p, int begin, int end, float m, int *s_redi, int *s_first) {
+  int first = INT_MAX;
+  for (int c = begin + (int)threadIdx.x; c < end && first == INT_MAX; c += THREADS)
+    if (x[c] == m && m != -INFINITY) first = c;
+  first = block_min<THREADS>(first, s_redi);
+  if (threadIdx.x == 0) *s_first = first;
+  cl.sync();  // every rank has read its part: p may be x
+  for (int i = 0; i < (int)cl.num_blocks(); i++) first = min(first, *cl.map_shared_rank(s_first, i));
+  for (int c = begin + (int)threadIdx.x; c < end; c += THREADS) p[c] = c == first ? 1.f : 0.f;
+  cl.sync();  // the others' shared memory stays until they have read it
 }
 
-// PER: values of a row that a thread holds (0: rows too long for a cluster's
-// registers, read a second time)
+// PER: values of a row that a thread keeps
 template <int PER>
 __global__ void __launch_bounds__(kProbThreads) token_probs_kernel(const ProbArgs a) {
   cg::cluster_group cl = cg::this_cluster();
@@ -90,77 +110,143 @@ __global__ void __launch_bounds__(kProbThreads) token_probs_kernel(const ProbArg
   const float *x = a.x + (size_t)row * a.vocab;
   float *p = a.p + (size_t)row * a.vocab;
   const double t = a.temp ? (double)a.temp[row] : a.t;
-  const bool greedy = !(t >= 0.01);
-  float v[PER > 0 ? PER : 1];
+  float v[PER];
   float m = -INFINITY;
-  if constexpr (PER > 0) {
 #pragma unroll
-    for (int i = 0; i < PER; i++) {
-      const int c = begin + i * kProbThreads + (int)threadIdx.x;
-      v[i] = c < end ? __ldcs(x + c) : -INFINITY;
-    }
-#pragma unroll
-    for (int i = 0; i < PER; i++) m = fmaxf(m, v[i]);
-  } else {
-    for (int c = begin + (int)threadIdx.x; c < end; c += kProbThreads) m = fmaxf(m, x[c]);
+  for (int i = 0; i < PER; i++) {
+    const int c = begin + i * kProbThreads + (int)threadIdx.x;
+    v[i] = c < end ? __ldcs(x + c) : -INFINITY;
   }
-  m = block_max(m, s_red);
+#pragma unroll
+  for (int i = 0; i < PER; i++) m = fmaxf(m, v[i]);
+  m = block_max<kProbThreads>(m, s_red);
   if (threadIdx.x == 0) s_max = m;
   cl.sync();
   for (int i = 0; i < ranks; i++) m = fmaxf(m, *cl.map_shared_rank(&s_max, i));
-  if (greedy) {
-    int first = INT_MAX;
-    if constexpr (PER > 0) {
-#pragma unroll
-      for (int i = PER - 1; i >= 0; i--)
-        if (v[i] == m && m != -INFINITY) first = begin + i * kProbThreads + (int)threadIdx.x;
-    } else {
-      for (int c = begin + (int)threadIdx.x; c < end && first == INT_MAX; c += kProbThreads)
-        if (x[c] == m && m != -INFINITY) first = c;
-    }
-    first = block_min(first, s_redi);
-    if (threadIdx.x == 0) s_first = first;
-    cl.sync();
-    for (int i = 0; i < ranks; i++) first = min(first, *cl.map_shared_rank(&s_first, i));
-    for (int c = begin + (int)threadIdx.x; c < end; c += kProbThreads) p[c] = c == first ? 1.f : 0.f;
-    cl.sync();  // the others' shared memory stays until they have read it
+  if (!(t >= 0.01)) {
+    one_hot<kProbThreads>(cl, x, p, begin, end, m, s_redi, &s_first);
     return;
   }
-  const double c64 = 1.4426950408889634074 / t;
-  const float c = (float)c64, c_lo = (float)(c64 - (double)c);
+  const float c = log2e_over(t);
+  const float ref = m == -INFINITY ? 0.f : m;  // -inf alone gives zeros, NaN beside it NaN
   float sum = 0.f;
-  if (m != -INFINITY) {
-    if constexpr (PER > 0) {
 #pragma unroll
-      for (int i = 0; i < PER; i++) {
-        v[i] = exp_scaled(v[i] - m, c, c_lo);
-        sum += v[i];
-      }
-    } else {
-      for (int i = begin + (int)threadIdx.x; i < end; i += kProbThreads) sum += exp_scaled(x[i] - m, c, c_lo);
-    }
+  for (int i = 0; i < PER; i++) {
+    v[i] = exp_scaled(v[i] - ref, c);
+    sum += v[i];
   }
-  sum = block_sum(sum, s_red);
+  sum = block_sum<kProbThreads>(sum, s_red);
   if (threadIdx.x == 0) s_sum = sum;
   cl.sync();
   sum = 0.f;
   for (int i = 0; i < ranks; i++) sum += *cl.map_shared_rank(&s_sum, i);
-  const float inv = m == -INFINITY ? 0.f : 1.f / sum;
-  if constexpr (PER > 0) {
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-    for (int i = 0; i < PER; i++) {
-      const int k = begin + i * kProbThreads + (int)threadIdx.x;
-      if (k < end) p[k] = m == -INFINITY ? 0.f : v[i] * inv;
-    }
-  } else {
-    for (int k = begin + (int)threadIdx.x; k < end; k += kProbThreads)
-      p[k] = m == -INFINITY ? 0.f : exp_scaled(x[k] - m, c, c_lo) * inv;
+  for (int i = 0; i < PER; i++) {
+    const int k = begin + i * kProbThreads + (int)threadIdx.x;
+    if (k < end) p[k] = v[i] * inv;
   }
   cl.sync();
 }
 
+// Two passes over the row. Four values a load where x and p have the same
+// place within 16 bytes (VEC): `head` single ones lead to the first boundary,
+// the cluster's ranks share the fours, the last rank takes the rest.
+template <bool VEC>
+__global__ void __launch_bounds__(kRowThreads, 5) token_probs_rows_kernel(const ProbArgs a) {
+  cg::cluster_group cl = cg::this_cluster();
+  __shared__ float s_red[kRowThreads / 32];
+  __shared__ int s_redi[kRowThreads / 32];
+  __shared__ float s_max, s_sum;
+  __shared__ int s_first;
+  const int ranks = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+  const int row = (int)(blockIdx.x / ranks);
+  const float *x = a.x + (size_t)row * a.vocab;
+  float *p = a.p + (size_t)row * a.vocab;
+  const double t = a.temp ? (double)a.temp[row] : a.t;
+  const int head = VEC ? min((int)((16 - ((uintptr_t)x & 15)) & 15) / 4, a.vocab) : 0;
+  const int fours = VEC ? (a.vocab - head) / 4 : 0, share = (fours + ranks - 1) / ranks;
+  const int b4 = min(rank * share, fours), e4 = min(b4 + share, fours);
+  const float4 *x4 = reinterpret_cast<const float4 *>(x + head);
+  float4 *p4 = reinterpret_cast<float4 *>(p + head);
+  // single values of this rank: VEC the head (rank 0) and the rest (last rank), else a slice
+  const int rest = head + 4 * fours;
+  const int s0 = VEC ? (rank == ranks - 1 ? rest : a.vocab) : min(rank * a.slice, a.vocab);
+  const int s1 = VEC ? a.vocab : min(s0 + a.slice, a.vocab);
+  if (!(t >= 0.01)) {
+    const int begin = min(rank * a.slice, a.vocab), end = min(begin + a.slice, a.vocab);
+    float m = -INFINITY;
+    for (int k = begin + (int)threadIdx.x; k < end; k += kRowThreads) m = fmaxf(m, x[k]);
+    m = block_max<kRowThreads>(m, s_red);
+    if (threadIdx.x == 0) s_max = m;
+    cl.sync();
+    for (int i = 0; i < ranks; i++) m = fmaxf(m, *cl.map_shared_rank(&s_max, i));
+    one_hot<kRowThreads>(cl, x, p, begin, end, m, s_redi, &s_first);
+    return;
+  }
+  const float c = log2e_over(t);
+  // running maximum and sum of this thread
+  float m = -INFINITY, sum = 0.f;
+  auto take = [&](float top, auto &&weights) {  // weights(ref): sum of exp of the new values
+    if (top > m) {
+      sum *= exp_scaled(m - top, c);
+      m = top;
+    }
+    sum += weights(m == -INFINITY ? 0.f : m);
+  };
+  auto e = [&](float y) { return exp_scaled(y, c); };
+  constexpr int U = 4;  // loads under way
+  for (int k = b4 + (int)threadIdx.x; k < e4; k += U * kRowThreads) {
+    float4 u[U];
+#pragma unroll
+    for (int i = 0; i < U; i++)
+      u[i] = k + i * kRowThreads < e4 ? x4[k + i * kRowThreads] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < U; i++) top = fmaxf(top, fmaxf(fmaxf(u[i].x, u[i].y), fmaxf(u[i].z, u[i].w)));
+    take(top, [&](float r) {
+      float w[U];
+#pragma unroll
+      for (int i = 0; i < U; i++) w[i] = (e(u[i].x - r) + e(u[i].y - r)) + (e(u[i].z - r) + e(u[i].w - r));
+      return (w[0] + w[1]) + (w[2] + w[3]);
+    });
+  }
+  auto single = [&](auto &&f) {
+    if (VEC && rank == 0)
+      for (int k = (int)threadIdx.x; k < head; k += kRowThreads) f(k);
+    for (int k = s0 + (int)threadIdx.x; k < s1; k += kRowThreads) f(k);
+  };
+  single([&](int k) {
+    const float y = x[k];
+    take(y, [&](float r) { return e(y - r); });
+  });
+  // the row's, from those of the threads
+  float top = block_max<kRowThreads>(m, s_red);
+  if (threadIdx.x == 0) s_max = top;
+  cl.sync();
+  for (int i = 0; i < ranks; i++) top = fmaxf(top, *cl.map_shared_rank(&s_max, i));
+  sum = block_sum<kRowThreads>(m == -INFINITY ? sum : sum * e(m - top), s_red);
+  if (threadIdx.x == 0) s_sum = sum;
+  cl.sync();
+  sum = 0.f;
+  for (int i = 0; i < ranks; i++) sum += *cl.map_shared_rank(&s_sum, i);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum, ref = top == -INFINITY ? 0.f : top;
+  for (int k = b4 + (int)threadIdx.x; k < e4; k += U * kRowThreads) {
+    float4 u[U];
+#pragma unroll
+    for (int i = 0; i < U; i++)
+      if (k + i * kRowThreads < e4) u[i] = __ldcs(x4 + k + i * kRowThreads);
+#pragma unroll
+    for (int i = 0; i < U; i++)
+      if (k + i * kRowThreads < e4)
+        __stcs(p4 + k + i * kRowThreads, make_float4(e(u[i].x - ref) * inv, e(u[i].y - ref) * inv, e(u[i].z - ref) * inv, e(u[i].w - ref) * inv));
+  }
+  single([&](int k) { p[k] = e(x[k] - ref) * inv; });
+  cl.sync();
+}
+
 // ------------------------------------------------------------------ verification
-constexpr int kVerifyThreads = 256, kVerifyWarps = kVerifyThreads / 32;
+constexpr int kVerifyThreads = 512, kVerifyWarps = kVerifyThreads / 32;
 constexpr int kRequests = 512;  // of one launch
 
 struct VerifyArgs {
@@ -172,13 +258,36 @@ struct VerifyArgs {
 };
 static_assert(sizeof(VerifyArgs) <= 4096, "kernel parameters");
 
-// mass of index v: max(p - q, 0) in f64, p alone without q; NaN counts as 0
-__device__ __forceinline__ double mass(const float *p, const float *q, int point, int v) {
-  double r = (double)__ldg(p + v);
-  if (q) r -= (double)__ldg(q + v);
-  else if (v == point) r -= 1.0;
-  return r > 0.0 ? r : 0.0;
+// Mass of an index: max(p - q, 0) in f64, p alone without q; NaN counts as 0.
+// (`point`: the index whose q is 1 when the drafts were not drawn.)
+__device__ __forceinline__ double mass(float p, float q) {
+  return p > q ? (double)p - (double)q : 0.0;
 }
+struct Row {
+  const float *p, *q;
+  int point, end;
+  // masses of the indices v + 32 u, u < N: all loads before the arithmetic
+  template <int N>
+  __device__ __forceinline__ void get(int v, double (&m)[N]) const {
+    float a[N], b[N];
+    if (q) {
+#pragma unroll
+      for (int u = 0; u < N; u++) {
+        const bool in = v + u * 32 < end;
+        a[u] = in ? __ldg(p + v + u * 32) : 0.f;
+        b[u] = in ? __ldg(q + v + u * 32) : 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < N; u++) {
+        a[u] = v + u * 32 < end ? __ldg(p + v + u * 32) : 0.f;
+        b[u] = v + u * 32 == point ? 1.f : 0.f;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < N; u++) m[u] = mass(a[u], b[u]);
+  }
+};
 
 __global__ void __launch_bounds__(kVerifyThreads) verify_drafts_kernel(const __grid_constant__ VerifyArgs a) {
   cg::cluster_group cl = cg::this_cluster();
@@ -203,20 +312,28 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafts_kernel(const __g
   }
   __syncthreads();
   const int r = s_refused;
-  const float *p = a.target + (row0 + r) * a.vocab;
-  const float *q = r < g && a.draft ? a.draft + (size_t)(d0 + r) * a.vocab : nullptr;
-  int point = r < g && !a.draft ? a.drafts[d0 + r] : -1;
+  Row row;
+  row.p = a.target + (row0 + r) * a.vocab;
+  row.q = r < g && a.draft ? a.draft + (size_t)(d0 + r) * a.vocab : nullptr;
+  row.point = r < g && !a.draft ? a.drafts[d0 + r] : -1;
   // run k = rank * kVerifyWarps + warp of the cluster: a.slice consecutive indices
   const int begin = (int)min((long long)(rank * kVerifyWarps + warp) * a.slice, (long long)a.vocab);
   const int end = (int)min((long long)begin + a.slice, (long long)a.vocab);
+  row.end = end;
   // sums of two runs per lane, and the sums up to and with each: the same
   // operations in the same order in every warp, so all agree on them
   constexpr int EACH = kMaxCluster * kVerifyWarps / 32;
   double sum[EACH], upto[EACH], total = 0.0;
   for (int pass = 0; pass < 2; pass++) {
-    double mine = 0.0;
-#pragma unroll 8
-    for (int v = begin + lane; v < end; v += 32) mine += mass(p, q, point, v);
+    // four sums a lane: f64 additions take their time
+    double part[4] = {0.0, 0.0, 0.0, 0.0};
+    for (int v = begin + lane; v < end; v += 512) {
+      double m[16];
+      row.get(v, m);
+#pragma unroll
+      for (int u = 0; u < 16; u++) part[u & 3] += m[u];
+    }
+    double mine = (part[0] + part[1]) + (part[2] + part[3]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
     if (lane == 0) s_warp[warp] = mine;
@@ -238,9 +355,9 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafts_kernel(const __g
     }
     total = carry;
     // differences without mass (p and q equal but for rounding): p itself
-    if (total > 0.0 || (!q && point < 0)) break;
-    q = nullptr;
-    point = -1;
+    if (total > 0.0 || (!row.q && row.point < 0)) break;
+    row.q = nullptr;
+    row.point = -1;
     __syncthreads();  // s_warp and s_all are written again
   }
   const double want = (double)a.u_sample[req] * total;
@@ -263,21 +380,47 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafts_kernel(const __g
       const double y = __shfl_sync(0xffffffffu, upto[e], (pick - 1) & 31);
       if (pick > 0 && (pick - 1) / 32 == e) run = y;
     }
+    // in steps of 32 blocks of 32 indices: the blocks' sums (eight reductions at
+    // a time: their chains overlap), the block that passes `want`, the index in it
     int found = -1, last = begin;
-    for (int v0 = begin; v0 < end && found < 0; v0 += 32) {
-      const int v = v0 + lane;
-      const double x = v < end ? mass(p, q, point, v) : 0.0;
-      double s = x;
+    for (int v0 = begin; v0 < end && found < 0; v0 += 1024) {
+      double block = 0.0;  // lane b: sum of block b
+      for (int b0 = 0; b0 < 32; b0 += 8) {
+        double t[8];
+        row.get(v0 + b0 * 32 + lane, t);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+          for (int u = 0; u < 8; u++) t[u] += __shfl_xor_sync(0xffffffffu, t[u], o);
+#pragma unroll
+        for (int u = 0; u < 8; u++) block = lane == b0 + u ? t[u] : block;
+      }
+      double sum = block;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const double y = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += y;
+        const double y = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += y;
       }
-      const unsigned hit = __ballot_sync(0xffffffffu, x > 0.0 && run + s > want);
-      const unsigned any = __ballot_sync(0xffffffffu, x > 0.0);
-      if (any) last = v0 + 31 - __clz(any);
-      if (hit) found = v0 + __ffs(hit) - 1;
-      run += __shfl_sync(0xffffffffu, s, 31);
+      const unsigned hit = __ballot_sync(0xffffffffu, block > 0.0 && run + sum > want);
+      const unsigned any = __ballot_sync(0xffffffffu, block > 0.0);
+      if (hit || any) {
+        // inside the block that passes, or the last with mass
+        const int b = hit ? __ffs(hit) - 1 : 31 - __clz(any);
+        const double before = run + __shfl_sync(0xffffffffu, sum, b) - __shfl_sync(0xffffffffu, block, b);
+        double m[1];
+        row.get(v0 + b * 32 + lane, m);
+        const double x = m[0];
+        double upto_v = x;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double y = __shfl_up_sync(0xffffffffu, upto_v, o);
+          if (lane >= o) upto_v += y;
+        }
+        const unsigned in = __ballot_sync(0xffffffffu, x > 0.0 && before + upto_v > want);
+        last = v0 + b * 32 + 31 - __clz(__ballot_sync(0xffffffffu, x > 0.0));
+        if (hit) found = in ? v0 + b * 32 + __ffs(in) - 1 : last;
+      }
+      run += __shfl_sync(0xffffffffu, sum, 31);
     }
     if (lane == 0) out[r] = found >= 0 ? found : last;
   }
@@ -321,18 +464,28 @@ VXB_API int vxb_token_probs(vxb_ctx *ctx, const float *d_logits, int rows, int v
   if (rows > INT_MAX / kMaxCluster) return set_error(ctx, VXB_EINVAL, "vxb_token_probs: %d rows", rows);
   ProbArgs a{d_logits, d_temperature, d_probs, vocab, 0, temperature};
   const int sms = ctx->num_sms > 0 ? ctx->num_sms : 148;
-  // the smallest cluster that holds a row in registers, a larger one while SMs are idle
-  int cluster = 1;
-  while (cluster < kMaxCluster && (long long)cluster * kProbThreads * 32 < vocab) cluster *= 2;
-  while (cluster < kMaxCluster && (long long)rows * cluster * 2 <= sms && vocab > cluster * kProbThreads) cluster *= 2;
-  a.slice = (vocab + cluster - 1) / cluster;
-  const int per = (a.slice + kProbThreads - 1) / kProbThreads;
   cudaStream_t st = (cudaStream_t)stream;
-  if (per <= 4) return launch_clusters(ctx, token_probs_kernel<4>, a, rows, cluster, kProbThreads, st, "token_probs_kernel");
-  if (per <= 8) return launch_clusters(ctx, token_probs_kernel<8>, a, rows, cluster, kProbThreads, st, "token_probs_kernel");
-  if (per <= 16) return launch_clusters(ctx, token_probs_kernel<16>, a, rows, cluster, kProbThreads, st, "token_probs_kernel");
-  if (per <= 32) return launch_clusters(ctx, token_probs_kernel<32>, a, rows, cluster, kProbThreads, st, "token_probs_kernel");
-  return launch_clusters(ctx, token_probs_kernel<0>, a, rows, cluster, kProbThreads, st, "token_probs_kernel");
+  // Rows that fit the SMs' registers at once (two CTAs of up to 16 values a
+  // thread, or one of 32) stay there; others are read twice.
+  int cluster = 1;
+  while (cluster < kMaxCluster && vocab > cluster * kProbThreads * 4) cluster *= 2;
+  const int per = ((vocab + cluster - 1) / cluster + kProbThreads - 1) / kProbThreads;
+  if (per <= 32 && (long long)rows * cluster <= (per <= 16 ? 2 : 1) * sms) {
+    a.slice = (vocab + cluster - 1) / cluster;
+    if (per <= 4) return launch_clusters(ctx, token_probs_kernel<4>, a, rows, cluster, kProbThreads, st, "token_probs_kernel");
+    if (per <= 8) return launch_clusters(ctx, token_probs_kernel<8>, a, rows, cluster, kProbThreads, st, "token_probs_kernel");
+    if (per <= 16) return launch_clusters(ctx, token_probs_kernel<16>, a, rows, cluster, kProbThreads, st, "token_probs_kernel");
+    return launch_clusters(ctx, token_probs_kernel<32>, a, rows, cluster, kProbThreads, st, "token_probs_kernel");
+  }
+  // as many ranks to a row as keep one wave of resident CTAs (5 per SM), with a
+  // round of loads a thread at least: a second wave of a few CTAs costs as much
+  // as the first (400 rows of 32,000: 1 rank 22.3 us, 2 ranks 25.8)
+  cluster = 1;
+  while (cluster < kMaxCluster && (long long)rows * cluster * 2 <= 5 * sms && vocab > cluster * kRowThreads * 16) cluster *= 2;
+  a.slice = (vocab + cluster - 1) / cluster;
+  if (((uintptr_t)d_logits & 15) == ((uintptr_t)d_probs & 15))
+    return launch_clusters(ctx, token_probs_rows_kernel<true>, a, rows, cluster, kRowThreads, st, "token_probs_rows_kernel");
+  return launch_clusters(ctx, token_probs_rows_kernel<false>, a, rows, cluster, kRowThreads, st, "token_probs_rows_kernel");
 }
 
 VXB_API int vxb_verify_drafts(vxb_ctx *ctx, int n, const int32_t *h_n_drafts, int vocab, const int32_t *d_drafts,
@@ -361,7 +514,9 @@ VXB_API int vxb_verify_drafts(vxb_ctx *ctx, int n, const int32_t *h_n_drafts, in
   a.accepted = d_n_accepted;
   a.vocab = vocab;
   int cluster = 1;
-  while (cluster < kMaxCluster && vocab > cluster * kVerifyThreads * 4) cluster *= 2;
+  // (two CTAs fit an SM: a cluster size that needs a second wave is too large)
+  const int sms = ctx->num_sms > 0 ? ctx->num_sms : 148;
+  while (cluster < kMaxCluster && vocab > cluster * kVerifyThreads * 4 && (long long)n * cluster * 2 <= 2 * sms) cluster *= 2;
   a.slice = (int)(((long long)vocab + cluster * kVerifyThreads - 1) / (cluster * kVerifyThreads) * 32);
   long long at = 0;
   for (int i = 0; i < n; i += kRequests) {

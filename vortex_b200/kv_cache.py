@@ -16,25 +16,37 @@ BF16 = N.BF16
 I8 = N.I8
 
 
+_I64 = np.dtype(np.int64)
+
+
+def _host_array(values, dtype):
+    """values as a contiguous 1-D array of dtype (itself where it is one)."""
+    if type(values) is np.ndarray and values.dtype == dtype and values.ndim == 1 and values.flags.c_contiguous:
+        return values
+    return np.ascontiguousarray(np.atleast_1d(values), dtype=dtype)
+
+
 def _ids_counts(who: str, seq_ids, counts, dtype=np.int32):
     """Host arrays of one sequence id and one count (or length) each."""
-    ids = np.ascontiguousarray(np.atleast_1d(seq_ids), dtype=np.int64)
-    c = np.atleast_1d(np.asarray(counts))
-    if c.size and not np.issubdtype(c.dtype, np.integer):
-        raise N.VxbError(N.VXB_EINVAL, f"{who}: the counts must be whole numbers")
-    if ids.ndim != 1 or c.ndim != 1 or ids.size != c.size:
-        raise N.VxbError(N.VXB_EINVAL, f"{who}: {ids.size} sequences and {c.size} counts")
-    if c.size and (int(c.min()) < 0 or int(c.max()) > np.iinfo(dtype).max):
-        raise N.VxbError(N.VXB_EINVAL, f"{who}: a count is negative or too large")
-    return ids, np.ascontiguousarray(c, dtype=dtype)
+    ids = _host_array(seq_ids, _I64)
+    if not (type(counts) is np.ndarray and counts.dtype == dtype):
+        counts = np.atleast_1d(np.asarray(counts))
+        if counts.size and (not np.issubdtype(counts.dtype, np.integer) or int(counts.max()) > np.iinfo(dtype).max):
+            raise N.VxbError(N.VXB_EINVAL, f"{who}: the counts must be whole numbers up to {np.iinfo(dtype).max}")
+    if ids.ndim != 1 or counts.ndim != 1 or ids.size != counts.size:
+        raise N.VxbError(N.VXB_EINVAL, f"{who}: {ids.size} sequences and {counts.size} counts")
+    c = _host_array(counts, dtype)
+    if c.size and min(c.tolist()) < 0:
+        raise N.VxbError(N.VXB_EINVAL, f"{who}: a count is negative")
+    return ids, c
 
 
 def _device_rows(who: str, name: str, t, shape, device: int):
-    """t as a contiguous bf16 tensor of this shape on the cache's device."""
+    """t as a contiguous, 16-byte aligned bf16 tensor of this shape on the cache's device."""
     import torch
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or not t.is_cuda or t.device.index != device:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or not t.is_cuda or t.get_device() != device:
         raise N.VxbError(N.VXB_EINVAL, f"{who}: {name} must be a bf16 tensor on cuda:{device}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise N.VxbError(N.VXB_EINVAL, f"{who}: {name} must be {tuple(shape)}, got {tuple(t.shape)}")
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
@@ -105,17 +117,17 @@ class PagedKVCache:
         sequence, their rows packed one sequence after another: k, v bf16
         [sum(n_tokens), H, D]."""
         ids, counts = _ids_counts("append_chunks", seq_ids, n_tokens)
-        want = (int(counts.sum()), self.num_heads, self.head_dim)
+        want = (sum(counts.tolist()), self.num_heads, self.head_dim)
         k = _device_rows("append_chunks", "k", k, want, self.ctx.device)
         v = _device_rows("append_chunks", "v", v, want, self.ctx.device)
-        self._check(N.lib().vxb_kv_append_chunks(self.ptr, layer, ids.size, ids.ctypes.data, counts.ctypes.data,
+        self._check(N.lib().vxb_kv_append_chunks(self.ptr, layer, ids.size, ids.tobytes(), counts.tobytes(),
                                                  k.data_ptr(), v.data_ptr(), _stream_on(self.ctx.device)))
 
     def truncate(self, seq_ids, lengths):
         """Takes appended tokens back: every layer of seq_ids[i] holds at most
         lengths[i] tokens afterwards."""
         ids, lens = _ids_counts("truncate", seq_ids, lengths, np.int64)
-        self._check(N.lib().vxb_kv_truncate(self.ptr, ids.size, ids.ctypes.data, lens.ctypes.data,
+        self._check(N.lib().vxb_kv_truncate(self.ptr, ids.size, ids.tobytes(), lens.tobytes(),
                                             _stream_on(self.ctx.device)))
 
     def pages(self) -> dict:
@@ -208,7 +220,7 @@ class PagedKVCache:
         Hq] if given). Rows that see nothing are zeros with lse -inf."""
         import torch
         ids, counts = _ids_counts("chunk_attention", seq_ids, n_queries)
-        rows, dev = int(counts.sum()), self.ctx.device
+        rows, dev = sum(counts.tolist()), self.ctx.device
         if q.dim() != 3:
             raise N.VxbError(N.VXB_EINVAL, "chunk_attention: q must be [rows, Hq, D]")
         Hq = q.shape[1]
@@ -218,8 +230,8 @@ class PagedKVCache:
             out = torch.empty_like(q)
         elif out is not _device_rows("chunk_attention", "out", out, shape, dev):
             raise N.VxbError(N.VXB_EINVAL, "chunk_attention: out must be contiguous and 16-byte aligned")
-        if lse is not None and (lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous()
-                                or tuple(lse.shape) != shape[:2]):
+        if lse is not None and (lse.dtype != torch.float32 or lse.get_device() != dev or not lse.is_contiguous()
+                                or lse.shape != shape[:2]):
             raise N.VxbError(N.VXB_EINVAL, f"chunk_attention: lse must be contiguous f32 {shape[:2]} on cuda:{dev}")
         need = self._chunk_ws.get(Hq)
         if need is None:
@@ -228,7 +240,7 @@ class PagedKVCache:
             need = self._chunk_ws[Hq] = n.value
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(self.head_dim)
-        self._check(N.lib().vxb_chunk_attention(self.ptr, layer, ids.size, ids.ctypes.data, counts.ctypes.data,
+        self._check(N.lib().vxb_chunk_attention(self.ptr, layer, ids.size, ids.tobytes(), counts.tobytes(),
                                                 q.data_ptr(), Hq, scale, int(causal), out.data_ptr(),
                                                 lse.data_ptr() if lse is not None else None, ws.data_ptr(), need,
                                                 _stream_on(dev)))

@@ -41,7 +41,7 @@ def _f32_rows(who: str, name: str, t, shape=None, device=None):
     import torch
     if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.float32:
         raise N.VxbError(N.VXB_EINVAL, f"{who}: {name} must be an f32 tensor on the GPU")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise N.VxbError(N.VXB_EINVAL, f"{who}: {name} must be {tuple(shape)}, got {tuple(t.shape)}")
     if device is not None and t.device != device:
         raise N.VxbError(N.VXB_EINVAL, f"{who}: {name} is on {t.device}, not on {device}")
@@ -85,12 +85,16 @@ def verify_drafts(drafts, n_drafts, target_probs, draft_probs, u_accept, u_sampl
     Returns (tokens int32 [D + n]: accepted drafts, the drawn token, then -1,
     per request; accepted int32 [n])."""
     import torch
-    counts = np.atleast_1d(np.asarray(n_drafts))
-    if counts.ndim != 1 or (counts.size and (not np.issubdtype(counts.dtype, np.integer) or int(counts.min()) < 0
-                                             or int(counts.max()) > np.iinfo(np.int32).max)):
-        raise N.VxbError(N.VXB_EINVAL, "verify_drafts: n_drafts must be whole numbers, none negative")
+    counts = n_drafts
+    if not (type(counts) is np.ndarray and counts.dtype == np.int32):
+        counts = np.atleast_1d(np.asarray(counts))
+        if counts.size and (not np.issubdtype(counts.dtype, np.integer) or int(counts.max()) > np.iinfo(np.int32).max):
+            raise N.VxbError(N.VXB_EINVAL, "verify_drafts: n_drafts must be whole numbers of 32 bits")
     counts = np.ascontiguousarray(counts, dtype=np.int32)
-    n, total = counts.size, int(counts.sum())
+    per = counts.tolist()
+    if counts.ndim != 1 or (per and min(per) < 0):
+        raise N.VxbError(N.VXB_EINVAL, "verify_drafts: n_drafts must be one list of numbers, none negative")
+    n, total = len(per), sum(per)
     if not isinstance(target_probs, torch.Tensor) or target_probs.dim() != 2 or target_probs.shape[1] == 0:
         raise N.VxbError(N.VXB_EINVAL, "verify_drafts: target_probs must be [rows, vocab]")
     vocab = target_probs.shape[1]
@@ -98,13 +102,13 @@ def verify_drafts(drafts, n_drafts, target_probs, draft_probs, u_accept, u_sampl
     q = None if draft_probs is None else _f32_rows("verify_drafts", "draft_probs", draft_probs, (total, vocab), p.device)
     ua = _f32_rows("verify_drafts", "u_accept", u_accept, (total,), p.device)
     us = _f32_rows("verify_drafts", "u_sample", u_sample, (n,), p.device)
-    if not isinstance(drafts, torch.Tensor) or drafts.dtype != torch.int32 or drafts.device != p.device or tuple(drafts.shape) != (total,):
+    if not isinstance(drafts, torch.Tensor) or drafts.dtype != torch.int32 or drafts.device != p.device or drafts.shape != (total,):
         raise N.VxbError(N.VXB_EINVAL, f"verify_drafts: drafts must be int32 ({total},) on {p.device}")
     drafts = drafts.contiguous()
     tokens = torch.empty(total + n, dtype=torch.int32, device=p.device)
     accepted = torch.empty(n, dtype=torch.int32, device=p.device)
     dev = p.device.index
-    context(dev).call("vxb_verify_drafts", n, counts.ctypes.data, vocab, drafts.data_ptr(), p.data_ptr(),
+    context(dev).call("vxb_verify_drafts", n, counts.tobytes(), vocab, drafts.data_ptr(), p.data_ptr(),
                       q.data_ptr() if q is not None else None, ua.data_ptr(), us.data_ptr(), tokens.data_ptr(),
                       accepted.data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
     return tokens, accepted
