@@ -226,25 +226,36 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
         }
       }
       if (warp_live) {
-        float s[N];
-#pragma unroll
-        for (int c = 0; c < N / 32; c++) tmem_ld32(tS + c * 32, *reinterpret_cast<float(*)[32]>(s + c * 32));
-        tmem_wait_ld();
+        // int8 reads S twice, 32 columns at a time: its threads have too few
+        // registers for 64 scores (spilled, they took twice as long)
+        constexpr int KEEP = INT8 ? 32 : N;
+        float s[KEEP];
         // K and V scales of this tile: there until its V is released, after P
         const float *key_scale = reinterpret_cast<const float *>(sm + C::OFF_SCALE) + (kv / 2 % C::SLOTS) * 2 * BN + half * N;
-        if constexpr (INT8) scale_keys<N>(s, key_scale);
         const bool masked = !__all_sync(0xffffffffu, kh + N - 1 <= lim);
-        if (masked) {
+        auto scores = [&](int c0) {
 #pragma unroll
-          for (int c = 0; c < N; c++) s[c] = kh + c <= lim ? s[c] : -INFINITY;
+          for (int c = 0; c < KEEP; c += 32) tmem_ld32(tS + c0 + c, *reinterpret_cast<float(*)[32]>(s + c));
+          tmem_wait_ld();
+          if constexpr (INT8) scale_keys<KEEP>(s, key_scale + c0);
+          if (masked) {
+#pragma unroll
+            for (int c = 0; c < KEEP; c++) s[c] = kh + c0 + c <= lim ? s[c] : -INFINITY;
+          }
+        };
+        float mx = -INFINITY;
+#pragma unroll
+        for (int c0 = 0; c0 < N; c0 += KEEP) {
+          scores(c0);
+          float mx4[4] = {mx, s[0], s[1], s[2]};
+#pragma unroll
+          for (int c = 3; c + 7 < KEEP; c += 8) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) mx4[e] = max3(mx4[e], s[c + 2 * e], s[c + 2 * e + 1]);
+          }
+          mx4[0] = max3(mx4[0], s[KEEP - 5], s[KEEP - 4]);
+          mx = max3(max3(mx4[0], mx4[1], mx4[2]), max3(mx4[3], s[KEEP - 3], s[KEEP - 2]), s[KEEP - 1]);
         }
-        float mx4[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-        for (int c = 4; c + 7 < N; c += 8) {
-#pragma unroll
-          for (int e = 0; e < 4; e++) mx4[e] = max3(mx4[e], s[c + 2 * e], s[c + 2 * e + 1]);
-        }
-        float mx = max3(max3(mx4[0], mx4[1], mx4[2]), max3(mx4[3], s[N - 4], s[N - 3]), fmaxf(s[N - 2], s[N - 1]));
         // the row's maximum over both halves (the next S, so the next write
         // here, waits for both halves' P)
         *x_mine = mx;
@@ -273,7 +284,8 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
         float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int c = 0; c < N / 32; c++) {
-          float *v = s + c * 32;
+          if constexpr (INT8) scores(c * 32);
+          float *v = s + c * 32 % KEEP;
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
             const float2 x = fma2(make_float2(v[e], v[e + 1]), scale2, ref2);
@@ -941,7 +953,21 @@ int chunk_attention(vxb_kv *kv, int layer, int n, const int64_t *ids, const int3
   a.mbps = kv->max_blocks_per_seq;
   a.scale_log2 = scale * 1.44269504088896340736f;
   a.box = bs % 128 == 0 ? 128 : bs % 64 == 0 ? 64 : bs % 32 == 0 ? 32 : 16;  // tokens of a page copy: within a block
-  // chunks of few rows and the others go to a kernel each
+  // Chunks of few rows and the others go to a kernel each; a few of the former
+  // beside the latter stay with them (a launch of its own has a fixed part of
+  // about 8 us, and leaves most SMs idle when it has few tiles).
+  auto is_few = [&](int i) { return (int64_t)counts[i] * a.G <= kFewRows; };
+  std::vector<int> lens(n, 0);
+  bool all_few = true;
+  int64_t few_tiles = 0;
+  for (int i = 0; i < n; i++) {
+    if (counts[i] == 0) continue;
+    auto it = kv->tables.find(std::make_pair(layer, ids[i]));
+    if (it != kv->tables.end()) lens[i] = (int)it->second.len;
+    if (is_few(i)) few_tiles += (int64_t)(lens[i] + BN - 1) / BN * Hkv;
+    else all_few = false;
+  }
+  const bool together = !all_few && few_tiles < 8 * ctas_of(ctx);
   for (int few = 0; few < 2; few++) {
     a.sh = {few ? kFewRows : BM / a.G, causal != 0};
     int row = 0;
@@ -951,10 +977,8 @@ int chunk_attention(vxb_kv *kv, int layer, int n, const int64_t *ids, const int3
       for (; i < n && a.n < kSeqs; i++) {
         const int at = row;
         row += counts[i];
-        if (counts[i] == 0 || ((int64_t)counts[i] * a.G <= kFewRows) != (few == 1)) continue;
-        auto it = kv->tables.find(std::make_pair(layer, ids[i]));
-        const int len = it == kv->tables.end() ? 0 : (int)it->second.len;
-        a.seq[a.n++] = {len > 0 ? kv->slot_of.at(ids[i]) : 0, at, counts[i], len};
+        if (counts[i] == 0 || (!together && is_few(i)) != (few == 1)) continue;
+        a.seq[a.n++] = {lens[i] > 0 ? kv->slot_of.at(ids[i]) : 0, at, counts[i], lens[i]};
         max_rows = max_rows > counts[i] ? max_rows : counts[i];
       }
       if (a.n == 0) continue;
