@@ -4,7 +4,7 @@
 // columns:
 //
 //   S^T = K Q^T         A = the K tile, B = the query rows
-//   P^T = 2^(S^T - m)   thread = key and half of the rows
+//   P^T = 2^(S^T - m)   thread = key and some of the rows
 //   O^T += V^T P^T      A = the V tile read MN-major, B = P from shared memory
 //
 // With the queries as rows (chunk_attn.cu) a tile costs 128 exponentials per
@@ -63,13 +63,13 @@ struct Cfg {
   static constexpr int OFF_RED = OFF_SCALE + SCALES * 2 * BN * 4;  // per-warp results and per-row values of the softmax
   static constexpr int OFF_BARS = OFF_RED + 7 * NR * 4;
   static constexpr int SMEM = OFF_BARS + 320;
-  // Warpgroups: two of softmax, PER_SLOT each that load K and V (int8 converts
-  // as it loads), one with the MMA and Q warps.
-  static constexpr int PER_SLOT = INT8 ? 2 : 1, LOADERS = 8 * PER_SLOT;  // warpgroups of a group; warps in all
-  static constexpr int THREADS = 256 + LOADERS * 32 + 128;
-  static constexpr int REGS = INT8 ? 72 : 96;  // at launch
-  static constexpr int REG_SOFT = NR < 64 ? 96 : INT8 ? 112 : 128, REG_LOAD = INT8 ? (NR < 64 ? 64 : 56) : NR < 64 ? 96 : 80, REG_MMA = 56;
-  static_assert(2 * REG_SOFT + 2 * PER_SLOT * REG_LOAD + REG_MMA <= THREADS / 128 * REGS, "registers");
+  // Warpgroups: SOFT of softmax (up to 16 rows each), PER_SLOT each that load K
+  // and V (int8 converts as it loads), one with the MMA and Q warps; registers
+  // at launch and of each.
+  static constexpr int SOFT = NR == 64 ? 4 : 2, PER_SLOT = INT8 && NR < 64 ? 2 : 1;
+  static constexpr int THREADS = (SOFT + 2 * PER_SLOT + 1) * 128, REGS = THREADS == 640 ? 96 : 72;
+  static constexpr int REG_SOFT = NR == 64 ? 72 : 96, REG_LOAD = NR == 64 ? 80 : INT8 ? 64 : 96, REG_MMA = 56;
+  static_assert(SOFT * REG_SOFT + 2 * PER_SLOT * REG_LOAD + REG_MMA <= THREADS / 128 * REGS, "registers");
   static constexpr int COLS = (AHEAD + 2) * NR <= 128 ? 128 : (AHEAD + 2) * NR <= 256 ? 256 : 512;  // TMEM: S x AHEAD, O, O
   static_assert(SMEM <= 232448, "shared memory");
 };
@@ -144,18 +144,18 @@ __device__ __forceinline__ void halve(float *v, int lane) {
   }
 }
 
-// ------------------------------------------------------------------ softmax: thread = (key, half of the rows)
-// Rows go to the two warpgroups in groups of eight in turn; groups without a
-// live row are passed over.
+// ------------------------------------------------------------------ softmax: thread = (key, the warpgroup's rows)
+// Rows go to the warpgroups in groups of eight in turn; groups without a live
+// row are passed over.
 template <int D, bool INT8, int NR>
 __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, BarsOf<D, INT8, NR> &bars) {
   using C = Cfg<D, INT8, NR>;
-  constexpr int N = NR / 2, GROUPS = N / 8;  // rows of this warpgroup
+  constexpr int W = C::SOFT, N = NR / W, GROUPS = N / 8;  // warpgroups; rows of this one
   constexpr float SHIFT = INT8 ? 6.f : 0.f;  // P (and l) hold 2^SHIFT times the weights
   const int wg = threadIdx.x >> 7, key = threadIdx.x & 127, warp = key >> 5, lane = key & 31;
   const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
   // row n of the warpgroup's N is row row_of(n) of the item
-  auto row_of = [&](int n) { return (n >> 3) * 16 + wg * 8 + (n & 7); };
+  auto row_of = [&](int n) { return ((n >> 3) * W + wg) * 8 + (n & 7); };
   // this warpgroup's: per-warp results [4][N]; per row the negated reference, a factor, a change of the reference
   float *red = reinterpret_cast<float *>(sm + C::OFF_RED) + wg * 7 * N, *ref_s = red + 4 * N, *f_s = ref_s + N, *d_s = f_s + N;
   const float *scales = reinterpret_cast<const float *>(sm + C::OFF_SCALE);
@@ -168,7 +168,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
   bar_sync(bar, 128);
   while (run.next(a, p)) {
     const int T = max(0, p.te - p.tb), live = p.ntok * a.G;
-    const int groups = live > wg * 8 ? (live - wg * 8 + 15) / 16 : 0;  // of this warpgroup's, with a live row
+    const int groups = live > wg * 8 ? (live - wg * 8 + W * 8 - 1) / (W * 8) : 0;  // of this warpgroup's, with a live row
     const int base = p.s.len - p.s.rows + p.tok0;  // last key that the first token sees
     const uint32_t tO = bars.tmem + lane_off + (C::AHEAD + (pieces & 1)) * NR + wg * 8;
     float l[N];
@@ -197,7 +197,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
       auto load = [&](auto all) {
 #pragma unroll
         for (int j = 0; j < GROUPS; j++)
-          if (decltype(all)::value || j < groups) tmem_ld8(tS + j * 16, *reinterpret_cast<float(*)[8]>(x + j * 8));
+          if (decltype(all)::value || j < groups) tmem_ld8(tS + j * W * 8, *reinterpret_cast<float(*)[8]>(x + j * 8));
         tmem_wait_ld();
 #pragma unroll
         for (int j = 0; j < GROUPS; j++)
@@ -253,7 +253,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
           for (int j = 0; j < GROUPS; j++)
             if (j < groups) {
               float o[8];
-              tmem_ld8(tO + j * 16, o);
+              tmem_ld8(tO + j * W * 8, o);
               tmem_wait_ld();
 #pragma unroll
               for (int n = 0; n < 8; n++) {
@@ -261,7 +261,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
                 o[n] *= f;
                 l[j * 8 + n] *= f;
               }
-              tmem_st8(tO + j * 16, o);
+              tmem_st8(tO + j * W * 8, o);
             }
           tmem_wait_st();
         }
@@ -290,8 +290,8 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
                 l[n + 1] += w1;
                 pair = pack_bf16(w0, w1);
               }
-              *reinterpret_cast<uint16_t *>(prow + j * 2048 + e * 128 + ((chunk ^ e) << 4)) = (uint16_t)pair;
-              *reinterpret_cast<uint16_t *>(prow + j * 2048 + (e + 1) * 128 + ((chunk ^ (e + 1)) << 4)) = (uint16_t)(pair >> 16);
+              *reinterpret_cast<uint16_t *>(prow + j * W * 1024 + e * 128 + ((chunk ^ e) << 4)) = (uint16_t)pair;
+              *reinterpret_cast<uint16_t *>(prow + j * W * 1024 + (e + 1) * 128 + ((chunk ^ (e + 1)) << 4)) = (uint16_t)(pair >> 16);
             }
           }
       };
@@ -304,19 +304,19 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
           wait(&bars.v_full[g % C::VS], (g / C::VS) & 1);
           uint8_t *V = sm + C::OFF_V + (g % C::VS) * C::TILE;
           uint32_t found = 0;
-          for (int c = threadIdx.x; c < valid * (D / 8); c += 256) {
+          for (int c = threadIdx.x; c < valid * (D / 8); c += W * 128) {
             const uint4 w = *reinterpret_cast<const uint4 *>(V + chunk_off(c / (D / 8), c % (D / 8)));
             found |= odd_bf16(w.x) | odd_bf16(w.y) | odd_bf16(w.z) | odd_bf16(w.w);
           }
           __syncwarp();
-          if (bar_or(3, 256, found != 0)) {
+          if (bar_or(W + 1, W * 128, found != 0)) {
             // rare: lane d of O^T takes every non-finite value of column d of V
             if (t > 0) {
               wait(&bars.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
               tc_fence_after();
             } else {
               const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-              for (int j = 0; j < GROUPS; j++) tmem_st8(tO + j * 16, z);
+              for (int j = 0; j < GROUPS; j++) tmem_st8(tO + j * W * 8, z);
               tmem_wait_st();
               if (threadIdx.x == 0) bars.acc = 1;
             }
@@ -331,14 +331,14 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
                 if (r < first) continue;
                 const uint32_t off = (uint32_t)(i >> 6) * (NR * 128) + (uint32_t)r * 128 + ((((uint32_t)(i & 63) >> 3) ^ ((uint32_t)n & 7)) << 4) + (i & 7) * 2;
                 const float w = __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t *>(P + off) << 16);
-                const uint32_t at = tO + (n >> 3) * 16 + (n & 7);
+                const uint32_t at = tO + (n >> 3) * W * 8 + (n & 7);
                 const float o = tmem_ld1(at);
                 tmem_st1(at, odd ? fmaf(w, __uint_as_float(bits << 16), o) : o);
                 tmem_wait_st();
               }
             }
-            bar_sync(3, 256);
-            for (int c = threadIdx.x; c < valid * (D / 8); c += 256) {
+            bar_sync(W + 1, W * 128);
+            for (int c = threadIdx.x; c < valid * (D / 8); c += W * 128) {
               uint4 *at = reinterpret_cast<uint4 *>(V + chunk_off(c / (D / 8), c % (D / 8)));
               *at = make_uint4(even_bf16(at->x), even_bf16(at->y), even_bf16(at->z), even_bf16(at->w));
             }
@@ -381,10 +381,10 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
     for (int j = 0; j < groups; j++) {
       float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       if (T > 0) {
-        tmem_ld8(tO + j * 16, o);
+        tmem_ld8(tO + j * W * 8, o);
         tmem_wait_ld();
       }
-      const int r0 = j * 16 + wg * 8, count = key < D ? live - r0 : 0;
+      const int r0 = (j * W + wg) * 8, count = key < D ? live - r0 : 0;
       const float *f8 = f_s + j * 8;
       if (whole) {
         int h = r0 % a.G;
@@ -691,10 +691,10 @@ __global__ void __launch_bounds__(Cfg<D, INT8, NR>::THREADS, 1) chunk_few_kernel
     for (int i = 0; i < 2; i++) {
       mbar_init(&bars.q_full[i], 1);
       mbar_init(&bars.q_empty[i], 1);
-      mbar_init(&bars.p_full[i], 8);
+      mbar_init(&bars.p_full[i], C::SOFT * 4);
       mbar_init(&bars.pv_done[i], 1);
       mbar_init(&bars.o_full[i], 1);
-      mbar_init(&bars.o_free[i], 8);
+      mbar_init(&bars.o_free[i], C::SOFT * 4);
     }
     for (int i = 0; i < C::AHEAD; i++) mbar_init(&bars.s_full[i], 1);
     bars.acc = 0;
@@ -704,12 +704,14 @@ __global__ void __launch_bounds__(Cfg<D, INT8, NR>::THREADS, 1) chunk_few_kernel
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars.tmem;
-  if (warp < 8) {
+  constexpr int SOFT_WARPS = C::SOFT * 4, LOAD_WARPS = C::PER_SLOT * 4;
+  if (warp < SOFT_WARPS) {
     if constexpr (C::REG_SOFT > C::REGS) regs_inc<C::REG_SOFT>();
     softmax_role<D, INT8, NR>(a, sm, bars);
-  } else if (warp < 8 + C::LOADERS) {
+  } else if (warp < SOFT_WARPS + 2 * LOAD_WARPS) {
     if constexpr (C::REG_LOAD < C::REGS) regs_dec<C::REG_LOAD>();
-    const bool v = warp >= 8 + C::LOADERS / 2;
+    if constexpr (C::REG_LOAD > C::REGS) regs_inc<C::REG_LOAD>();
+    const bool v = warp >= SOFT_WARPS + LOAD_WARPS;
     if constexpr (INT8) {
       if (v) load_role_i8<D, NR, true>(a, sm, bars);
       else load_role_i8<D, NR, false>(a, sm, bars);
@@ -719,9 +721,9 @@ __global__ void __launch_bounds__(Cfg<D, INT8, NR>::THREADS, 1) chunk_few_kernel
     }
   } else {
     regs_dec<C::REG_MMA>();
-    if (warp == 8 + C::LOADERS) {
+    if (warp == SOFT_WARPS + 2 * LOAD_WARPS) {
       mma_role<D, INT8, NR>(a, sm, bars);
-    } else if (warp == 9 + C::LOADERS) {
+    } else if (warp == SOFT_WARPS + 2 * LOAD_WARPS + 1) {
       q_role<D, INT8, NR>(a, sm, bars);
     }
   }
