@@ -17,8 +17,8 @@ constexpr float RESCALE_THRESHOLD = 8.f;  // O is rescaled when a row's maximum 
 struct ChunkSeq {
   int32_t slot, row0, rows, len;
 };
-struct Start {  // a CTA's first item and the first of its key tiles
-  int32_t seq, head, pair, tile;
+struct Start {  // a CTA's first item, the first of its key tiles, and the key tiles of the run
+  int32_t seq, head, pair, tile, units;
 };
 struct Shape {
   int tpt;  // tokens of a 128-row tile
@@ -36,9 +36,8 @@ struct ChunkArgs {
   int n, Hq, Hkv, G, bs, mbps, box, n_ctas;
   Shape sh;
   float scale_log2;
-  long long units;
   ChunkSeq seq[kSeqs];
-  Start start[kMaxCtas + 1];
+  Start start[kMaxCtas];
 };
 static_assert(sizeof(ChunkArgs) <= 8192, "kernel parameters");
 
@@ -88,8 +87,7 @@ struct Run {
   Run() = default;
   __device__ Run(const ChunkArgs &a) {
     at = a.start[blockIdx.x];
-    const long long u0 = a.units * blockIdx.x / a.n_ctas, u1 = a.units * (blockIdx.x + 1) / a.n_ctas;
-    left = (int)(u1 - u0);
+    left = at.units;
   }
   __device__ __forceinline__ bool next(const ChunkArgs &a, Piece &p) {
     if (left <= 0) return false;
@@ -216,7 +214,7 @@ __device__ __forceinline__ uint32_t even_bf16(uint32_t w) {  // the pair with ze
 // Scratch of an item's part: 256 rows of D sums, then (maximum, sum) pairs.
 inline size_t part_floats(int D) { return (size_t)kRowsItem * (D + 2); }
 
-// Chunks of up to kFewRows rows per kv head (few_rows.cu); everything else goes
+// Chunks of up to kFewRows rows per kv head (chunk_few.cu); everything else goes
 // to the kernel in chunk_attn.cu.
 constexpr int kFewRows = 64;
 int launch_few(vxb_kv *kv, const ChunkArgs &a, int max_rows, cudaStream_t st);

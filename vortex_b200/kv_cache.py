@@ -10,7 +10,7 @@ import math
 import numpy as np
 
 from . import _native as N
-from .quant import _dptr, _stream_ptr, context
+from .quant import _dptr, _stream_on, _stream_ptr, context
 
 BF16 = N.BF16
 I8 = N.I8
@@ -50,12 +50,6 @@ def _device_rows(who: str, name: str, t, shape, device: int):
         raise N.VxbError(N.VXB_EINVAL, f"{who}: {name} must be {tuple(shape)}, got {tuple(t.shape)}")
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
-def _stream_on(device: int) -> int:
-    """The current stream of the cache's device (which need not be the current device)."""
-    import torch
-    return torch.cuda.current_stream(device).cuda_stream
 
 
 class _DeviceArray:

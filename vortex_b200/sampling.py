@@ -10,7 +10,7 @@ import ctypes
 import numpy as np
 
 from . import _native as N
-from .quant import _dptr, _stream_ptr, context
+from .quant import _dptr, _stream_on, _stream_ptr, context
 
 
 def argmax(logits):
@@ -69,7 +69,7 @@ def token_probs(logits, temperature=1.0, out=None):
     dev = lg.device.index
     context(dev).call("vxb_token_probs", lg.data_ptr(), rows, vocab, per_row.data_ptr() if per_row is not None else None,
                       1.0 if per_row is not None else float(temperature), out.data_ptr(),
-                      torch.cuda.current_stream(dev).cuda_stream)
+                      _stream_on(dev))
     return out
 
 
@@ -110,7 +110,7 @@ def verify_drafts(drafts, n_drafts, target_probs, draft_probs, u_accept, u_sampl
     dev = p.device.index
     context(dev).call("vxb_verify_drafts", n, counts.tobytes(), vocab, drafts.data_ptr(), p.data_ptr(),
                       q.data_ptr() if q is not None else None, ua.data_ptr(), us.data_ptr(), tokens.data_ptr(),
-                      accepted.data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
+                      accepted.data_ptr(), _stream_on(dev))
     return tokens, accepted
 
 
