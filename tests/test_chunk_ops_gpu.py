@@ -311,6 +311,50 @@ def test_chunk_attention_few_rows(KV, H, G, bs, lens, counts, D, int8, causal):
     assert torch.equal(out, c.chunk_attention(0, range(n), counts, q, causal=causal)), "not deterministic"
 
 
+RUNS = [
+    # H kv, G, block, lens, counts: few items of many key tiles, which are cut, and many of few, several to a run
+    (1, 4, 16, [2500], [300]),
+    (2, 3, 16, [2300, 130, 4000], [100, 90, 60]),
+    (1, 1, 32, [1500, 3100, 7], [129, 300, 5]),
+    (1, 128, 64, [1900], [5]),
+    (8, 1, 16, [130 + 29 * i for i in range(20)], [70 + 13 * (i * 7 % 20) for i in range(20)]),
+    (4, 2, 16, [65 + 40 * i for i in range(16)], [65 + 3 * i for i in range(16)]),
+    (8, 4, 16, [100 + 33 * (i * 5 % 33) for i in range(33)], [1 + i % 16 for i in range(33)]),
+]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("H,G,bs,lens,counts", RUNS)
+def test_chunk_attention_cut_and_whole_runs(KV, H, G, bs, lens, counts, D, int8, causal):
+    n = len(lens)
+    c = make(KV, 1, H, D, bs, sum(-(-x // bs) for x in lens), n, int8)
+    c.append_chunks(0, range(n), lens, rnd((sum(lens), H, D), 1), rnd((sum(lens), H, D), 2))
+    q = rnd((sum(counts), H * G, D), 3, 2.0)
+    lse = torch.full((sum(counts), H * G), 7.0, device="cuda")
+    out = c.chunk_attention(0, range(n), counts, q, causal=causal, lse=lse)
+    check_rows(out, lse, q, c, 0, range(n), counts, causal, 1 / math.sqrt(D))
+    assert torch.equal(out, c.chunk_attention(0, range(n), counts, q, causal=causal)), "not deterministic"
+
+
+@pytest.mark.parametrize("m", [200, 64])
+def test_chunk_attention_non_finite_values_in_cut_items(KV, m):
+    H, n, D = 1, 2600, 128  # the chunk's own keys end far behind the first cut
+    k, v, q = rnd((n, H, D), 1), rnd((n, H, D), 2), rnd((m, H, D), 3)
+    outs = []
+    for poison in (False, True):
+        c = make(KV, 1, H, D, 16, 170, 1)
+        vv = v.clone()
+        if poison:
+            vv[n - 40, 0, 5] = float("nan")
+        c.append_chunks(0, [0], [n], k, vv)
+        outs.append(c.chunk_attention(0, [0], [m], q))
+    clean, dirty = outs
+    assert torch.equal(clean[:m - 40], dirty[:m - 40])
+    assert torch.equal(clean[..., 6:], dirty[..., 6:]) and bool(torch.isnan(dirty[m - 40:, 0, 5]).all())
+
+
 @pytest.mark.parametrize("int8", [False, True])
 def test_chunk_attention_rows_that_see_nothing(KV, int8):
     # empty and unknown sequences, more queries than tokens, sequences without queries
