@@ -157,6 +157,21 @@ __device__ __forceinline__ void scale_keys(float *v, const float *f) {
   }
 }
 
+// w[j] of lane q (of four) and w[q] of lane j change places
+__device__ __forceinline__ void transpose4(uint4 (&w)[4], int lane) {
+  auto swap = [&](uint4 &lo, uint4 &hi, int bit) {  // lanes with the bit give lo and get it, the others hi
+    const bool up = lane & bit;
+    const uint4 give = up ? lo : hi;
+    const uint4 got = make_uint4(__shfl_xor_sync(0xffffffffu, give.x, bit), __shfl_xor_sync(0xffffffffu, give.y, bit),
+                                 __shfl_xor_sync(0xffffffffu, give.z, bit), __shfl_xor_sync(0xffffffffu, give.w, bit));
+    (up ? lo : hi) = got;
+  };
+  swap(w[0], w[1], 1);
+  swap(w[2], w[3], 1);
+  swap(w[0], w[2], 2);
+  swap(w[1], w[3], 2);
+}
+
 // ------------------------------------------------------------------ softmax: thread = (stream, row, half of a tile's keys)
 template <int D, bool INT8, class B>
 __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B &bars) {
@@ -215,13 +230,15 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
             fence_async_smem();
           }
           if (diagonal) {
-            uint32_t found = 0;
-            for (int c = tid; c < valid * (D / 8); c += 256) {
-              const uint4 w = *reinterpret_cast<const uint4 *>(sv_tile + chunk_off(c / (D / 8), c % (D / 8)));
-              found |= odd_bf16(w.x) | odd_bf16(w.y) | odd_bf16(w.z) | odd_bf16(w.w);
+            uint32_t found[2] = {0u, 0u};
+#pragma unroll
+            for (int n = 0; n < BN * (D / 8) / 256; n++) {
+              const int c = tid + n * 256;
+              if (c / (D / 8) < valid)
+                found[n & 1] = add_odd(found[n & 1], *reinterpret_cast<const uint4 *>(sv_tile + chunk_off(c / (D / 8), c % (D / 8))));
             }
             __syncwarp();
-            odd = bar_or(2 + st, 256, found != 0);
+            odd = bar_or(2 + st, 256, (odd_bf16(found[0]) | odd_bf16(found[1])) != 0);
           }
         }
       }
@@ -394,31 +411,50 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
     const int prow = p.both ? st * BM + r : r;
     if (warp_live) {
       const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
-      // the row's threads take D / 2 columns each, or D / 4
-      const int width = p.both ? D / 2 : D / 4, first = p.both ? half * width : (st * 2 + half) * width;
+      // the threads of a row take D / 2 columns each, or D / 4 but 32 at least
+      const int width = p.both ? D / 2 : D / 4 > 32 ? D / 4 : 32, first = p.both ? half * width : (st * (D == 128 ? 2 : 1) + half) * width;
+      const int tq0 = (r & ~3) / a.G, gq0 = (r & ~3) - tq0 * a.G;
       const bool has0 = steps > 0, has1 = !p.both && p.steps(st ^ 1) > 0;
       f0 *= inv;
       f1 *= inv;
 #pragma unroll 1
-      for (int c = first; c < first + width; c += 16) {
-        float o[16], x[16];
+      for (int c = first; c < (D == 64 && !p.both && half ? 0 : first + width); c += 32) {
+        uint4 w[4];
 #pragma unroll
-        for (int e = 0; e < 16; e++) o[e] = x[e] = 0.f;
-        if (has0) tmem_ld16(tO + c, o);
-        if (has1) tmem_ld16(tO_other + c, x);
-        tmem_wait_ld();
+        for (int h = 0; h < 2; h++) {
+          float o[16], x[16];
 #pragma unroll
-        for (int e = 0; e < 16; e++) o[e] = has1 ? fmaf(x[e], f1, o[e] * f0) : o[e] * f0;
-        if (mine && whole) {
-          uint4 *dst = reinterpret_cast<uint4 *>(a.out + row * D + c);
+          for (int e = 0; e < 16; e++) o[e] = x[e] = 0.f;
+          if (has0) tmem_ld16(tO + c + h * 16, o);
+          if (has1) tmem_ld16(tO_other + c + h * 16, x);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; e++) o[e] = has1 ? fmaf(x[e], f1, o[e] * f0) : o[e] * f0;
+          if (!whole) {
+            float4 *dst = reinterpret_cast<float4 *>(part + ((size_t)((c + h * 16) / 8) * kRowsItem + prow) * 8);
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+              if (mine) __stcg(dst + (q >> 1) * (kRowsItem * 2) + (q & 1), make_float4(o[q * 4], o[q * 4 + 1], o[q * 4 + 2], o[q * 4 + 3]));
+          }
 #pragma unroll
           for (int q = 0; q < 2; q++)
-            dst[q] = make_uint4(pack_bf16(o[q * 8], o[q * 8 + 1]), pack_bf16(o[q * 8 + 2], o[q * 8 + 3]), pack_bf16(o[q * 8 + 4], o[q * 8 + 5]),
-                                pack_bf16(o[q * 8 + 6], o[q * 8 + 7]));
-        } else if (mine) {
-          float4 *dst = reinterpret_cast<float4 *>(part + (size_t)prow * D + c);
+            w[h * 2 + q] = make_uint4(pack_bf16(o[q * 8], o[q * 8 + 1]), pack_bf16(o[q * 8 + 2], o[q * 8 + 3]),
+                                      pack_bf16(o[q * 8 + 4], o[q * 8 + 5]), pack_bf16(o[q * 8 + 6], o[q * 8 + 7]));
+        }
+        if (whole) {
+          // four lanes exchange their 64 bytes, so that they write one row at
+          // a time (each its own row took twice as long: 32 lines a store)
+          transpose4(w, lane);
+          int tq = tq0, gq = gq0;
 #pragma unroll
-          for (int q = 0; q < 4; q++) __stcg(dst + q, make_float4(o[q * 4], o[q * 4 + 1], o[q * 4 + 2], o[q * 4 + 3]));
+          for (int q = 0; q < 4; q++) {
+            if ((r & ~3) + q < live)
+              *reinterpret_cast<uint4 *>(a.out + (((size_t)(p.s.row0 + tile_tok + tq) * a.Hq) + (size_t)p.head * a.G + gq) * D + c + (r & 3) * 8) = w[q];
+            if (++gq == a.G) {
+              gq = 0;
+              tq++;
+            }
+          }
         }
       }
       if (mine && half == 0 && (p.both || st == 0)) {
@@ -573,7 +609,7 @@ __device__ __forceinline__ void tma_role(const CUtensorMap *tq, const CUtensorMa
       const int tok = (t + lane / per_tile) * BN + lane % per_tile * a.box;
       if (tok < p.s.len && t + lane / per_tile < p.te) {
         const int b = tok / a.bs;
-        rows = (int)(((long long)__ldg(table + b) * a.Hkv + p.head) * a.bs + (tok - b * a.bs));
+        rows = (int)(((long long)table[b] * a.Hkv + p.head) * a.bs + (tok - b * a.bs));
       }
     };
     auto load = [&](const CUtensorMap *map, int t) {
@@ -602,11 +638,11 @@ __device__ __forceinline__ void tma_role(const CUtensorMap *tq, const CUtensorMa
       }
       __syncwarp();
     };
-    if (p.te <= p.tb) load_q();
+    if (p.te <= p.tb || pieces == 0) load_q();
     for (int t = p.tb; t < p.te; t++) {
       if ((t - p.tb) % group == 0) look_up(t);
       load(tk, t);
-      if (t == p.tb) load_q();  // behind the first keys: the last piece may still use Q
+      if (t == p.tb && pieces > 0) load_q();  // behind the first keys: the last piece may still use Q
       load(tv, t);
     }
     pieces++;
@@ -629,7 +665,7 @@ __device__ __forceinline__ void convert_role(const ChunkArgs &a, uint8_t *sm, B 
     for (int t = p.tb; t < p.te; t++) {
       const int tok = t * BN + r, valid = min(BN, p.s.len - t * BN);
       size_t row = 0;
-      if (r < valid) row = ((size_t)__ldg(table + tok / a.bs) * a.Hkv + p.head) * a.bs + tok % a.bs;
+      if (r < valid) row = ((size_t)table[tok / a.bs] * a.Hkv + p.head) * a.bs + tok % a.bs;
       const float scale = r < valid ? __ldcg((v_scale ? a.sv : a.sk) + row) : 0.f;
 #pragma unroll
       for (int v = 0; v < 2; v++, idx++) {
@@ -695,6 +731,9 @@ __global__ void __launch_bounds__(Cfg<D, INT8>::THREADS, 1)
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem)), "r"(512u));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  if (threadIdx.x == 17 * 32) {
+    for (const CUtensorMap *map : {&tq, &tk, &tv}) asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+  }
   if (threadIdx.x == 32) {
     bars.run = Run(a);
     mbar_init(&bars.q_full, 1);
@@ -719,6 +758,7 @@ __global__ void __launch_bounds__(Cfg<D, INT8>::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // what the last kernels wrote is there, and what they read is free
   const uint32_t tmem = bars.tmem;
   if (warp < 16) {
     regs_inc<C::REG_SOFT>();
@@ -745,9 +785,10 @@ __global__ void __launch_bounds__(Cfg<D, INT8>::THREADS, 1)
 // Joins the parts of the items that CTA boundaries cut: block x belongs to the
 // boundary before CTA x + 1 and takes the item if that boundary is its first.
 constexpr int kJoinThreads = 128;
-template <int D>
+// A part's sums lie [row][D] (few rows) or [D / 8][256 rows][8], as their writers' lanes run.
+template <int D, bool FEW>
 __global__ void __launch_bounds__(kJoinThreads) chunk_join_kernel(const __grid_constant__ ChunkArgs a) {
-  constexpr int ROWS = kJoinThreads / (D / 4);
+  constexpr int OCTETS = D / 8, ROWS = kJoinThreads / OCTETS;  // 8 columns a thread
   const int c = (int)blockIdx.x + 1;
   const Start it = a.start[c], before = a.start[c - 1];
   auto same = [&](const Start &x) { return x.seq == it.seq && x.head == it.head && x.pair == it.pair && x.tile > 0; };
@@ -759,30 +800,31 @@ __global__ void __launch_bounds__(kJoinThreads) chunk_join_kernel(const __grid_c
   int last = c;  // CTAs c - 1 .. last hold parts
   while (last + 1 < a.n_ctas && same(a.start[last + 1])) last++;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int col = threadIdx.x % (D / 4);
-  for (int r = (int)blockIdx.y * ROWS + threadIdx.x / (D / 4); r < rows; r += gridDim.y * ROWS) {
+  const int tid = threadIdx.x;
+  const int oct = FEW ? tid % OCTETS : tid / 8 % OCTETS, first = FEW ? tid / OCTETS : tid / (8 * OCTETS) * 8 + tid % 8;
+  for (int r = (int)blockIdx.y * ROWS + first; r < rows; r += gridDim.y * ROWS) {
     // row r of the item in the scratch: the second tile starts at 128
     const int tile_rows = a.sh.tpt * a.G, prow = both && r >= tile_rows ? BM + r - tile_rows : r;
     auto part = [&](int x) { return a.ws + (size_t)(x * 2 + (x == c - 1 ? 1 : 0)) * (kRowsItem * (D + 2)); };
+    const size_t at = FEW ? (size_t)prow * D + oct * 8 : ((size_t)oct * kRowsItem + prow) * 8;
     float m = -INFINITY;
     for (int x = c - 1; x <= last; x++) m = fmaxf(m, __ldcg(reinterpret_cast<const float2 *>(part(x) + (size_t)kRowsItem * D) + prow).x);
-    float l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (int x = c - 1; x <= last; x++) {
       const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part(x) + (size_t)kRowsItem * D) + prow);
       const float f = ml.x == -INFINITY ? 1.f : ex2(ml.x - m);  // without a maximum l and O are 0, or NaN
-      const float4 y = __ldcg(reinterpret_cast<const float4 *>(part(x) + (size_t)prow * D) + col);
+      const float4 y = __ldcg(reinterpret_cast<const float4 *>(part(x) + at)), z = __ldcg(reinterpret_cast<const float4 *>(part(x) + at) + 1);
+      const float v[8] = {y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w};
       l = fmaf(ml.y, f, l);
-      o.x = fmaf(y.x, f, o.x);
-      o.y = fmaf(y.y, f, o.y);
-      o.z = fmaf(y.z, f, o.z);
-      o.w = fmaf(y.w, f, o.w);
+#pragma unroll
+      for (int e = 0; e < 8; e++) o[e] = fmaf(v[e], f, o[e]);
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int tok = tok0 + r / a.G;
     const size_t row = (size_t)(s.row0 + tok) * a.Hq + (size_t)it.head * a.G + r % a.G;
-    *reinterpret_cast<uint2 *>(a.out + row * D + col * 4) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
-    if (col == 0 && a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+    *reinterpret_cast<uint4 *>(a.out + row * D + oct * 8) = make_uint4(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv),
+                                                                       pack_bf16(o[4] * inv, o[5] * inv), pack_bf16(o[6] * inv, o[7] * inv));
+    if (oct == 0 && a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
   }
 }
 
@@ -826,8 +868,7 @@ int launch_many(vxb_kv *kv, const CUtensorMap &q, const CUtensorMap &k, const CU
     VXB_CUDA_TRY(kv->ctx, cudaFuncSetAttribute(chunk_attn_kernel<D, INT8>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     configured[kv->ctx->device & 63] = true;
   }
-  chunk_attn_kernel<D, INT8><<<a.n_ctas, C::THREADS, C::SMEM, st>>>(q, k, v, a);
-  return launch_check(kv->ctx, "chunk_attn_kernel");
+  return launch_early(kv->ctx, "chunk_attn_kernel", chunk_attn_kernel<D, INT8>, dim3((unsigned)a.n_ctas), C::THREADS, C::SMEM, st, q, k, v, a);
 }
 
 int launch_many(vxb_kv *kv, const ChunkArgs &a, int64_t rows, cudaStream_t st) {
@@ -855,20 +896,12 @@ int launch_many(vxb_kv *kv, const ChunkArgs &a, int64_t rows, cudaStream_t st) {
   return i8 ? launch_many<64, true>(kv, mq, mk, mv, a, st) : launch_many<64, false>(kv, mq, mk, mv, a, st);
 }
 
-int launch_join(vxb_kv *kv, const ChunkArgs &a, int max_rows, cudaStream_t st) {
-  const int rows = kJoinThreads / (kv->head_dim / 4);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.n_ctas - 1), (unsigned)((max_rows + rows - 1) / rows));
-  cfg.blockDim = dim3(kJoinThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (kv->head_dim == 128) VXB_CUDA_TRY(kv->ctx, cudaLaunchKernelEx(&cfg, chunk_join_kernel<128>, a));
-  else VXB_CUDA_TRY(kv->ctx, cudaLaunchKernelEx(&cfg, chunk_join_kernel<64>, a));
-  return launch_check(kv->ctx, "chunk_join_kernel");
+int launch_join(vxb_kv *kv, const ChunkArgs &a, bool few, int max_rows, cudaStream_t st) {
+  const int rows = kJoinThreads / (kv->head_dim / 8);
+  auto *kernel = kv->head_dim == 128 ? (few ? chunk_join_kernel<128, true> : chunk_join_kernel<128, false>)
+                                     : (few ? chunk_join_kernel<64, true> : chunk_join_kernel<64, false>);
+  return launch_early(kv->ctx, "chunk_join_kernel", kernel, dim3((unsigned)(a.n_ctas - 1), (unsigned)((max_rows + rows - 1) / rows)), kJoinThreads,
+                      0, st, a);
 }
 
 int ctas_of(const vxb_ctx *ctx) {
@@ -1026,7 +1059,7 @@ int chunk_attention(vxb_kv *kv, int layer, int n, const int64_t *ids, const int3
       max_rows = (max_rows < 2 * a.sh.tpt ? max_rows : 2 * a.sh.tpt) * a.G;
       if (int rc = few ? launch_few(kv, a, max_rows, st) : launch_many(kv, a, total, st)) return rc;
       if (cut)
-        if (int rc = launch_join(kv, a, max_rows, st)) return rc;
+        if (int rc = launch_join(kv, a, few, max_rows, st)) return rc;
     }
   }
   return VXB_OK;

@@ -200,6 +200,13 @@ __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.a
 template <int N>
 __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
+// Adds 0 * x of every element: NaN in a lane of acc once an element was inf or NaN
+__device__ __forceinline__ uint32_t add_odd(uint32_t acc, const uint4 &x) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int i = 0; i < 4; i++) asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(w[i]), "r"(0u));
+  return acc;
+}
 __device__ __forceinline__ uint32_t odd_bf16(uint32_t w) {  // a non-finite element in a pair
   return (uint32_t)((w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u);
 }
@@ -208,6 +215,31 @@ __device__ __forceinline__ uint32_t even_bf16(uint32_t w) {  // the pair with ze
   if ((w & 0x7F80u) == 0x7F80u) w &= 0xFFFF0000u;
   if ((w & 0x7F800000u) == 0x7F800000u) w &= 0xFFFFu;
   return w;
+}
+#endif
+
+#ifdef __CUDACC__
+// Launches a kernel that may start its CTAs before the stream's last kernel has
+// ended; it waits for that itself (griddepcontrol.wait) before it touches memory.
+template <typename T>
+struct Same {
+  using type = T;
+};
+template <typename... P>
+int launch_early(vxb_ctx *ctx, const char *what, void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t st,
+                 const typename Same<P>::type &...args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  VXB_CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, kernel, args...));
+  return launch_check(ctx, what);
 }
 #endif
 

@@ -490,7 +490,7 @@ __device__ __forceinline__ int group_row(const ChunkArgs &a, const Piece &p, con
   const int tok = tile * BN + (threadIdx.x & 7) * 16;
   if (tok >= p.s.len) return 0;
   const int b = a.bs == 16 ? tok >> 4 : tok / a.bs;
-  return (__ldg(table + b) * a.Hkv + p.head) * a.bs + (tok - b * a.bs);
+  return (table[b] * a.Hkv + p.head) * a.bs + (tok - b * a.bs);
 }
 
 // Q warp: the query rows of each piece (zeros behind the last)
@@ -703,6 +703,7 @@ __global__ void __launch_bounds__(Cfg<D, INT8, NR>::THREADS, 1) chunk_few_kernel
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // what the last kernels wrote is there, and what they read is free
   const uint32_t tmem = bars.tmem;
   constexpr int SOFT_WARPS = C::SOFT * 4, LOAD_WARPS = C::PER_SLOT * 4;
   if (warp < SOFT_WARPS) {
@@ -741,8 +742,7 @@ int launch(vxb_kv *kv, const ChunkArgs &a, cudaStream_t st) {
     VXB_CUDA_TRY(kv->ctx, cudaFuncSetAttribute(chunk_few_kernel<D, INT8, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     configured[kv->ctx->device & 63] = true;
   }
-  chunk_few_kernel<D, INT8, NR><<<a.n_ctas, C::THREADS, C::SMEM, st>>>(a);
-  return launch_check(kv->ctx, "chunk_few_kernel");
+  return launch_early(kv->ctx, "chunk_few_kernel", chunk_few_kernel<D, INT8, NR>, dim3((unsigned)a.n_ctas), C::THREADS, C::SMEM, st, a);
 }
 
 template <int D, bool INT8>
