@@ -216,8 +216,9 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
       // V elements that only some rows may see, and rows behind the last token
       bool odd = false;
       const bool both_here = p.both && i < p.n0;  // the other stream works on the same tile
-      // a tile that hides keys from some row of either stream that uses it
-      const bool diagonal = (both_here ? lim_item : lim_first) < min(k0 + BN, p.s.len) - 1;
+      // the tile's first key that is hidden from some row of either stream that uses it
+      const int hidden = max(0, (both_here ? lim_item : lim_first) + 1 - k0);
+      const bool diagonal = hidden < min(BN, p.s.len - k0);
       if constexpr (!INT8) {
         if (diagonal || p.s.len - k0 < BN) {
           const int valid = min(BN, p.s.len - k0);
@@ -231,12 +232,9 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
           }
           if (diagonal) {
             uint32_t found[2] = {0u, 0u};
-#pragma unroll
-            for (int n = 0; n < BN * (D / 8) / 256; n++) {
-              const int c = tid + n * 256;
-              if (c / (D / 8) < valid)
-                found[n & 1] = add_odd(found[n & 1], *reinterpret_cast<const uint4 *>(sv_tile + chunk_off(c / (D / 8), c % (D / 8))));
-            }
+#pragma unroll 4
+            for (int c = hidden * (D / 8) + tid, n = 0; c < valid * (D / 8); c += 256, n ^= 1)
+              found[n] = add_odd(found[n], *reinterpret_cast<const uint4 *>(sv_tile + chunk_off(c / (D / 8), c % (D / 8))));
             __syncwarp();
             odd = bar_or(2 + st, 256, (odd_bf16(found[0]) | odd_bf16(found[1])) != 0);
           }
@@ -339,7 +337,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
                 for (int c = 0; c < D; c += 8) tmem_st8(tO + c, z);
                 tmem_wait_st();
               }
-              for (int k = half * N; k < min(valid, (half + 1) * N); k++)
+              for (int k = max(hidden, half * N); k < min(valid, (half + 1) * N); k++)
                 for (int c = 0; c < D / 8; c++) {
                   const uint4 w = *reinterpret_cast<const uint4 *>(sv_tile + chunk_off(k, c));
                   if (!(odd_bf16(w.x) | odd_bf16(w.y) | odd_bf16(w.z) | odd_bf16(w.w))) continue;
@@ -364,7 +362,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
           // every row has taken the odd elements: out of the tile with them
           if (both_here) bar_sync(1, 512);
           if (!(both_here && st == 1)) {
-            for (int c = tid; c < valid * (D / 8); c += 256) {
+            for (int c = hidden * (D / 8) + tid; c < valid * (D / 8); c += 256) {
               uint4 *at = reinterpret_cast<uint4 *>(sv_tile + chunk_off(c / (D / 8), c % (D / 8)));
               *at = make_uint4(even_bf16(at->x), even_bf16(at->y), even_bf16(at->z), even_bf16(at->w));
             }
@@ -788,7 +786,7 @@ constexpr int kJoinThreads = 128;
 // A part's sums lie [row][D] (few rows) or [D / 8][256 rows][8], as their writers' lanes run.
 template <int D, bool FEW>
 __global__ void __launch_bounds__(kJoinThreads) chunk_join_kernel(const __grid_constant__ ChunkArgs a) {
-  constexpr int OCTETS = D / 8, ROWS = kJoinThreads / OCTETS;  // 8 columns a thread
+  constexpr int COLS = FEW ? 4 : 8, ACROSS = D / COLS, ROWS = kJoinThreads / ACROSS;  // columns of a thread, threads of a row
   const int c = (int)blockIdx.x + 1;
   const Start it = a.start[c], before = a.start[c - 1];
   auto same = [&](const Start &x) { return x.seq == it.seq && x.head == it.head && x.pair == it.pair && x.tile > 0; };
@@ -801,30 +799,50 @@ __global__ void __launch_bounds__(kJoinThreads) chunk_join_kernel(const __grid_c
   while (last + 1 < a.n_ctas && same(a.start[last + 1])) last++;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int tid = threadIdx.x;
-  const int oct = FEW ? tid % OCTETS : tid / 8 % OCTETS, first = FEW ? tid / OCTETS : tid / (8 * OCTETS) * 8 + tid % 8;
+  const int col = FEW ? tid % ACROSS : tid / 8 % ACROSS, first = FEW ? tid / ACROSS : tid / (8 * ACROSS) * 8 + tid % 8;
   for (int r = (int)blockIdx.y * ROWS + first; r < rows; r += gridDim.y * ROWS) {
     // row r of the item in the scratch: the second tile starts at 128
     const int tile_rows = a.sh.tpt * a.G, prow = both && r >= tile_rows ? BM + r - tile_rows : r;
     auto part = [&](int x) { return a.ws + (size_t)(x * 2 + (x == c - 1 ? 1 : 0)) * (kRowsItem * (D + 2)); };
-    const size_t at = FEW ? (size_t)prow * D + oct * 8 : ((size_t)oct * kRowsItem + prow) * 8;
-    float m = -INFINITY;
-    for (int x = c - 1; x <= last; x++) m = fmaxf(m, __ldcg(reinterpret_cast<const float2 *>(part(x) + (size_t)kRowsItem * D) + prow).x);
-    float l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int x = c - 1; x <= last; x++) {
-      const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part(x) + (size_t)kRowsItem * D) + prow);
-      const float f = ml.x == -INFINITY ? 1.f : ex2(ml.x - m);  // without a maximum l and O are 0, or NaN
-      const float4 y = __ldcg(reinterpret_cast<const float4 *>(part(x) + at)), z = __ldcg(reinterpret_cast<const float4 *>(part(x) + at) + 1);
-      const float v[8] = {y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w};
-      l = fmaf(ml.y, f, l);
+    const size_t at = FEW ? (size_t)prow * D + col * 4 : ((size_t)col * kRowsItem + prow) * 8;
+    float m = -INFINITY, l = 0.f, o[COLS];
 #pragma unroll
-      for (int e = 0; e < 8; e++) o[e] = fmaf(v[e], f, o[e]);
+    for (int e = 0; e < COLS; e++) o[e] = 0.f;
+    for (int x = c - 1; x <= last; x += 2) {  // two parts at a time are mostly all of them: every load before its first use
+      float2 ml[2];
+      float4 y[2][COLS / 4];
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const float *from = part(min(x + h, last));
+        ml[h] = __ldcg(reinterpret_cast<const float2 *>(from + (size_t)kRowsItem * D) + prow);
+#pragma unroll
+        for (int e = 0; e < COLS / 4; e++) y[h][e] = __ldcg(reinterpret_cast<const float4 *>(from + at) + e);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        if (x + h > last) break;
+        const float top = fmaxf(m, ml[h].x);
+        // without a maximum l and O are 0, or NaN
+        const float f0 = m == -INFINITY ? 1.f : ex2(m - top), f1 = ml[h].x == -INFINITY ? 1.f : ex2(ml[h].x - top);
+        m = top;
+        l = fmaf(ml[h].y, f1, l * f0);
+#pragma unroll
+        for (int e = 0; e < COLS / 4; e++) {
+          o[e * 4] = fmaf(y[h][e].x, f1, o[e * 4] * f0);
+          o[e * 4 + 1] = fmaf(y[h][e].y, f1, o[e * 4 + 1] * f0);
+          o[e * 4 + 2] = fmaf(y[h][e].z, f1, o[e * 4 + 2] * f0);
+          o[e * 4 + 3] = fmaf(y[h][e].w, f1, o[e * 4 + 3] * f0);
+        }
+      }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int tok = tok0 + r / a.G;
     const size_t row = (size_t)(s.row0 + tok) * a.Hq + (size_t)it.head * a.G + r % a.G;
-    *reinterpret_cast<uint4 *>(a.out + row * D + oct * 8) = make_uint4(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv),
-                                                                       pack_bf16(o[4] * inv, o[5] * inv), pack_bf16(o[6] * inv, o[7] * inv));
-    if (oct == 0 && a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+#pragma unroll
+    for (int e = 0; e < COLS; e += 4)
+      *reinterpret_cast<uint2 *>(a.out + row * D + col * COLS + e) =
+          make_uint2(pack_bf16(o[e] * inv, o[e + 1] * inv), pack_bf16(o[e + 2] * inv, o[e + 3] * inv));
+    if (col == 0 && a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
   }
 }
 
@@ -897,7 +915,7 @@ int launch_many(vxb_kv *kv, const ChunkArgs &a, int64_t rows, cudaStream_t st) {
 }
 
 int launch_join(vxb_kv *kv, const ChunkArgs &a, bool few, int max_rows, cudaStream_t st) {
-  const int rows = kJoinThreads / (kv->head_dim / 8);
+  const int rows = kJoinThreads / (kv->head_dim / (few ? 4 : 8));
   auto *kernel = kv->head_dim == 128 ? (few ? chunk_join_kernel<128, true> : chunk_join_kernel<128, false>)
                                      : (few ? chunk_join_kernel<64, true> : chunk_join_kernel<64, false>);
   return launch_early(kv->ctx, "chunk_join_kernel", kernel, dim3((unsigned)(a.n_ctas - 1), (unsigned)((max_rows + rows - 1) / rows)), kJoinThreads,

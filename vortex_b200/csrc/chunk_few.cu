@@ -298,18 +298,15 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
       if (groups == GROUPS) weights(std::true_type{});
       else weights(std::false_type{});
       if constexpr (!INT8) {
-        if (a.sh.causal && min(k0 + BN, p.s.len) - 1 > base) {
-          // some row does not see all of this tile's keys
-          const int valid = min(BN, p.s.len - k0);
+        const int valid = min(BN, p.s.len - k0), hidden = a.sh.causal ? max(0, base + 1 - k0) : valid;
+        if (hidden < valid) {  // some row does not see the keys from here on
           wait(&bars.v_full[g % C::VS], (g / C::VS) & 1);
           uint8_t *V = sm + C::OFF_V + (g % C::VS) * C::TILE;
           uint32_t found = 0;
-          for (int c = threadIdx.x; c < valid * (D / 8); c += W * 128) {
-            const uint4 w = *reinterpret_cast<const uint4 *>(V + chunk_off(c / (D / 8), c % (D / 8)));
-            found |= odd_bf16(w.x) | odd_bf16(w.y) | odd_bf16(w.z) | odd_bf16(w.w);
-          }
+          for (int c = hidden * (D / 8) + (int)threadIdx.x; c < valid * (D / 8); c += W * 128)
+            found = add_odd(found, *reinterpret_cast<const uint4 *>(V + chunk_off(c / (D / 8), c % (D / 8))));
           __syncwarp();
-          if (bar_or(W + 1, W * 128, found != 0)) {
+          if (bar_or(W + 1, W * 128, odd_bf16(found) != 0)) {
             // rare: lane d of O^T takes every non-finite value of column d of V
             if (t > 0) {
               wait(&bars.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
@@ -321,7 +318,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
               if (threadIdx.x == 0) bars.acc = 1;
             }
             const int d = key % D;
-            for (int i = 0; i < valid; i++) {
+            for (int i = hidden; i < valid; i++) {
               const uint32_t bits = *reinterpret_cast<const uint16_t *>(V + chunk_off(i, d >> 3) + (d & 7) * 2);
               const bool odd = (bits & 0x7F80u) == 0x7F80u;
               if (!__any_sync(0xffffffffu, odd)) continue;
@@ -338,7 +335,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
               }
             }
             bar_sync(W + 1, W * 128);
-            for (int c = threadIdx.x; c < valid * (D / 8); c += W * 128) {
+            for (int c = hidden * (D / 8) + (int)threadIdx.x; c < valid * (D / 8); c += W * 128) {
               uint4 *at = reinterpret_cast<uint4 *>(V + chunk_off(c / (D / 8), c % (D / 8)));
               *at = make_uint4(even_bf16(at->x), even_bf16(at->y), even_bf16(at->z), even_bf16(at->w));
             }

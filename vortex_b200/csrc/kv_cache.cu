@@ -77,24 +77,29 @@ __global__ void kv_append_kernel(const KVPlace *__restrict__ places, int layer, 
 // A launch covers consecutive packed rows of the call: `n` pieces, piece i the
 // rows [row0_i, row0_{i+1}) that become tokens pos0_i, pos0_i + 1, ... of one
 // sequence; ids lists the pool blocks of its positions from block pos0_i /
-// block_size on, starting at ids[blk0_i]. The record travels by value (within
-// the 4 KB of kernel parameters that every launch carries), so an append needs
-// no host-to-device copy and no staging buffer that a later call could
-// overwrite.
-constexpr int kPieces = 64, kPieceIds = 640;
+// block_size on, starting at ids[blk0_i]. The record travels by value (a kernel
+// has up to 32,764 bytes of parameters), so an append needs no host-to-device
+// copy and no staging buffer that a later call could overwrite.
 struct ChunkPiece {
   int32_t slot, pos0, row0, blk0;
 };
-struct ChunkArgs {
+template <int PIECES, int IDS>
+struct ChunkArgsOf {
+  static constexpr int kPieces = PIECES, kIds = IDS;
   const uint16_t *k, *v;
   void *pool_k, *pool_v;
   float *scale_k, *scale_v;
   int32_t *tables, *lens;  // of the layer
   int H, bs, mbps, n, row_end, tokens;
-  ChunkPiece piece[kPieces];
-  int32_t ids[kPieceIds];
+  ChunkPiece piece[PIECES];
+  int32_t ids[IDS];
 };
-static_assert(sizeof(ChunkArgs) <= 4096, "kernel parameters");
+// A record of 4 KB for drafts (an append for 40 sequences and its truncate take
+// 17.3 us, 19.5 us with the large one), one of 32 KB for prompts (15,300 tokens of
+// 8 heads of 128: 34.5 us in launches of 640 blocks, 27.6 us in one).
+using FewChunks = ChunkArgsOf<64, 640>;
+using ManyChunks = ChunkArgsOf<256, 6912>;
+static_assert(sizeof(FewChunks) <= 4096 && sizeof(ManyChunks) <= 32764, "kernel parameters");
 
 constexpr int kChunkThreads = 256;
 constexpr int kChunkTokens = 64;  // most tokens of a CTA
@@ -104,8 +109,8 @@ constexpr int kChunkTokens = 64;  // most tokens of a CTA
 // rows are read once and written once (bf16), and the destination of a row is
 // 2 D contiguous bytes. A CTA takes `tokens` tokens, enough for two rounds of
 // loads at few heads.
-template <int D, bool INT8>
-__global__ void __launch_bounds__(kChunkThreads) kv_append_chunks_kernel(const __grid_constant__ ChunkArgs a) {
+template <int D, bool INT8, class Args>
+__global__ void __launch_bounds__(kChunkThreads) kv_append_chunks_kernel(const __grid_constant__ Args a) {
   __shared__ int32_t s_block[kChunkTokens], s_off[kChunkTokens];
   const int first = a.piece[0].row0 + (int)blockIdx.x * a.tokens;
   const int count = min(a.tokens, a.row_end - first);
@@ -463,75 +468,19 @@ void cut_table(vxb_kv *kv, vxb_kv::Table &t, int64_t len) {
   t.len = len;
 }
 
-int append_chunks(vxb_kv *kv, int layer, int n, const int64_t *ids, const int32_t *counts, const uint16_t *d_k,
-                  const uint16_t *d_v, cudaStream_t st) {
+struct AppendSeq {
+  vxb_kv::Table *table;  // null: not there yet, or no tokens
+  int64_t len;           // tokens before the call
+  int slot;              // -1: none yet
+};
+
+// The launches of an append whose tables already hold the new tokens' blocks
+template <class Args>
+int write_chunks(vxb_kv *kv, int layer, const std::vector<AppendSeq> &seqs, const int32_t *counts, const uint16_t *d_k,
+                 const uint16_t *d_v, cudaStream_t st) {
   vxb_ctx *ctx = kv->ctx;
-  const int bs = kv->block_size;
-  int64_t total = 0, need = 0;
-  size_t new_slots = 0;
-  for (int i = 0; i < n; i++) {
-    if (counts[i] < 0) return set_error(ctx, VXB_EINVAL, "vxb_kv_append_chunks: sequence %lld has %d tokens", (long long)ids[i], counts[i]);
-    total += counts[i];
-  }
-  if (total > INT_MAX) return set_error(ctx, VXB_EINVAL, "vxb_kv_append_chunks: %lld rows", (long long)total);
-  if (total == 0) return VXB_OK;
-  if (!d_k || !d_v || ((uintptr_t)d_k | (uintptr_t)d_v) % 16)
-    return set_error(ctx, VXB_EINVAL, "vxb_kv_append_chunks: d_k and d_v must be 16-byte aligned device pointers");
-  if (listed_twice(ids, n))
-    return set_error(ctx, VXB_EINVAL, "vxb_kv_append_chunks: a sequence is listed twice");
-  // everything is checked before anything is taken
-  struct Seq {
-    vxb_kv::Table *table;  // null: not there yet, or no tokens
-    int64_t len;
-    int slot;  // -1: none yet
-  };
-  std::vector<Seq> seqs(n, Seq{nullptr, 0, -1});
-  for (int i = 0; i < n; i++) {
-    if (counts[i] == 0) continue;
-    auto it = kv->tables.find(std::make_pair(layer, ids[i]));
-    auto si = kv->slot_of.find(ids[i]);
-    Seq &q = seqs[i];
-    if (it != kv->tables.end()) {
-      q.table = &it->second;
-      q.len = it->second.len;
-    }
-    if (si == kv->slot_of.end()) new_slots++;
-    else q.slot = si->second;
-    const int64_t have = (q.len + bs - 1) / bs, want = (q.len + counts[i] + bs - 1) / bs;
-    if (want > kv->max_blocks_per_seq || q.len + counts[i] > INT_MAX)
-      return set_error(ctx, VXB_ENOBLOCKS, "sequence %lld exceeds max_blocks_per_seq=%d", (long long)ids[i], kv->max_blocks_per_seq);
-    need += want - have;
-  }
-  if (need > (int64_t)kv->free_blocks.size()) return set_error(ctx, VXB_ENOBLOCKS, "KV cache out of blocks");
-  if (new_slots > kv->free_slots.size())
-    return set_error(ctx, VXB_ENOBLOCKS, "KV cache has no free sequence slot (max_seqs=%d)", kv->max_seqs);
-
-  // host tables: blocks and lengths, remembered for the launches. What may
-  // throw comes before what takes blocks.
-  for (int i = 0; i < n; i++) {
-    if (counts[i] == 0) continue;
-    Seq &q = seqs[i];
-    if (!q.table) q.table = &kv->tables[std::make_pair(layer, ids[i])];
-    const int64_t want = (q.len + counts[i] + bs - 1) / bs;
-    if ((int64_t)q.table->blocks.capacity() < want) q.table->blocks.reserve((size_t)std::max<int64_t>(want, 2 * q.len / bs));
-    if (q.slot < 0) {
-      q.slot = kv->slot_of[ids[i]] = kv->free_slots.back();
-      kv->free_slots.pop_back();
-    }
-  }
-  for (int i = 0; i < n; i++) {
-    if (counts[i] == 0) continue;
-    vxb_kv::Table &t = *seqs[i].table;
-    const int64_t want = (t.len + counts[i] + bs - 1) / bs;
-    while ((int64_t)t.blocks.size() < want) {
-      t.blocks.push_back(kv->free_blocks.back());
-      kv->refs[kv->free_blocks.back()] = 1;
-      kv->free_blocks.pop_back();
-    }
-    t.len += counts[i];
-  }
-
-  ChunkArgs a;
+  const int bs = kv->block_size, n = (int)seqs.size();
+  Args a;
   a.k = d_k;
   a.v = d_v;
   a.pool_k = kv->pool_k;
@@ -558,11 +507,11 @@ int append_chunks(vxb_kv *kv, int layer, int n, const int64_t *ids, const int32_
     const unsigned grid = (unsigned)((rows + a.tokens - 1) / a.tokens);
     const bool i8 = kv->dtype == VXB_I8;
     if (kv->head_dim == 128) {
-      if (i8) kv_append_chunks_kernel<128, true><<<grid, kChunkThreads, 0, st>>>(a);
-      else kv_append_chunks_kernel<128, false><<<grid, kChunkThreads, 0, st>>>(a);
+      if (i8) kv_append_chunks_kernel<128, true, Args><<<grid, kChunkThreads, 0, st>>>(a);
+      else kv_append_chunks_kernel<128, false, Args><<<grid, kChunkThreads, 0, st>>>(a);
     } else {
-      if (i8) kv_append_chunks_kernel<64, true><<<grid, kChunkThreads, 0, st>>>(a);
-      else kv_append_chunks_kernel<64, false><<<grid, kChunkThreads, 0, st>>>(a);
+      if (i8) kv_append_chunks_kernel<64, true, Args><<<grid, kChunkThreads, 0, st>>>(a);
+      else kv_append_chunks_kernel<64, false, Args><<<grid, kChunkThreads, 0, st>>>(a);
     }
     rc = launch_check(ctx, "kv_append_chunks_kernel");
     a.n = 0;
@@ -572,10 +521,10 @@ int append_chunks(vxb_kv *kv, int layer, int n, const int64_t *ids, const int32_
     int64_t pos = seqs[i].len;
     int left = counts[i];
     while (left > 0 && !rc) {
-      if (a.n == kPieces || used == kPieceIds) flush();
+      if (a.n == Args::kPieces || used == Args::kIds) flush();
       // as many of the chunk's tokens as the remaining ids reach
       const int64_t b0 = pos / bs;
-      const int64_t room = (int64_t)(kPieceIds - used) * bs - pos % bs;
+      const int64_t room = (int64_t)(Args::kIds - used) * bs - pos % bs;
       const int take = (int)std::min<int64_t>(left, room);
       const int64_t b1 = (pos + take + bs - 1) / bs;
       a.piece[a.n++] = {seqs[i].slot, (int32_t)pos, row, used};
@@ -586,6 +535,75 @@ int append_chunks(vxb_kv *kv, int layer, int n, const int64_t *ids, const int32_
     }
   }
   flush();
+  return rc;
+}
+
+int append_chunks(vxb_kv *kv, int layer, int n, const int64_t *ids, const int32_t *counts, const uint16_t *d_k,
+                  const uint16_t *d_v, cudaStream_t st) {
+  vxb_ctx *ctx = kv->ctx;
+  const int bs = kv->block_size;
+  int64_t total = 0, need = 0, spanned = 0;  // rows; new blocks; blocks that take rows
+  size_t new_slots = 0;
+  for (int i = 0; i < n; i++) {
+    if (counts[i] < 0) return set_error(ctx, VXB_EINVAL, "vxb_kv_append_chunks: sequence %lld has %d tokens", (long long)ids[i], counts[i]);
+    total += counts[i];
+  }
+  if (total > INT_MAX) return set_error(ctx, VXB_EINVAL, "vxb_kv_append_chunks: %lld rows", (long long)total);
+  if (total == 0) return VXB_OK;
+  if (!d_k || !d_v || ((uintptr_t)d_k | (uintptr_t)d_v) % 16)
+    return set_error(ctx, VXB_EINVAL, "vxb_kv_append_chunks: d_k and d_v must be 16-byte aligned device pointers");
+  if (listed_twice(ids, n))
+    return set_error(ctx, VXB_EINVAL, "vxb_kv_append_chunks: a sequence is listed twice");
+  // everything is checked before anything is taken
+  std::vector<AppendSeq> seqs(n, AppendSeq{nullptr, 0, -1});
+  for (int i = 0; i < n; i++) {
+    if (counts[i] == 0) continue;
+    auto it = kv->tables.find(std::make_pair(layer, ids[i]));
+    auto si = kv->slot_of.find(ids[i]);
+    AppendSeq &q = seqs[i];
+    if (it != kv->tables.end()) {
+      q.table = &it->second;
+      q.len = it->second.len;
+    }
+    if (si == kv->slot_of.end()) new_slots++;
+    else q.slot = si->second;
+    const int64_t have = (q.len + bs - 1) / bs, want = (q.len + counts[i] + bs - 1) / bs;
+    if (want > kv->max_blocks_per_seq || q.len + counts[i] > INT_MAX)
+      return set_error(ctx, VXB_ENOBLOCKS, "sequence %lld exceeds max_blocks_per_seq=%d", (long long)ids[i], kv->max_blocks_per_seq);
+    need += want - have;
+    spanned += want - q.len / bs;
+  }
+  if (need > (int64_t)kv->free_blocks.size()) return set_error(ctx, VXB_ENOBLOCKS, "KV cache out of blocks");
+  if (new_slots > kv->free_slots.size())
+    return set_error(ctx, VXB_ENOBLOCKS, "KV cache has no free sequence slot (max_seqs=%d)", kv->max_seqs);
+
+  // host tables: blocks and lengths, remembered for the launches. What may
+  // throw comes before what takes blocks.
+  for (int i = 0; i < n; i++) {
+    if (counts[i] == 0) continue;
+    AppendSeq &q = seqs[i];
+    if (!q.table) q.table = &kv->tables[std::make_pair(layer, ids[i])];
+    const int64_t want = (q.len + counts[i] + bs - 1) / bs;
+    if ((int64_t)q.table->blocks.capacity() < want) q.table->blocks.reserve((size_t)std::max<int64_t>(want, 2 * q.len / bs));
+    if (q.slot < 0) {
+      q.slot = kv->slot_of[ids[i]] = kv->free_slots.back();
+      kv->free_slots.pop_back();
+    }
+  }
+  for (int i = 0; i < n; i++) {
+    if (counts[i] == 0) continue;
+    vxb_kv::Table &t = *seqs[i].table;
+    const int64_t want = (t.len + counts[i] + bs - 1) / bs;
+    while ((int64_t)t.blocks.size() < want) {
+      t.blocks.push_back(kv->free_blocks.back());
+      kv->refs[kv->free_blocks.back()] = 1;
+      kv->free_blocks.pop_back();
+    }
+    t.len += counts[i];
+  }
+
+  const int rc = n <= FewChunks::kPieces && spanned <= FewChunks::kIds ? write_chunks<FewChunks>(kv, layer, seqs, counts, d_k, d_v, st)
+                                                                      : write_chunks<ManyChunks>(kv, layer, seqs, counts, d_k, d_v, st);
   if (rc)  // nothing was launched behind the failed launch: the tokens are taken back
     for (int i = n - 1; i >= 0; i--)
       if (seqs[i].table) cut_table(kv, *seqs[i].table, seqs[i].len);

@@ -149,6 +149,8 @@ __global__ void __launch_bounds__(kProbThreads) token_probs_kernel(const ProbArg
   cl.sync();
 }
 
+constexpr int kKeep = 8;  // fours of a thread that the second pass finds in shared memory, not in L2 (39.3 -> 38.0 us)
+
 // Two passes over the row. Four values a load where x and p have the same
 // place within 16 bytes (VEC): `head` single ones lead to the first boundary,
 // the cluster's ranks share the fours, the last rank takes the rest.
@@ -196,11 +198,17 @@ __global__ void __launch_bounds__(kRowThreads, 5) token_probs_rows_kernel(const 
   };
   auto e = [&](float y) { return exp_scaled(y, c); };
   constexpr int U = 4;  // loads under way
-  for (int k = b4 + (int)threadIdx.x; k < e4; k += U * kRowThreads) {
+  // the first of the share stay in shared memory (each thread's own)
+  __shared__ float4 s_keep[VEC ? kKeep : 1][kRowThreads];
+  int n = 0;
+  for (int k = b4 + (int)threadIdx.x; k < e4; k += U * kRowThreads, n += U) {
     float4 u[U];
 #pragma unroll
     for (int i = 0; i < U; i++)
       u[i] = k + i * kRowThreads < e4 ? x4[k + i * kRowThreads] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+#pragma unroll
+    for (int i = 0; i < U; i++)
+      if (n + i < kKeep) s_keep[n + i][threadIdx.x] = u[i];
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < U; i++) top = fmaxf(top, fmaxf(fmaxf(u[i].x, u[i].y), fmaxf(u[i].z, u[i].w)));
@@ -231,11 +239,12 @@ __global__ void __launch_bounds__(kRowThreads, 5) token_probs_rows_kernel(const 
   sum = 0.f;
   for (int i = 0; i < ranks; i++) sum += *cl.map_shared_rank(&s_sum, i);
   const float inv = sum == 0.f ? 0.f : 1.f / sum, ref = top == -INFINITY ? 0.f : top;
-  for (int k = b4 + (int)threadIdx.x; k < e4; k += U * kRowThreads) {
+  n = 0;
+  for (int k = b4 + (int)threadIdx.x; k < e4; k += U * kRowThreads, n += U) {
     float4 u[U];
 #pragma unroll
     for (int i = 0; i < U; i++)
-      if (k + i * kRowThreads < e4) u[i] = __ldcs(x4 + k + i * kRowThreads);
+      if (k + i * kRowThreads < e4) u[i] = n + i < kKeep ? s_keep[n + i][threadIdx.x] : __ldcs(x4 + k + i * kRowThreads);
 #pragma unroll
     for (int i = 0; i < U; i++)
       if (k + i * kRowThreads < e4)
