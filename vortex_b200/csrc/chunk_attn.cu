@@ -66,8 +66,9 @@ struct Cfg {
   static constexpr int RAWS = INT8 ? (D == 128 ? 3 : 6) : 0;
   static constexpr int OFF_KV = 2 * TILE;
   static constexpr int OFF_RAW = OFF_KV + SLOTS * TILE;
-  static constexpr int OFF_SCALE = OFF_RAW + RAWS * RAW;  // f32 per key: K and V scales of the last SLOTS tiles
-  static constexpr int OFF_X = OFF_SCALE + (INT8 ? SLOTS * 2 * BN * 4 : 0);  // what the two halves of a row tell each other
+  // int8: three f32 per key of the last SLOTS tiles, K's scale times a.scale_log2, log2 of V's, 1 / V's
+  static constexpr int OFF_SCALE = OFF_RAW + RAWS * RAW;
+  static constexpr int OFF_X = OFF_SCALE + (INT8 ? SLOTS * 3 * BN * 4 : 0);  // what the two halves of a row tell each other
   static constexpr int OFF_BARS = OFF_X + 4 * BM * 4;
   static constexpr int SMEM = OFF_BARS + 768;
   // warpgroups: two of softmax for each stream, one of the MMA and TMA warps,
@@ -80,7 +81,7 @@ struct Cfg {
 
 template <int SLOTS, int RAWS>
 struct Bars {
-  uint64_t q_full, q_empty, o_free, s_full[2], p_full[2], o_full[2], full[SLOTS], empty[SLOTS], raw_full[RAWS + 1],
+  uint64_t q_full, q_empty, o_free, s_full[2], p_full[2], o_full[2], full[SLOTS], empty[SLOTS], keyed[SLOTS], raw_full[RAWS + 1],
       raw_empty[RAWS + 1];
   uint32_t tmem;
   int acc[2];  // the stream's O already holds values that its first product adds to
@@ -116,11 +117,6 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(as_u64(a)), "l"(as_u64(b)), "l"(as_u64(c)));
   return as_f2(d);
 }
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(as_u64(a)), "l"(as_u64(b)));
-  return as_f2(d);
-}
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   uint64_t d;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(as_u64(a)), "l"(as_u64(b)));
@@ -143,18 +139,11 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
   for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
 }
 
-// v[i] *= f[i], f in shared memory (the same for every lane)
-template <int N>
-__device__ __forceinline__ void scale_keys(float *v, const float *f) {
-#pragma unroll
-  for (int c = 0; c < N; c += 4) {
-    const float4 x = *reinterpret_cast<const float4 *>(f + c);
-    const float2 lo = mul2(make_float2(v[c], v[c + 1]), make_float2(x.x, x.y)), hi = mul2(make_float2(v[c + 2], v[c + 3]), make_float2(x.z, x.w));
-    v[c] = lo.x;
-    v[c + 1] = lo.y;
-    v[c + 2] = hi.x;
-    v[c + 3] = hi.y;
-  }
+// four f32 of shared memory (the same for every lane) as two pairs
+__device__ __forceinline__ void four_keys(const float *f, float2 &lo, float2 &hi) {
+  const float4 x = *reinterpret_cast<const float4 *>(f);
+  lo = make_float2(x.x, x.y);
+  hi = make_float2(x.z, x.w);
 }
 
 // w[j] of lane q (of four) and w[q] of lane j change places
@@ -177,6 +166,7 @@ template <int D, bool INT8, class B>
 __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B &bars) {
   using C = Cfg<D, INT8>;
   constexpr int N = BN / 2;
+  constexpr float SHIFT = INT8 ? 6.f : 0.f;  // P, O and l hold 2^SHIFT times the weights
   const int st = threadIdx.x >> 8, half = (threadIdx.x >> 7) & 1, warp4 = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
   const int r = warp4 * 32 + lane, tid = threadIdx.x & 255;  // row of the tile; thread of the stream
   const uint32_t lane_off = (uint32_t)(warp4 * 32) << 16;
@@ -245,14 +235,28 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
         // registers for 64 scores (spilled, they took twice as long)
         constexpr int KEEP = INT8 ? 32 : N;
         float s[KEEP];
-        // K and V scales of this tile: there until its V is released, after P
-        const float *key_scale = reinterpret_cast<const float *>(sm + C::OFF_SCALE) + (kv / 2 % C::SLOTS) * 2 * BN + half * N;
+        // what the scales of this tile's keys make: there until its V is released, after P
+        const float *keys = reinterpret_cast<const float *>(sm + C::OFF_SCALE) + (kv / 2 % C::SLOTS) * 3 * BN + half * N;
+        if constexpr (INT8) wait(&bars.keyed[kv / 2 % C::SLOTS], (kv / 2 / C::SLOTS) & 1);
         const bool masked = !__all_sync(0xffffffffu, kh + N - 1 <= lim);
         auto scores = [&](int c0) {
 #pragma unroll
           for (int c = 0; c < KEEP; c += 32) tmem_ld32(tS + c0 + c, *reinterpret_cast<float(*)[32]>(s + c));
           tmem_wait_ld();
-          if constexpr (INT8) scale_keys<KEEP>(s, key_scale + c0);
+          if constexpr (INT8) {
+#pragma unroll
+            for (int c = 0; c < KEEP; c += 4) {
+              float2 k[2], v[2];
+              four_keys(keys + c0 + c, k[0], k[1]);
+              four_keys(keys + BN + c0 + c, v[0], v[1]);
+#pragma unroll
+              for (int e = 0; e < 2; e++) {
+                const float2 y = fma2(make_float2(s[c + 2 * e], s[c + 2 * e + 1]), k[e], v[e]);
+                s[c + 2 * e] = y.x;
+                s[c + 2 * e + 1] = y.y;
+              }
+            }
+          }
           if (masked) {
 #pragma unroll
             for (int c = 0; c < KEEP; c++) s[c] = kh + c0 + c <= lim ? s[c] : -INFINITY;
@@ -275,7 +279,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
         // here, waits for both halves' P)
         *x_mine = mx;
         bar_sync(pair, 64);
-        mx = fmaxf(mx, *x_half) * a.scale_log2;
+        mx = fmaxf(mx, *x_half) * (INT8 ? 1.f : a.scale_log2);
         const bool grow = mx > m + RESCALE_THRESHOLD;
         const float m_new = grow ? mx : m;
         const float mb = m_new == -INFINITY ? 0.f : m_new;
@@ -294,30 +298,41 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
             tmem_st8(tO + c, o);
           }
         }
-        if constexpr (INT8) wait(&bars.full[(kv + 1) % C::SLOTS], ((kv + 1) / C::SLOTS) & 1);  // V's scales come with V
-        const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), ref2 = make_float2(-mb, -mb);
+        const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), ref2 = make_float2(SHIFT - mb, SHIFT - mb);
         float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int c = 0; c < N / 32; c++) {
           if constexpr (INT8) scores(c * 32);
           float *v = s + c * 32 % KEEP;
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float2 x = fma2(make_float2(v[e], v[e + 1]), scale2, ref2);
-            v[e] = ex2(x.x);
-            v[e + 1] = ex2(x.y);
-            sum2[(e >> 1) & 1] = add2(sum2[(e >> 1) & 1], make_float2(v[e], v[e + 1]));
-          }
-          if constexpr (INT8) {
-            scale_keys<32>(v, key_scale + BN + c * 32);
-            if (masked) {  // 0 * a scale that is not finite
+          for (int e0 = 0; e0 < 32; e0 += 4) {
+            float2 inv[2];
+            if constexpr (INT8) {
+              four_keys(keys + 2 * BN + c * 32 + e0, inv[0], inv[1]);
+              if (masked) {  // 0 * what is not finite
 #pragma unroll
-              for (int e = 0; e < 32; e++) v[e] = kh + c * 32 + e <= lim ? v[e] : 0.f;
+                for (int e = 0; e < 2; e++) {
+                  inv[e].x = kh + c * 32 + e0 + 2 * e <= lim ? inv[e].x : 0.f;
+                  inv[e].y = kh + c * 32 + e0 + 2 * e + 1 <= lim ? inv[e].y : 0.f;
+                }
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              float *y = v + e0 + 2 * e;
+              const float2 x = INT8 ? add2(make_float2(y[0], y[1]), ref2) : fma2(make_float2(y[0], y[1]), scale2, ref2);
+              const float2 w = make_float2(ex2(x.x), ex2(x.y));
+              y[0] = w.x;
+              y[1] = w.y;
+              sum2[e] = INT8 ? fma2(w, inv[e], sum2[e]) : add2(sum2[e], w);
             }
           }
           uint32_t h[16];
 #pragma unroll
-          for (int e = 0; e < 16; e++) h[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
+          for (int e = 0; e < 16; e++) {
+            if constexpr (INT8) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h[e]) : "f"(v[2 * e + 1]), "f"(v[2 * e]));
+            else h[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
+          }
           tmem_st16u(tS + c * 16, h);
         }
         l = l * alpha + ((sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y));
@@ -376,6 +391,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.p_full[st]);
     }
+    m -= SHIFT;
     // ---------------- end of the piece: l of both halves, of a shared row of
     // both streams, then O
     bar_sync(pair, 64);  // the last step's maxima have been read
@@ -485,7 +501,9 @@ struct Slot {
 template <int D, bool INT8, class B>
 __device__ __forceinline__ void mma_role(const ChunkArgs &a, uint8_t *sm, B &bars) {
   using C = Cfg<D, INT8>;
-  constexpr uint32_t ID_QK = idesc_bf16(BM, BN, false), ID_PV = idesc_bf16(BM, D, true);
+  constexpr uint32_t ID_QK = idesc_bf16(BM, BN, false);
+  // int8: P and V in f16 (bits 7 and 10 of the types say bf16)
+  constexpr uint32_t ID_PV = INT8 ? idesc_bf16(BM, D, true) & ~((1u << 7) | (1u << 10)) : idesc_bf16(BM, D, true);
   constexpr uint64_t KMAJOR = desc_base(16, 1024), VMAJOR = desc_base(C::SLAB, 1024);
   const uint32_t s_q = smem_u32(sm) >> 4, s_kv = smem_u32(sm + C::OFF_KV) >> 4;
   const uint32_t tmem = __shfl_sync(0xffffffffu, bars.tmem, 0);
@@ -664,7 +682,7 @@ __device__ __forceinline__ void convert_role(const ChunkArgs &a, uint8_t *sm, B 
       const int tok = t * BN + r, valid = min(BN, p.s.len - t * BN);
       size_t row = 0;
       if (r < valid) row = ((size_t)table[tok / a.bs] * a.Hkv + p.head) * a.bs + tok % a.bs;
-      const float scale = r < valid ? __ldcg((v_scale ? a.sv : a.sk) + row) : 0.f;
+      const float scale = r < valid ? __ldcg((v_scale ? a.sv : a.sk) + row) : 1.f;
 #pragma unroll
       for (int v = 0; v < 2; v++, idx++) {
         const uint32_t raw = idx % C::RAWS, slot = idx % C::SLOTS;
@@ -672,9 +690,17 @@ __device__ __forceinline__ void convert_role(const ChunkArgs &a, uint8_t *sm, B 
         if (idx >= C::SLOTS) wait(&bars.empty[slot], (idx / C::SLOTS - 1) & 1);
         const uint8_t *src = sm + C::OFF_RAW + raw * C::RAW;
         uint8_t *dst = sm + C::OFF_KV + slot * C::TILE;
-        // V of tile t holds its slot until the softmax has used both of the
-        // tile's scales, so this warpgroup is less than SLOTS tiles ahead
-        if (v_scale == v) reinterpret_cast<float *>(sm + C::OFF_SCALE)[(idx / 2 % C::SLOTS * 2 + v) * BN + r] = scale;
+        // The slot was free: with 3 slots V of the tile before the last has
+        // been used, with 6 K of the third last, whose S came behind P of the
+        // tile before it. So the softmax is done with the tile SLOTS before
+        // this one, and its place takes this tile's scales.
+        if (!v) {
+          float *keys = reinterpret_cast<float *>(sm + C::OFF_SCALE) + idx / 2 % C::SLOTS * 3 * BN + r;
+          keys[v_scale * BN] = v_scale ? log2f(scale) : scale * a.scale_log2;
+          if (v_scale) keys[2 * BN] = 1.f / scale;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars.keyed[idx / 2 % C::SLOTS]);
+        }
         // 16 codes at a time; rows behind the last token become zeros
         uint4 codes[N];
 #pragma unroll
@@ -691,12 +717,17 @@ __device__ __forceinline__ void convert_role(const ChunkArgs &a, uint8_t *sm, B 
           for (int e = 0; e < 4; e++)
 #pragma unroll
             for (int half = 0; half < 2; half++) {
-              // bytes (b0, b1) -> bf16 pair of the codes: low 7 bits on the magic
-              // 0x43 give 128 + low7, the sign bit on it 128 or 256; their
-              // difference is the code, exactly
-              const uint32_t x = __byte_perm(in[e], 0x43434343u, half ? 0x4342u : 0x4140u);
               uint32_t d;
-              asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(x & 0xFF7FFF7Fu), "r"(x & 0xFF80FF80u));
+              if (v) {
+                // f16: (code ^ 0x80) under the magic 0x64 is 1024 + 128 + code
+                const uint32_t x = __byte_perm(in[e] ^ 0x80808080u, 0x64646464u, half ? 0x4342u : 0x4140u);
+                asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(0x64806480u));
+              } else {
+                // bf16: the low 7 bits under the magic 0x43 are 128 + low7, the
+                // sign bit alone 128 or 256; their difference is the code
+                const uint32_t x = __byte_perm(in[e], 0x43434343u, half ? 0x4342u : 0x4140u);
+                asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(x & 0xFF7FFF7Fu), "r"(x & 0xFF80FF80u));
+              }
               o[e * 2 + half] = d;
             }
           *reinterpret_cast<uint4 *>(dst + chunk_off(row_t, 2 * ch)) = make_uint4(o[0], o[1], o[2], o[3]);
@@ -746,6 +777,7 @@ __global__ void __launch_bounds__(Cfg<D, INT8>::THREADS, 1)
     for (int i = 0; i < C::SLOTS; i++) {
       mbar_init(&bars.full[i], INT8 ? 8 : 1);
       mbar_init(&bars.empty[i], 1);
+      mbar_init(&bars.keyed[i], 8);  // int8: the tile's scales
     }
     for (int i = 0; i < C::RAWS; i++) {
       mbar_init(&bars.raw_full[i], 1);
