@@ -1082,9 +1082,10 @@ int chunk_attention(vxb_kv *kv, int layer, int n, const int64_t *ids, const int3
   std::vector<int> lens(n, 0);
   bool all_few = true;
   int64_t few_tiles = 0;
+  TableFinder find(kv, layer);
   for (int i = 0; i < n; i++) {
     if (counts[i] == 0) continue;
-    auto it = kv->tables.find(std::make_pair(layer, ids[i]));
+    auto it = find(ids[i]);
     if (it != kv->tables.end()) lens[i] = (int)it->second.len;
     if (is_few(i)) few_tiles += (int64_t)(lens[i] + BN - 1) / BN * Hkv;
     else all_few = false;

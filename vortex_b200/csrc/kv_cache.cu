@@ -445,12 +445,9 @@ namespace {
 
 // A sequence listed twice in one call (the calls below change each sequence once)
 bool listed_twice(const int64_t *ids, int n) {
-  if (n <= 48) {
-    for (int i = 1; i < n; i++)
-      for (int j = 0; j < i; j++)
-        if (ids[i] == ids[j]) return true;
-    return false;
-  }
+  int rising = 1;
+  while (rising < n && ids[rising - 1] < ids[rising]) rising++;
+  if (rising >= n) return false;
   std::vector<int64_t> sorted(ids, ids + n);
   std::sort(sorted.begin(), sorted.end());
   return std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end();
@@ -556,9 +553,10 @@ int append_chunks(vxb_kv *kv, int layer, int n, const int64_t *ids, const int32_
     return set_error(ctx, VXB_EINVAL, "vxb_kv_append_chunks: a sequence is listed twice");
   // everything is checked before anything is taken
   std::vector<AppendSeq> seqs(n, AppendSeq{nullptr, 0, -1});
+  TableFinder find(kv, layer);
   for (int i = 0; i < n; i++) {
     if (counts[i] == 0) continue;
-    auto it = kv->tables.find(std::make_pair(layer, ids[i]));
+    auto it = find(ids[i]);
     auto si = kv->slot_of.find(ids[i]);
     AppendSeq &q = seqs[i];
     if (it != kv->tables.end()) {
@@ -628,22 +626,25 @@ int truncate(vxb_kv *kv, int n, const int64_t *ids, const int64_t *lens, cudaStr
     if (si != kv->slot_of.end()) slots[i] = si->second;
   }
   int64_t freed = 0;
-  for (int layer = kv->num_layers - 1; layer >= 0; layer--)
-    for (int i = n - 1; i >= 0; i--) {
+  for (int layer = 0; layer < kv->num_layers; layer++) {
+    TableFinder find(kv, layer);
+    for (int i = 0; i < n; i++) {
       if (slots[i] < 0) continue;
-      auto it = kv->tables.find(std::make_pair(layer, ids[i]));
+      auto it = find(ids[i]);
       if (it == kv->tables.end() || it->second.len <= lens[i]) continue;
       vxb_kv::Table &t = it->second;
       cuts.push_back({&t, lens[i], layer, slots[i]});
       for (size_t b = (size_t)((lens[i] + bs - 1) / bs); b < t.blocks.size(); b++) freed += kv->refs[t.blocks[b]] == 1;
       if (lens[i] % bs && kv->refs[t.blocks[(size_t)(lens[i] / bs)]] > 1) moves.push_back(cuts.back());
     }
+  }
   if (cuts.empty()) return VXB_OK;
   if ((int64_t)moves.size() > (int64_t)kv->free_blocks.size() + freed) return set_error(ctx, VXB_ENOBLOCKS, "KV cache out of blocks");
   CutArgs a;
   a.lens = kv->d_lens;
   a.max_seqs = kv->max_seqs;
-  for (const Cut &c : cuts) cut_table(kv, *c.table, c.len);
+  // in the opposite order of the appends, so that they get the same blocks again
+  for (auto c = cuts.rbegin(); c != cuts.rend(); ++c) cut_table(kv, *c->table, c->len);
   for (const Cut &c : moves) {
     const size_t index = (size_t)(c.len / bs);
     const int32_t from = c.table->blocks[index];

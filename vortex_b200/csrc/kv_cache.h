@@ -39,6 +39,20 @@ struct vxb_kv {
   std::vector<int> free_slots;                        // stack of unused slots
 };
 
+// Finds the tables of one layer; the one behind the last found is tried first,
+// since calls mostly list their sequences in order.
+struct TableFinder {
+  vxb_kv *kv;
+  int layer;
+  std::map<std::pair<int, int64_t>, vxb_kv::Table>::iterator last;
+  TableFinder(vxb_kv *kv, int layer) : kv(kv), layer(layer), last(kv->tables.end()) {}
+  auto operator()(int64_t id) {
+    const std::pair<int, int64_t> key(layer, id);
+    if (last != kv->tables.end() && ++last != kv->tables.end() && last->first == key) return last;
+    return last = kv->tables.find(key);
+  }
+};
+
 namespace vxb {
 
 // Reserve placement for one appended token of (layer, seq_id): pops a block

@@ -29,6 +29,8 @@ def _host_array(values, dtype):
 def _ids_counts(who: str, seq_ids, counts, dtype=np.int32):
     """Host arrays of one sequence id and one count (or length) each."""
     ids = _host_array(seq_ids, _I64)
+    if type(counts) is np.ndarray and counts.dtype == dtype and counts.ndim == 1 and counts.size == ids.size:
+        return ids, counts  # (a negative one is refused by the call)
     if not (type(counts) is np.ndarray and counts.dtype == dtype):
         counts = np.atleast_1d(np.asarray(counts))
         if counts.size and (not np.issubdtype(counts.dtype, np.integer) or int(counts.max()) > np.iinfo(dtype).max):
@@ -48,7 +50,8 @@ def _device_rows(who: str, name: str, t, shape, device: int):
         raise N.VxbError(N.VXB_EINVAL, f"{who}: {name} must be a bf16 tensor on cuda:{device}")
     if t.shape != shape:
         raise N.VxbError(N.VXB_EINVAL, f"{who}: {name} must be {tuple(shape)}, got {tuple(t.shape)}")
-    t = t.contiguous()
+    if not t.is_contiguous():
+        t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 

@@ -43,9 +43,9 @@ def _f32_rows(who: str, name: str, t, shape=None, device=None):
         raise N.VxbError(N.VXB_EINVAL, f"{who}: {name} must be an f32 tensor on the GPU")
     if shape is not None and t.shape != shape:
         raise N.VxbError(N.VXB_EINVAL, f"{who}: {name} must be {tuple(shape)}, got {tuple(t.shape)}")
-    if device is not None and t.device != device:
-        raise N.VxbError(N.VXB_EINVAL, f"{who}: {name} is on {t.device}, not on {device}")
-    return t.contiguous()
+    if device is not None and t.get_device() != device:
+        raise N.VxbError(N.VXB_EINVAL, f"{who}: {name} is on {t.device}, not on cuda:{device}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def token_probs(logits, temperature=1.0, out=None):
@@ -61,12 +61,12 @@ def token_probs(logits, temperature=1.0, out=None):
     rows = lg.numel() // vocab
     if out is None:
         out = torch.empty_like(lg)
-    elif _f32_rows("token_probs", "out", out, lg.shape, lg.device) is not out:
+    elif _f32_rows("token_probs", "out", out, lg.shape, lg.get_device()) is not out:
         raise N.VxbError(N.VXB_EINVAL, "token_probs: out must be contiguous")
     per_row = None
     if isinstance(temperature, torch.Tensor):
-        per_row = _f32_rows("token_probs", "temperature", temperature.reshape(-1), (rows,), lg.device)
-    dev = lg.device.index
+        per_row = _f32_rows("token_probs", "temperature", temperature.reshape(-1), (rows,), lg.get_device())
+    dev = lg.get_device()
     context(dev).call("vxb_token_probs", lg.data_ptr(), rows, vocab, per_row.data_ptr() if per_row is not None else None,
                       1.0 if per_row is not None else float(temperature), out.data_ptr(),
                       _stream_on(dev))
@@ -86,11 +86,11 @@ def verify_drafts(drafts, n_drafts, target_probs, draft_probs, u_accept, u_sampl
     per request; accepted int32 [n])."""
     import torch
     counts = n_drafts
-    if not (type(counts) is np.ndarray and counts.dtype == np.int32):
+    if not (type(counts) is np.ndarray and counts.dtype == np.int32 and counts.ndim == 1):
         counts = np.atleast_1d(np.asarray(counts))
         if counts.size and (not np.issubdtype(counts.dtype, np.integer) or int(counts.max()) > np.iinfo(np.int32).max):
             raise N.VxbError(N.VXB_EINVAL, "verify_drafts: n_drafts must be whole numbers of 32 bits")
-    counts = np.ascontiguousarray(counts, dtype=np.int32)
+        counts = counts.astype(np.int32)
     per = counts.tolist()
     if counts.ndim != 1 or (per and min(per) < 0):
         raise N.VxbError(N.VXB_EINVAL, "verify_drafts: n_drafts must be one list of numbers, none negative")
@@ -99,15 +99,15 @@ def verify_drafts(drafts, n_drafts, target_probs, draft_probs, u_accept, u_sampl
         raise N.VxbError(N.VXB_EINVAL, "verify_drafts: target_probs must be [rows, vocab]")
     vocab = target_probs.shape[1]
     p = _f32_rows("verify_drafts", "target_probs", target_probs, (total + n, vocab))
-    q = None if draft_probs is None else _f32_rows("verify_drafts", "draft_probs", draft_probs, (total, vocab), p.device)
-    ua = _f32_rows("verify_drafts", "u_accept", u_accept, (total,), p.device)
-    us = _f32_rows("verify_drafts", "u_sample", u_sample, (n,), p.device)
-    if not isinstance(drafts, torch.Tensor) or drafts.dtype != torch.int32 or drafts.device != p.device or drafts.shape != (total,):
-        raise N.VxbError(N.VXB_EINVAL, f"verify_drafts: drafts must be int32 ({total},) on {p.device}")
-    drafts = drafts.contiguous()
-    tokens = torch.empty(total + n, dtype=torch.int32, device=p.device)
-    accepted = torch.empty(n, dtype=torch.int32, device=p.device)
-    dev = p.device.index
+    dev = p.get_device()
+    q = None if draft_probs is None else _f32_rows("verify_drafts", "draft_probs", draft_probs, (total, vocab), dev)
+    ua = _f32_rows("verify_drafts", "u_accept", u_accept, (total,), dev)
+    us = _f32_rows("verify_drafts", "u_sample", u_sample, (n,), dev)
+    if not isinstance(drafts, torch.Tensor) or drafts.dtype != torch.int32 or drafts.get_device() != dev or drafts.shape != (total,):
+        raise N.VxbError(N.VXB_EINVAL, f"verify_drafts: drafts must be int32 ({total},) on cuda:{dev}")
+    if not drafts.is_contiguous():
+        drafts = drafts.contiguous()
+    tokens, accepted = drafts.new_empty(total + n), drafts.new_empty(n)
     context(dev).call("vxb_verify_drafts", n, counts.tobytes(), vocab, drafts.data_ptr(), p.data_ptr(),
                       q.data_ptr() if q is not None else None, ua.data_ptr(), us.data_ptr(), tokens.data_ptr(),
                       accepted.data_ptr(), _stream_on(dev))
