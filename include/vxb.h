@@ -372,7 +372,8 @@ int vxb_sample_top_p(vxb_ctx *ctx, const float *d_logits, int rows, int vocab, d
  * or, when d_temperature is NULL, `temperature` (finite). A temperature that
  * is not at least 0.01 is greedy, as in the generate loop (argmax below it): 1
  * at the first maximum, 0 elsewhere. -inf logits get 0; a row of -inf alone
- * gives zeros. A NaN logit makes its row NaN (greedy: it is passed over). d_probs may be d_logits. Allocates nothing. */
+ * gives zeros. A NaN logit makes its row NaN (greedy: it is passed over).
+ * vocab <= 2^30. d_probs may be d_logits. Allocates nothing. */
 int vxb_token_probs(vxb_ctx *ctx, const float *d_logits, int rows, int vocab, const float *d_temperature,
                     double temperature, float *d_probs, void *stream);
 
@@ -389,7 +390,8 @@ int vxb_token_probs(vxb_ctx *ctx, const float *d_logits, int rows, int vocab, co
  * sum. Products, differences and sums are f64. A row of max(p - q, 0) without
  * mass draws from p; a p without mass gives token 0; NaN counts as 0.
  * d_tokens int32 [sum of h_n_drafts + n] gets each request's accepted drafts,
- * the drawn token, then -1; d_n_accepted int32 [n]. Allocates nothing. */
+ * the drawn token, then -1; d_n_accepted int32 [n]. vocab <= 2^30. Allocates
+ * nothing. */
 int vxb_verify_drafts(vxb_ctx *ctx, int n, const int32_t *h_n_drafts, int vocab, const int32_t *d_drafts,
                       const float *d_target_probs, const float *d_draft_probs, const float *d_u_accept,
                       const float *d_u_sample, int32_t *d_tokens, int32_t *d_n_accepted, void *stream);

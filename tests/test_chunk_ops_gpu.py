@@ -710,3 +710,37 @@ def test_speculative_steps_together(KV, SM):
     # a decode step reads the same cache
     qq = rnd((n, Hq, D), 8)
     assert torch.equal(c.attention(0, ids, qq), plain.attention(0, ids, qq))
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_calls_in_a_row_without_waiting(KV, int8):
+    # each call starts while the last may still run: appends, attention whose
+    # items are cut and joined, and few rows, all over one scratch allocator
+    H, G, D, lens = 1, 4, 128, [2000, 700]
+    c = make(KV, 1, H, D, 16, 300, 2, int8)
+    c.append_chunks(0, [0, 1], lens, rnd((sum(lens), H, D), 1), rnd((sum(lens), H, D), 2))
+    torch.cuda.synchronize()
+    got = []
+    for step, counts in enumerate([[200, 3], [5, 1], [1, 140], [70, 70], [2, 2], [300, 0]]):
+        k, v = rnd((sum(counts), H, D), 10 + step), rnd((sum(counts), H, D), 20 + step)
+        q, lse = rnd((sum(counts), H * G, D), 30 + step, 2.0), torch.empty(sum(counts), H * G, device="cuda")
+        c.append_chunks(0, [0, 1], counts, k, v)
+        got.append((counts, q, c.chunk_attention(0, [0, 1], counts, q, lse=lse), lse))
+    total = [a + sum(x[0][i] for x in got) for i, a in enumerate(lens)]
+    for counts, q, out, lse in got[::-1]:
+        c.truncate([0, 1], total)
+        check_rows(out, lse, q, c, 0, [0, 1], counts, True, 1 / math.sqrt(D))
+        total = [a - b for a, b in zip(total, counts)]
+
+
+def test_probabilities_of_too_large_a_vocabulary_are_refused(SM):
+    from vortex_b200 import _native as N
+    from vortex_b200.quant import context
+    ctx, x = context(0), torch.zeros(8, device="cuda")
+    with pytest.raises(N.VxbError) as e:
+        ctx.call("vxb_token_probs", x.data_ptr(), 1, 2 ** 30 + 1, None, 1.0, x.data_ptr(), None)
+    assert e.value.code == N.VXB_EUNSUPPORTED
+    with pytest.raises(N.VxbError) as e:
+        ctx.call("vxb_verify_drafts", 1, np.zeros(1, np.int32).tobytes(), 2 ** 30 + 1, None, x.data_ptr(), None, None,
+                 x.data_ptr(), x.data_ptr(), x.data_ptr(), None)
+    assert e.value.code == N.VXB_EUNSUPPORTED

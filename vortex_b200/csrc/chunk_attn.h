@@ -54,11 +54,10 @@ __host__ __device__ inline int units_of(const ChunkSeq &s, const Shape &sh, int 
 }
 
 #ifdef __CUDACC__
-// Bounded wait; once one has run out, the following ones of this thread do not
-// wait again, and the kernel ends.
 using namespace vxb::tc;
 
-template <bool WARP>  // every lane of a warp waits, and they go on together
+// Bounded wait of a whole warp; once one has run out, the following ones do not
+// wait again, and the kernel ends.
 struct Waiter {
   int *err;
   bool dead = false;
@@ -67,7 +66,7 @@ struct Waiter {
       dead = true;
       atomicExch(err, 1);
     }
-    if (WARP) __syncwarp();
+    __syncwarp();
   }
 };
 
