@@ -639,7 +639,7 @@ __device__ __forceinline__ void tma_role(const CUtensorMap *tq, const CUtensorMa
       const int tok = (t + lane / per_tile) * BN + lane % per_tile * a.box;
       if (tok < p.s.len && t + lane / per_tile < p.te) {
         const int b = tok / a.bs;
-        rows = (int)(((long long)table[b] * a.Hkv + p.head) * a.bs + (tok - b * a.bs));
+        rows = (int)(((long long)__ldcg(table + b) * a.Hkv + p.head) * a.bs + (tok - b * a.bs));
       }
     };
     auto load = [&](const CUtensorMap *map, int t) {
@@ -695,7 +695,7 @@ __device__ __forceinline__ void convert_role(const ChunkArgs &a, uint8_t *sm, B 
     for (int t = p.tb; t < p.te; t++) {
       const int tok = t * BN + r, valid = min(BN, p.s.len - t * BN);
       size_t row = 0;
-      if (r < valid) row = ((size_t)table[tok / a.bs] * a.Hkv + p.head) * a.bs + tok % a.bs;
+      if (r < valid) row = ((size_t)__ldcg(table + tok / a.bs) * a.Hkv + p.head) * a.bs + tok % a.bs;
       const float scale = r < valid ? __ldcg((v_scale ? a.sv : a.sk) + row) : 1.f;
 #pragma unroll
       for (int v = 0; v < 2; v++, idx++) {

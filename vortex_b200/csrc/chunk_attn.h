@@ -219,7 +219,9 @@ __device__ __forceinline__ uint32_t even_bf16(uint32_t w) {  // the pair with ze
 
 #ifdef __CUDACC__
 // Launches a kernel that may start its CTAs before the stream's last kernel has
-// ended; it waits for that itself (griddepcontrol.wait) before it touches memory.
+// ended; it waits for that itself (griddepcontrol.wait) before it touches memory,
+// and reads through L2 alone: a line in L1 may be one that an earlier kernel
+// read on this SM, before a kernel in between wrote it.
 template <typename T>
 struct Same {
   using type = T;

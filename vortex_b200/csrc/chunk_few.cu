@@ -113,9 +113,6 @@ __device__ __forceinline__ uint32_t chunk_off(int r, int c) {
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void cp4(uint32_t dst, const void *src, bool live) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
-}
 __device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -492,12 +489,17 @@ __device__ __forceinline__ void mma_role(const ChunkArgs &a, uint8_t *sm, BarsOf
 
 // ------------------------------------------------------------------ loaders
 // What a loader warp knows of a tile: lane i < 8 has the pool row of the tile's
-// 16-token group i (of a block: block_size is a multiple of 16).
-__device__ __forceinline__ int group_row(const ChunkArgs &a, const Piece &p, const int32_t *table, int tile) {
+// 16-token group i (of a block: block_size is a multiple of 16). The table's
+// entry is read a tile ahead and used only then.
+__device__ __forceinline__ int group_block(const ChunkArgs &a, const Piece &p, int tile) {
   const int tok = tile * BN + (threadIdx.x & 7) * 16;
   if (tok >= p.s.len) return 0;
-  const int b = a.bs == 16 ? tok >> 4 : tok / a.bs;
-  return (table[b] * a.Hkv + p.head) * a.bs + (tok - b * a.bs);
+  return __ldcg(a.tables + (size_t)p.s.slot * a.mbps + (a.bs == 16 ? tok >> 4 : tok / a.bs));
+}
+__device__ __forceinline__ int group_row(const ChunkArgs &a, const Piece &p, int tile, int block) {
+  const int tok = tile * BN + (threadIdx.x & 7) * 16;
+  if (tok >= p.s.len) return 0;
+  return (block * a.Hkv + p.head) * a.bs + (a.bs == 16 ? 0 : tok % a.bs);
 }
 
 // Q warp: the query rows of each piece (zeros behind the last)
@@ -544,9 +546,8 @@ struct Tiles {
     } while (more && T == 0);
   }
   __device__ __forceinline__ int tile() const { return p.tb + t; }
-  __device__ __forceinline__ int rows(const ChunkArgs &a) const {
-    return more ? group_row(a, p, a.tables + (size_t)p.s.slot * a.mbps, tile()) : 0;
-  }
+  __device__ __forceinline__ int block(const ChunkArgs &a) const { return more ? group_block(a, p, tile()) : 0; }
+  __device__ __forceinline__ int rows(const ChunkArgs &a, int block) const { return group_row(a, p, tile(), block); }
 };
 
 // One group of four warps loads K, the other V.
@@ -562,11 +563,11 @@ __device__ __forceinline__ void load_role(const ChunkArgs &a, uint8_t *sm, BarsO
   Waiter wait{a.err};
   Tiles c(a);
   Ring<V ? C::VS : C::KS> at;
-  int next = c.rows(a);
+  int next = c.block(a);
   for (bool first = true; c.more; at.next()) {
-    const int valid = c.p.s.len - c.tile() * BN, rows = next;
+    const int valid = c.p.s.len - c.tile() * BN, rows = c.rows(a, next);
     c.next(a);
-    next = c.rows(a);  // the table's answer comes while this tile is copied
+    next = c.block(a);  // the table's answer comes while this tile is copied
     if (!first) wait(&empty[at.slot], at.phase ^ 1);
     if (at.slot + 1 == (V ? C::VS : C::KS)) first = false;
     const uint32_t dst = ring + at.slot * C::TILE;
@@ -598,12 +599,12 @@ __device__ __forceinline__ void load_role_i8(const ChunkArgs &a, uint8_t *sm, Ba
   const uint8_t *pool = reinterpret_cast<const uint8_t *>(V ? a.pool_v : a.pool_k) + ch * 16;
   Waiter wait{a.err};
   Tiles f(a), c(a);  // what is fetched, what is converted
-  int next = f.rows(a);
+  int next = f.block(a);
   auto fetch = [&](uint32_t stage) {
     if (f.more) {
-      const int valid = f.p.s.len - f.tile() * BN, rows = next;
+      const int valid = f.p.s.len - f.tile() * BN, rows = f.rows(a, next);
       f.next(a);
-      next = f.rows(a);
+      next = f.block(a);
       const uint32_t dst = smem_u32(raw + stage * C::RAW) + tid * 16;
 #pragma unroll
       for (int i = 0; i < N; i++) {
@@ -611,11 +612,9 @@ __device__ __forceinline__ void load_role_i8(const ChunkArgs &a, uint8_t *sm, Ba
         const int row = __shfl_sync(0xffffffffu, rows, r >> 4) + (r & 15);
         cp16(dst + i * (THREADS * 16), pool + (size_t)row * D, r < valid);
       }
-      if (!V && tid < BN) {  // both scales come with K
-        const int row = __shfl_sync(0xffffffffu, rows, tid >> 4) + (tid & 15);
-        const uint32_t at = smem_u32(raw + stage * C::RAW + BN * D) + tid * 8;
-        cp4(at, a.sk + row, tid < valid);
-        cp4(at + 4, a.sv + row, tid < valid);
+      if (!V && tid < 64) {  // both scales come with K: four keys' of K, or of V, a thread
+        const int k = lane * 4, row = __shfl_sync(0xffffffffu, rows, k >> 4) + (k & 15);
+        cp16(smem_u32(raw + stage * C::RAW + BN * D) + tid * 16, (tid < 32 ? a.sk : a.sv) + row, k < valid);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -633,12 +632,11 @@ __device__ __forceinline__ void load_role_i8(const ChunkArgs &a, uint8_t *sm, Ba
     for (int i = 0; i < N; i++) x[i] = *reinterpret_cast<const uint4 *>(src + i * (THREADS * 16) + tid * 16);
     if (!first) wait(&empty[at.slot], at.phase ^ 1);
     if (at.slot + 1 == (V ? C::VS : C::KS)) first = false;
-    if (!V && tid < BN) {
-      const bool live = tid < c.p.s.len - c.tile() * BN;  // a key that does not exist has scale 1
-      const float2 f2 = *reinterpret_cast<const float2 *>(src + BN * D + tid * 8);
-      float *to = reinterpret_cast<float *>(sm + C::OFF_SCALE) + scales.slot * 2 * BN + tid;
-      to[0] = live ? f2.x : 1.f;
-      to[BN] = live ? f2.y : 1.f;
+    if (!V && tid < 64) {
+      const int k = lane * 4, live = c.p.s.len - c.tile() * BN - k;  // a key that does not exist has scale 1
+      const float4 f = *reinterpret_cast<const float4 *>(src + BN * D + tid * 16);
+      float *to = reinterpret_cast<float *>(sm + C::OFF_SCALE) + scales.slot * 2 * BN + (tid < 32 ? 0 : BN) + k;
+      *reinterpret_cast<float4 *>(to) = make_float4(live > 0 ? f.x : 1.f, live > 1 ? f.y : 1.f, live > 2 ? f.z : 1.f, live > 3 ? f.w : 1.f);
     }
     uint8_t *dst = ring + at.slot * C::TILE;
 #pragma unroll
