@@ -29,13 +29,13 @@
 // Values of V that only some rows may see and that are not finite are taken
 // out of the tile and added to the rows that see them, as in chunk_attn.cu.
 //
-// Measured: 32 x 32 heads, ctx 2k, 4 rows 169 us (6.3 TB/s); 32 x 8 heads, ctx
-// 8k, 24 rows 177 us (6.1 TB/s), int8 16 rows 162 us (3.4 TB/s), 64 rows 238;
-// heads of 64, ctx 8k, 16 rows 101 us (5.3 TB/s); 32 heads, 333 keys, 4 rows
-// 6.5 us. bf16 tiles of 128 columns wait for memory. int8 tiles cost half the
-// bytes and 1.5 us each for their conversion and softmax, tiles of 64 columns
-// 0.9 us (16 rows) to 1.4 us (64 rows) against 0.75 us of memory time: the chain
-// vote, exponentials, P to shared memory, announcement of one tile.
+// Measured: 32 x 32 heads, ctx 2k, 4 rows 162 us (6.6 TB/s); 32 x 8 heads, ctx
+// 8k, 24 rows 165 us (6.5 TB/s), 64 rows 177, int8 16 rows 164 (3.4 TB/s), 64
+// rows 229; heads of 64, ctx 8k, 16 rows 93 us (5.8 TB/s), 64 rows 142; 32
+// heads, 333 keys, 4 rows 6.6 us. bf16 tiles of 128 columns wait for memory.
+// int8 halves the bytes and fills 63% of the issue slots with conversions and
+// softmax; tiles of 64 columns wait for the chain vote, exponentials, P to
+// shared memory, announcement (up to 1.3 us a tile against 0.75 us of memory).
 #include <atomic>
 #include <climits>
 #include <cmath>

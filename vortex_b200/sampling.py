@@ -67,7 +67,7 @@ def token_probs(logits, temperature=1.0, out=None):
     if isinstance(temperature, torch.Tensor):
         per_row = _f32_rows("token_probs", "temperature", temperature.reshape(-1), (rows,), lg.get_device())
     dev = lg.get_device()
-    context(dev).call("vxb_token_probs", lg.data_ptr(), rows, vocab, per_row.data_ptr() if per_row is not None else None,
+    N.Context.get(dev).call("vxb_token_probs", lg.data_ptr(), rows, vocab, per_row.data_ptr() if per_row is not None else None,
                       1.0 if per_row is not None else float(temperature), out.data_ptr(),
                       _stream_on(dev))
     return out
@@ -108,7 +108,7 @@ def verify_drafts(drafts, n_drafts, target_probs, draft_probs, u_accept, u_sampl
     if not drafts.is_contiguous():
         drafts = drafts.contiguous()
     tokens, accepted = drafts.new_empty(total + n), drafts.new_empty(n)
-    context(dev).call("vxb_verify_drafts", n, counts.tobytes(), vocab, drafts.data_ptr(), p.data_ptr(),
+    N.Context.get(dev).call("vxb_verify_drafts", n, counts.tobytes(), vocab, drafts.data_ptr(), p.data_ptr(),
                       q.data_ptr() if q is not None else None, ua.data_ptr(), us.data_ptr(), tokens.data_ptr(),
                       accepted.data_ptr(), _stream_on(dev))
     return tokens, accepted
