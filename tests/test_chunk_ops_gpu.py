@@ -215,7 +215,7 @@ def stored(c, layer, s):
     return k.double(), v.double()
 
 
-def exact_rows(q, k, v, m, causal, scale):
+def exact_rows(q, k, v, m, causal, scale, far=False):
     """out, lse and the two tolerances of the m rows q [m, Hq, D] over k, v [len, Hkv, D] (64 bits)."""
     n, hkv, D = k.shape
     G = q.shape[1] // hkv
@@ -231,14 +231,20 @@ def exact_rows(q, k, v, m, causal, scale):
     b = (torch.einsum("mhd,nhd->mhn", q.abs(), k.abs()) * scale).masked_fill(~sees[:, None], 0.0)
     b = b.amax(-1) if n else torch.zeros_like(lse)
     extra = 2 * D * 2.0 ** -24 * b + 2.0 ** -20
-    return out, lse, 2.0 ** -8 * out.abs() + (2.0 ** -8 + extra[..., None]) * (1 + 2.0 ** -8) * a, extra + 2.0 ** -22 * lse.abs()
+    tol = 2.0 ** -8 * out.abs() + (2.0 ** -8 + extra[..., None]) * (1 + 2.0 ** -8) * a
+    if far:
+        # int8 caches whose V scales lie far apart: a weight p_k s_k (s_k the V scale) is kept as f16 in a unit in which
+        # the row's largest is 2^6 or more, so below 2^-14 it is off by half of f16's least step, 2^-25: by
+        # 2^-31 max(p s). It multiplies a code of at most 127, and max |v_k| = 127 s_k: n 2^-31 max(p_k max |v_k|) in all.
+        tol = tol + n * 2.0 ** -31 * (p * v.abs().amax(-1).transpose(0, 1)[None]).amax(-1)[..., None]
+    return out, lse, tol, extra + 2.0 ** -22 * lse.abs()
 
 
-def check_rows(out, lse, q, c, layer, ids, counts, causal, scale):
+def check_rows(out, lse, q, c, layer, ids, counts, causal, scale, far=False):
     at = 0
     for s, m in zip(ids, counts):
         k, v = stored(c, layer, s)
-        o, z, to, tz = exact_rows(q[at:at + m], k, v, m, causal, scale)
+        o, z, to, tz = exact_rows(q[at:at + m], k, v, m, causal, scale, far)
         g, y = out[at:at + m].double(), lse[at:at + m].double()
         none = torch.isinf(z)
         assert torch.equal(torch.isinf(y) & (y < 0), none), s
@@ -336,6 +342,23 @@ def test_chunk_attention_cut_and_whole_runs(KV, H, G, bs, lens, counts, D, int8,
     out = c.chunk_attention(0, range(n), counts, q, causal=causal, lse=lse)
     check_rows(out, lse, q, c, 0, range(n), counts, causal, 1 / math.sqrt(D))
     assert torch.equal(out, c.chunk_attention(0, range(n), counts, q, causal=causal)), "not deterministic"
+
+
+@pytest.mark.parametrize("m", [150, 60, 24, 5])
+@pytest.mark.parametrize("D", [64, 128])
+def test_chunk_attention_int8_scales_far_apart(KV, D, m):
+    # values near the least and the largest that bf16 holds beside ordinary ones, and keys alike
+    H, n = 2, 700
+    k, v, q = rnd((n, H, D), 1), rnd((n, H, D), 2), rnd((m, H, D), 3)
+    v[3::7] *= 1e-39
+    v[5::11] *= 1e-20
+    v[n - 2:, 1] *= 1e30
+    k[2::9] *= 1e-39
+    c = make(KV, 1, H, D, 16, 50, 1, True)
+    c.append_chunks(0, [0], [n], k, v)
+    lse = torch.zeros(m, H, device="cuda")
+    out = c.chunk_attention(0, [0], [m], q, lse=lse)
+    check_rows(out, lse, q, c, 0, [0], [m], True, 1 / math.sqrt(D), far=True)
 
 
 @pytest.mark.parametrize("m", [200, 64])

@@ -48,7 +48,7 @@
 // of w / scale in f32. Every wait is bounded.
 //
 // Measured: 4096 tokens behind 12288 (8 x 4 heads of 128) 775-800 us, 1.2
-// PFLOP/s of 1.6; 4 x 512 of 2048 (8 x 4 heads) 73 us, of 32 heads in int8 122;
+// PFLOP/s of 1.6; 4 x 512 of 2048 (8 x 4 heads) 73 us, of 32 heads in int8 127;
 // 300 of 500 (8 x 4 heads) 16 us. A step of both streams (256 rows x 128 keys)
 // takes 3,400 to 4,000 cycles, of which the tensor core needs 2,100 and the 32
 // thousand exponentials 2,050: the chain S, maximum, P, O of a stream hides
@@ -104,6 +104,7 @@ struct Bars {
   Run run;
   Piece piece[2];
   int more[2];
+  alignas(4) uint8_t far[SLOTS][4];  // int8: a V scale with an inverse over kFarInverse among 32 keys of a tile
 };
 
 // 16-byte chunk c (8 columns) of row r of a bf16 tile in shared memory
@@ -173,6 +174,22 @@ __device__ __forceinline__ void transpose4(uint4 (&w)[4], int lane) {
   swap(w[2], w[3], 1);
   swap(w[0], w[2], 2);
   swap(w[1], w[3], 2);
+}
+
+// int8: a row's sum of 2^(score + ref) over N keys of S, the first `last` + 1 of
+// them visible. Rare (kFarInverse): a function of its own leaves the softmax its registers.
+template <int N>
+__device__ __noinline__ float far_sum(uint32_t tS, const float *keys, int last, float ref) {
+  float sum = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < N; c += 8) {
+    float v[8];
+    tmem_ld8(tS + c, v);
+    tmem_wait_ld();
+#pragma unroll
+    for (int e = 0; e < 8; e++) sum += c + e <= last ? ex2(fmaf(v[e], keys[c + e], ref)) : 0.f;
+  }
+  return sum;
 }
 
 // ------------------------------------------------------------------ softmax: thread = (stream, row, half of a tile's keys)
@@ -276,6 +293,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
             for (int c = 0; c < KEEP; c++) s[c] = kh + c0 + c <= lim ? s[c] : -INFINITY;
           }
         };
+        auto far = [&]() { return INT8 && *reinterpret_cast<const volatile uint32_t *>(bars.far[kv / 2 % C::SLOTS]) != 0; };
         float mx = -INFINITY;
 #pragma unroll
         for (int c0 = 0; c0 < N; c0 += KEEP) {
@@ -314,6 +332,9 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
         }
         const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), ref2 = make_float2(SHIFT - mb, SHIFT - mb);
         float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        if constexpr (INT8) {
+          if (far()) l = l * alpha + far_sum<N>(tS, keys, lim - kh, ref2.x);
+        }
 #pragma unroll
         for (int c = 0; c < N / 32; c++) {
           if constexpr (INT8) scores(c * 32);
@@ -349,7 +370,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
           }
           tmem_st16u(tS + c * 16, h);
         }
-        l = l * alpha + ((sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y));
+        if (!far()) l = l * alpha + ((sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y));
         tmem_wait_st();
       }
       if constexpr (!INT8) {
@@ -710,8 +731,16 @@ __device__ __forceinline__ void convert_role(const ChunkArgs &a, uint8_t *sm, B 
         // this one, and its place takes this tile's scales.
         if (!v) {
           float *keys = reinterpret_cast<float *>(sm + C::OFF_SCALE) + idx / 2 % C::SLOTS * 3 * BN + r;
-          keys[v_scale * BN] = v_scale ? log2f(scale) : scale * a.scale_log2;
-          if (v_scale) keys[2 * BN] = 1.f / scale;
+          if (v_scale) {
+            const float sv = scale < kLeastScale ? kLeastScale : scale;
+            const float inv = 1.f / sv;
+            keys[BN] = log2f(sv);
+            keys[2 * BN] = inv;
+            const bool far = __any_sync(0xffffffffu, inv > kFarInverse);
+            if (lane == 0) bars.far[idx / 2 % C::SLOTS][(tid >> 5) & 3] = far;
+          } else {
+            keys[0] = scale * a.scale_log2;
+          }
           __syncwarp();
           if (lane == 0) mbar_arrive(&bars.keyed[idx / 2 % C::SLOTS]);
         }

@@ -19,7 +19,7 @@
 // TB/s, 16-byte copies the memory rate), int8 rows by cp.async into a place of
 // the thread that then converts them, K to bf16 and V to f16 (codes are exact
 // in both). Rows behind the last token become zeros. Two warpgroups take the
-// softmax of up to 32 rows, four of more (int8, 64 rows: 295 and 262 us).
+// softmax of up to 32 rows, four of more (int8, 64 rows: 295 and 262 us then).
 //
 // int8 weights carry the V scale, w = p * scale, with the reference maximum
 // taken over log2(w), and go into P as f16 times 2^6: 11 significant bits, and
@@ -31,7 +31,7 @@
 //
 // Measured: 32 x 32 heads, ctx 2k, 4 rows 162 us (6.6 TB/s); 32 x 8 heads, ctx
 // 8k, 24 rows 165 us (6.5 TB/s), 64 rows 177, int8 16 rows 164 (3.4 TB/s), 64
-// rows 229; heads of 64, ctx 8k, 16 rows 93 us (5.8 TB/s), 64 rows 142; 32
+// rows 238; heads of 64, ctx 8k, 16 rows 93 us (5.8 TB/s), 64 rows 142; 32
 // heads, 333 keys, 4 rows 6.6 us. bf16 tiles of 128 columns wait for memory.
 // int8 halves the bytes and fills 63% of the issue slots with conversions and
 // softmax; tiles of 64 columns wait for the chain vote, exponentials, P to
@@ -151,6 +151,10 @@ __device__ __forceinline__ void halve(float *v, int lane) {
   }
 }
 
+// 2^(score + ref) of a row and the thread's key. Rare (kFarInverse): a function
+// of its own leaves the softmax its registers.
+__device__ __noinline__ float far_weight(uint32_t tS, float sc, float ref) { return ex2(fmaf(tmem_ld1(tS), sc, ref)); }
+
 // ------------------------------------------------------------------ softmax: thread = (key, the warpgroup's rows)
 // Rows go to the warpgroups in groups of eight in turn; groups without a live
 // row are passed over.
@@ -193,7 +197,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
       if constexpr (INT8) {
         const float *tile = scales + g % C::SCALES * 2 * BN;
         sc *= tile[key];
-        const float sv = tile[BN + key];
+        const float sv = tile[BN + key] < kLeastScale ? kLeastScale : tile[BN + key];
         add += log2f(sv);
         isv = 1.f / sv;
       }
@@ -278,6 +282,18 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
       if (g >= 2) wait(&bars.pv_done[g & 1], ((g - 2) >> 1) & 1);
       uint8_t *prow = P + (key >> 6) * (NR * 128) + wg * 8 * 128 + (key & 7) * 2;
       const uint32_t chunk = (uint32_t)(key & 63) >> 3;
+      if (INT8 && __any_sync(0xffffffffu, isv > kFarInverse)) {
+#pragma unroll
+        for (int j = 0; j < GROUPS; j++)
+          if (j < groups) {
+#pragma unroll
+            for (int n = j * 8; n < j * 8 + 8; n++) {
+              const float w = far_weight(tS + j * W * 8 + (n & 7), sc, SHIFT + ref_s[n]);
+              l[n] = row_of(n) >= n_min ? l[n] + w : l[n];
+            }
+          }
+        isv = 0.f;
+      }
       auto weights = [&](auto all) {
 #pragma unroll
         for (int j = 0; j < GROUPS; j++)
