@@ -15,10 +15,11 @@ constexpr int kRowsItem = 2 * BM;
 constexpr float RESCALE_THRESHOLD = 8.f;  // O is rescaled when a row's maximum grows by more (log2)
 
 // int8: weights carry the V scale, and the sum l takes the weight times its
-// inverse. A scale of 0 or a subnormal one counts as the least normal number
-// (NaN stays); the l of a tile that has one with an inverse over kFarInverse comes
-// from the scores alone, since such weights may leave the range of f32 beside large ones.
-constexpr float kLeastScale = 1.17549435e-38f, kFarInverse = 1073741824.f;  // 2^30
+// inverse. A scale under 2^-100 (values under 1e-28) counts as that, so that l
+// stays within f32 where a row sees nothing larger (NaN stays); the l of a tile
+// with an inverse over kFarInverse comes from the scores alone, since such
+// weights may leave the range of f32 beside large ones.
+constexpr float kLeastScale = 7.8886091e-31f, kFarInverse = 1073741824.f;  // 2^-100, 2^30
 struct ChunkSeq {
   int32_t slot, row0, rows, len;
 };
