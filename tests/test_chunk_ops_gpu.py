@@ -736,6 +736,25 @@ def test_speculative_steps_together(KV, SM):
 
 
 @pytest.mark.parametrize("int8", [False, True])
+def test_pages_behind_four_gigabytes(KV, int8):
+    H, D, bs = 32, 128, 1024
+    fill = 1100 if int8 else 560  # sequences of one token, each with a block of its own
+    c = make(KV, 1, H, D, bs, fill + 4, fill + 1, int8)
+    one = rnd((fill, H, D), 0)
+    c.append_chunks(0, range(fill), [1] * fill, one, one)
+    n = 2500
+    c.append_chunks(0, [fill], [n], rnd((n, H, D), 1), rnd((n, H, D), 2))
+    assert min(c.block_table(0, fill)) * H * bs * D * (1 if int8 else 2) > 2 ** 32
+    for m in (3, 200):
+        q, lse = rnd((m, H, D), 3, 2.0), torch.empty(m, H, device="cuda")
+        out = c.chunk_attention(0, [fill], [m], q, lse=lse)
+        check_rows(out, lse, q, c, 0, [fill], [m], True, 1 / math.sqrt(D))
+    assert torch.equal(c.get_kv(0, 7)[0][0], c.get_kv(0, 7)[1][0])
+    c.truncate([fill], [n - 40])
+    assert c.pages()["lens"][0, fill].item() == n - 40
+
+
+@pytest.mark.parametrize("int8", [False, True])
 def test_calls_in_a_row_without_waiting(KV, int8):
     # each call starts while the last may still run: appends, attention whose
     # items are cut and joined, and few rows, all over one scratch allocator
