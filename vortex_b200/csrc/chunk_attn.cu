@@ -733,8 +733,10 @@ __device__ __forceinline__ void convert_role(const ChunkArgs &a, uint8_t *sm, B 
           float *keys = reinterpret_cast<float *>(sm + C::OFF_SCALE) + idx / 2 % C::SLOTS * 3 * BN + r;
           if (v_scale) {
             const float sv = scale < kLeastScale ? kLeastScale : scale;
-            const float inv = 1.f / sv;
-            keys[BN] = log2f(sv);
+            // (a factor 2^lv in the weight and 2^-lv in the sum: what the
+            // approximate logarithm is off by, under 2^-16, is V's alone)
+            const float lv = __log2f(sv), inv = ex2(-lv);
+            keys[BN] = lv;
             keys[2 * BN] = inv;
             const bool far = __any_sync(0xffffffffu, inv > kFarInverse);
             if (lane == 0) bars.far[idx / 2 % C::SLOTS][(tid >> 5) & 3] = far;

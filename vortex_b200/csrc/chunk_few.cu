@@ -198,8 +198,9 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
         const float *tile = scales + g % C::SCALES * 2 * BN;
         sc *= tile[key];
         const float sv = tile[BN + key] < kLeastScale ? kLeastScale : tile[BN + key];
-        add += log2f(sv);
-        isv = 1.f / sv;
+        const float lv = __log2f(sv);  // off by under 2^-16, in V's factor alone
+        add += lv;
+        isv = ex2(-lv);
       }
       float x[N];  // log2 of what goes into P
       // (the usual case of only live groups has code without their branches,
