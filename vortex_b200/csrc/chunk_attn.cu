@@ -45,7 +45,8 @@
 // weights carry the V scale, log2(w) = log2(p) + log2(scale), the reference is
 // the maximum of those, and w goes into P as f16 times 2^6: 11 significant
 // bits, and weights down to 2^-30 of the row's largest keep at least one; l is
-// of w / scale in f32. Every wait is bounded.
+// of w / scale in f32 (or, beside a scale under 2^-30, of the scores: kFarInverse).
+// Every wait is bounded.
 //
 // Measured: 4096 tokens behind 12288 (8 x 4 heads of 128) 775-800 us, 1.2
 // PFLOP/s of 1.6; 4 x 512 of 2048 (8 x 4 heads) 73 us, of 32 heads in int8 127;
@@ -104,7 +105,6 @@ struct Bars {
   Run run;
   Piece piece[2];
   int more[2];
-  alignas(4) uint8_t far[SLOTS][4];  // int8: a V scale with an inverse over kFarInverse among 32 keys of a tile
 };
 
 // 16-byte chunk c (8 columns) of row r of a bf16 tile in shared memory
@@ -293,7 +293,8 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
             for (int c = 0; c < KEEP; c++) s[c] = kh + c0 + c <= lim ? s[c] : -INFINITY;
           }
         };
-        auto far = [&]() { return INT8 && *reinterpret_cast<const volatile uint32_t *>(bars.far[kv / 2 % C::SLOTS]) != 0; };
+        const float inv_max = INT8 ? fmaxf(keys[2 * BN + lane], keys[2 * BN + lane + 32]) : 0.f;
+        const bool far = INT8 && __any_sync(0xffffffffu, inv_max > kFarInverse);
         float mx = -INFINITY;
 #pragma unroll
         for (int c0 = 0; c0 < N; c0 += KEEP) {
@@ -333,7 +334,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
         const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), ref2 = make_float2(SHIFT - mb, SHIFT - mb);
         float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         if constexpr (INT8) {
-          if (far()) l = l * alpha + far_sum<N>(tS, keys, lim - kh, ref2.x);
+          if (far) l = l * alpha + far_sum<N>(tS, keys, lim - kh, ref2.x);
         }
 #pragma unroll
         for (int c = 0; c < N / 32; c++) {
@@ -370,7 +371,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
           }
           tmem_st16u(tS + c * 16, h);
         }
-        if (!far()) l = l * alpha + ((sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y));
+        if (!far) l = l * alpha + ((sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y));
         tmem_wait_st();
       }
       if constexpr (!INT8) {
@@ -735,11 +736,9 @@ __device__ __forceinline__ void convert_role(const ChunkArgs &a, uint8_t *sm, B 
             const float sv = scale < kLeastScale ? kLeastScale : scale;
             // (a factor 2^lv in the weight and 2^-lv in the sum: what the
             // approximate logarithm is off by, under 2^-16, is V's alone)
-            const float lv = __log2f(sv), inv = ex2(-lv);
+            const float lv = __log2f(sv);
             keys[BN] = lv;
-            keys[2 * BN] = inv;
-            const bool far = __any_sync(0xffffffffu, inv > kFarInverse);
-            if (lane == 0) bars.far[idx / 2 % C::SLOTS][(tid >> 5) & 3] = far;
+            keys[2 * BN] = ex2(-lv);
           } else {
             keys[0] = scale * a.scale_log2;
           }

@@ -30,8 +30,8 @@
 // out of the tile and added to the rows that see them, as in chunk_attn.cu.
 //
 // Measured: 32 x 32 heads, ctx 2k, 4 rows 162 us (6.6 TB/s); 32 x 8 heads, ctx
-// 8k, 24 rows 165 us (6.5 TB/s), 64 rows 177, int8 16 rows 164 (3.4 TB/s), 64
-// rows 238; heads of 64, ctx 8k, 16 rows 93 us (5.8 TB/s), 64 rows 142; 32
+// 8k, 24 rows 165 us (6.5 TB/s), 64 rows 177, int8 16 rows 158 (3.5 TB/s), 64
+// rows 227; heads of 64, ctx 8k, 16 rows 93 us (5.8 TB/s), 64 rows 142; 32
 // heads, 333 keys, 4 rows 6.6 us. bf16 tiles of 128 columns wait for memory.
 // int8 halves the bytes and fills 63% of the issue slots with conversions and
 // softmax; tiles of 64 columns wait for the chain vote, exponentials, P to
