@@ -232,7 +232,7 @@ def exact_rows(q, k, v, m, causal, scale, far=False):
     b = b.amax(-1) if n else torch.zeros_like(lse)
     extra = 2 * D * 2.0 ** -24 * b + 2.0 ** -20
     tol = 2.0 ** -8 * out.abs() + (2.0 ** -8 + extra[..., None]) * (1 + 2.0 ** -8) * a
-    if far:
+    if far and n:
         # int8 caches whose V scales lie far apart: a weight p_k s_k (s_k the V scale) is kept as f16 in a unit in which
         # the row's largest is 2^6 or more, so below 2^-14 it is off by half of f16's least step, 2^-25: by
         # 2^-31 max(p s). It multiplies a code of at most 127, and max |v_k| = 127 s_k: n 2^-31 max(p_k max |v_k|) in all.
