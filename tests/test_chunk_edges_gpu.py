@@ -1,0 +1,131 @@
+"""Chunk operators where their numbers are hard: int8 value rows of zeros and
+of scales far apart, infinities and NaN, rows whose first keys count for
+nothing, caches without a block to spare. Every result has to be finite where
+the definition's is, and within the bound; the definition is computed in 64
+bits from the codes and scales that the cache holds.
+
+Tolerances. Half a step is 2^-8 of a bf16 value, 2^-11 of an f16, 2^-24 of an
+f32. A softmax weight is off by
+  - its rounding: bf16 caches 2^-8; int8 caches, whose weights times the value's
+    scale s are f16 in a unit in which the row's largest p s is 2^6 at least,
+    2^-11, or 2^-25 / 2^6 of that largest below f16's least normal number,
+  - its score, a sum of D products in f32: 2 D 2^-24 B, B the largest
+    scale * sum |q k| that the row sees,
+  - the exponent, score + log2 s less the row's reference: at most eight
+    roundings of numbers up to 2 (B log2 e + max |log2 s| + 14):
+    2^-20 (B log2 e + max |log2 s| + 14),
+  - the exponential and the sums: 2^-20.
+E is the sum of the last three, w the rounding. With A = sum of p |v|:
+  |out - exact| <= 2^-8 |exact| + (1 + 2^-8) ((w + E) A + n 127 max(p s) 2^-31)
+  |lse - exact| <= E + 2^-22 |exact|
+and 127 * 2^-100 for V scales under 2^-100, which count as that.
+"""
+import math
+
+import numpy as np
+import pytest
+
+from tests.test_chunk_ops_gpu import CHUNKS, FEW, KV, RUNS, SM, make, rnd  # noqa: F401 (fixtures)
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+def held(c, layer, s):
+    """(k, v, V scales) of a sequence in 64 bits: [len, H, D] twice and [len, H] (0 for rows of zeros; None in bf16)."""
+    n, bs = c.seq_len(layer, s), c.block_size
+    p, t = c.pages(), torch.arange(n, device="cuda")
+    blocks = torch.tensor(c.block_table(layer, s), dtype=torch.long, device="cuda")[t // bs] if n else t
+    k, v = (p[x][blocks, :, t % bs].double() for x in ("k", "v"))
+    if "k_scale" not in p:
+        return k, v, None
+    sk, sv = (p[x + "_scale"][blocks, :, t % bs].double() for x in ("k", "v"))
+    return k * sk[..., None], v * sv[..., None], torch.where((v == 0).all(-1), 0.0, sv)
+
+
+def definition(q, k, v, sv, m, causal):
+    """out, lse and their tolerances; what a row does not see never enters."""
+    n, hkv, D = k.shape
+    G, scale = q.shape[1] // hkv, 1 / math.sqrt(D)
+    k, v = (t.repeat_interleave(G, 1) for t in (k, v))
+    q = q.double()
+    last = torch.arange(m, device=q.device) + (n - m) if causal else torch.full((m,), n - 1, device=q.device)
+    sees = (torch.arange(n, device=q.device)[None] <= last[:, None])[:, None]
+    s = (torch.einsum("mhd,nhd->mhn", q, k) * scale).masked_fill(~sees, -math.inf)
+    if n == 0:
+        none = torch.full((m, q.shape[1]), -math.inf, device=q.device, dtype=torch.float64)
+        zero = torch.zeros(m, q.shape[1], D, device=q.device, dtype=torch.float64)
+        return zero, none, zero, torch.zeros_like(none)
+    lse = torch.logsumexp(s, -1)
+    p = torch.exp(s - lse[..., None]).nan_to_num(0.0)
+    hide = (p == 0)[..., None] & ~torch.isfinite(v).transpose(0, 1)[None] if not bool(torch.isfinite(v).all()) else None
+    if hide is None:
+        out, a = torch.einsum("mhn,nhd->mhd", p, v), torch.einsum("mhn,nhd->mhd", p, v.abs())
+    else:
+        pv = (p[..., None] * v.transpose(0, 1)[None]).masked_fill(hide, 0.0)
+        out, a = pv.sum(2), pv.abs().sum(2)
+    b = (torch.einsum("mhd,nhd->mhn", q.abs(), k.abs()) * scale).masked_fill(~sees | torch.isinf(s), 0.0).amax(-1)
+    tiny = torch.zeros_like(b)
+    mag = b * math.log2(math.e) + 14
+    if sv is not None:
+        sv = sv.repeat_interleave(G, 1)
+        ok = torch.isfinite(sv) & (sv > 0)
+        spread = torch.where(ok, sv, 1.0).log2().abs().amax(0)
+        mag = mag + spread
+        tiny = 127 * (n * 2.0 ** -31 * (p * torch.where(ok, sv, 0.0).transpose(0, 1)).amax(-1) + 2.0 ** -100)
+    e = 2 * D * 2.0 ** -24 * b + 2.0 ** -20 * mag + 2.0 ** -20
+    w = 2.0 ** -8 if sv is None else 2.0 ** -11
+    tol = 2.0 ** -8 * out.abs() + (1 + 2.0 ** -8) * ((w + e[..., None]) * a + tiny[..., None]) + 2.0 ** -130
+    return out, lse, tol, e + 2.0 ** -22 * lse.abs()
+
+
+def check(out, lse, q, c, layer, ids, counts, causal=True, rows=None, lse_only=False):
+    """Every row (or those of `rows`, a mask over the packed ones) against the definition."""
+    at = 0
+    for s, m in zip(ids, counts):
+        o, z, to, tz = definition(q[at:at + m], *held(c, layer, s), m, causal)
+        g, y = out[at:at + m].double(), lse[at:at + m].double()
+        if rows is not None:
+            o, z, to, tz, g, y = (t[rows[at:at + m]] for t in (o, z, to, tz, g, y))
+        none = torch.isinf(z)
+        assert torch.equal(torch.isinf(y) & (y < 0), none), s
+        dz = (y - z)[~none].abs()
+        assert bool((dz <= tz[~none]).all()), (s, "lse", float(dz.max()), float(tz[~none].max()))
+        if not lse_only:
+            assert bool(torch.isfinite(to).all()) and bool((g[none] == 0).all()), s
+            off = (g - o).abs()
+            assert bool((off <= to).all()), (s, float((off / to).nan_to_num(math.inf).max()), int((~(off <= to)).sum()))
+        at += m
+
+
+def attend(c, ids, counts, q, causal=True, **kw):
+    lse = torch.full((q.shape[0], q.shape[1]), 7.0, device="cuda")
+    out = c.chunk_attention(0, ids, counts, q, causal=causal, lse=lse)
+    check(out, lse, q, c, 0, ids, counts, causal, **kw)
+    return out, lse
+
+
+def filled(KV, k, v, int8, bs=16):
+    n, H, D = k.shape
+    c = make(KV, 1, H, D, bs, -(-n // bs) + 2, 1, int8)
+    c.append_chunks(0, [0], [n], k, v)
+    return c
+
+
+ROWS = [150, 60, 24, 5]  # queries of a chunk: the many-row kernel, and the few-row one with 64, 32 and 16 columns
+SHAPES = [(2, 600), (2, 1500), (16, 1500)]  # heads, keys: whole items, items cut tile by tile, items cut into pieces of several
+
+
+# ---------------------------------------------------------------- attention, both caches
+
+@pytest.mark.parametrize("m", ROWS)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("score", [-3.0, -60.0, -150.0, 150.0])
+def test_keys_of_score_minus_infinity_before_the_others(KV, D, m, score):
+    # a row's unit comes from the first key that counts, not from the first key
+    for H, n in SHAPES:
+        k, v, q = rnd((n, H, D), 1), rnd((n, H, D), 2), rnd((m, H, D), 3)
+        q[..., 0], q[..., 1] = 1.0, 8.0
+        k[..., 0], k[..., 1] = 0.0, score * math.sqrt(D) / 8.0
+        k[:260, :, 0] = -math.inf
+        attend(filled(KV, k, v, False), [0], [m], q)

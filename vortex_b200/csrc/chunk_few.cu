@@ -151,6 +151,11 @@ __device__ __forceinline__ void halve(float *v, int lane) {
   }
 }
 
+// Negated reference of a row that has seen no finite score yet: the first one
+// passes it, and the vote for new references is called. A sum with it has lost
+// the score's last bits, so that tile's exponents are formed again.
+constexpr float kUnset = 1048576.f;
+
 // 2^(score + ref) of a row and the thread's key. Rare (kFarInverse): a function
 // of its own leaves the softmax its registers.
 __device__ __noinline__ float far_weight(uint32_t tS, float sc, float ref) { return ex2(fmaf(tmem_ld1(tS), sc, ref)); }
@@ -202,6 +207,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
         add += lv;
         isv = ex2(-lv);
       }
+    again:
       float x[N];  // log2 of what goes into P
       // (the usual case of only live groups has code without their branches,
       // which keep the rows' chains apart)
@@ -233,8 +239,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
       else load(std::false_type{});
       if (t == 0 || bar_or(bar, 128, top > RESCALE_THRESHOLD + SHIFT)) {
         // New references: a first tile's maximum, later the maximum of the rows
-        // that passed it, becomes 2^SHIFT. (A row without a visible key in its
-        // first tile has none in the others.)
+        // that passed it, becomes 2^SHIFT.
         float most = -INFINITY;
 #pragma unroll
         for (int j = 0; j < GROUPS; j++)
@@ -250,14 +255,26 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
         bar_sync(bar, 128);
         if (key < N) {
           const float m = fmaxf(fmaxf(red[key], red[N + key]), fmaxf(red[2 * N + key], red[3 * N + key]));
-          const float d = t == 0 ? (m > -INFINITY ? SHIFT - m : 0.f) : fminf(SHIFT - m, 0.f);
-          ref_s[key] += d;
-          d_s[key] = d;
+          const float d = t == 0 ? (m > -INFINITY ? SHIFT - m : kUnset) : fminf(SHIFT - m, 0.f);
+          const float ref = ref_s[key] + d;
+          d_s[key] = ref_s[key] >= kUnset / 2 && ref < kUnset / 2 ? NAN : d;
+          ref_s[key] = ref;
           f_s[key] = ex2(d);
         }
         bar_sync(bar, 128);
+        // (bf16 forms its exponents anew in any case: this costs its heads of 64
+        // 1% of a call, the branch for the rare case 5%; int8 the other way round)
+        bool coarse = false;
+        if constexpr (INT8) {
 #pragma unroll
-        for (int n = 0; n < N; n++) x[n] += d_s[n];
+          for (int n = 0; n < N; n++) {
+            const float d = d_s[n];
+            x[n] += d;
+            coarse |= isnan(d);
+          }
+        } else {
+          load(std::false_type{});
+        }
         if (t > 0) {
           wait(&bars.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
           tc_fence_after();
@@ -277,6 +294,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
             }
           tmem_wait_st();
         }
+        if (coarse) goto again;  // (once for a row: its reference never rises)
       }
       // P of two tiles ago has been used
       uint8_t *P = sm + C::OFF_P + (g & 1) * C::P;
