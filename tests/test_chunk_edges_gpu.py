@@ -116,6 +116,42 @@ ROWS = [150, 60, 24, 5]  # queries of a chunk: the many-row kernel, and the few-
 SHAPES = [(2, 600), (2, 1500), (16, 1500)]  # heads, keys: whole items, items cut tile by tile, items cut into pieces of several
 
 
+# ---------------------------------------------------------------- attention over int8 caches
+
+@pytest.mark.parametrize("m", ROWS)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("big,small", [(2.0 ** 115, 2.0 ** -20), (2.0 ** 120, 1.0), (2.0 ** 100, 2.0 ** -90), (2.0 ** 30, 2.0 ** -30)])
+@pytest.mark.parametrize("where", ["first", "last", "each tile", "one"])
+def test_int8_equal_scores_and_value_scales_far_apart(KV, D, m, big, small, where):
+    # the sum of the weights knows nothing of the values' sizes
+    for H, n in SHAPES:
+        k, v = torch.zeros(n, H, D, dtype=torch.bfloat16, device="cuda"), rnd((n, H, D), 2, small)
+        at = {"first": slice(0, 200), "last": slice(400, n), "each tile": slice(7, n, 50), "one": slice(3, 4)}[where]
+        v[at] = rnd((n, H, D), 3, big)[at]
+        attend(filled(KV, k, v, True), [0], [m], rnd((m, H, D), 4))
+
+
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+@pytest.mark.parametrize("m", [200, 64, 20])
+@pytest.mark.parametrize("D", [64, 128])
+def test_int8_values_that_are_not_finite(KV, D, m, bad):
+    # a value row with an infinity has the scale inf: NaN for the rows that see
+    # it, whose lse knows nothing of it; nothing for the others
+    H, n, at = 2, 300, 290
+    k, v, q = rnd((n, H, D), 1), rnd((n, H, D), 2), rnd((m, H, D), 3)
+    if math.isinf(bad):
+        v[at, 0, 3] = bad
+    c = filled(KV, k, v, True)
+    if math.isnan(bad):
+        c.pages()["v_scale"][c.block_table(0, 0)[at // 16], 0, at % 16] = bad
+    lse = torch.full((m, H), 7.0, device="cuda")
+    out = c.chunk_attention(0, [0], [m], q, lse=lse)
+    sees = torch.arange(m, device="cuda") + n - m >= at
+    check(out, lse, q, c, 0, [0], [m], lse_only=True)
+    check(out, lse, q, c, 0, [0], [m], rows=~sees)
+    assert bool(torch.isnan(out[sees, 0]).all()) and bool(torch.isfinite(out[:, 1]).all())
+
+
 # ---------------------------------------------------------------- attention, both caches
 
 @pytest.mark.parametrize("m", ROWS)

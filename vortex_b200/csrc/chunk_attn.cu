@@ -45,7 +45,7 @@
 // weights carry the V scale, log2(w) = log2(p) + log2(scale), the reference is
 // the maximum of those, and w goes into P as f16 times 2^6: 11 significant
 // bits, and weights down to 2^-30 of the row's largest keep at least one; l is
-// of w / scale in f32 (or, beside a scale under 2^-30, of the scores: kFarInverse).
+// of w / scale in f32 or, beside scales out of 2^+-30, of the scores alone (kFarLog2).
 // Every wait is bounded.
 //
 // Measured: 4096 tokens behind 12288 (8 x 4 heads of 128) 775-800 us, 1.2
@@ -84,7 +84,8 @@ struct Cfg {
   // int8: three f32 per key of the last SLOTS tiles, K's scale times a.scale_log2, log2 of V's, 1 / V's
   static constexpr int OFF_SCALE = OFF_RAW + RAWS * RAW;
   static constexpr int OFF_X = OFF_SCALE + (INT8 ? SLOTS * 3 * BN * 4 : 0);  // what the two halves of a row tell each other
-  static constexpr int OFF_BARS = OFF_X + 4 * BM * 4;
+  static constexpr int OFF_FAR = OFF_X + 4 * BM * 4;  // int8: the threads' maximum of scores (kFarLog2), +inf while they need none
+  static constexpr int OFF_BARS = OFF_FAR + (INT8 ? 4 * BM * 4 : 0);
   static constexpr int SMEM = OFF_BARS + 768;
   // warpgroups: two of softmax for each stream, one of the MMA and TMA warps,
   // int8: two that convert; registers at launch and of each
@@ -176,20 +177,31 @@ __device__ __forceinline__ void transpose4(uint4 (&w)[4], int lane) {
   swap(w[1], w[3], 2);
 }
 
-// int8: a row's sum of 2^(score + ref) over N keys of S, the first `last` + 1 of
-// them visible. Rare (kFarInverse): a function of its own leaves the softmax its registers.
+// int8: N keys' scores alone, the first `last` + 1 of them visible, added to a
+// row's maximum and sum of 2^(score - maximum). Rare (kFarLog2): a function of its
+// own leaves the softmax its registers.
 template <int N>
-__device__ __noinline__ float far_sum(uint32_t tS, const float *keys, int last, float ref) {
-  float sum = 0.f;
+__device__ __noinline__ float2 far_row(uint32_t tS, const float *keys, int last, float top, float sum) {
+  float m = top;
 #pragma unroll 1
   for (int c = 0; c < N; c += 8) {
     float v[8];
     tmem_ld8(tS + c, v);
     tmem_wait_ld();
 #pragma unroll
-    for (int e = 0; e < 8; e++) sum += c + e <= last ? ex2(fmaf(v[e], keys[c + e], ref)) : 0.f;
+    for (int e = 0; e < 8; e++) m = c + e <= last ? fmaxf(m, v[e] * keys[c + e]) : m;
   }
-  return sum;
+  const float ref = m == -INFINITY ? 0.f : m;
+  sum = top == -INFINITY ? sum : sum * ex2(top - ref);
+#pragma unroll 1
+  for (int c = 0; c < N; c += 8) {
+    float v[8];
+    tmem_ld8(tS + c, v);
+    tmem_wait_ld();
+#pragma unroll
+    for (int e = 0; e < 8; e++) sum += c + e <= last ? ex2(fmaf(v[e], keys[c + e], -ref)) : 0.f;
+  }
+  return make_float2(m, sum);
 }
 
 // ------------------------------------------------------------------ softmax: thread = (stream, row, half of a tile's keys)
@@ -205,6 +217,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
   const uint32_t tO = bars.tmem + 256 + st * 128 + lane_off, tO_other = bars.tmem + 256 + (st ^ 1) * 128 + lane_off;
   float *x_row = reinterpret_cast<float *>(sm + C::OFF_X) + r;  // [stream][half][row]
   float *x_mine = x_row + (st * 2 + half) * BM, *x_half = x_row + (st * 2 + (half ^ 1)) * BM;
+  float *far_row_s = reinterpret_cast<float *>(sm + C::OFF_FAR) + r, *far_s = far_row_s + (st * 2 + half) * BM;  // int8
   const int pair = 4 + st * 4 + warp4;  // barrier of the two warps that share these rows
   Waiter wait{a.err};
   uint32_t step = 0, pieces = 0, ring = 0;  // this stream's steps; pieces; first ring index of the piece
@@ -228,6 +241,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
     const int lim_first = a.sh.causal ? p.s.len - p.s.rows + tile_tok : p.s.len - 1, lim_item = a.sh.causal ? p.s.len - p.s.rows + p.tok0 : p.s.len - 1;
     const bool warp_live = warp4 * 32 < live;
     float m = -INFINITY, l = 0.f;
+    if constexpr (INT8) *far_s = INFINITY;
     const int steps = p.steps(st);
     for (int i = 0; i < steps; i++, step++) {
       const int t = p.tile(st, i), k0 = t * BN, kh = k0 + half * N;
@@ -293,8 +307,17 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
             for (int c = 0; c < KEEP; c++) s[c] = kh + c0 + c <= lim ? s[c] : -INFINITY;
           }
         };
-        const float inv_max = INT8 ? fmaxf(keys[2 * BN + lane], keys[2 * BN + lane + 32]) : 0.f;
-        const bool far = INT8 && __any_sync(0xffffffffu, inv_max > kFarInverse);
+        // the same for both halves: a scale of the tile, or of one before it
+        bool far = false;
+        if constexpr (INT8) {
+          const float *inv = keys - half * N + 2 * BN + lane;
+          bool key = false;
+#pragma unroll
+          for (int e = 0; e < BN; e += 32) key |= !(inv[e] >= 1.f / kFarInverse && inv[e] <= kFarInverse);
+          const bool was = *far_s < INFINITY;
+          far = __any_sync(0xffffffffu, key) || was;
+          if (far && !was) *far_s = l == 0.f ? -INFINITY : m - SHIFT;
+        }
         float mx = -INFINITY;
 #pragma unroll
         for (int c0 = 0; c0 < N; c0 += KEEP) {
@@ -334,7 +357,11 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
         const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), ref2 = make_float2(SHIFT - mb, SHIFT - mb);
         float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         if constexpr (INT8) {
-          if (far) l = l * alpha + far_sum<N>(tS, keys, lim - kh, ref2.x);
+          if (far) {
+            const float2 y = far_row<N>(tS, keys, lim - kh, *far_s, l);
+            *far_s = y.x;
+            l = y.y;
+          }
         }
 #pragma unroll
         for (int c = 0; c < N / 32; c++) {
@@ -433,11 +460,22 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
     bar_sync(pair, 64);  // the last step's maxima have been read
     *x_mine = l;
     bar_sync(pair, 64);
-    l += *x_half;
-    float f0 = 1.f, f1 = 0.f;  // factors of this stream's and the other's O
+    float own = 1.f;  // factor that brings this stream's O to the unit of l
+    if (INT8 && *far_s < INFINITY) {
+      // O and the sum have units of their own: O is divided by the sum, which then is 1
+      const float top = *far_s, other = far_row_s[(st * 2 + (half ^ 1)) * BM], ol = *x_half, t = fmaxf(top, other);
+      l = (top == -INFINITY ? l : l * ex2(top - t)) + (other == -INFINITY ? ol : ol * ex2(other - t));
+      own = l > 0.f ? ex2(m - t) / l : 0.f;
+      m = l > 0.f ? t + log2f(l) : -INFINITY;
+      l = l > 0.f ? 1.f : l;
+    } else {
+      l += *x_half;
+    }
+    float f0 = own, f1 = 0.f;  // factors of this stream's and the other's O
     if (!p.both) {
       bar_sync(1, 512);
       *x_mine = half ? l : m;
+      if (INT8 && half == 0) *far_s = own;
       bar_sync(1, 512);
       const float om = x_row[(st ^ 1) * 2 * BM], ol = x_row[((st ^ 1) * 2 + 1) * BM];
       const float top = fmaxf(m, om);
@@ -446,6 +484,10 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
       // NaN sums stay: a stream with steps whose maximum is -inf has l = 0 or NaN
       l = (m == -INFINITY ? l : l * f0) + (om == -INFINITY ? ol : ol * f1);
       m = top;
+      if constexpr (INT8) {
+        f0 *= own;
+        f1 *= far_row_s[(st ^ 1) * 2 * BM];
+      }
       bar_sync(1, 512);  // read by all
       wait(&bars.o_full[st ^ 1], pieces & 1);
     } else {

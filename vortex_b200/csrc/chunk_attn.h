@@ -14,12 +14,14 @@ constexpr int kMaxCtas = 160;
 constexpr int kRowsItem = 2 * BM;
 constexpr float RESCALE_THRESHOLD = 8.f;  // O is rescaled when a row's maximum grows by more (log2)
 
-// int8: weights carry the V scale, and the sum l takes the weight times its
-// inverse. A scale under 2^-100 (values under 1e-28) counts as that, so that l
-// stays within f32 where a row sees nothing larger (NaN stays); the l of a tile
-// with an inverse over kFarInverse comes from the scores alone, since such
-// weights may leave the range of f32 beside large ones.
-constexpr float kLeastScale = 7.8886091e-31f, kFarInverse = 1073741824.f;  // 2^-100, 2^30
+// int8: weights carry the V scale, and a row's unit follows the largest of them.
+// The sum l takes the weight times the scale's inverse, as long as all scales of
+// the tiles so far are within 2^+-kFarLog2: a weight that f32 flushes then is
+// under 2^-50 of the row's largest p. From the first tile with another scale on,
+// l is formed from the scores alone, with their own maximum, and meets O at the
+// end: it knows nothing of the values' sizes, infinite ones included. A scale
+// under 2^-100 (values under 1e-28) counts as that.
+constexpr float kLeastScale = 7.8886091e-31f, kFarLog2 = 30.f, kFarInverse = 1073741824.f;  // 2^-100, 2^30
 struct ChunkSeq {
   int32_t slot, row0, rows, len;
 };

@@ -56,8 +56,8 @@ struct Cfg {
   static constexpr int TILE = SLAB * (D / 64);
   static constexpr int AHEAD = 3;               // tiles whose S may be computed before the oldest one's P is there
   // int8: tiles of codes on their way, in shared memory of the thread that will
-  // convert them (RAWS each of K and V)
-  static constexpr int RAWS = INT8 ? 2 : 0, RAW = BN * D + BN * 8;
+  // convert them (RAWS each of K and V; K's bring the scales of both)
+  static constexpr int RAWS = INT8 ? 2 : 0, RAW_V = BN * D, RAW_K = RAW_V + BN * 8;
   // ring slots of K and of V
   static constexpr int KS = D == 64 ? (INT8 ? 4 : 5) : INT8 ? (NR == 64 ? 1 : 2) : NR == 64 ? 2 : 3;
   static constexpr int VS = D == 64 ? (INT8 ? 4 : 5) : INT8 ? 2 : 3;
@@ -66,12 +66,13 @@ struct Cfg {
   static constexpr int OFF_V = KS * TILE, OFF_Q = OFF_V + VS * TILE;
   static constexpr int OFF_P = OFF_Q + QBUFS * Q;  // two tiles
   static constexpr int OFF_RAW = OFF_P + 2 * P;
-  static constexpr int OFF_SCALE = OFF_RAW + 2 * RAWS * RAW;
+  static constexpr int OFF_SCALE = OFF_RAW + RAWS * (RAW_K + RAW_V);
   // Tiles whose K and V scales are kept: K of tile t is written when S of tile
   // t - KS is done, for which the softmax of the tile AHEAD before it is.
   static constexpr int SCALES = INT8 ? AHEAD + KS : 0;
   static constexpr int OFF_RED = OFF_SCALE + SCALES * 2 * BN * 4;  // per-warp results and per-row values of the softmax
-  static constexpr int OFF_BARS = OFF_RED + 7 * NR * 4;
+  static constexpr int PER_ROW = INT8 ? 15 : 7;
+  static constexpr int OFF_BARS = OFF_RED + PER_ROW * NR * 4;
   static constexpr int SMEM = OFF_BARS + 320;
   // Warpgroups: SOFT of softmax (up to 16 rows each), PER_SLOT each that load K
   // and V (int8 converts as it loads), one with the MMA and Q warps; registers
@@ -88,7 +89,8 @@ template <int KS, int VS>
 struct Bars {
   uint64_t k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], q_full[2], q_empty[2], s_full[3], p_full[2], pv_done[2], o_full[2], o_free[2];
   uint32_t tmem;
-  int acc;  // O already holds values that the piece's first product adds to
+  int acc;     // O already holds values that the piece's first product adds to
+  int far[4];  // int8, of each softmax warpgroup: the piece has met V scales out of kFarLog2
 };
 template <int D, bool INT8, int NR>
 using BarsOf = Bars<Cfg<D, INT8, NR>::KS, Cfg<D, INT8, NR>::VS>;
@@ -156,9 +158,29 @@ __device__ __forceinline__ void halve(float *v, int lane) {
 // the score's last bits, so that tile's exponents are formed again.
 constexpr float kUnset = 1048576.f;
 
-// 2^(score + ref) of a row and the thread's key. Rare (kFarInverse): a function
-// of its own leaves the softmax its registers.
-__device__ __noinline__ float far_weight(uint32_t tS, float sc, float ref) { return ex2(fmaf(tmem_ld1(tS), sc, ref)); }
+// int8: a tile's scores alone, added to each row's maximum and sum of 2^(score -
+// maximum) over the warp's keys. Rare (kFarLog2): a function of its own leaves the
+// softmax its registers. Row e of group j is row first + j * step + e of the item,
+// its scores in column j * step + e.
+__device__ __noinline__ void far_rows(uint32_t tS, int groups, int step, int first, float sc, int n_min, float *top, float *sum) {
+#pragma unroll 1
+  for (int j = 0; j < groups; j++)
+#pragma unroll 1
+    for (int e = 0; e < 8; e++) {
+      const int n = j * 8 + e;
+      const float s = tmem_ld1(tS + j * step + e);
+      const bool sees = first + j * step + e >= n_min;
+      float most;
+      asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(most) : "f"(sees ? s * sc : -INFINITY));
+      const float before = top[n], m = fmaxf(before, most), ref = m == -INFINITY ? 0.f : m;
+      const float w = warp_sum(sees ? ex2(fmaf(s, sc, -ref)) : 0.f);
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) {
+        sum[n] = (before == -INFINITY ? sum[n] : sum[n] * ex2(before - m)) + w;
+        top[n] = m;
+      }
+    }
+}
 
 // ------------------------------------------------------------------ softmax: thread = (key, the warpgroup's rows)
 // Rows go to the warpgroups in groups of eight in turn; groups without a live
@@ -173,7 +195,9 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
   // row n of the warpgroup's N is row row_of(n) of the item
   auto row_of = [&](int n) { return ((n >> 3) * W + wg) * 8 + (n & 7); };
   // this warpgroup's: per-warp results [4][N]; per row the negated reference, a factor, a change of the reference
-  float *red = reinterpret_cast<float *>(sm + C::OFF_RED) + wg * 7 * N, *ref_s = red + 4 * N, *f_s = ref_s + N, *d_s = f_s + N;
+  float *red = reinterpret_cast<float *>(sm + C::OFF_RED) + wg * C::PER_ROW * N, *ref_s = red + 4 * N, *f_s = ref_s + N, *d_s = f_s + N;
+  float *far_top = d_s + N, *far_sum = far_top + 4 * N;  // int8: of each warp, see far_rows
+  int *far_s = &bars.far[wg];
   const float *scales = reinterpret_cast<const float *>(sm + C::OFF_SCALE);
   const int bar = 1 + wg;
   Waiter wait{a.err};
@@ -199,6 +223,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
       const int n_min = k >= p.s.len ? INT_MAX : a.sh.causal && k > base ? (k - base) * a.G : 0;
       const bool masked = k0 + BN > p.s.len || (a.sh.causal && k0 + BN - 1 > base);
       float sc = a.scale_log2, add = SHIFT, isv = 1.f;
+      bool far_key = false;
       if constexpr (INT8) {
         const float *tile = scales + g % C::SCALES * 2 * BN;
         sc *= tile[key];
@@ -206,6 +231,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
         const float lv = __log2f(sv);  // off by under 2^-16, in V's factor alone
         add += lv;
         isv = ex2(-lv);
+        far_key = !(fabsf(lv) <= kFarLog2);
       }
     again:
       float x[N];  // log2 of what goes into P
@@ -237,7 +263,21 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
       };
       if (groups == GROUPS) load(std::true_type{});
       else load(std::false_type{});
-      if (t == 0 || bar_or(bar, 128, top > RESCALE_THRESHOLD + SHIFT)) {
+      if (t == 0 || bar_or(bar, 128, top > RESCALE_THRESHOLD + SHIFT || far_key)) {
+        bool far = false;
+        if constexpr (INT8) {
+          const bool was = t > 0 && *far_s != 0;
+          far = bar_or(bar, 128, far_key) || was;
+          if (far && !was) {  // the sums so far become each warp's own
+            halve<N, 16>(l, lane);
+            if (lane % (32 / N) == 0) {
+              const int n = lane / (32 / N);
+              far_top[warp * N + n] = l[0] == 0.f ? -INFINITY : -ref_s[n] - SHIFT;
+              far_sum[warp * N + n] = l[0];
+            }
+            __syncwarp();
+          }
+        }
         // New references: a first tile's maximum, later the maximum of the rows
         // that passed it, becomes 2^SHIFT.
         float most = -INFINITY;
@@ -261,6 +301,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
           ref_s[key] = ref;
           f_s[key] = ex2(d);
         }
+        if (INT8 && key == 0) *far_s = far;
         bar_sync(bar, 128);
         // (bf16 forms its exponents anew in any case: this costs its heads of 64
         // 1% of a call, the branch for the rare case 5%; int8 the other way round)
@@ -301,16 +342,8 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
       if (g >= 2) wait(&bars.pv_done[g & 1], ((g - 2) >> 1) & 1);
       uint8_t *prow = P + (key >> 6) * (NR * 128) + wg * 8 * 128 + (key & 7) * 2;
       const uint32_t chunk = (uint32_t)(key & 63) >> 3;
-      if (INT8 && __any_sync(0xffffffffu, isv > kFarInverse)) {
-#pragma unroll
-        for (int j = 0; j < GROUPS; j++)
-          if (j < groups) {
-#pragma unroll
-            for (int n = j * 8; n < j * 8 + 8; n++) {
-              const float w = far_weight(tS + j * W * 8 + (n & 7), sc, SHIFT + ref_s[n]);
-              l[n] = row_of(n) >= n_min ? l[n] + w : l[n];
-            }
-          }
+      if (INT8 && *(volatile int *)far_s) {
+        far_rows(tS, groups, W * 8, wg * 8, sc, n_min, far_top + warp * N, far_sum + warp * N);
         isv = 0.f;
       }
       auto weights = [&](auto all) {
@@ -402,9 +435,24 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
     float *part = a.ws + (size_t)(blockIdx.x * 2 + (p.tb > 0 ? 0 : 1)) * (kRowsItem * (D + 2));
     const size_t row0 = (size_t)(p.s.row0 + p.tok0) * a.Hq + (size_t)p.head * a.G;
     if (key < N) {
-      const float L = red[key] + red[N + key] + red[2 * N + key] + red[3 * N + key];
-      const float m = L == 0.f ? -INFINITY : -ref_s[key] - SHIFT;
-      f_s[key] = whole ? (L == 0.f ? 0.f : 1.f / L) : 1.f;
+      float L = red[key] + red[N + key] + red[2 * N + key] + red[3 * N + key];
+      const float unit = -ref_s[key] - SHIFT;  // of O (log2)
+      float m = L == 0.f ? -INFINITY : unit, f = whole ? (L == 0.f ? 0.f : 1.f / L) : 1.f;
+      if (INT8 && T > 0 && *far_s) {
+        // O and the sum have units of their own: O is divided by the sum here,
+        // also in a part, whose sum then is 1
+        const float *tops = far_top + key, *sums = far_sum + key;
+        const float top = fmaxf(fmaxf(tops[0], tops[N]), fmaxf(tops[2 * N], tops[3 * N]));
+        L = 0.f;
+        for (int w = 0; w < 4; w++) L += tops[w * N] == -INFINITY ? sums[w * N] : sums[w * N] * ex2(tops[w * N] - top);
+        f = L > 0.f ? ex2(unit - top) / L : L;
+        m = top;
+        if (!whole) {
+          m = L > 0.f ? top + log2f(L) : -INFINITY;
+          L = L > 0.f ? 1.f : L;
+        }
+      }
+      f_s[key] = f;
       ref_s[key] = 0.f;
       const int r = row_of(key);
       if (r < live) {
@@ -442,7 +490,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
         float *to = part + (size_t)r0 * D + d;
 #pragma unroll
         for (int e = 0; e < 8; e++)
-          if (e < count) __stcg(to + e * D, o[e]);
+          if (e < count) __stcg(to + e * D, INT8 ? o[e] * f8[e] : o[e]);
       }
       __syncwarp();
     }
@@ -625,12 +673,12 @@ __device__ __forceinline__ void load_role(const ChunkArgs &a, uint8_t *sm, BarsO
 template <int D, int NR, bool V>
 __device__ __forceinline__ void load_role_i8(const ChunkArgs &a, uint8_t *sm, BarsOf<D, true, NR> &bars) {
   using C = Cfg<D, true, NR>;
-  constexpr int THREADS = 128 * C::PER_SLOT;
+  constexpr int THREADS = 128 * C::PER_SLOT, RAW = V ? C::RAW_V : C::RAW_K;
   const int tid = threadIdx.x % THREADS, lane = threadIdx.x & 31;
   constexpr int CHUNKS = D / 16, STEP = THREADS / CHUNKS, N = BN / STEP;
   const int ch = tid % CHUNKS, r0 = tid / CHUNKS;
   uint64_t *full = V ? bars.v_full : bars.k_full, *empty = V ? bars.v_empty : bars.k_empty;
-  uint8_t *ring = sm + (V ? C::OFF_V : 0), *raw = sm + C::OFF_RAW + (V ? C::RAWS * C::RAW : 0);
+  uint8_t *ring = sm + (V ? C::OFF_V : 0), *raw = sm + C::OFF_RAW + (V ? C::RAWS * C::RAW_K : 0);
   const uint8_t *pool = reinterpret_cast<const uint8_t *>(V ? a.pool_v : a.pool_k) + ch * 16;
   Waiter wait{a.err};
   Tiles f(a), c(a);  // what is fetched, what is converted
@@ -640,7 +688,7 @@ __device__ __forceinline__ void load_role_i8(const ChunkArgs &a, uint8_t *sm, Ba
       const int valid = f.p.s.len - f.tile() * BN, rows = f.rows(a, next);
       f.next(a);
       next = f.block(a);
-      const uint32_t dst = smem_u32(raw + stage * C::RAW) + tid * 16;
+      const uint32_t dst = smem_u32(raw + stage * RAW) + tid * 16;
 #pragma unroll
       for (int i = 0; i < N; i++) {
         const int r = r0 + i * STEP;
@@ -649,7 +697,7 @@ __device__ __forceinline__ void load_role_i8(const ChunkArgs &a, uint8_t *sm, Ba
       }
       if (!V && tid < 64) {  // both scales come with K: four keys' of K, or of V, a thread
         const int k = lane * 4, row = __shfl_sync(0xffffffffu, rows, k >> 4) + (k & 15);
-        cp16(smem_u32(raw + stage * C::RAW + BN * D) + tid * 16, (tid < 32 ? a.sk : a.sv) + row, k < valid);
+        cp16(smem_u32(raw + stage * RAW + BN * D) + tid * 16, (tid < 32 ? a.sk : a.sv) + row, k < valid);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -661,7 +709,7 @@ __device__ __forceinline__ void load_role_i8(const ChunkArgs &a, uint8_t *sm, Ba
   Ring<V ? 1 : C::SCALES> scales;
   for (bool first = true; c.more; at.next(), stage.next(), scales.next(), c.next(a)) {
     cp_wait<C::RAWS - 1>();
-    const uint8_t *src = raw + stage.slot * C::RAW;
+    const uint8_t *src = raw + stage.slot * RAW;
     uint4 x[N];
 #pragma unroll
     for (int i = 0; i < N; i++) x[i] = *reinterpret_cast<const uint4 *>(src + i * (THREADS * 16) + tid * 16);
