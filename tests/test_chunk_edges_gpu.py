@@ -131,6 +131,32 @@ def test_int8_equal_scores_and_value_scales_far_apart(KV, D, m, big, small, wher
         attend(filled(KV, k, v, True), [0], [m], rnd((m, H, D), 4))
 
 
+@pytest.mark.parametrize("m", ROWS)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("size,logit", [(1.0, 0.0), (0.02, 10.0), (0.002, 12.0), (1e-4, 12.0), (1e-4, 30.0), (1.0, 100.0)])
+@pytest.mark.parametrize("where", ["one", "some", "first", "all"])
+def test_int8_value_rows_of_zeros(KV, D, m, size, logit, where):
+    # padding or an attention sink: nothing for the output, a share of the sum
+    for H, n in SHAPES:
+        k, v, q = rnd((n, H, D), 1), rnd((n, H, D), 2, size), rnd((m, H, D), 3)
+        at = {"one": slice(5, 6), "some": slice(3, n, 41), "first": slice(0, 300), "all": slice(0, n)}[where]
+        q[..., 0], k[..., 0] = 4.0, 0.0
+        k[at, :, 0] = logit * math.sqrt(D) / 4.0
+        v[at] = 0.0
+        attend(filled(KV, k, v, True), [0], [m], q)
+
+
+@pytest.mark.parametrize("m", ROWS)
+@pytest.mark.parametrize("D", [64, 128])
+def test_int8_rows_of_full_range_are_not_zeros(KV, D, m):
+    # scale 1 as a row of zeros has, but with codes; the first values are 0
+    H, n = 2, 400
+    k, v = rnd((n, H, D), 1), torch.zeros(n, H, D, dtype=torch.bfloat16, device="cuda")
+    v[..., D - 1], v[::2, :, D - 2] = 127.0, -127.0
+    v[::3] = rnd((n, H, D), 2, 1e-3)[::3]
+    attend(filled(KV, k, v, True), [0], [m], rnd((m, H, D), 3))
+
+
 @pytest.mark.parametrize("bad", [math.inf, math.nan])
 @pytest.mark.parametrize("m", [200, 64, 20])
 @pytest.mark.parametrize("D", [64, 128])

@@ -29,8 +29,9 @@
 //
 // Warps: 0-15 softmax (two warpgroups to a stream, each half of a tile's keys:
 // thread = row = TMEM lane; the halves tell each other their maxima), 16 issues
-// the MMAs, 17 the TMA copies; int8 caches add 20-27, which turn int8 pages
-// into K tiles of bf16 and V tiles of f16 (codes are exact in both). Pages come
+// the MMAs, 17 the TMA copies; int8 caches use 18, which looks the V scales over,
+// and add 20-27, which turn int8 pages into K tiles of bf16 and V tiles of f16
+// (codes are exact in both). Pages come
 // through one ring of tiles in the order K, V, K, V, ...; a page box is up to
 // 128 tokens of one block, of which only those that hold tokens are copied.
 //
@@ -81,9 +82,11 @@ struct Cfg {
   static constexpr int RAWS = INT8 ? (D == 128 ? 3 : 6) : 0;
   static constexpr int OFF_KV = 2 * TILE;
   static constexpr int OFF_RAW = OFF_KV + SLOTS * TILE;
-  // int8: three f32 per key of the last SLOTS tiles, K's scale times a.scale_log2, log2 of V's, 1 / V's
+  // int8: three f32 per key of the last SLOTS tiles, K's scale times a.scale_log2, log2 of V's, 1 / V's;
+  // then what is unusual about them (scale_role)
+  static constexpr int KEYS = 3 * BN + 4;
   static constexpr int OFF_SCALE = OFF_RAW + RAWS * RAW;
-  static constexpr int OFF_X = OFF_SCALE + (INT8 ? SLOTS * 3 * BN * 4 : 0);  // what the two halves of a row tell each other
+  static constexpr int OFF_X = OFF_SCALE + (INT8 ? SLOTS * KEYS * 4 : 0);  // what the two halves of a row tell each other
   static constexpr int OFF_FAR = OFF_X + 4 * BM * 4;  // int8: the threads' maximum of scores (kFarLog2), +inf while they need none
   static constexpr int OFF_BARS = OFF_FAR + (INT8 ? 4 * BM * 4 : 0);
   static constexpr int SMEM = OFF_BARS + 768;
@@ -97,7 +100,7 @@ struct Cfg {
 
 template <int SLOTS, int RAWS>
 struct Bars {
-  uint64_t q_full, q_empty, o_free, s_full[2], p_full[2], o_full[2], full[SLOTS], empty[SLOTS], keyed[SLOTS], raw_full[RAWS + 1],
+  uint64_t q_full, q_empty, o_free, s_full[2], p_full[2], o_full[2], full[SLOTS], empty[SLOTS], keyed[SLOTS], scaled[SLOTS], raw_full[RAWS + 1],
       raw_empty[RAWS + 1];
   uint32_t tmem;
   int acc[2];  // the stream's O already holds values that its first product adds to
@@ -177,31 +180,59 @@ __device__ __forceinline__ void transpose4(uint4 (&w)[4], int lane) {
   swap(w[1], w[3], 2);
 }
 
-// int8: N keys' scores alone, the first `last` + 1 of them visible, added to a
-// row's maximum and sum of 2^(score - maximum). Rare (kFarLog2): a function of its
-// own leaves the softmax its registers.
+// int8: what the sum of weights gets from a tile with unusual scales (scale_role),
+// from N keys of S, the first `last` + 1 of them visible. The keys whose value row is
+// zero (log2 scale -inf) add 2^(score + ref). Where the sum has a maximum of its own
+// (`far`), and from here on where such a share is too large or the row has no unit
+// but such keys, all keys add 2^(score - maximum). Rare: a function of its own leaves
+// the softmax its registers. Called by whole warps.
 template <int N>
-__device__ __noinline__ float2 far_row(uint32_t tS, const float *keys, int last, float top, float sum) {
-  float m = top;
+__device__ __noinline__ float odd_tile(uint32_t tS, const float *keys, int last, float ref, float m, float l, bool far, float *far_s) {
+  constexpr float SHIFT = 6.f;
+  float v[8];
+  if (!far) {
+    float share = 0.f;
+#pragma unroll 1
+    for (int c = 0; c < N; c += 8) {
+      tmem_ld8(tS + c, v);
+      tmem_wait_ld();
+#pragma unroll
+      for (int e = 0; e < 8; e++) share += c + e <= last && keys[BN + c + e] == -INFINITY ? ex2(fmaf(v[e], keys[c + e], ref)) : 0.f;
+    }
+    if (!__any_sync(0xffffffffu, !(share <= kMostShare) || m == -INFINITY)) return l + share;
+    *far_s = l == 0.f ? -INFINITY : m - SHIFT;
+  }
+  const float before = *far_s;
+  float top = before;
 #pragma unroll 1
   for (int c = 0; c < N; c += 8) {
-    float v[8];
     tmem_ld8(tS + c, v);
     tmem_wait_ld();
 #pragma unroll
-    for (int e = 0; e < 8; e++) m = c + e <= last ? fmaxf(m, v[e] * keys[c + e]) : m;
+    for (int e = 0; e < 8; e++) top = c + e <= last ? fmaxf(top, v[e] * keys[c + e]) : top;
   }
-  const float ref = m == -INFINITY ? 0.f : m;
-  sum = top == -INFINITY ? sum : sum * ex2(top - ref);
+  const float own = top == -INFINITY ? 0.f : -top;
+  l = before == -INFINITY ? l : l * ex2(before - top);
 #pragma unroll 1
   for (int c = 0; c < N; c += 8) {
-    float v[8];
     tmem_ld8(tS + c, v);
     tmem_wait_ld();
 #pragma unroll
-    for (int e = 0; e < 8; e++) sum += c + e <= last ? ex2(fmaf(v[e], keys[c + e], -ref)) : 0.f;
+    for (int e = 0; e < 8; e++) l += c + e <= last ? ex2(fmaf(v[e], keys[c + e], own)) : 0.f;
   }
-  return make_float2(m, sum);
+  *far_s = top;
+  return l;
+}
+
+// The end of a row whose sums have maxima of their own (+inf: a half that needed
+// none, its sum is in O's unit m): O is divided by the sum, which then is 1. The
+// factor of O, the row's maximum and the sum.
+__device__ __noinline__ float3 far_join(float m, float l0, float l1, float top0, float top1) {
+  top0 = top0 < INFINITY ? top0 : l0 == 0.f ? -INFINITY : m;
+  top1 = top1 < INFINITY ? top1 : l1 == 0.f ? -INFINITY : m;
+  const float t = fmaxf(top0, top1);
+  const float l = (top0 == -INFINITY ? l0 : l0 * ex2(top0 - t)) + (top1 == -INFINITY ? l1 : l1 * ex2(top1 - t));
+  return l > 0.f ? make_float3(ex2(m - t) / l, t + log2f(l), 1.f) : make_float3(0.f, -INFINITY, l);
 }
 
 // ------------------------------------------------------------------ softmax: thread = (stream, row, half of a tile's keys)
@@ -281,8 +312,8 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
         constexpr int KEEP = INT8 ? 32 : N;
         float s[KEEP];
         // what the scales of this tile's keys make: there until its V is released, after P
-        const float *keys = reinterpret_cast<const float *>(sm + C::OFF_SCALE) + (kv / 2 % C::SLOTS) * 3 * BN + half * N;
-        if constexpr (INT8) wait(&bars.keyed[kv / 2 % C::SLOTS], (kv / 2 / C::SLOTS) & 1);
+        const float *keys = reinterpret_cast<const float *>(sm + C::OFF_SCALE) + (kv / 2 % C::SLOTS) * C::KEYS + half * N;
+        if constexpr (INT8) wait(&bars.scaled[kv / 2 % C::SLOTS], (kv / 2 / C::SLOTS) & 1);
         const bool masked = !__all_sync(0xffffffffu, kh + N - 1 <= lim);
         auto scores = [&](int c0) {
 #pragma unroll
@@ -307,15 +338,14 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
             for (int c = 0; c < KEEP; c++) s[c] = kh + c0 + c <= lim ? s[c] : -INFINITY;
           }
         };
-        // the same for both halves: a scale of the tile, or of one before it
+        // the sum has a maximum of its own from here on: a scale of the tile (of both
+        // halves' keys), or of one before it
+        uint32_t odd = 0;
         bool far = false;
         if constexpr (INT8) {
-          const float *inv = keys - half * N + 2 * BN + lane;
-          bool key = false;
-#pragma unroll
-          for (int e = 0; e < BN; e += 32) key |= !(inv[e] >= 1.f / kFarInverse && inv[e] <= kFarInverse);
+          odd = reinterpret_cast<const uint32_t *>(keys)[3 * BN - half * N];
           const bool was = *far_s < INFINITY;
-          far = __any_sync(0xffffffffu, key) || was;
+          far = was || (odd & 1);
           if (far && !was) *far_s = l == 0.f ? -INFINITY : m - SHIFT;
         }
         float mx = -INFINITY;
@@ -339,7 +369,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
         const bool grow = mx > m + RESCALE_THRESHOLD;
         const float m_new = grow ? mx : m;
         const float mb = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = grow ? ex2(m - mb) : 1.f;
+        float alpha = grow ? ex2(m - mb) : 1.f;
         m = m_new;
         if (i > 0 && __any_sync(0xffffffffu, grow)) {
           // s_full of this step came behind the products of the last: O is whole.
@@ -357,10 +387,10 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
         const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), ref2 = make_float2(SHIFT - mb, SHIFT - mb);
         float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         if constexpr (INT8) {
-          if (far) {
-            const float2 y = far_row<N>(tS, keys, lim - kh, *far_s, l);
-            *far_s = y.x;
-            l = y.y;
+          if (odd || far) {
+            l = odd_tile<N>(tS, keys, lim - kh, ref2.x, m, l * (far ? 1.f : alpha), far, far_s);
+            far = *far_s < INFINITY;
+            alpha = 1.f;
           }
         }
 #pragma unroll
@@ -461,13 +491,11 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
     *x_mine = l;
     bar_sync(pair, 64);
     float own = 1.f;  // factor that brings this stream's O to the unit of l
-    if (INT8 && *far_s < INFINITY) {
-      // O and the sum have units of their own: O is divided by the sum, which then is 1
-      const float top = *far_s, other = far_row_s[(st * 2 + (half ^ 1)) * BM], ol = *x_half, t = fmaxf(top, other);
-      l = (top == -INFINITY ? l : l * ex2(top - t)) + (other == -INFINITY ? ol : ol * ex2(other - t));
-      own = l > 0.f ? ex2(m - t) / l : 0.f;
-      m = l > 0.f ? t + log2f(l) : -INFINITY;
-      l = l > 0.f ? 1.f : l;
+    if (INT8 && (*far_s < INFINITY || far_row_s[(st * 2 + (half ^ 1)) * BM] < INFINITY)) {
+      const float3 y = far_join(m, l, *x_half, *far_s, far_row_s[(st * 2 + (half ^ 1)) * BM]);
+      own = y.x;
+      m = y.y;
+      l = y.z;
     } else {
       l += *x_half;
     }
@@ -743,6 +771,52 @@ __device__ __forceinline__ void tma_role(const CUtensorMap *tq, const CUtensorMa
   }
 }
 
+// ------------------------------------------------------------------ scale warp (int8)
+// Looks a tile's V scales over: bit 0 one out of 2^+-kFarLog2, bit 1 a value row of
+// zeros. Such a row (only scale 1 can be one, so V is looked at in that rare case
+// alone) gets the log2 scale -inf and the inverse 0.
+template <int D, class B>
+__device__ __forceinline__ void scale_role(const ChunkArgs &a, uint8_t *sm, B &bars) {
+  using C = Cfg<D, true>;
+  const int lane = threadIdx.x & 31;
+  Waiter wait{a.err};
+  Run run(a);
+  Piece p{};
+  uint32_t idx = 0;
+  while (run.next(a, p)) {
+    for (int t = p.tb; t < p.te; t++, idx++) {
+      const uint32_t slot = idx % C::SLOTS, v = 2 * idx + 1;
+      float *keys = reinterpret_cast<float *>(sm + C::OFF_SCALE) + slot * C::KEYS;
+      wait(&bars.keyed[slot], (idx / C::SLOTS) & 1);
+      auto far = [&](int k) { return !(keys[2 * BN + k] >= 1.f / kFarInverse && keys[2 * BN + k] <= kFarInverse); };
+      uint32_t odd = 0;
+      bool look = false;
+      for (int k = lane; k < BN; k += 32) look |= far(k) || (keys[2 * BN + k] == 1.f && t * BN + k < p.s.len);
+      if (__any_sync(0xffffffffu, look)) {
+        wait(&bars.full[v % C::SLOTS], (v / C::SLOTS) & 1);
+        const uint8_t *tile = sm + C::OFF_KV + v % C::SLOTS * C::TILE;
+        for (int k = lane; k < BN; k += 32) {
+          if (far(k)) odd |= 1u;
+          if (keys[2 * BN + k] != 1.f || t * BN + k >= p.s.len) continue;
+          uint32_t any = 0;
+          for (int c = 0; c < D / 8 && !any; c++) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(tile + chunk_off(k, c));
+            any = x.x | x.y | x.z | x.w;
+          }
+          if (any) continue;
+          keys[BN + k] = -INFINITY;
+          keys[2 * BN + k] = 0.f;
+          odd |= 2u;
+        }
+        odd = __reduce_or_sync(0xffffffffu, odd);
+      }
+      if (lane == 0) reinterpret_cast<uint32_t *>(keys)[3 * BN] = odd;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.scaled[slot]);
+    }
+  }
+}
+
 // ------------------------------------------------------------------ converter warpgroup (int8)
 template <int D, class B>
 __device__ __forceinline__ void convert_role(const ChunkArgs &a, uint8_t *sm, B &bars) {
@@ -773,7 +847,7 @@ __device__ __forceinline__ void convert_role(const ChunkArgs &a, uint8_t *sm, B 
         // tile before it. So the softmax is done with the tile SLOTS before
         // this one, and its place takes this tile's scales.
         if (!v) {
-          float *keys = reinterpret_cast<float *>(sm + C::OFF_SCALE) + idx / 2 % C::SLOTS * 3 * BN + r;
+          float *keys = reinterpret_cast<float *>(sm + C::OFF_SCALE) + idx / 2 % C::SLOTS * C::KEYS + r;
           if (v_scale) {
             const float sv = scale < kLeastScale ? kLeastScale : scale;
             // (a factor 2^lv in the weight and 2^-lv in the sum: what the
@@ -864,6 +938,7 @@ __global__ void __launch_bounds__(Cfg<D, INT8>::THREADS, 1)
       mbar_init(&bars.full[i], INT8 ? 8 : 1);
       mbar_init(&bars.empty[i], 1);
       mbar_init(&bars.keyed[i], 8);  // int8: the tile's scales
+      mbar_init(&bars.scaled[i], 1);
     }
     for (int i = 0; i < C::RAWS; i++) {
       mbar_init(&bars.raw_full[i], 1);
@@ -886,6 +961,8 @@ __global__ void __launch_bounds__(Cfg<D, INT8>::THREADS, 1)
       mma_role<D, INT8>(a, sm, bars);
     } else if (warp == 17) {
       tma_role<D, INT8>(&tq, &tk, &tv, a, sm, bars);
+    } else if (INT8 && warp == 18) {
+      if constexpr (INT8) scale_role<D>(a, sm, bars);
     }
   } else {
     if constexpr (INT8) {

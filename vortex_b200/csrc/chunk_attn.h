@@ -21,6 +21,12 @@ constexpr float RESCALE_THRESHOLD = 8.f;  // O is rescaled when a row's maximum 
 // l is formed from the scores alone, with their own maximum, and meets O at the
 // end: it knows nothing of the values' sizes, infinite ones included. A scale
 // under 2^-100 (values under 1e-28) counts as that.
+//
+// The cache gives a row of zeros the scale 1. Its weight, which the output has no
+// use for, would set the unit and leave smaller values' weights few bits, or none:
+// such a key counts for the sum alone. While its share is under 2^60 of the unit
+// that is one more term, else the sum takes its own maximum as above.
+constexpr float kMostShareLog2 = 60.f, kMostShare = 1152921504606846976.f;
 constexpr float kLeastScale = 7.8886091e-31f, kFarLog2 = 30.f, kFarInverse = 1073741824.f;  // 2^-100, 2^30
 struct ChunkSeq {
   int32_t slot, row0, rows, len;

@@ -24,7 +24,8 @@
 // int8 weights carry the V scale, w = p * scale, with the reference maximum
 // taken over log2(w), and go into P as f16 times 2^6: 11 significant bits, and
 // weights down to 2^-30 of the row's largest keep at least one. bf16 P rounds
-// at 2^-9 (the type of V decides).
+// at 2^-9 (the type of V decides). A value row of zeros counts for the sum alone
+// (chunk_attn.h): its key's thread keeps it out of the reference.
 //
 // Values of V that only some rows may see and that are not finite are taken
 // out of the tile and added to the rows that see them, as in chunk_attn.cu.
@@ -182,6 +183,16 @@ __device__ __noinline__ void far_rows(uint32_t tS, int groups, int step, int fir
     }
 }
 
+// A key's row of the V tile is zero. Rare (only scale 1 can be such a row).
+template <int D>
+__device__ __noinline__ bool zero_row(const uint8_t *tile, int key) {
+  for (int c = 0; c < D / 8; c++) {
+    const uint4 x = *reinterpret_cast<const uint4 *>(tile + chunk_off(key, c));
+    if (x.x | x.y | x.z | x.w) return false;
+  }
+  return true;
+}
+
 // ------------------------------------------------------------------ softmax: thread = (key, the warpgroup's rows)
 // Rows go to the warpgroups in groups of eight in turn; groups without a live
 // row are passed over.
@@ -214,6 +225,15 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
     float l[N];
 #pragma unroll
     for (int n = 0; n < N; n++) l[n] = 0.f;
+    auto own_sums = [&]() {  // int8: the sums so far become each warp's own (far_rows)
+      halve<N, 16>(l, lane);
+      if (lane % (32 / N) == 0) {
+        const int n = lane / (32 / N);
+        far_top[warp * N + n] = l[0] == 0.f ? -INFINITY : -ref_s[n] - SHIFT;
+        far_sum[warp * N + n] = l[0];
+      }
+      __syncwarp();
+    };
     for (int t = 0; t < T; t++, g++) {
       const int k0 = (p.tb + t) * BN, k = k0 + key;
       const uint32_t tS = bars.tmem + lane_off + (g % C::AHEAD) * NR + wg * 8;
@@ -223,11 +243,15 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
       const int n_min = k >= p.s.len ? INT_MAX : a.sh.causal && k > base ? (k - base) * a.G : 0;
       const bool masked = k0 + BN > p.s.len || (a.sh.causal && k0 + BN - 1 > base);
       float sc = a.scale_log2, add = SHIFT, isv = 1.f;
-      bool far_key = false;
+      bool far_key = false, zero = false;  // zero: the key's value row is
       if constexpr (INT8) {
         const float *tile = scales + g % C::SCALES * 2 * BN;
         sc *= tile[key];
         const float sv = tile[BN + key] < kLeastScale ? kLeastScale : tile[BN + key];
+        if (__any_sync(0xffffffffu, sv == 1.f && k < p.s.len)) {
+          wait(&bars.v_full[g % C::VS], (g / C::VS) & 1);
+          zero = sv == 1.f && zero_row<D>(sm + C::OFF_V + g % C::VS * C::TILE, key);
+        }
         const float lv = __log2f(sv);  // off by under 2^-16, in V's factor alone
         add += lv;
         isv = ex2(-lv);
@@ -263,20 +287,16 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
       };
       if (groups == GROUPS) load(std::true_type{});
       else load(std::false_type{});
+      if (INT8 && zero) {  // (w is p then: its share of the sum)
+        far_key = top > kMostShareLog2;
+        top = -INFINITY;
+      }
       if (t == 0 || bar_or(bar, 128, top > RESCALE_THRESHOLD + SHIFT || far_key)) {
         bool far = false;
         if constexpr (INT8) {
           const bool was = t > 0 && *far_s != 0;
           far = bar_or(bar, 128, far_key) || was;
-          if (far && !was) {  // the sums so far become each warp's own
-            halve<N, 16>(l, lane);
-            if (lane % (32 / N) == 0) {
-              const int n = lane / (32 / N);
-              far_top[warp * N + n] = l[0] == 0.f ? -INFINITY : -ref_s[n] - SHIFT;
-              far_sum[warp * N + n] = l[0];
-            }
-            __syncwarp();
-          }
+          if (far && !was) own_sums();
         }
         // New references: a first tile's maximum, later the maximum of the rows
         // that passed it, becomes 2^SHIFT.
@@ -287,7 +307,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
 #pragma unroll
             for (int n = j * 8; n < j * 8 + 8; n++) {
               float y;
-              asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x[n]));
+              asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(INT8 && zero ? -INFINITY : x[n]));
               most = lane == n ? y : most;
             }
           }
@@ -336,6 +356,18 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
           tmem_wait_st();
         }
         if (coarse) goto again;  // (once for a row: its reference never rises)
+        if constexpr (INT8) {
+          if (!far) {  // a row of zeros whose share of the sum is too large in the new unit
+            float share = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < N; n++) share = n / 8 < groups ? fmaxf(share, x[n]) : share;
+            if (bar_or(bar, 128, zero && share > kMostShareLog2)) {
+              own_sums();
+              if (key == 0) *far_s = 1;
+              bar_sync(bar, 128);
+            }
+          }
+        }
       }
       // P of two tiles ago has been used
       uint8_t *P = sm + C::OFF_P + (g & 1) * C::P;
@@ -359,7 +391,8 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
                 // a row without this key: no product with a scale that is not finite
                 l[n] = !masked || row_of(n) >= n_min ? fmaf(w0, isv, l[n]) : l[n];
                 l[n + 1] = !masked || row_of(n + 1) >= n_min ? fmaf(w1, isv, l[n + 1]) : l[n + 1];
-                asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(pair) : "f"(w1), "f"(w0));
+                // (finite beside a row of zeros, whose weight has no bound)
+                asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(pair) : "f"(w1), "f"(w0));
               } else {
                 l[n] += w0;
                 l[n + 1] += w1;
