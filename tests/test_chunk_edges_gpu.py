@@ -191,3 +191,64 @@ def test_keys_of_score_minus_infinity_before_the_others(KV, D, m, score):
         k[..., 0], k[..., 1] = 0.0, score * math.sqrt(D) / 8.0
         k[:260, :, 0] = -math.inf
         attend(filled(KV, k, v, False), [0], [m], q)
+
+
+# ---------------------------------------------------------------- cache
+
+def test_truncate_of_every_holder_needs_the_blocks_it_frees(KV):
+    # a full pool; both holders of every block are cut: two blocks come free
+    # and one copy of the block with the cut is needed
+    k = rnd((64, 1, 64), 0)
+    c = make(KV, 1, 1, 64, 16, 4, 2)
+    c.append_chunks(0, [0], [64], k, -k)
+    c.fork(0, 1, 64)
+    assert c.free_block_count() == 0
+    c.truncate([0, 1], [20, 20])
+    assert c.free_block_count() == 1 and c.block_table(0, 0)[0] == c.block_table(0, 1)[0]
+    assert c.block_table(0, 0)[1] != c.block_table(0, 1)[1]
+    for s in (0, 1):
+        gk, gv = c.get_kv(0, s)
+        assert torch.equal(gk, k[:20].float()) and torch.equal(gv, -k[:20].float())
+
+
+@pytest.mark.parametrize("blocks", [7, 6])
+def test_truncate_of_several_holders_at_different_places(KV, blocks):
+    # two cuts inside block 2, which the fourth sequence keeps, one inside block
+    # 0, which all others keep: three copies
+    from vortex_b200 import _native as N
+    k = rnd((64, 1, 64), 0)
+    c = make(KV, 1, 1, 64, 16, blocks, 4)
+    c.append_chunks(0, [0], [64], k, -k)
+    for s in (1, 2, 3):
+        c.fork(0, s, 64)
+    lens = [40, 47, 9, 64]
+    if blocks == 6:
+        with pytest.raises(N.VxbError) as e:
+            c.truncate(range(4), lens)
+        assert e.value.code == N.VXB_ENOBLOCKS
+        lens = [64] * 4
+    else:
+        c.truncate(range(4), lens)
+        assert c.free_block_count() == 0
+        assert len({c.block_table(0, s)[2] for s in (0, 1, 3)}) == 3
+    for s in range(4):
+        gk, gv = c.get_kv(0, s)
+        assert torch.equal(gk, k[:lens[s]].float()) and torch.equal(gv, -k[:lens[s]].float())
+
+
+def test_truncate_without_a_block_to_spare_changes_nothing(KV):
+    from vortex_b200 import _native as N
+    k = rnd((64, 1, 64), 0)
+    c = make(KV, 1, 1, 64, 16, 4, 3)
+    c.append_chunks(0, [0], [64], k, -k)
+    c.fork(0, 1, 64)
+    before = c.stats(), [c.block_table(0, s) for s in (0, 1)], c.pages()["lens"].tolist()
+    with pytest.raises(N.VxbError) as e:
+        c.truncate([0], [20])  # the other sequence keeps every block
+    assert e.value.code == N.VXB_ENOBLOCKS
+    assert (c.stats(), [c.block_table(0, s) for s in (0, 1)], c.pages()["lens"].tolist()) == before
+    # cut inside a block that stays shared with one that is cut behind it
+    with pytest.raises(N.VxbError) as e:
+        c.truncate([0, 1], [20, 64])
+    assert e.value.code == N.VXB_ENOBLOCKS
+    assert (c.stats(), [c.block_table(0, s) for s in (0, 1)], c.pages()["lens"].tolist()) == before

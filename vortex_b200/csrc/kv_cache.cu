@@ -626,7 +626,6 @@ int truncate(vxb_kv *kv, int n, const int64_t *ids, const int64_t *lens, cudaStr
     auto si = kv->slot_of.find(ids[i]);
     if (si != kv->slot_of.end()) slots[i] = si->second;
   }
-  int64_t freed = 0;
   for (int layer = 0; layer < kv->num_layers; layer++) {
     TableFinder find(kv, layer);
     for (int i = 0; i < n; i++) {
@@ -635,12 +634,31 @@ int truncate(vxb_kv *kv, int n, const int64_t *ids, const int64_t *lens, cudaStr
       if (it == kv->tables.end() || it->second.len <= lens[i]) continue;
       vxb_kv::Table &t = it->second;
       cuts.push_back({&t, lens[i], layer, slots[i]});
-      for (size_t b = (size_t)((lens[i] + bs - 1) / bs); b < t.blocks.size(); b++) freed += kv->refs[t.blocks[b]] == 1;
       if (lens[i] % bs && kv->refs[t.blocks[(size_t)(lens[i] / bs)]] > 1) moves.push_back(cuts.back());
     }
   }
   if (cuts.empty()) return VXB_OK;
-  if ((int64_t)moves.size() > (int64_t)kv->free_blocks.size() + freed) return set_error(ctx, VXB_ENOBLOCKS, "KV cache out of blocks");
+  if (moves.size() > kv->free_blocks.size()) {
+    // Do the blocks suffice that the cuts themselves free? Of every block: the
+    // references that cuts in front of it take, and the cuts inside it, each of
+    // which needs a copy, but for the last where no other sequence keeps the block.
+    struct Use {
+      int taken = 0, inside = 0;
+    };
+    std::map<int32_t, Use> uses;
+    for (const Cut &c : cuts) {
+      const std::vector<int32_t> &blocks = c.table->blocks;
+      if (c.len % bs) uses[blocks[(size_t)(c.len / bs)]].inside++;
+      for (size_t b = (size_t)((c.len + bs - 1) / bs); b < blocks.size(); b++) uses[blocks[b]].taken++;
+    }
+    int64_t left = (int64_t)kv->free_blocks.size();
+    for (const auto &[block, use] : uses) {
+      const int kept = kv->refs[block] - use.taken;  // references behind the cuts
+      left += kept == 0;
+      if (use.inside) left -= use.inside - (kept == use.inside);
+    }
+    if (left < 0) return set_error(ctx, VXB_ENOBLOCKS, "KV cache out of blocks");
+  }
   CutArgs a;
   a.lens = kv->d_lens;
   a.max_seqs = kv->max_seqs;
