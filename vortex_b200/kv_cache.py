@@ -19,27 +19,25 @@ I8 = N.I8
 _I64 = np.dtype(np.int64)
 
 
-def _host_array(values, dtype):
-    """values as a contiguous 1-D array of dtype (itself where it is one)."""
-    if type(values) is np.ndarray and values.dtype == dtype and values.ndim == 1 and values.flags.c_contiguous:
-        return values
-    return np.ascontiguousarray(np.atleast_1d(values), dtype=dtype)
+def _whole_numbers(who: str, name: str, values, dtype, least=None):
+    """values as a contiguous 1-D host array of dtype (itself where it is one);
+    refused: fractions, other shapes, numbers that dtype does not hold and, in
+    an array of another type, numbers under `least`."""
+    if type(values) is np.ndarray and values.dtype == dtype and values.ndim == 1:
+        return values if values.flags.c_contiguous else np.ascontiguousarray(values)
+    a = np.atleast_1d(np.asarray(values))
+    lo, hi = np.iinfo(dtype).min if least is None else least, np.iinfo(dtype).max
+    if a.ndim != 1 or (a.size and (not np.issubdtype(a.dtype, np.integer) or int(a.min()) < lo or int(a.max()) > hi)):
+        raise N.VxbError(N.VXB_EINVAL, f"{who}: {name} must be one list of whole numbers from {lo} to {hi}")
+    return a.astype(dtype)
 
 
-def _ids_counts(who: str, seq_ids, counts, dtype=np.int32):
+def _ids_counts(who: str, seq_ids, counts, dtype=np.dtype(np.int32)):
     """Host arrays of one sequence id and one count (or length) each."""
-    ids = _host_array(seq_ids, _I64)
-    if type(counts) is np.ndarray and counts.dtype == dtype and counts.ndim == 1 and counts.size == ids.size:
-        return ids, counts  # (a negative one is refused by the call)
-    if not (type(counts) is np.ndarray and counts.dtype == dtype):
-        counts = np.atleast_1d(np.asarray(counts))
-        if counts.size and (not np.issubdtype(counts.dtype, np.integer) or int(counts.max()) > np.iinfo(dtype).max):
-            raise N.VxbError(N.VXB_EINVAL, f"{who}: the counts must be whole numbers up to {np.iinfo(dtype).max}")
-    if ids.ndim != 1 or counts.ndim != 1 or ids.size != counts.size:
-        raise N.VxbError(N.VXB_EINVAL, f"{who}: {ids.size} sequences and {counts.size} counts")
-    c = _host_array(counts, dtype)
-    if c.size and min(c.tolist()) < 0:
-        raise N.VxbError(N.VXB_EINVAL, f"{who}: a count is negative")
+    ids = _whole_numbers(who, "seq_ids", seq_ids, _I64)
+    c = _whole_numbers(who, "the counts", counts, dtype, least=0)  # (a negative one in an array of dtype is refused by the call)
+    if ids.size != c.size:
+        raise N.VxbError(N.VXB_EINVAL, f"{who}: {ids.size} sequences and {c.size} counts")
     return ids, c
 
 
@@ -123,7 +121,7 @@ class PagedKVCache:
     def truncate(self, seq_ids, lengths):
         """Takes appended tokens back: every layer of seq_ids[i] holds at most
         lengths[i] tokens afterwards."""
-        ids, lens = _ids_counts("truncate", seq_ids, lengths, np.int64)
+        ids, lens = _ids_counts("truncate", seq_ids, lengths, _I64)
         self._check(N.lib().vxb_kv_truncate(self.ptr, ids.size, ids.tobytes(), lens.tobytes(),
                                             _stream_on(self.ctx.device)))
 

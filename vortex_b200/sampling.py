@@ -10,7 +10,10 @@ import ctypes
 import numpy as np
 
 from . import _native as N
+from .kv_cache import _whole_numbers
 from .quant import _dptr, _stream_on, _stream_ptr, context
+
+_I32 = np.dtype(np.int32)
 
 
 def argmax(logits):
@@ -85,15 +88,10 @@ def verify_drafts(drafts, n_drafts, target_probs, draft_probs, u_accept, u_sampl
     Returns (tokens int32 [D + n]: accepted drafts, the drawn token, then -1,
     per request; accepted int32 [n])."""
     import torch
-    counts = n_drafts
-    if not (type(counts) is np.ndarray and counts.dtype == np.int32 and counts.ndim == 1):
-        counts = np.atleast_1d(np.asarray(counts))
-        if counts.size and (not np.issubdtype(counts.dtype, np.integer) or int(counts.max()) > np.iinfo(np.int32).max):
-            raise N.VxbError(N.VXB_EINVAL, "verify_drafts: n_drafts must be whole numbers of 32 bits")
-        counts = counts.astype(np.int32)
+    counts = _whole_numbers("verify_drafts", "n_drafts", n_drafts, _I32, least=0)
     per = counts.tolist()
-    if counts.ndim != 1 or (per and min(per) < 0):
-        raise N.VxbError(N.VXB_EINVAL, "verify_drafts: n_drafts must be one list of numbers, none negative")
+    if per and min(per) < 0:
+        raise N.VxbError(N.VXB_EINVAL, "verify_drafts: n_drafts must not be negative")
     n, total = len(per), sum(per)
     if not isinstance(target_probs, torch.Tensor) or target_probs.dim() != 2 or target_probs.shape[1] == 0:
         raise N.VxbError(N.VXB_EINVAL, "verify_drafts: target_probs must be [rows, vocab]")
