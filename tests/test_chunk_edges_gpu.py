@@ -252,3 +252,31 @@ def test_truncate_without_a_block_to_spare_changes_nothing(KV):
         c.truncate([0, 1], [20, 64])
     assert e.value.code == N.VXB_ENOBLOCKS
     assert (c.stats(), [c.block_table(0, s) for s in (0, 1)], c.pages()["lens"].tolist()) == before
+
+
+def test_an_append_that_cannot_be_launched_takes_nothing(KV):
+    # a stream whose capture has been broken off takes no launches: the host's
+    # tables and the device's lengths stay as they were, and later calls work
+    import ctypes
+    from vortex_b200 import _native as N
+    rt = ctypes.CDLL("libcudart.so.12")
+    c = make(KV, 1, 2, 64, 16, 700, 400)
+    k = rnd((5000, 2, 64), 0)
+    c.append_chunks(0, [1, 2], [20, 3], k[:23], k[:23])
+    torch.cuda.synchronize()
+    before = c.free_block_count(), [c.block_table(0, s) for s in (1, 2)], c.pages()["lens"].tolist()
+    side = torch.cuda.Stream()
+    raw, graph = ctypes.c_void_p(side.cuda_stream), ctypes.c_void_p()
+    assert rt.cudaStreamBeginCapture(raw, 0) == 0
+    assert rt.cudaStreamSynchronize(raw) != 0  # not allowed in a capture, which ends with it
+    with torch.cuda.stream(side):
+        for ids, counts in (([1, 2], [30, 1]), (list(range(1, 301)), [9] * 300)):
+            with pytest.raises(N.VxbError) as e:
+                c.append_chunks(0, ids, counts, k[:sum(counts)], k[:sum(counts)])
+            assert e.value.code == N.VXB_ECUDA and "append" in str(e.value)
+    assert rt.cudaStreamEndCapture(raw, ctypes.byref(graph)) != 0
+    rt.cudaGetLastError()
+    assert c.free_block_count() == before[0] and [c.block_table(0, s) for s in (1, 2)] == before[1] and [c.seq_len(0, s) for s in (1, 2, 3)] == [20, 3, 0]
+    assert c.pages()["lens"].tolist() == before[2]
+    c.append_chunks(0, [1, 2], [30, 1], k[23:54], k[23:54])
+    assert torch.equal(c.get_kv(0, 1)[0], torch.cat([k[:20], k[23:53]]).float())

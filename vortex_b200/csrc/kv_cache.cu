@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(kChunkThreads) kv_append_chunks_kernel(const _
   }
 }
 
-// lens[layer][slot] = min(lens[layer][slot], len) for every layer
+// lens[layer][slot] = min(lens[layer][slot], len) for consecutive layers
 constexpr int kCutSeqs = 256;
 struct CutArgs {
   int32_t *lens;
@@ -466,6 +466,23 @@ void cut_table(vxb_kv *kv, vxb_kv::Table &t, int64_t len) {
   t.len = len;
 }
 
+// The device's lengths of (slot, length) pairs, in `layers` layers from one on
+int cut_lens(vxb_kv *kv, int layer, int layers, const std::vector<std::pair<int, int64_t>> &cuts, cudaStream_t st) {
+  CutArgs a;
+  a.lens = kv->d_lens + (size_t)layer * kv->max_seqs;
+  a.max_seqs = kv->max_seqs;
+  for (size_t i = 0; i < cuts.size();) {
+    a.n = 0;
+    for (; i < cuts.size() && a.n < kCutSeqs; i++) {
+      a.slot[a.n] = cuts[i].first;
+      a.len[a.n++] = (int32_t)std::min<int64_t>(cuts[i].second, INT_MAX);
+    }
+    kv_cut_lens_kernel<<<layers, std::min(128, (a.n + 31) / 32 * 32), 0, st>>>(a);
+    if (int rc = launch_check(kv->ctx, "kv_cut_lens_kernel")) return rc;
+  }
+  return VXB_OK;
+}
+
 struct AppendSeq {
   vxb_kv::Table *table;  // null: not there yet, or no tokens
   int64_t len;           // tokens before the call
@@ -603,9 +620,18 @@ int append_chunks(vxb_kv *kv, int layer, int n, const int64_t *ids, const int32_
 
   const int rc = n <= FewChunks::kPieces && spanned <= FewChunks::kIds ? write_chunks<FewChunks>(kv, layer, seqs, counts, d_k, d_v, st)
                                                                       : write_chunks<ManyChunks>(kv, layer, seqs, counts, d_k, d_v, st);
-  if (rc)  // nothing was launched behind the failed launch: the tokens are taken back
+  if (rc) {
+    // nothing was launched behind the failed launch: the tokens are taken back,
+    // on the host and, as far as the stream still takes launches, in the lengths
+    // that the launches before it wrote
     for (int i = n - 1; i >= 0; i--)
       if (seqs[i].table) cut_table(kv, *seqs[i].table, seqs[i].len);
+    const std::string what = ctx->err;
+    std::vector<std::pair<int, int64_t>> cuts;
+    for (const AppendSeq &q : seqs)
+      if (q.table) cuts.emplace_back(q.slot, q.len);
+    if (cut_lens(kv, layer, 1, cuts, st)) set_error(ctx, rc, "%s", what.c_str());
+  }
   return rc;
 }
 
@@ -659,9 +685,9 @@ int truncate(vxb_kv *kv, int n, const int64_t *ids, const int64_t *lens, cudaStr
     }
     if (left < 0) return set_error(ctx, VXB_ENOBLOCKS, "KV cache out of blocks");
   }
-  CutArgs a;
-  a.lens = kv->d_lens;
-  a.max_seqs = kv->max_seqs;
+  std::vector<std::pair<int, int64_t>> kept;  // (what may throw comes before what changes)
+  for (int i = 0; i < n; i++)
+    if (slots[i] >= 0) kept.emplace_back(slots[i], lens[i]);
   // in the opposite order of the appends, so that they get the same blocks again
   for (auto c = cuts.rbegin(); c != cuts.rend(); ++c) cut_table(kv, *c->table, c->len);
   for (const Cut &c : moves) {
@@ -679,18 +705,7 @@ int truncate(vxb_kv *kv, int n, const int64_t *ids, const int64_t *lens, cudaStr
     kv_set_entry_kernel<<<1, 1, 0, st>>>(kv->d_tables + ((size_t)c.layer * kv->max_seqs + c.slot) * kv->max_blocks_per_seq + index, to);
     if (int rc = launch_check(ctx, "kv_set_entry_kernel")) return rc;
   }
-  for (int i0 = 0; i0 < n;) {
-    a.n = 0;
-    for (; i0 < n && a.n < kCutSeqs; i0++) {
-      if (slots[i0] < 0 || lens[i0] > INT_MAX) continue;
-      a.slot[a.n] = slots[i0];
-      a.len[a.n++] = (int32_t)lens[i0];
-    }
-    if (a.n == 0) continue;
-    kv_cut_lens_kernel<<<kv->num_layers, std::min(128, (a.n + 31) / 32 * 32), 0, st>>>(a);
-    if (int rc = launch_check(ctx, "kv_cut_lens_kernel")) return rc;
-  }
-  return VXB_OK;
+  return cut_lens(kv, 0, kv->num_layers, kept, st);
 }
 
 }  // namespace
