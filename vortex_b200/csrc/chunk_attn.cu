@@ -100,7 +100,7 @@ struct Cfg {
 
 template <int SLOTS, int RAWS>
 struct Bars {
-  uint64_t q_full, q_empty, o_free, s_full[2], p_full[2], o_full[2], full[SLOTS], empty[SLOTS], keyed[SLOTS], scaled[SLOTS], raw_full[RAWS + 1],
+  uint64_t q_full, q_empty, o_free, drained, s_full[2], p_full[2], o_full[2], full[SLOTS], empty[SLOTS], keyed[SLOTS], scaled[SLOTS], raw_full[RAWS + 1],
       raw_empty[RAWS + 1];
   uint32_t tmem;
   int acc[2];  // the stream's O already holds values that its first product adds to
@@ -705,6 +705,9 @@ __device__ __forceinline__ void mma_role(const ChunkArgs &a, uint8_t *sm, B &bar
     ring.phase ^= 1;
     pieces++;
   }
+  // (behind a wait that has run out, products may be under way that nobody waits for)
+  mma_commit(one, &bars.drained);
+  wait.last(&bars.drained, 0);
 }
 
 // ------------------------------------------------------------------ TMA warp
@@ -721,7 +724,7 @@ __device__ __forceinline__ void tma_role(const CUtensorMap *tq, const CUtensorMa
   Waiter wait{a.err};
   Run run(a);
   Piece p{};
-  uint32_t idx = 0, pieces = 0;
+  uint32_t idx = 0, pieces = 0, issued = 0, queries = 0;
   while (run.next(a, p)) {
     const int32_t *table = a.tables + (size_t)p.s.slot * a.mbps;
     // pool rows of this lane's box in the tiles t .. t + 32 / per_tile - 1
@@ -739,19 +742,22 @@ __device__ __forceinline__ void tma_role(const CUtensorMap *tq, const CUtensorMa
       uint64_t *full = INT8 ? &bars.raw_full[slot] : &bars.full[slot], *empty = INT8 ? &bars.raw_empty[slot] : &bars.empty[slot];
       if (idx >= RING) wait(empty, (idx / RING - 1) & 1);
       const int boxes = (min(BN, p.s.len - t * BN) + a.box - 1) / a.box;
-      if (lane == 0) mbar_expect_tx(full, (uint32_t)(boxes * SLABS * a.box * ROW));
+      // (behind a wait that has run out nothing is copied any more)
+      if (lane == 0 && !wait.dead) mbar_expect_tx(full, (uint32_t)(boxes * SLABS * a.box * ROW));
       __syncwarp();
       const int row = __shfl_sync(0xffffffffu, rows, (t - p.tb) % group * per_tile + lane / SLABS % per_tile);
-      if (lane < boxes * SLABS) {
+      if (lane < boxes * SLABS && !wait.dead) {
         const int b = lane / SLABS, sl = lane % SLABS;
         tma_load_2d(tiles + slot * (INT8 ? C::RAW : C::TILE) + sl * C::SLAB + b * a.box * ROW, map, sl * 64, row, full);
       }
       __syncwarp();
       idx++;
+      if (!wait.dead) issued = idx;
     };
     auto load_q = [&]() {
       if (pieces > 0) wait(&bars.q_empty, (pieces - 1) & 1);
-      if (lane == 0) {
+      if (lane == 0 && !wait.dead) {
+        queries = pieces + 1;
         const int halves = p.both ? 2 : 1;
         mbar_expect_tx(&bars.q_full, (uint32_t)(halves * (D / 64) * a.sh.tpt * a.G * 128));
         for (int h = 0; h < halves; h++)
@@ -769,6 +775,12 @@ __device__ __forceinline__ void tma_role(const CUtensorMap *tq, const CUtensorMa
     }
     pieces++;
   }
+  // no copy is under way when the CTA ends, also behind a wait that has run out
+  issued = __reduce_max_sync(0xffffffffu, issued);
+  queries = __reduce_max_sync(0xffffffffu, queries);
+  for (uint32_t i = issued > RING ? issued - RING : 0; i < issued; i++)
+    wait.last(INT8 ? &bars.raw_full[i % RING] : &bars.full[i % RING], (i / RING) & 1);
+  if (queries > 0) wait.last(&bars.q_full, (queries - 1) & 1);
 }
 
 // ------------------------------------------------------------------ scale warp (int8)
@@ -928,6 +940,7 @@ __global__ void __launch_bounds__(Cfg<D, INT8>::THREADS, 1)
     mbar_init(&bars.q_full, 1);
     mbar_init(&bars.q_empty, 1);
     mbar_init(&bars.o_free, 16);
+    mbar_init(&bars.drained, 1);
     for (int i = 0; i < 2; i++) {
       mbar_init(&bars.s_full[i], 1);
       mbar_init(&bars.p_full[i], 8);

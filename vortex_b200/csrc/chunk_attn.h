@@ -82,6 +82,11 @@ struct Waiter {
     }
     __syncwarp();
   }
+  // For what the warp itself has under way, at its end: waited for in any case.
+  __device__ __forceinline__ void last(uint64_t *bar, uint32_t parity) {
+    if (!mbar_wait(bar, parity)) atomicExch(err, 1);
+    __syncwarp();
+  }
 };
 
 // The run of a CTA as pieces: consecutive key tiles of one item.

@@ -88,7 +88,7 @@ struct Cfg {
 
 template <int KS, int VS>
 struct Bars {
-  uint64_t k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], q_full[2], q_empty[2], s_full[3], p_full[2], pv_done[2], o_full[2], o_free[2];
+  uint64_t k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], q_full[2], q_empty[2], s_full[3], p_full[2], pv_done[2], o_full[2], o_free[2], drained;
   uint32_t tmem;
   int acc;     // O already holds values that the piece's first product adds to
   int far[4];  // int8, of each softmax warpgroup: the piece has met V scales out of kFarLog2
@@ -601,6 +601,9 @@ __device__ __forceinline__ void mma_role(const ChunkArgs &a, uint8_t *sm, BarsOf
     mma_commit(one, &bars.o_full[pb]);
     pieces++;
   }
+  // (behind a wait that has run out, products may be under way that nobody waits for)
+  mma_commit(one, &bars.drained);
+  wait.last(&bars.drained, 0);
 }
 
 // ------------------------------------------------------------------ loaders
@@ -819,6 +822,7 @@ __global__ void __launch_bounds__(Cfg<D, INT8, NR>::THREADS, 1) chunk_few_kernel
       mbar_init(&bars.o_free[i], C::SOFT * 4);
     }
     for (int i = 0; i < C::AHEAD; i++) mbar_init(&bars.s_full[i], 1);
+    mbar_init(&bars.drained, 1);
     bars.acc = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
