@@ -193,6 +193,46 @@ def test_keys_of_score_minus_infinity_before_the_others(KV, D, m, score):
         attend(filled(KV, k, v, False), [0], [m], q)
 
 
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("H,G,D,bs,lens,counts", CHUNKS + [(x[0], x[1], D, *x[2:]) for x in FEW + RUNS for D in (64, 128)])
+def test_every_row_is_finite_and_within_the_bound(KV, H, G, D, bs, lens, counts, int8):
+    n = len(lens)
+    c = make(KV, 1, H, D, bs, sum(-(-x // bs) for x in lens), n, int8)
+    v = rnd((sum(lens), H, D), 2)
+    v[::5] *= 100.0
+    v[1::7] *= 0.001
+    c.append_chunks(0, range(n), lens, rnd((sum(lens), H, D), 1), v)
+    for causal in (True, False):
+        attend(c, range(n), counts, rnd((sum(counts), H * G, D), 3, 2.0), causal)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_rows_that_see_nothing_and_rows_that_do(KV, int8):
+    H, D = 2, 128
+    c = make(KV, 1, H, D, 16, 32, 8, int8)
+    c.append_chunks(0, [1, 2, 3], [3, 150, 16], rnd((169, H, D), 1), rnd((169, H, D), 2))
+    c.truncate([3], [0])
+    ids, counts = [1, 4, 3, 2, 1], [9, 5, 2, 140, 0]
+    for causal in (True, False):
+        attend(c, ids, counts, rnd((sum(counts), 4, D), 3), causal)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_attention_behind_four_gigabytes_is_finite(KV, int8):
+    H, D, bs = 32, 128, 1024
+    fill = 1100 if int8 else 560
+    c = make(KV, 1, H, D, bs, fill + 4, fill + 1, int8)
+    one = rnd((fill, H, D), 0)
+    c.append_chunks(0, range(fill), [1] * fill, one, one)
+    n = 2500
+    v = rnd((n, H, D), 2)
+    v[9::100] = 0.0
+    c.append_chunks(0, [fill], [n], rnd((n, H, D), 1), v)
+    assert min(c.block_table(0, fill)) * H * bs * D * (1 if int8 else 2) > 2 ** 32
+    for m in (3, 70):
+        attend(c, [fill], [m], rnd((m, H, D), 3, 2.0))
+
+
 # ---------------------------------------------------------------- cache
 
 def test_truncate_of_every_holder_needs_the_blocks_it_frees(KV):
@@ -280,3 +320,33 @@ def test_an_append_that_cannot_be_launched_takes_nothing(KV):
     assert c.pages()["lens"].tolist() == before[2]
     c.append_chunks(0, [1, 2], [30, 1], k[23:54], k[23:54])
     assert torch.equal(c.get_kv(0, 1)[0], torch.cat([k[:20], k[23:53]]).float())
+
+
+def test_append_int8_scales_of_keys_and_values(KV):
+    D = 64
+    rows = [torch.linspace(-1, 1, D) * m * (1 + j / 16) for m in (1.0, 127.0, 3.0, 1e-38, 1e38, 2.0 ** -133) for j in range(16)]
+    rows += [torch.zeros(D), torch.full((D,), 5.0), torch.tensor([math.inf] + [1.0] * (D - 1)), torch.tensor([math.nan] * D)]
+    k = torch.stack(rows)[:, None].to(torch.bfloat16).cuda()
+    a, b = (make(KV, 1, 1, D, 16, 16, 1, True) for _ in range(2))
+    a.append_chunks(0, [0], [k.shape[0]], k, -k.flip(0))
+    b.append_seq(0, 0, k, -k.flip(0))
+    pa, pb = a.pages(), b.pages()
+    for name in ("k", "v"):
+        assert torch.equal(pa[name], pb[name])
+        assert torch.equal(pa[name + "_scale"].view(torch.int32), pb[name + "_scale"].view(torch.int32))
+
+
+# ---------------------------------------------------------------- probabilities
+
+@pytest.mark.parametrize("rows,vocab", [(2, 2000), (300, 30001)])
+@pytest.mark.parametrize("t", [0.011, 1.4091, 0.3])
+def test_probs_far_below_the_maximum(SM, rows, vocab, t):
+    # d = x - max is off by 2^-24 of it, log2(e) / t and their product by 2^-24
+    # each, so the exponent by 3 * 2^-24 |d| / t; the exponential by 2^-22, the
+    # sums by at most 64 * 2^-24 and two more roundings: 2^-17 in all
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = -85.0 * t * torch.rand(rows, vocab, generator=g, device="cuda") + 3.0
+    p = SM.token_probs(x, t).double()
+    d = (x.double() - x.double().amax(-1, keepdim=True)) / t
+    want = torch.softmax(d, -1)
+    assert bool(((p - want).abs() <= (2.0 ** -17 + 3 * 2.0 ** -24 * d.abs()) * want + 2.0 ** -125).all())
