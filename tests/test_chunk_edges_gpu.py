@@ -146,6 +146,23 @@ def test_int8_value_rows_of_zeros(KV, D, m, size, logit, where):
         attend(filled(KV, k, v, True), [0], [m], q)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("G", [3, 5, 7, 48])
+def test_int8_unusual_scales_beside_rows_without_a_token(KV, G, D, causal):
+    # 128 is no multiple of G: a tile's last rows hold no token, but what an
+    # earlier call left in shared memory, here values that make scores infinite
+    H, lens, counts = 1, [319, 8, 83, 530, 118, 700], [319, 8, 64, 17, 65, 2]
+    for far in (True, False):
+        k, v, q = rnd((sum(lens), H, D), 1), rnd((sum(lens), H, D), 2), rnd((sum(counts), H * G, D), 3)
+        v[3::11] *= 2.0 ** 60 if far else 0.0
+        c = make(KV, 1, H, D, 16, sum(-(-x // 16) for x in lens), len(lens), True)
+        c.append_chunks(0, range(len(lens)), lens, k, v)
+        for _ in range(3):
+            c.chunk_attention(0, range(len(lens)), counts, torch.full_like(q, 3e38) * k.new_tensor([1.0, -1.0]).repeat(D // 2), causal=causal)
+            attend(c, range(len(lens)), counts, q, causal)
+
+
 @pytest.mark.parametrize("m", ROWS)
 @pytest.mark.parametrize("D", [64, 128])
 def test_int8_rows_of_full_range_are_not_zeros(KV, D, m):

@@ -58,6 +58,7 @@
 // (polynomial of degree 5) made short chunks 3% faster and long ones 6% slower.
 // A call's fixed part is 11 us: 3 until the first scores, 2 at the end.
 #include <atomic>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <cuda.h>
@@ -200,7 +201,7 @@ __device__ __noinline__ float odd_tile(uint32_t tS, const float *keys, int last,
       for (int e = 0; e < 8; e++) share += c + e <= last && keys[BN + c + e] == -INFINITY ? ex2(fmaf(v[e], keys[c + e], ref)) : 0.f;
     }
     if (!__any_sync(0xffffffffu, !(share <= kMostShare) || m == -INFINITY)) return l + share;
-    *far_s = l == 0.f ? -INFINITY : m - SHIFT;
+    *far_s = l == 0.f ? -INFINITY : fminf(m - SHIFT, FLT_MAX);
   }
   const float before = *far_s;
   float top = before;
@@ -220,7 +221,9 @@ __device__ __noinline__ float odd_tile(uint32_t tS, const float *keys, int last,
 #pragma unroll
     for (int e = 0; e < 8; e++) l += c + e <= last ? ex2(fmaf(v[e], keys[c + e], own)) : 0.f;
   }
-  *far_s = top;
+  // (a row without a token has what lies in shared memory for queries: no
+  // maximum of its may read as "none", since whole warps have one or none)
+  *far_s = fminf(top, FLT_MAX);
   return l;
 }
 
@@ -346,7 +349,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
           odd = reinterpret_cast<const uint32_t *>(keys)[3 * BN - half * N];
           const bool was = *far_s < INFINITY;
           far = was || (odd & 1);
-          if (far && !was) *far_s = l == 0.f ? -INFINITY : m - SHIFT;
+          if (far && !was) *far_s = l == 0.f ? -INFINITY : fminf(m - SHIFT, FLT_MAX);
         }
         float mx = -INFINITY;
 #pragma unroll

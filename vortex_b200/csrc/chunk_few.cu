@@ -180,6 +180,7 @@ __device__ __noinline__ void far_rows(uint32_t tS, int groups, int step, int fir
         sum[n] = (before == -INFINITY ? sum[n] : sum[n] * ex2(before - m)) + w;
         top[n] = m;
       }
+      __syncwarp();
     }
 }
 
@@ -251,6 +252,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
         if (__any_sync(0xffffffffu, sv == 1.f && k < p.s.len)) {
           wait(&bars.v_full[g % C::VS], (g / C::VS) & 1);
           zero = sv == 1.f && zero_row<D>(sm + C::OFF_V + g % C::VS * C::TILE, key);
+          __syncwarp();
         }
         const float lv = __log2f(sv);  // off by under 2^-16, in V's factor alone
         add += lv;
