@@ -158,9 +158,11 @@ def test_int8_unusual_scales_beside_rows_without_a_token(KV, G, D, causal):
         v[3::11] *= 2.0 ** 60 if far else 0.0
         c = make(KV, 1, H, D, 16, sum(-(-x // 16) for x in lens), len(lens), True)
         c.append_chunks(0, range(len(lens)), lens, k, v)
-        for _ in range(3):
-            c.chunk_attention(0, range(len(lens)), counts, torch.full_like(q, 3e38) * k.new_tensor([1.0, -1.0]).repeat(D // 2), causal=causal)
-            attend(c, range(len(lens)), counts, q, causal)
+        first = attend(c, range(len(lens)), counts, q, causal)
+        for scale in (3e38, 1e4, 0.0):
+            c.chunk_attention(0, range(len(lens)), counts, torch.full_like(q, scale) * k.new_tensor([1.0, -1.0]).repeat(D // 2), causal=causal)
+            for a, b in zip(first, attend(c, range(len(lens)), counts, q, causal)):
+                assert torch.equal(a, b), "not deterministic"
 
 
 @pytest.mark.parametrize("m", ROWS)

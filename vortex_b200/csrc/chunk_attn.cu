@@ -186,9 +186,10 @@ __device__ __forceinline__ void transpose4(uint4 (&w)[4], int lane) {
 // zero (log2 scale -inf) add 2^(score + ref). Where the sum has a maximum of its own
 // (`far`), and from here on where such a share is too large or the row has no unit
 // but such keys, all keys add 2^(score - maximum). Rare: a function of its own leaves
-// the softmax its registers. Called by whole warps.
+// the softmax its registers. Called by whole warps; rows without a token (`token`)
+// have no say.
 template <int N>
-__device__ __noinline__ float odd_tile(uint32_t tS, const float *keys, int last, float ref, float m, float l, bool far, float *far_s) {
+__device__ __noinline__ float odd_tile(uint32_t tS, const float *keys, int last, float ref, float m, float l, bool token, bool far, float *far_s) {
   constexpr float SHIFT = 6.f;
   float v[8];
   if (!far) {
@@ -200,7 +201,7 @@ __device__ __noinline__ float odd_tile(uint32_t tS, const float *keys, int last,
 #pragma unroll
       for (int e = 0; e < 8; e++) share += c + e <= last && keys[BN + c + e] == -INFINITY ? ex2(fmaf(v[e], keys[c + e], ref)) : 0.f;
     }
-    if (!__any_sync(0xffffffffu, !(share <= kMostShare) || m == -INFINITY)) return l + share;
+    if (!__any_sync(0xffffffffu, token && (!(share <= kMostShare) || m == -INFINITY))) return l + share;
     *far_s = l == 0.f ? -INFINITY : fminf(m - SHIFT, FLT_MAX);
   }
   const float before = *far_s;
@@ -391,7 +392,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
         float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         if constexpr (INT8) {
           if (odd || far) {
-            l = odd_tile<N>(tS, keys, lim - kh, ref2.x, m, l * (far ? 1.f : alpha), far, far_s);
+            l = odd_tile<N>(tS, keys, lim - kh, ref2.x, m, l * (far ? 1.f : alpha), r < live, far, far_s);
             far = *far_s < INFINITY;
             alpha = 1.f;
           }
