@@ -252,6 +252,19 @@ def test_attention_behind_four_gigabytes_is_finite(KV, int8):
         attend(c, [fill], [m], rnd((m, H, D), 3, 2.0))
 
 
+def test_chunk_attention_refuses_what_is_no_tensor_and_scales_that_overflow(KV):
+    from vortex_b200 import _native as N
+    c = filled(KV, rnd((20, 2, 64), 1), rnd((20, 2, 64), 2), False)
+    q = rnd((4, 2, 64), 3)
+    for args in (dict(q=q.cpu().float().numpy()), dict(q=None), dict(lse=[[0.0, 0.0]] * 4), dict(lse=q.float().cpu().numpy()[..., 0]),
+                 dict(softmax_scale=3e38), dict(softmax_scale=1e39)):
+        with pytest.raises(N.VxbError) as e:
+            c.chunk_attention(0, [0], [4], **{"q": q, **args})
+        assert e.value.code == N.VXB_EINVAL
+    out = c.chunk_attention(0, [0], [4], torch.zeros_like(q), softmax_scale=2e38)
+    assert bool(torch.isfinite(out).all())
+
+
 # ---------------------------------------------------------------- cache
 
 def test_truncate_of_every_holder_needs_the_blocks_it_frees(KV):

@@ -1328,7 +1328,8 @@ VXB_API int vxb_chunk_attention(vxb_kv *kv, int layer, int n, const int64_t *h_s
   vxb_ctx *ctx = kv->ctx;
   if (layer < 0 || layer >= kv->num_layers) return set_error(ctx, VXB_EINVAL, "vxb_chunk_attention: layer %d out of range", layer);
   if (n < 0 || (n > 0 && (!h_seq_ids || !h_n_queries))) return set_error(ctx, VXB_EINVAL, "vxb_chunk_attention: bad arguments");
-  if (!(softmax_scale > 0.f) || std::isinf(softmax_scale)) return set_error(ctx, VXB_EINVAL, "vxb_chunk_attention: scale must be positive and finite");
+  if (!(softmax_scale > 0.f) || std::isinf(softmax_scale * 1.44269504088896340736f))  // (times log2 e: as the kernels use it)
+    return set_error(ctx, VXB_EINVAL, "vxb_chunk_attention: scale must be positive and finite");
   size_t need = 0;
   if (int rc = vxb_chunk_attention_ws(kv, num_q_heads, &need)) return rc;
   if (n == 0) return VXB_OK;

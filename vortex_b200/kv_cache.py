@@ -216,7 +216,7 @@ class PagedKVCache:
         import torch
         ids, counts = _ids_counts("chunk_attention", seq_ids, n_queries)
         rows, dev = sum(counts.tolist()), self.ctx.device
-        if q.dim() != 3:
+        if not isinstance(q, torch.Tensor) or q.dim() != 3:
             raise N.VxbError(N.VXB_EINVAL, "chunk_attention: q must be [rows, Hq, D]")
         Hq = q.shape[1]
         shape = (rows, Hq, self.head_dim)
@@ -225,7 +225,7 @@ class PagedKVCache:
             out = torch.empty_like(q)
         elif out is not _device_rows("chunk_attention", "out", out, shape, dev):
             raise N.VxbError(N.VXB_EINVAL, "chunk_attention: out must be contiguous and 16-byte aligned")
-        if lse is not None and (lse.dtype != torch.float32 or lse.get_device() != dev or not lse.is_contiguous()
+        if lse is not None and (not isinstance(lse, torch.Tensor) or lse.dtype != torch.float32 or lse.get_device() != dev or not lse.is_contiguous()
                                 or lse.shape != shape[:2]):
             raise N.VxbError(N.VXB_EINVAL, f"chunk_attention: lse must be contiguous f32 {shape[:2]} on cuda:{dev}")
         need = self._chunk_ws.get(Hq)
