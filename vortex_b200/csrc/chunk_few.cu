@@ -294,11 +294,14 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
         top = -INFINITY;
       }
       if (t == 0 || bar_or(bar, 128, top > RESCALE_THRESHOLD + SHIFT || far_key)) {
-        bool far = false;
+        bool odd = false, far = false;  // a key to look at; sums with maxima of their own
         if constexpr (INT8) {
-          const bool was = t > 0 && *far_s != 0;
-          far = bar_or(bar, 128, far_key) || was;
-          if (far && !was) own_sums();
+          odd = bar_or(bar, 128, far_key || zero);
+          far = t > 0 && *far_s != 0;
+          if (odd && bar_or(bar, 128, far_key) && !far) {
+            own_sums();
+            far = true;
+          }
         }
         // New references: a first tile's maximum, later the maximum of the rows
         // that passed it, becomes 2^SHIFT.
@@ -358,16 +361,14 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
           tmem_wait_st();
         }
         if (coarse) goto again;  // (once for a row: its reference never rises)
-        if constexpr (INT8) {
-          if (!far) {  // a row of zeros whose share of the sum is too large in the new unit
-            float share = -INFINITY;
+        if (INT8 && odd && !far) {  // a row of zeros whose share of the sum is too large in the new unit
+          float share = -INFINITY;
 #pragma unroll
-            for (int n = 0; n < N; n++) share = n / 8 < groups ? fmaxf(share, x[n]) : share;
-            if (bar_or(bar, 128, zero && share > kMostShareLog2)) {
-              own_sums();
-              if (key == 0) *far_s = 1;
-              bar_sync(bar, 128);
-            }
+          for (int n = 0; n < N; n++) share = n / 8 < groups ? fmaxf(share, x[n]) : share;
+          if (bar_or(bar, 128, zero && share > kMostShareLog2)) {
+            own_sums();
+            if (key == 0) *far_s = 1;
+            bar_sync(bar, 128);
           }
         }
       }
