@@ -280,8 +280,12 @@ int vxb_decode_attention(vxb_kv *kv, int layer, int n, const int64_t *h_seq_ids,
  * r (causal != 0) or to all len (causal == 0). out as q, lse (optional) f32
  * [rows, Hq], natural log. A row that sees no key (an empty or unknown
  * sequence, more queries than tokens) gives zeros and lse -inf; what the cache
- * holds behind a sequence's last token is never used. In an int8 cache a V
- * scale under 2^-100 counts as that. Query head j reads kv
+ * holds behind a sequence's last token is never used. A softmax weight is
+ * rounded once before it meets V: to bf16 (off by 2^-8 of it at most), in an
+ * int8 cache times the V scale to f16 (2^-11); vxb_decode_attention keeps more
+ * bits. Sums are f32: a weight under 2^-126 of its row's largest counts as 0,
+ * and bf16 values near the end of the range may overflow when added up. In an
+ * int8 cache a V scale under 2^-100 counts as that. Query head j reads kv
  * head j / (Hq / Hkv), Hq / Hkv <= 128. Tensors are 16-byte aligned.
  * d_ws: ws_bytes of device scratch (16-byte aligned), at least what
  * vxb_chunk_attention_ws gives for this cache and head count, not shared with

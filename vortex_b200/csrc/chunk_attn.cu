@@ -31,9 +31,9 @@
 // thread = row = TMEM lane; the halves tell each other their maxima), 16 issues
 // the MMAs, 17 the TMA copies; int8 caches use 18, which looks the V scales over,
 // and add 20-27, which turn int8 pages into K tiles of bf16 and V tiles of f16
-// (codes are exact in both). Pages come
-// through one ring of tiles in the order K, V, K, V, ...; a page box is up to
-// 128 tokens of one block, of which only those that hold tokens are copied.
+// (codes are exact in both). Pages come through one ring of tiles in the order K,
+// V, K, V, ...; a page box is up to 128 tokens of one block, of which only those
+// that hold tokens are copied.
 //
 // Keys behind the last token never count: S is masked by selection, the
 // MMA stops at the last 16 keys with a token and the rest of those 16 V rows
@@ -41,17 +41,22 @@
 // elements of V are taken out of the tile before the product and added to the
 // rows that see them (0 * inf would reach the others).
 //
-// Roundings. bf16 caches: P to bf16 once (2^-9 of a weight; the output's own
-// rounding is as large), the sums l are of the f32 weights. int8 caches: the
-// weights carry the V scale, log2(w) = log2(p) + log2(scale), the reference is
-// the maximum of those, and w goes into P as f16 times 2^6: 11 significant
-// bits, and weights down to 2^-30 of the row's largest keep at least one; l is
-// of w / scale in f32 or, beside scales out of 2^+-30, of the scores alone (kFarLog2).
-// Every wait is bounded.
+// Roundings. bf16 caches: P to bf16 once (2^-8 of a weight at most, as the
+// output's own; decode attention keeps a second part of P, which here would be
+// half as much tensor core work again), the sums l are of the f32 weights. int8 caches: the weights carry the V scale,
+// log2(w) = log2(p) + log2(scale), the reference is the maximum of those, and w
+// goes into P as f16 times 2^6: 2^-11 of a weight, and weights down to 2^-30 of
+// the row's largest keep at least one bit; l is of w / scale in f32 or, beside
+// scales out of 2^+-30, of the scores alone (kFarLog2). Value rows of zeros count
+// for l alone: warp 18 finds them, a few scales at a time, while S is formed.
+// Every wait is bounded, and a CTA ends behind its own copies and products.
 //
-// Measured: 4096 tokens behind 12288 (8 x 4 heads of 128) 775-800 us, 1.2
-// PFLOP/s of 1.6; 4 x 512 of 2048 (8 x 4 heads) 73 us, of 32 heads in int8 127;
-// 300 of 500 (8 x 4 heads) 16 us. A step of both streams (256 rows x 128 keys)
+// Measured: 4096 tokens behind 12288 (8 x 4 heads of 128) 810 us in a dozen
+// calls (1965 MHz, 1.19 PFLOP/s of 1.6), 920 in thousands (1640 MHz, power cap
+// of 1000 W, 1.05); 4 x 512 of 2048 (8 x 4 heads) 74 us, of 32 heads in int8 130
+// (127 before zero rows and scales far apart were handled); 300 of 500 (8 x 4
+// heads) 16 us; heads of 64, 4 x 512 of 2048 69 us, in int8 112. One zero row in
+// each tile costs int8 90%. A step of both streams (256 rows x 128 keys)
 // takes 3,400 to 4,000 cycles, of which the tensor core needs 2,100 and the 32
 // thousand exponentials 2,050: the chain S, maximum, P, O of a stream hides
 // only behind the other one's. A fourth of the exponentials on the FMA pipe

@@ -22,21 +22,25 @@
 // softmax of up to 32 rows, four of more (int8, 64 rows: 295 and 262 us then).
 //
 // int8 weights carry the V scale, w = p * scale, with the reference maximum
-// taken over log2(w), and go into P as f16 times 2^6: 11 significant bits, and
-// weights down to 2^-30 of the row's largest keep at least one. bf16 P rounds
-// at 2^-9 (the type of V decides). A value row of zeros counts for the sum alone
-// (chunk_attn.h): its key's thread keeps it out of the reference.
+// taken over log2(w), and go into P as f16 times 2^6: off by 2^-11 at most, and
+// weights down to 2^-30 of the row's largest keep at least one bit. bf16 P is off
+// by 2^-8 (the type of V decides; decode attention keeps a second part of P). A
+// value row of zeros counts for the sum alone (chunk_attn.h): its key's thread
+// keeps it out of the reference. A row takes its reference from its first tile
+// with a finite score (kUnset).
 //
 // Values of V that only some rows may see and that are not finite are taken
 // out of the tile and added to the rows that see them, as in chunk_attn.cu.
 //
 // Measured: 32 x 32 heads, ctx 2k, 4 rows 162 us (6.6 TB/s); 32 x 8 heads, ctx
-// 8k, 24 rows 165 us (6.5 TB/s), 64 rows 177, int8 16 rows 158 (3.5 TB/s), 64
-// rows 227; heads of 64, ctx 8k, 16 rows 93 us (5.8 TB/s), 64 rows 142; 32
-// heads, 333 keys, 4 rows 6.6 us. bf16 tiles of 128 columns wait for memory.
-// int8 halves the bytes and fills 63% of the issue slots with conversions and
-// softmax; tiles of 64 columns wait for the chain vote, exponentials, P to
+// 8k, 24 rows 164 us (6.6 TB/s), 64 rows 176, int8 16 rows 166 (3.3 TB/s), 64
+// rows 234; heads of 64, ctx 8k, 16 rows 93 us (5.7 TB/s), 64 rows 146, int8 133
+// and 195; 32 heads, 333 keys, 4 rows 6.6 us. bf16 tiles of 128 columns wait for
+// memory. int8 halves the bytes and fills 61% of the issue slots with conversions
+// and softmax; tiles of 64 columns wait for the chain vote, exponentials, P to
 // shared memory, announcement (up to 1.3 us a tile against 0.75 us of memory).
+// Looking for value rows of zeros and scales far apart costs int8 2 to 3%, heads
+// of 64 4 to 7%; rows of zeros in every tile cost 40%.
 #include <atomic>
 #include <climits>
 #include <cmath>

@@ -74,8 +74,9 @@ __device__ int block_min(int v, int *s) {
   return r;
 }
 
-// exp(d / t) with d = x - max <= 0 and c = log2(e) / t: the roundings of c and
-// of the product cost 1.5 * 2^-24 of |d| / t, the special-function unit 2 ulp.
+// exp(d / t) with d = x - max <= 0 and c = log2(e) / t: the roundings of d, of c
+// and of the product cost up to 2^-24 of |d| / t each, the special-function unit
+// 2 ulp.
 __device__ __forceinline__ float exp_scaled(float d, float c) {
   float e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(d * c));

@@ -212,7 +212,9 @@ class PagedKVCache:
         seq_ids[i] (packed, q bf16 [sum(n_queries), Hq, D]) are its last
         n_queries[i] cached tokens; each sees the tokens up to its own (all of
         them with causal=False). Returns bf16 like q (and fills lse f32 [rows,
-        Hq] if given). Rows that see nothing are zeros with lse -inf."""
+        Hq] if given). Rows that see nothing are zeros with lse -inf. Softmax
+        weights are rounded once, to bf16 (int8 caches: f16); attention() keeps
+        more bits of them."""
         import torch
         ids, counts = _ids_counts("chunk_attention", seq_ids, n_queries)
         rows, dev = sum(counts.tolist()), self.ctx.device
