@@ -159,9 +159,14 @@ __device__ __forceinline__ void halve(float *v, int lane) {
 }
 
 // Negated reference of a row that has seen no finite score yet: the first one
-// passes it, and the vote for new references is called. A sum with it has lost
-// the score's last bits, so that tile's exponents are formed again.
-constexpr float kUnset = 1048576.f;
+// passes it, and the vote for new references is called. The exponents of that
+// tile were formed with it and have lost the score's last bits. bf16 forms them
+// anew behind every vote (1% of a call for heads of 64). In int8 that, or a branch
+// to it, took 3 to 9% of a call: there the unit is less far away, so that the
+// weights of that one tile are off by 2^-14 ln 2 at most (f16 rounds at 2^-11),
+// and scores are told from none down to -700 (nats).
+template <bool INT8>
+constexpr float kUnset = INT8 ? 1024.f : 1048576.f;
 
 // int8: a tile's scores alone, added to each row's maximum and sum of 2^(score -
 // maximum) over the warp's keys. Rare (kFarLog2): a function of its own leaves the
@@ -263,7 +268,6 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
         isv = ex2(-lv);
         far_key = !(fabsf(lv) <= kFarLog2);
       }
-    again:
       float x[N];  // log2 of what goes into P
       // (the usual case of only live groups has code without their branches,
       // which keep the rows' chains apart)
@@ -324,24 +328,16 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
         bar_sync(bar, 128);
         if (key < N) {
           const float m = fmaxf(fmaxf(red[key], red[N + key]), fmaxf(red[2 * N + key], red[3 * N + key]));
-          const float d = t == 0 ? (m > -INFINITY ? SHIFT - m : kUnset) : fminf(SHIFT - m, 0.f);
-          const float ref = ref_s[key] + d;
-          d_s[key] = ref_s[key] >= kUnset / 2 && ref < kUnset / 2 ? NAN : d;
-          ref_s[key] = ref;
+          const float d = t == 0 ? (m > -INFINITY ? SHIFT - m : kUnset<INT8>) : fminf(SHIFT - m, 0.f);
+          ref_s[key] += d;
+          d_s[key] = d;
           f_s[key] = ex2(d);
         }
         if (INT8 && key == 0) *far_s = far;
         bar_sync(bar, 128);
-        // (bf16 forms its exponents anew in any case: this costs its heads of 64
-        // 1% of a call, the branch for the rare case 5%; int8 the other way round)
-        bool coarse = false;
         if constexpr (INT8) {
 #pragma unroll
-          for (int n = 0; n < N; n++) {
-            const float d = d_s[n];
-            x[n] += d;
-            coarse |= isnan(d);
-          }
+          for (int n = 0; n < N; n++) x[n] += d_s[n];
         } else {
           load(std::false_type{});
         }
@@ -364,7 +360,6 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
             }
           tmem_wait_st();
         }
-        if (coarse) goto again;  // (once for a row: its reference never rises)
         if (INT8 && odd && !far) {  // a row of zeros whose share of the sum is too large in the new unit
           float share = -INFINITY;
 #pragma unroll
