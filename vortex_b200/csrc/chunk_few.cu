@@ -94,8 +94,7 @@ template <int KS, int VS>
 struct Bars {
   uint64_t k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], q_full[2], q_empty[2], s_full[3], p_full[2], pv_done[2], o_full[2], o_free[2], drained;
   uint32_t tmem;
-  int acc;     // O already holds values that the piece's first product adds to
-  int far[4];  // int8, of each softmax warpgroup: the piece has met V scales out of kFarLog2
+  int acc;  // O already holds values that the piece's first product adds to
 };
 template <int D, bool INT8, int NR>
 using BarsOf = Bars<Cfg<D, INT8, NR>::KS, Cfg<D, INT8, NR>::VS>;
@@ -218,7 +217,6 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
   // this warpgroup's: per-warp results [4][N]; per row the negated reference, a factor, a change of the reference
   float *red = reinterpret_cast<float *>(sm + C::OFF_RED) + wg * C::PER_ROW * N, *ref_s = red + 4 * N, *f_s = ref_s + N, *d_s = f_s + N;
   float *far_top = d_s + N, *far_sum = far_top + 4 * N;  // int8: of each warp, see far_rows
-  int *far_s = &bars.far[wg];
   const float *scales = reinterpret_cast<const float *>(sm + C::OFF_SCALE);
   const int bar = 1 + wg;
   Waiter wait{a.err};
@@ -244,6 +242,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
       }
       __syncwarp();
     };
+    bool own = false;  // int8: the sums have maxima of their own (far_rows)
     for (int t = 0; t < T; t++, g++) {
       const int k0 = (p.tb + t) * BN, k = k0 + key;
       const uint32_t tS = bars.tmem + lane_off + (g % C::AHEAD) * NR + wg * 8;
@@ -302,13 +301,12 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
         top = -INFINITY;
       }
       if (t == 0 || bar_or(bar, 128, top > RESCALE_THRESHOLD + SHIFT || far_key)) {
-        bool odd = false, far = false;  // a key to look at; sums with maxima of their own
+        bool odd = false;  // a key to look at
         if constexpr (INT8) {
           odd = bar_or(bar, 128, far_key || zero);
-          far = t > 0 && *far_s != 0;
-          if (odd && bar_or(bar, 128, far_key) && !far) {
+          if (odd && bar_or(bar, 128, far_key) && !own) {
             own_sums();
-            far = true;
+            own = true;
           }
         }
         // New references: a first tile's maximum, later the maximum of the rows
@@ -333,7 +331,6 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
           d_s[key] = d;
           f_s[key] = ex2(d);
         }
-        if (INT8 && key == 0) *far_s = far;
         bar_sync(bar, 128);
         if constexpr (INT8) {
 #pragma unroll
@@ -360,14 +357,13 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
             }
           tmem_wait_st();
         }
-        if (INT8 && odd && !far) {  // a row of zeros whose share of the sum is too large in the new unit
+        if (INT8 && odd && !own) {  // a row of zeros whose share of the sum is too large in the new unit
           float share = -INFINITY;
 #pragma unroll
           for (int n = 0; n < N; n++) share = n / 8 < groups ? fmaxf(share, x[n]) : share;
           if (bar_or(bar, 128, zero && share > kMostShareLog2)) {
             own_sums();
-            if (key == 0) *far_s = 1;
-            bar_sync(bar, 128);
+            own = true;
           }
         }
       }
@@ -376,7 +372,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
       if (g >= 2) wait(&bars.pv_done[g & 1], ((g - 2) >> 1) & 1);
       uint8_t *prow = P + (key >> 6) * (NR * 128) + wg * 8 * 128 + (key & 7) * 2;
       const uint32_t chunk = (uint32_t)(key & 63) >> 3;
-      if (INT8 && *(volatile int *)far_s) {
+      if (INT8 && own) {
         far_rows(tS, groups, W * 8, wg * 8, sc, n_min, far_top + warp * N, far_sum + warp * N);
         isv = 0.f;
       }
@@ -473,7 +469,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, Ba
       float L = red[key] + red[N + key] + red[2 * N + key] + red[3 * N + key];
       const float unit = -ref_s[key] - SHIFT;  // of O (log2)
       float m = L == 0.f ? -INFINITY : unit, f = whole ? (L == 0.f ? 0.f : 1.f / L) : 1.f;
-      if (INT8 && T > 0 && *far_s) {
+      if (INT8 && own) {
         // O and the sum have units of their own: O is divided by the sum here,
         // also in a part, whose sum then is 1
         const float *tops = far_top + key, *sums = far_sum + key;
