@@ -282,6 +282,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
     const bool warp_live = warp4 * 32 < live;
     float m = -INFINITY, l = 0.f;
     if constexpr (INT8) *far_s = INFINITY;
+    bool far = false;  // int8: the sum has a maximum of its own from here on
     const int steps = p.steps(st);
     for (int i = 0; i < steps; i++, step++) {
       const int t = p.tile(st, i), k0 = t * BN, kh = k0 + half * N;
@@ -347,15 +348,14 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
             for (int c = 0; c < KEEP; c++) s[c] = kh + c0 + c <= lim ? s[c] : -INFINITY;
           }
         };
-        // the sum has a maximum of its own from here on: a scale of the tile (of both
-        // halves' keys), or of one before it
+        // a scale of the tile (of both halves' keys), or of one before it
         uint32_t odd = 0;
-        bool far = false;
         if constexpr (INT8) {
           odd = reinterpret_cast<const uint32_t *>(keys)[3 * BN - half * N];
-          const bool was = *far_s < INFINITY;
-          far = was || (odd & 1);
-          if (far && !was) *far_s = l == 0.f ? -INFINITY : fminf(m - SHIFT, FLT_MAX);
+          if ((odd & 1) && !far) {
+            far = true;
+            *far_s = l == 0.f ? -INFINITY : fminf(m - SHIFT, FLT_MAX);
+          }
         }
         float mx = -INFINITY;
 #pragma unroll
@@ -398,7 +398,7 @@ __device__ __forceinline__ void softmax_role(const ChunkArgs &a, uint8_t *sm, B 
         if constexpr (INT8) {
           if (odd || far) {
             l = odd_tile<N>(tS, keys, lim - kh, ref2.x, m, l * (far ? 1.f : alpha), r < live, far, far_s);
-            far = *far_s < INFINITY;
+            far = __any_sync(0xffffffffu, *far_s < INFINITY);  // (a warp's lanes agree)
             alpha = 1.f;
           }
         }
