@@ -53,9 +53,9 @@
 //
 // Measured: 4096 tokens behind 12288 (8 x 4 heads of 128) 810 us in a dozen
 // calls (1965 MHz, 1.19 PFLOP/s of 1.6), 920 in thousands (1640 MHz, power cap
-// of 1000 W, 1.05); 4 x 512 of 2048 (8 x 4 heads) 74 us, of 32 heads in int8 130
+// of 1000 W, 1.05); 4 x 512 of 2048 (8 x 4 heads) 74 us, of 32 heads in int8 129
 // (127 before zero rows and scales far apart were handled); 300 of 500 (8 x 4
-// heads) 16 us; heads of 64, 4 x 512 of 2048 69 us, in int8 112. One zero row in
+// heads) 16 us; heads of 64, 4 x 512 of 2048 69 us, in int8 114. One zero row in
 // each tile costs int8 90%. A step of both streams (256 rows x 128 keys)
 // takes 3,400 to 4,000 cycles, of which the tensor core needs 2,100 and the 32
 // thousand exponentials 2,050: the chain S, maximum, P, O of a stream hides

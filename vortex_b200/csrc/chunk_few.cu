@@ -33,14 +33,14 @@
 // out of the tile and added to the rows that see them, as in chunk_attn.cu.
 //
 // Measured: 32 x 32 heads, ctx 2k, 4 rows 162 us (6.6 TB/s); 32 x 8 heads, ctx
-// 8k, 24 rows 164 us (6.6 TB/s), 64 rows 176, int8 16 rows 166 (3.3 TB/s), 64
-// rows 234; heads of 64, ctx 8k, 16 rows 93 us (5.7 TB/s), 64 rows 146, int8 133
-// and 195; 32 heads, 333 keys, 4 rows 6.6 us. bf16 tiles of 128 columns wait for
+// 8k, 24 rows 164 us (6.6 TB/s), 64 rows 176, int8 16 rows 161 (3.4 TB/s), 64
+// rows 229; heads of 64, ctx 8k, 16 rows 93 us (5.7 TB/s), 64 rows 146, int8 131
+// and 188; 32 heads, 333 keys, 4 rows 6.6 us. bf16 tiles of 128 columns wait for
 // memory. int8 halves the bytes and fills 61% of the issue slots with conversions
 // and softmax; tiles of 64 columns wait for the chain vote, exponentials, P to
 // shared memory, announcement (up to 1.3 us a tile against 0.75 us of memory).
-// Looking for value rows of zeros and scales far apart costs int8 2 to 3%, heads
-// of 64 4 to 7%; rows of zeros in every tile cost 40%.
+// Looking for value rows of zeros and scales far apart costs int8 1 to 3%, heads
+// of 64 and launches of 32 rows 3 to 6%; a row of zeros in every tile 30 to 40%.
 #include <atomic>
 #include <climits>
 #include <cmath>
